@@ -240,6 +240,55 @@ int nmg_spmm_noalloc(const void *val, const int16_t *idx, int64_t M, int64_t K, 
                      const void *act, int64_t ld_act, int64_t tokens, const void *bias, void *out, int64_t ld_out,
                      int layout, void *stream);
 
+/* Rows of logits over a vocabulary (the two operators below; no counterpart in the reference, which leaves every loss to the
+ * model code).  Row r < rows begins at element (r / inner_rows) * ld_outer + (r % inner_rows) * ld of `logits` and has `vocab`
+ * consecutive elements of `dtype`; base and strides need no alignment beyond the element's.  z = x / temperature, everything
+ * is computed in 32 bits.  Logits may be -inf (masked).  A row that is -inf throughout has no distribution: its log-sum-exp
+ * and log-probabilities are -inf, its entropy, its divergence and its gradient 0.  A row that holds NaN or +inf gives NaN.
+ *
+ * nmg_token_log_probs writes, in fp32 and for every row,
+ *   log_prob  log softmax(z) at targets[r]; 0 where that is ignore_index, NaN where there is no such token (targets and log_prob
+ *             may both be NULL)
+ *   entropy   -sum p log p
+ *   lse       log sum exp z
+ *   norm      [rows][2], may be NULL: lse in two parts, for the backward pass (8-byte aligned)
+ *   top_log_prob, top_ids   [rows][top] log-probabilities and columns of the `top` (0 .. 128) largest logits, largest first, equal
+ *             ones in the order of their columns (-0 equals 0, NaN counts as larger than all)
+ * nmg_token_log_probs_backward writes d_logits (row pitches ld_d, ld_d_outer) from the gradients of those outputs, any of which
+ * may be NULL; it reads norm always, entropy with g_entropy, top_ids with g_top. */
+int nmg_token_log_probs(const void *logits, int64_t rows, int64_t inner_rows, int64_t ld, int64_t ld_outer, int64_t vocab, int dtype,
+                        const int64_t *targets, int64_t ignore_index, float temperature, int top, float *log_prob, float *entropy,
+                        float *lse, float *top_log_prob, int64_t *top_ids, float *norm, void *stream);
+int nmg_token_log_probs_backward(const void *logits, int64_t rows, int64_t inner_rows, int64_t ld, int64_t ld_outer, int64_t vocab,
+                                 int dtype, const int64_t *targets, int64_t ignore_index, float temperature, int top,
+                                 const int64_t *top_ids, const float *norm, const float *entropy, const float *g_log_prob,
+                                 const float *g_entropy, const float *g_lse, const float *g_top, void *d_logits, int64_t ld_d,
+                                 int64_t ld_d_outer, void *stream);
+
+/* Divergence of a student's rows of logits from a teacher of whom the `kept` (1 .. 256) top log-probabilities of each row are
+ * known: ids[rows][kept] (id_bytes 4 or 8 each; negative: padding), log_probs[rows][kept] of teacher_dtype, at the same temperature.
+ *   remainder = 0: q = softmax of the kept log_probs (so any logits divided by the temperature will do)
+ *   remainder = 1: q_i = exp(log_prob), and 1 - sum q (at least 0) is held against the student's probability of all other tokens
+ *                  together (left out where the student has no finite logit among them); vocab at most 2^20
+ *   row_loss = temperature^2 * weight[r] * sum q (log q - log softmax(z));  weight may be NULL (all 1)
+ * A row of weight 0, without a kept token of non-zero q, or of logits -inf throughout has loss 0 and gradient 0.  An id of
+ * vocab or more makes its row NaN; an id that occurs twice in a row stands for one token of the summed q.
+ * reduction: NMG_REDUCE_NONE row_loss is the result; NMG_REDUCE_SUM loss = sum row_loss; NMG_REDUCE_MEAN that divided by the sum of
+ * the weights (by rows without weights; 0 where it is 0).  Sums over rows are added in 64 bits in a fixed order.
+ * norm [rows][4] (8-byte aligned) and total [1] are written for nmg_distill_backward.  d_logits, where not NULL (a reduction only), receives
+ * the gradient of `loss` in the same pass.
+ * nmg_distill_backward writes the gradient for upstream[rows] (NMG_REDUCE_NONE) or upstream[1], the gradient of the loss;
+ * with skip_if_one it leaves d_logits as it is when *upstream is 1, as after an nmg_distill that wrote it. */
+typedef enum { NMG_REDUCE_NONE = 0, NMG_REDUCE_SUM = 1, NMG_REDUCE_MEAN = 2 } nmg_reduction;
+int nmg_distill(const void *logits, int64_t rows, int64_t inner_rows, int64_t ld, int64_t ld_outer, int64_t vocab, int dtype,
+                const void *ids, int id_bytes, const void *log_probs, int teacher_dtype, int kept, int remainder, float temperature,
+                const float *weight, int reduction, float *row_loss, float *norm, float *total, float *loss,
+                void *d_logits, int64_t ld_d, int64_t ld_d_outer, void *stream);
+int nmg_distill_backward(const void *logits, int64_t rows, int64_t inner_rows, int64_t ld, int64_t ld_outer, int64_t vocab, int dtype,
+                         const void *ids, int id_bytes, const void *log_probs, int teacher_dtype, int kept, int remainder,
+                         float temperature, const float *weight, int reduction, const float *norm, const float *total, const float *upstream, int skip_if_one, void *d_logits, int64_t ld_d,
+                         int64_t ld_d_outer, void *stream);
+
 /* Measurement helpers (no counterpart in the reference; its profiling is wall-clock around whole operators,
  * src/sten/sten.py:30-49).
  * nmg_profile_next: the next nmg_spmm / nmg_spmm_t call made by this thread records `start_event` immediately before

@@ -16,9 +16,10 @@ NMG_ACT_TOKEN_MAJOR, NMG_ACT_K_MAJOR, NMG_ACT_TOKEN_MAJOR_OUT_ROWS = 0, 1, 2
 NMG_ALGO_AUTO, NMG_ALGO_SIMT, NMG_ALGO_TENSOR, NMG_ALGO_TENSOR_DENSE = 0, 1, 2, 3
 NMG_NOALLOC_SCRATCH_BYTES = 32 << 20
 NMG_EPI_NONE, NMG_EPI_GELU = 0, 1
+NMG_REDUCE_NONE, NMG_REDUCE_SUM, NMG_REDUCE_MEAN = 0, 1, 2
 
 # name -> (restype, argtypes); must list every function of include/nmg_b200.h (checked by the test-suite)
-_i64, _int, _vp, _sz = ctypes.c_int64, ctypes.c_int, ctypes.c_void_p, ctypes.c_size_t
+_i64, _int, _vp, _sz, _f32 = ctypes.c_int64, ctypes.c_int, ctypes.c_void_p, ctypes.c_size_t, ctypes.c_float
 SIGNATURES = {
     "nmg_version": (_int, []),
     "nmg_last_error": (ctypes.c_char_p, []),
@@ -51,6 +52,12 @@ SIGNATURES = {
     "nmg_spmm_replicated_workspace_bytes": (_sz, [_i64, _i64, _i64, _int, _int, _int, _int]),
     "nmg_spmm_replicated": (_int, [_vp, _vp, _i64, _i64, _int, _int, _int, _int, _vp, _i64, _i64, _vp, _vp, _int, _vp, _i64, _vp, _sz, _vp]),
     "nmg_spmm_noalloc": (_int, [_vp, _vp, _i64, _i64, _int, _int, _int, _int, _vp, _i64, _i64, _vp, _vp, _i64, _int, _vp]),
+    "nmg_token_log_probs": (_int, [_vp, _i64, _i64, _i64, _i64, _i64, _int, _vp, _i64, _f32, _int, _vp, _vp, _vp, _vp, _vp, _vp, _vp]),
+    "nmg_token_log_probs_backward": (_int, [_vp, _i64, _i64, _i64, _i64, _i64, _int, _vp, _i64, _f32, _int, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64,
+                                            _vp]),
+    "nmg_distill": (_int, [_vp, _i64, _i64, _i64, _i64, _i64, _int, _vp, _int, _vp, _int, _int, _int, _f32, _vp, _int, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _vp]),
+    "nmg_distill_backward": (_int, [_vp, _i64, _i64, _i64, _i64, _i64, _int, _vp, _int, _vp, _int, _int, _int, _f32, _vp, _int, _vp, _vp, _vp, _int, _vp, _i64, _i64,
+                                    _vp]),
     "nmg_profile_next": (_int, [_vp, _vp]),
     "nmg_measure_fma_peak": (_int, [ctypes.POINTER(ctypes.c_double), _vp]),
     "nmg_memcpy_2d_async": (_int, [_vp, _sz, _vp, _sz, _sz, _sz, _vp]),

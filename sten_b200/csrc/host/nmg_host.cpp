@@ -16,6 +16,7 @@
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
+#include <algorithm>
 #include <memory>
 #include <optional>
 #include <string>
@@ -879,6 +880,264 @@ PyObject *handle_gather(PyObject *self, PyObject *const *a, Py_ssize_t nargs) {
     NMG_PY_END
 }
 
+// ------------------------------------------------------------------------------------------------ rows of logits
+float float_arg(PyObject *o) {
+    const double v = PyFloat_AsDouble(o);
+    if (v == -1.0 && PyErr_Occurred()) throw PyRaised();
+    return (float)v;
+}
+
+int float_code(const at::Tensor &t, const char *what) {
+    switch (t.scalar_type()) {
+        case at::kFloat: return NMG_F32;
+        case at::kHalf: return NMG_F16;
+        case at::kBFloat16: return NMG_BF16;
+        default: break;
+    }
+    py_raise(PyExc_TypeError, std::string(what) + " must be float32, float16 or bfloat16, got " + c10::toString(t.scalar_type()));
+}
+
+// [..., vocab] as the library takes it: two levels of rows.  The copy is made only where the strides need more or the columns are apart.
+struct LogitRows {
+    at::Tensor t;
+    int64_t rows, inner, ld, ld_outer, vocab;
+    bool apart;  // no two rows share an element
+};
+LogitRows logit_rows(const at::Tensor &t0) {
+    if (t0.dim() < 1 || t0.size(-1) < 1) py_raise(PyExc_ValueError, "logits must have a last dimension of at least one token, got shape " + shape_str(t0.sizes()));
+    for (at::Tensor t = t0;; t = t0.contiguous()) {
+        LogitRows r{t, 1, 1, t.size(-1), 0, t.size(-1), true};
+        int64_t size[2] = {1, 1}, stride[2] = {0, 0};  // inner, outer
+        int levels = 0;
+        for (int64_t d = t.dim() - 2; d >= 0; d--) {
+            const int64_t n = t.size(d), st = t.stride(d);
+            r.rows *= n;
+            if (n == 1) continue;
+            if (levels > 0 && levels <= 2 && st == size[levels - 1] * stride[levels - 1]) {
+                size[levels - 1] *= n;
+            } else if (levels++ < 2) {
+                size[levels - 1] = n;
+                stride[levels - 1] = st;
+            }
+        }
+        if (r.rows > 0 && (levels > 2 || (r.vocab > 1 && t.stride(-1) != 1))) continue;
+        if (levels > 0) {
+            r.inner = size[0] > 0 ? size[0] : 1;
+            r.ld = stride[0];
+        }
+        r.ld_outer = levels > 1 ? stride[1] : r.inner * r.ld;
+        r.apart = (r.inner == 1 || r.ld >= r.vocab) && (levels < 2 || r.ld_outer >= (r.inner - 1) * r.ld + r.vocab);
+        return r;
+    }
+}
+std::vector<int64_t> lead_shape(const at::Tensor &t) { return std::vector<int64_t>(t.sizes().begin(), t.sizes().end() - 1); }
+
+// Tensor for the logits' gradient.  It takes the logits' strides and the place of their rows relative to 16-byte boundaries, so that
+// the kernels read and write whole vectors; a tensor of its own layout where that would leave much of the memory unused.
+LogitRows gradient_of(const LogitRows &x) {
+    LogitRows g = x;
+    const int64_t es = (int64_t)x.t.element_size(), phase = (int64_t)(reinterpret_cast<uintptr_t>(x.t.const_data_ptr()) % 16) / es;
+    const int64_t span = x.rows > 0 ? (x.rows / x.inner - 1) * x.ld_outer + (x.inner - 1) * x.ld + x.vocab : 0, numel = x.rows * x.vocab;
+    if (x.t.is_contiguous() && phase == 0) {
+        g.t = new_empty(x.t.sizes(), x.t.scalar_type());
+    } else if (x.apart && span <= numel + numel / 4) {
+        g.t = new_empty({span + phase}, x.t.scalar_type()).as_strided(x.t.sizes(), x.t.strides(), phase);
+        return g;
+    } else {
+        g.t = new_empty(x.t.sizes(), x.t.scalar_type());
+    }
+    g.ld = x.vocab;
+    g.ld_outer = x.inner * x.vocab;
+    g.apart = true;
+    return g;
+}
+
+void check_lead(const at::Tensor &t, const at::Tensor &logits, const char *what) {
+    if (t.sizes() != logits.sizes().slice(0, logits.dim() - 1))
+        py_raise(PyExc_ValueError, std::string(what) + " must have one entry per row of the logits: expected shape " + shape_str(logits.sizes().slice(0, logits.dim() - 1)) + ", got " + shape_str(t.sizes()));
+}
+const int64_t *targets_ptr(const at::Tensor &targets) { return targets.defined() ? static_cast<const int64_t *>(targets.const_data_ptr()) : nullptr; }
+at::Tensor checked_targets(PyObject *o, const at::Tensor &logits) {
+    const at::Tensor t = optional_tensor(o);
+    if (!t.defined()) return t;
+    if (t.scalar_type() != at::kLong) py_raise(PyExc_TypeError, std::string("targets must be int64, got ") + c10::toString(t.scalar_type()));
+    check_lead(t, logits, "targets");
+    return packed_rows(t);
+}
+const float *f32_ptr(const at::Tensor &t) { return t.defined() ? static_cast<const float *>(t.const_data_ptr()) : nullptr; }
+// gradient of an fp32 output, as the kernels read it
+at::Tensor upstream_arg(PyObject *o) {
+    const at::Tensor t = optional_tensor(o);
+    if (!t.defined()) return t;
+    if (t.scalar_type() != at::kFloat) py_raise(PyExc_TypeError, std::string("gradients of float32 outputs must be float32, got ") + c10::toString(t.scalar_type()));
+    return packed_rows(t);
+}
+void set_item(PyObject *tuple, Py_ssize_t i, const at::Tensor &t) { PyTuple_SET_ITEM(tuple, i, t.defined() ? THPVariable_Wrap(t) : Py_NewRef(Py_None)); }
+
+// token_log_probs(logits, targets, ignore_index, temperature, top, with_norm) -> (log_prob, entropy, lse, top_log_prob, top_ids, norm)
+PyObject *py_token_log_probs(PyObject *, PyObject *const *a, Py_ssize_t nargs) {
+    NMG_PY_BEGIN(6)
+    const at::Tensor &logits = tensor_arg(a[0]);
+    const at::Tensor raw = optional_tensor(a[1]);
+    const c10::Device dev = device_of({&logits, &raw});
+    const int code = float_code(logits, "logits");
+    const c10::cuda::CUDAGuard guard(dev);
+    const LogitRows x = logit_rows(logits);
+    const at::Tensor targets = checked_targets(a[1], logits);
+    const int64_t ignore = int_arg(a[2]), top = int_arg(a[4]);
+    const float temperature = float_arg(a[3]);
+    if (top < 0 || top > x.vocab) py_raise(PyExc_ValueError, "top must be between 0 and the vocabulary's " + std::to_string(x.vocab) + " tokens, got " + std::to_string(top));
+    const std::vector<int64_t> lead = lead_shape(logits);
+    std::vector<int64_t> many = lead;
+    many.push_back(top);
+    at::Tensor log_prob, top_log_prob, top_ids, norm;
+    const at::Tensor entropy = new_empty(lead, at::kFloat), lse = new_empty(lead, at::kFloat);
+    if (targets.defined()) log_prob = new_empty(lead, at::kFloat);
+    if (int_arg(a[5]) != 0) norm = new_empty({x.rows, 2}, at::kFloat);
+    if (top > 0) {
+        top_log_prob = new_empty(many, at::kFloat);
+        top_ids = new_empty(many, at::kLong);
+    }
+    if (x.rows > 0) {
+        void *st = stream_of(dev);
+        auto f32 = [](const at::Tensor &t) { return t.defined() ? static_cast<float *>(t.mutable_data_ptr()) : nullptr; };
+        PyThreadState *save = PyEval_SaveThread();
+        const int rc = nmg_token_log_probs(x.t.const_data_ptr(), x.rows, x.inner, x.ld, x.ld_outer, x.vocab, code, targets_ptr(targets), ignore, temperature, (int)std::min<int64_t>(top, 1 << 30),
+                                           f32(log_prob), f32(entropy), f32(lse), f32(top_log_prob), top > 0 ? static_cast<int64_t *>(top_ids.mutable_data_ptr()) : nullptr, f32(norm), st);
+        PyEval_RestoreThread(save);
+        check(rc);
+    }
+    PyObject *r = PyTuple_New(6);
+    set_item(r, 0, log_prob);
+    set_item(r, 1, entropy);
+    set_item(r, 2, lse);
+    set_item(r, 3, top_log_prob);
+    set_item(r, 4, top_ids);
+    set_item(r, 5, norm);
+    return r;
+    NMG_PY_END
+}
+
+// token_log_probs_backward(logits, targets, ignore_index, temperature, top_ids, norm, entropy, g_log_prob, g_entropy, g_lse, g_top) -> d_logits
+PyObject *py_token_log_probs_backward(PyObject *, PyObject *const *a, Py_ssize_t nargs) {
+    NMG_PY_BEGIN(11)
+    const at::Tensor &logits = tensor_arg(a[0]);
+    const c10::Device dev = device_of({&logits});
+    const int code = float_code(logits, "logits");
+    const c10::cuda::CUDAGuard guard(dev);
+    const LogitRows x = logit_rows(logits);
+    const at::Tensor targets = checked_targets(a[1], logits), top_ids = optional_tensor(a[4]), norm = tensor_arg(a[5]), entropy = optional_tensor(a[6]);
+    const at::Tensor g_log_prob = upstream_arg(a[7]), g_entropy = upstream_arg(a[8]), g_lse = upstream_arg(a[9]), g_top = upstream_arg(a[10]);
+    const LogitRows d = gradient_of(x);
+    if (x.rows > 0) {
+        void *st = stream_of(dev);
+        const int64_t ignore = int_arg(a[2]);
+        const float temperature = float_arg(a[3]);
+        PyThreadState *save = PyEval_SaveThread();
+        const int rc = nmg_token_log_probs_backward(x.t.const_data_ptr(), x.rows, x.inner, x.ld, x.ld_outer, x.vocab, code, targets_ptr(targets), ignore, temperature,
+                                                    top_ids.defined() ? (int)top_ids.size(-1) : 0, targets_ptr(top_ids), f32_ptr(norm), f32_ptr(entropy), f32_ptr(g_log_prob),
+                                                    f32_ptr(g_entropy), f32_ptr(g_lse), f32_ptr(g_top), d.t.mutable_data_ptr(), d.ld, d.ld_outer, st);
+        PyEval_RestoreThread(save);
+        check(rc);
+    }
+    return THPVariable_Wrap(d.t);
+    NMG_PY_END
+}
+
+struct Teacher {
+    at::Tensor ids, log_probs, weight;
+    int id_bytes, code;
+    int64_t kept;
+};
+Teacher teacher_args(PyObject *ids_, PyObject *log_probs_, PyObject *weight_, const at::Tensor &logits) {
+    const at::Tensor &ids = tensor_arg(ids_), &log_probs = tensor_arg(log_probs_);
+    const at::Tensor weight = optional_tensor(weight_);
+    if (ids.scalar_type() != at::kLong && ids.scalar_type() != at::kInt) py_raise(PyExc_TypeError, std::string("teacher_ids must be int64 or int32, got ") + c10::toString(ids.scalar_type()));
+    const int code = float_code(log_probs, "teacher_log_probs");
+    if (ids.dim() != logits.dim() || ids.sizes().slice(0, ids.dim() - 1) != logits.sizes().slice(0, logits.dim() - 1) || ids.size(-1) < 1)
+        py_raise(PyExc_ValueError, "teacher_ids must hold at least one token per row of the logits: logits " + shape_str(logits.sizes()) + ", teacher_ids " + shape_str(ids.sizes()));
+    if (log_probs.sizes() != ids.sizes()) py_raise(PyExc_ValueError, "teacher_log_probs must have the shape of teacher_ids " + shape_str(ids.sizes()) + ", got " + shape_str(log_probs.sizes()));
+    if (weight.defined()) {
+        if (weight.scalar_type() != at::kFloat) py_raise(PyExc_TypeError, std::string("weight must be float32, got ") + c10::toString(weight.scalar_type()));
+        check_lead(weight, logits, "weight");
+    }
+    return Teacher{packed_rows(ids), packed_rows(log_probs), weight.defined() ? packed_rows(weight) : weight, ids.scalar_type() == at::kLong ? 8 : 4, code, ids.size(-1)};
+}
+
+// distill(logits, ids, log_probs, weight, remainder, temperature, reduction, with_gradient) -> (loss, norm, total, d_logits)
+PyObject *py_distill(PyObject *, PyObject *const *a, Py_ssize_t nargs) {
+    NMG_PY_BEGIN(8)
+    const at::Tensor &logits = tensor_arg(a[0]), &ids = tensor_arg(a[1]), &log_probs = tensor_arg(a[2]);
+    const at::Tensor weight = optional_tensor(a[3]);
+    const c10::Device dev = device_of({&logits, &ids, &log_probs, &weight});
+    const int code = float_code(logits, "logits");
+    const c10::cuda::CUDAGuard guard(dev);
+    const LogitRows x = logit_rows(logits);
+    const Teacher t = teacher_args(a[1], a[2], a[3], logits);
+    const int remainder = int_arg(a[4]) != 0, reduction = (int)int_arg(a[6]);
+    const float temperature = float_arg(a[5]);
+    const std::vector<int64_t> lead = lead_shape(logits);
+    const at::Tensor row_loss = new_empty(lead, at::kFloat), norm = new_empty({x.rows, 4}, at::kFloat);
+    at::Tensor loss, total;
+    if (reduction != NMG_REDUCE_NONE) loss = new_empty({}, at::kFloat);
+    if (reduction == NMG_REDUCE_MEAN && t.weight.defined()) total = new_empty({1}, at::kFloat);
+    LogitRows d{at::Tensor(), 0, 1, 0, 0, 0, true};
+    if (int_arg(a[7]) != 0) d = gradient_of(x);
+    if (x.rows > 0) {
+        void *st = stream_of(dev);
+        auto f32 = [](const at::Tensor &v) { return v.defined() ? static_cast<float *>(v.mutable_data_ptr()) : nullptr; };
+        PyThreadState *save = PyEval_SaveThread();
+        const int rc = nmg_distill(x.t.const_data_ptr(), x.rows, x.inner, x.ld, x.ld_outer, x.vocab, code, t.ids.const_data_ptr(), t.id_bytes, t.log_probs.const_data_ptr(), t.code,
+                                   (int)std::min<int64_t>(t.kept, 1 << 30), remainder, temperature, f32_ptr(t.weight), reduction, f32(row_loss), f32(norm), f32(total), f32(loss),
+                                   d.t.defined() ? d.t.mutable_data_ptr() : nullptr, d.ld, d.ld_outer, st);
+        PyEval_RestoreThread(save);
+        check(rc);
+    } else if (loss.defined()) {
+        loss.zero_();
+    }
+    PyObject *r = PyTuple_New(4);
+    set_item(r, 0, reduction == NMG_REDUCE_NONE ? row_loss : loss);
+    set_item(r, 1, norm);
+    set_item(r, 2, total);
+    set_item(r, 3, d.t);
+    return r;
+    NMG_PY_END
+}
+
+// distill_backward(logits, ids, log_probs, weight, remainder, temperature, reduction, norm, total, upstream, d_logits) -> d_logits;
+// a d_logits that distill() wrote stays as it is where upstream is 1, and is written again where it is not
+PyObject *py_distill_backward(PyObject *, PyObject *const *a, Py_ssize_t nargs) {
+    NMG_PY_BEGIN(11)
+    const at::Tensor &logits = tensor_arg(a[0]);
+    const c10::Device dev = device_of({&logits});
+    const int code = float_code(logits, "logits");
+    const c10::cuda::CUDAGuard guard(dev);
+    const LogitRows x = logit_rows(logits);
+    const Teacher t = teacher_args(a[1], a[2], a[3], logits);
+    const int remainder = int_arg(a[4]) != 0, reduction = (int)int_arg(a[6]);
+    const float temperature = float_arg(a[5]);
+    const at::Tensor norm = tensor_arg(a[7]), total = optional_tensor(a[8]), upstream = upstream_arg(a[9]), made = optional_tensor(a[10]);
+    LogitRows d = gradient_of(x);
+    if (made.defined()) {
+        d = logit_rows(made);
+        if (d.inner != x.inner) {  // rows that collapse to one level here and to two there
+            d.inner = x.inner;
+            d.ld_outer = x.inner * d.ld;
+        }
+    }
+    if (x.rows > 0) {
+        void *st = stream_of(dev);
+        PyThreadState *save = PyEval_SaveThread();
+        const int rc = nmg_distill_backward(x.t.const_data_ptr(), x.rows, x.inner, x.ld, x.ld_outer, x.vocab, code, t.ids.const_data_ptr(), t.id_bytes, t.log_probs.const_data_ptr(), t.code,
+                                            (int)std::min<int64_t>(t.kept, 1 << 30), remainder, temperature, f32_ptr(t.weight), reduction, f32_ptr(norm), f32_ptr(total),
+                                            f32_ptr(upstream), made.defined(), d.t.mutable_data_ptr(), d.ld, d.ld_outer, st);
+        PyEval_RestoreThread(save);
+        check(rc);
+    }
+    return THPVariable_Wrap(d.t);
+    NMG_PY_END
+}
+
 PyMethodDef handle_methods[] = {
     NMG_METHOD("gather", handle_gather),
     NMG_METHOD("linear", handle_linear),
@@ -904,6 +1163,10 @@ PyMethodDef module_methods[] = {
     NMG_METHOD("gather", py_gather),
     NMG_METHOD("column_sum", py_column_sum),
     NMG_METHOD("densify", py_densify),
+    NMG_METHOD("token_log_probs", py_token_log_probs),
+    NMG_METHOD("token_log_probs_backward", py_token_log_probs_backward),
+    NMG_METHOD("distill", py_distill),
+    NMG_METHOD("distill_backward", py_distill_backward),
     NMG_METHOD("capturing", py_capturing),
     NMG_METHOD("check_weight", py_check_weight),
     NMG_METHOD("set_dispatch", py_set_dispatch),

@@ -1,0 +1,336 @@
+// Distillation from a teacher of whom only the top log-probabilities of every row were kept.
+//
+// A row has up to KEPT_MAX kept tokens i with teacher log-probabilities l_i (negative ids are padding), student logits z = x / tau,
+// p = softmax(z).  The teacher's distribution is
+//   without remainder:  q = softmax over the kept l_i;
+//   with remainder:     q_i = e^l_i, and q_0 = max(0, 1 - sum q_i) on all other tokens together, which the student gives
+//                       p_0 = sum of p over the tokens not kept.
+// loss = tau^2 w (sum q_i (log q_i - log p_i) + q_0 (log q_0 - log p_0)), and with r = softmax of z over the tokens not kept and
+// S = sum q_i + q_0,
+//   d loss / d x_j = tau w (S p_j - sum of q_i with id_i = j)   on kept tokens (without remainder: on all, S = 1),
+//                    tau w r_j (S p_0 - q_0)                    on the others.
+// p_0 is summed over the tokens not kept and never formed as 1 - sum p_i, whose rounding error is as large as p_0 itself once the
+// student is sure: the kept tokens are marked in a bitmap in shared memory, the pass over the row leaves them out, and the
+// kept logits, gathered beforehand, are added afterwards.
+//
+// distill_kernel<T, REST, STATS, GRAD>: STATS, the pass that finds the normalisers, and the loss; GRAD, the pass that writes the
+// gradient.  Both in one launch read a row from HBM once: the second pass finds it in L2.  GRAD alone takes the normalisers
+// of an earlier launch and a gradient of the loss.
+#include "nmg_vocab.cuh"
+
+namespace nmg {
+
+constexpr int KEPT_MAX = 256;
+constexpr int MAX_REST_VOCAB = 1 << 20;  // bitmap of 128 KB
+constexpr int FILTER_BITS = 1 << 16;     // without remainder the bits only have to tell whether an id may be there twice
+constexpr int BIT0 = 16;                 // bit of the column behind the lead: its vectors' bits begin at whole bytes (nibbles)
+
+struct DistillParams {
+    Logits x;
+    const void *ids, *log_probs;
+    int id_bytes, teacher_dtype, kept, parts;
+    float tau, inv_tau;
+    const float *weight, *total;  // total: what the losses are divided by, NULL for `divisor`
+    float divisor;
+    float *loss;                  // per row
+    Norm *norm;                   // two per row, of all tokens and of those not kept: written with STATS, read without
+    const float *upstream;        // GRAD without STATS: gradient of each row's loss, or with upstream_one of their sum
+    int upstream_one, skip_if_one;
+    void *dx;
+    int64_t ld_dx, ld_dx_outer;
+};
+
+struct KeptShared {
+    float q[KEPT_MAX], logq[KEPT_MAX], x[KEPT_MAX];
+    int id[KEPT_MAX];      // -1: padding
+    uint8_t first[KEPT_MAX];
+    float mass, rest, max_x, sum_x;  // S, q_0, and the statistics of the kept logits
+    int some, twice;
+};
+
+__device__ __forceinline__ float teacher_value(const void *p, int dtype, int64_t i) {
+    if (dtype == NMG_F32) return static_cast<const float *>(p)[i];
+    if (dtype == NMG_F16) return __half2float(static_cast<const __half *>(p)[i]);
+    return __bfloat162float(static_cast<const __nv_bfloat16 *>(p)[i]);
+}
+__device__ __forceinline__ float warp_max(float v) {
+#pragma unroll
+    for (int o = 16; o; o >>= 1) v = fmaxf(v, __shfl_xor_sync(FULL, v, o));
+    return v;
+}
+__device__ __forceinline__ float warp_sum(float v) {
+#pragma unroll
+    for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(FULL, v, o);
+    return v;
+}
+
+template <typename T, bool REST, bool STATS, bool GRAD> __global__ void __launch_bounds__(VT, VOCAB_CTAS) distill_kernel(DistillParams p) {
+    extern __shared__ __align__(16) uint32_t bits[];
+    __shared__ Stats red[VT / 32], part;
+    __shared__ KeptShared sh;
+    const int tid = (int)threadIdx.x, lane = tid & 31, warp = tid >> 5, rank = (int)(blockIdx.x % (unsigned)p.parts);
+    const int64_t r = blockIdx.x / (unsigned)p.parts;
+    const Slice<T> sl(static_cast<const T *>(p.x.x) + row_offset(r, p.x.inner, p.x.ld, p.x.ld_outer), p.x.vocab, rank, p.parts);
+    T *dx = GRAD ? static_cast<T *>(p.dx) + row_offset(r, p.x.inner, p.ld_dx, p.ld_dx_outer) : nullptr;
+    if (GRAD && !STATS && p.skip_if_one && *p.upstream == 1.f) return;  // the gradient that is there already is this one
+    const float weight = p.weight ? p.weight[r] : 1.f;
+    auto leave = [&] {  // a row that does not count
+        if constexpr (GRAD) grad_pass<4>(sl, dx, [](float) { return 0.f; });
+        if (STATS && rank == 0 && tid == 0) {
+            p.loss[r] = 0.f;
+            p.norm[2 * r] = p.norm[2 * r + 1] = Norm{neg_inf(), 0.f};
+        }
+    };
+    if (weight == 0.f) return leave();  // whatever its logits are, they are not read for the loss
+
+    // the kept tokens
+    const int words = REST ? (p.x.vocab + BIT0 + 31) / 32 : FILTER_BITS / 32;
+    auto bit_of = [&](int col) { return REST ? col - sl.lead + BIT0 : col & (FILTER_BITS - 1); };
+    for (int i = tid; i < words; i += VT) bits[i] = 0u;
+    int id = -1;
+    bool none_such = false;
+    if (tid < p.kept) {
+        const int64_t raw = p.id_bytes == 8 ? static_cast<const int64_t *>(p.ids)[r * p.kept + tid] : static_cast<const int *>(p.ids)[r * p.kept + tid];
+        none_such = raw >= p.x.vocab;
+        id = raw < 0 || none_such ? -1 : (int)raw;
+        sh.id[tid] = id;
+        sh.logq[tid] = id < 0 ? neg_inf() : teacher_value(p.log_probs, p.teacher_dtype, r * p.kept + tid);
+        sh.x[tid] = id < 0 ? neg_inf() : sl.at(id);
+        sh.first[tid] = 0;
+    }
+    if (tid == 0) sh.twice = 0;
+    const bool bad = __syncthreads_or(none_such);
+    if (id >= 0) {
+        const uint32_t bit = 1u << (bit_of(id) & 31);
+        if (atomicOr(&bits[bit_of(id) >> 5], bit) & bit) sh.twice = 1;  // without remainder: perhaps
+    }
+    __syncthreads();
+    if (sh.twice) {  // an id that is there more than once counts as one token with the sum of its q
+        if (id >= 0) {
+            bool first = true;
+            for (int i = 0; i < tid; i++) first = first && sh.id[i] != id;
+            sh.first[tid] = first;
+        }
+    } else if (id >= 0) {
+        sh.first[tid] = 1;
+    }
+    __syncthreads();
+    const float a = LOG2E * p.inv_tau, slack = 8.f * p.tau;
+    if (warp == 0) {
+        float top = neg_inf(), sum = 0.f, max_x = neg_inf(), sum_x = 0.f;
+        for (int i = lane; i < p.kept; i += 32) {
+            top = fmaxf(top, sh.logq[i]);
+            if (sh.first[i]) max_x = fmaxf(max_x, sh.x[i]);
+        }
+        top = REST ? 0.f : warp_max(top);
+        max_x = warp_max(max_x);
+        const float ref = top == neg_inf() ? 0.f : top, ref_x = max_x == neg_inf() ? 0.f : max_x;
+        for (int i = lane; i < p.kept; i += 32) {
+            const float q = expf(sh.logq[i] - ref);
+            sh.q[i] = q;
+            sum += q;
+            if (sh.first[i]) sum_x += exp2_fast((sh.x[i] - ref_x) * a);
+        }
+        sum = warp_sum(sum);
+        sum_x = warp_sum(sum_x);
+        if (!REST) {
+            const float norm = ref + logf(sum), inv = 1.f / sum;
+            for (int i = lane; i < p.kept; i += 32) {
+                sh.logq[i] -= norm;
+                sh.q[i] *= inv;
+            }
+        }
+        if (lane == 0) {
+            sh.some = REST || sum != 0.f;
+            sh.mass = REST ? sum : 1.f;
+            sh.rest = REST ? fmaxf(1.f - sum, 0.f) : 0.f;
+            sh.max_x = max_x;
+            sh.sum_x = sum_x;
+        }
+    }
+
+    // the normalisers: of all tokens, and of those not kept
+    Norm all, rest;
+    if constexpr (STATS) {
+        Stats st = Stats::none();
+        constexpr int U = 4, N = U * VEC<T>;
+        auto marked = [&](int bit) { return bits[bit >> 5] >> (bit & 31); };
+        for_vectors<U>(sl, [&](const uint4 *q, int v, int n) {
+            float x[N], top = neg_inf();
+#pragma unroll
+            for (int u = 0; u < U; u++) {
+                unpack<T>(q[u], x + u * VEC<T>);
+                if constexpr (REST) {
+                    const uint32_t out = u < n ? marked(BIT0 + (v + u * VT) * VEC<T>) & ((1u << VEC<T>) - 1) : 0u;
+                    if (out) {
+#pragma unroll
+                        for (int i = 0; i < VEC<T>; i++)
+                            if (out >> i & 1) x[u * VEC<T> + i] = neg_inf();
+                    }
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < N; i++) top = fmaxf(top, x[i]);
+            st.add<N, false>(x, a, slack, top);
+        });
+        if (const int col = sl.single(tid); col >= 0) {
+            const float x = REST && (marked(bit_of(col)) & 1) ? neg_inf() : sl.at(col);
+            st.add<1, false>(&x, a, slack, x);
+        }
+        st = block_merge(st, a, red);
+        if (p.parts > 1) {
+            if (tid == 0) part = st;
+            cluster_barrier_arrive();
+            cluster_barrier_wait();
+            st = peer_stats(&part, 0);
+            for (int i = 1; i < p.parts; i++) st.merge(peer_stats(&part, i), a);
+            cluster_barrier_arrive();  // waited for at the end: shared memory of all CTAs stays until then
+        }
+        rest = norm_of(st);
+        if constexpr (REST) st.merge(Stats{sh.max_x, sh.sum_x, 0.f}, a);
+        all = norm_of(st);
+    } else {
+        __syncthreads();
+        all = p.norm[2 * r];
+        rest = p.norm[2 * r + 1];
+    }
+    const bool counts = sh.some && !all.empty();
+    const float q0 = REST && !rest.empty() ? sh.rest : 0.f, mass = sh.mass + q0;
+    const float log_p0 = fmaf(rest.m - all.m, p.inv_tau, rest.ln - all.ln);
+    if constexpr (STATS) {
+        if (rank == 0 && warp == 0) {
+            float loss = 0.f;
+            for (int i = lane; i < p.kept; i += 32) {
+                const float q = sh.q[i];
+                if (q != 0.f) loss += q * (sh.logq[i] - all.log_prob(sh.x[i], p.inv_tau));
+            }
+            loss = warp_sum(loss);
+            if (lane == 0) {
+                if (q0 != 0.f) loss += q0 * (logf(q0) - log_p0);
+                p.loss[r] = bad ? __int_as_float(0x7fffffff) : counts ? p.tau * p.tau * weight * loss : 0.f;
+                p.norm[2 * r] = all;
+                p.norm[2 * r + 1] = rest;
+            }
+        }
+    }
+    if constexpr (GRAD) {
+        const float total = p.total ? *p.total : p.divisor;
+        float scale = total == 0.f ? 0.f : p.tau * weight / total;
+        if constexpr (!STATS) scale *= p.upstream_one ? *p.upstream : p.upstream[r];
+        if (bad) scale = __int_as_float(0x7fffffff);
+        if (!counts && !bad) {
+            grad_pass<4>(sl, dx, [](float) { return 0.f; });
+        } else {
+            // away from the kept tokens every element is a multiple of one exponential
+            const Norm of = REST ? rest : all;
+            const float m = of.empty() ? 0.f : of.m, ln2 = of.ln * LOG2E;
+            const float others = scale * (REST ? (rest.empty() ? 0.f : mass * exp2_fast(log_p0 * LOG2E) - q0) : 1.f);
+            grad_pass<4>(sl, dx, [&](float x) { return others * exp2_fast(fmaf(x - m, a, -ln2)); });
+            __syncthreads();  // the entries below replace what other threads wrote
+            if (tid < p.kept && sh.first[tid] && sl.holds(id)) {
+                float q = sh.q[tid];
+                if (sh.twice)
+                    for (int i = tid + 1; i < p.kept; i++) q += sh.id[i] == id ? sh.q[i] : 0.f;
+                dx[id] = DT<T>::from_f32(scale * ((REST ? mass : 1.f) * exp2_fast(all.log_prob(sh.x[tid], p.inv_tau) * LOG2E) - q));
+            }
+        }
+    }
+    if (STATS && p.parts > 1) cluster_barrier_wait();
+}
+
+// out = sum of v (divided by *by, or by 1; 0 where that is 0), added in 64 bits in a fixed order
+__global__ void __launch_bounds__(1024) ordered_sum_kernel(const float *v, int64_t n, const float *by, float divisor, float *out) {
+    __shared__ double part[32];
+    double s = 0.0;
+    for (int64_t i = threadIdx.x; i < n; i += 1024) s += v[i];
+#pragma unroll
+    for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(FULL, s, o);
+    if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = s;
+    __syncthreads();
+    if (threadIdx.x < 32) {
+        s = part[threadIdx.x];
+#pragma unroll
+        for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(FULL, s, o);
+        const float total = by ? *by : divisor;
+        if (threadIdx.x == 0) *out = total == 0.f ? 0.f : (float)(s / (double)total);
+    }
+}
+
+template <typename T, bool REST, bool STATS, bool GRAD> static int launch_distill(DistillParams &p, int dtype, cudaStream_t st) {
+    int sms, rc;
+    if ((rc = device_sms(&sms))) return rc;
+    p.parts = row_parts(p.x.rows, p.x.vocab, dtype, sms, STATS && GRAD);
+    const size_t smem = (REST ? ((size_t)p.x.vocab + BIT0 + 31) / 32 : FILTER_BITS / 32) * 4;
+    NMG_ALLOW_SMEM(smem, distill_kernel<T, REST, STATS, GRAD>);
+    return launch_rows(distill_kernel<T, REST, STATS, GRAD>, p.x.rows, p.parts, smem, st, p);
+}
+template <bool STATS, bool GRAD> static int launch_distill_any(DistillParams &p, int dtype, bool rest, cudaStream_t st) {
+    NMG_DISPATCH_DTYPE(dtype, T, { return rest ? launch_distill<T, true, STATS, GRAD>(p, dtype, st) : launch_distill<T, false, STATS, GRAD>(p, dtype, st); });
+    return NMG_OK;
+}
+
+static int check_distill(DistillParams &p, int64_t vocab, int dtype, int remainder) {
+    int rc;
+    if (vocab < 1 || vocab > INT32_MAX - 64) NMG_FAIL(NMG_ERR_INVALID, "vocab must be 1 .. 2^31 - 65, got %lld", (long long)vocab);
+    p.x.vocab = (int)vocab;
+    if ((rc = check_logits(p.x, dtype, p.tau))) return rc;
+    if (p.kept < 1) NMG_FAIL(NMG_ERR_INVALID, "a row needs at least one kept token, got %d", p.kept);
+    if (p.kept > KEPT_MAX) NMG_FAIL(NMG_ERR_UNSUPPORTED, "at most %d kept tokens a row, got %d", KEPT_MAX, p.kept);
+    if (!p.ids || !p.log_probs || !p.norm) NMG_FAIL(NMG_ERR_INVALID, "NULL operand pointer");
+    if (reinterpret_cast<uintptr_t>(p.norm) % 8) NMG_FAIL(NMG_ERR_INVALID, "norm must be 8-byte aligned");
+    if (p.id_bytes != 4 && p.id_bytes != 8) NMG_FAIL(NMG_ERR_INVALID, "ids have 4 or 8 bytes, got %d", p.id_bytes);
+    if (p.teacher_dtype != NMG_F32 && p.teacher_dtype != NMG_F16 && p.teacher_dtype != NMG_BF16) NMG_FAIL(NMG_ERR_INVALID, "teacher dtype must be NMG_F32, NMG_F16 or NMG_BF16, got %d", p.teacher_dtype);
+    if (remainder && vocab > MAX_REST_VOCAB) NMG_FAIL(NMG_ERR_UNSUPPORTED, "with a remainder the vocabulary has at most %d tokens, got %lld", MAX_REST_VOCAB, (long long)vocab);
+    if (p.dx && reinterpret_cast<uintptr_t>(p.dx) % dtype_size(dtype)) NMG_FAIL(NMG_ERR_INVALID, "d_logits must be aligned to its elements");
+    return NMG_OK;
+}
+
+}  // namespace nmg
+
+using namespace nmg;
+
+extern "C" int nmg_distill(const void *logits, int64_t rows, int64_t inner_rows, int64_t ld, int64_t ld_outer, int64_t vocab, int dtype,
+                           const void *ids, int id_bytes, const void *log_probs, int teacher_dtype, int kept, int remainder,
+                           float temperature, const float *weight, int reduction, float *row_loss, float *norm, float *total,
+                           float *loss, void *d_logits, int64_t ld_d, int64_t ld_d_outer, void *stream) {
+    DistillParams p{{logits, rows, inner_rows, ld, ld_outer, 0}, ids, log_probs, id_bytes, teacher_dtype, kept, 1, temperature, 1.f / temperature, weight, nullptr, 1.f,
+                    row_loss, reinterpret_cast<Norm *>(norm), nullptr, 0, 0, d_logits, ld_d, ld_d_outer};
+    int rc;
+    if ((rc = check_distill(p, vocab, dtype, remainder))) return rc;
+    if (reduction != NMG_REDUCE_NONE && reduction != NMG_REDUCE_SUM && reduction != NMG_REDUCE_MEAN) NMG_FAIL(NMG_ERR_INVALID, "unknown reduction %d", reduction);
+    if (!row_loss || (reduction != NMG_REDUCE_NONE && !loss) || (reduction == NMG_REDUCE_MEAN && weight && !total)) NMG_FAIL(NMG_ERR_INVALID, "row_loss, loss and total must be non-NULL where they are written");
+    if (d_logits && reduction == NMG_REDUCE_NONE) NMG_FAIL(NMG_ERR_INVALID, "without a reduction the gradient depends on that of every row's loss: nmg_distill_backward");
+    cudaStream_t st = (cudaStream_t)stream;
+    if (reduction == NMG_REDUCE_MEAN) {
+        p.divisor = (float)rows;
+        if (weight) {
+            ordered_sum_kernel<<<1, 1024, 0, st>>>(weight, rows, nullptr, 1.f, total);
+            NMG_CUDA(cudaGetLastError());
+            p.total = total;
+        }
+    }
+    if ((rc = d_logits ? launch_distill_any<true, true>(p, dtype, remainder != 0, st) : launch_distill_any<true, false>(p, dtype, remainder != 0, st))) return rc;
+    if (reduction != NMG_REDUCE_NONE) {
+        ordered_sum_kernel<<<1, 1024, 0, st>>>(row_loss, rows, p.total, p.divisor, loss);
+        NMG_CUDA(cudaGetLastError());
+    }
+    return NMG_OK;
+}
+
+extern "C" int nmg_distill_backward(const void *logits, int64_t rows, int64_t inner_rows, int64_t ld, int64_t ld_outer, int64_t vocab, int dtype,
+                                    const void *ids, int id_bytes, const void *log_probs, int teacher_dtype, int kept, int remainder,
+                                    float temperature, const float *weight, int reduction, const float *norm, const float *total, const float *upstream, int skip_if_one, void *d_logits, int64_t ld_d,
+                                    int64_t ld_d_outer, void *stream) {
+    DistillParams p{{logits, rows, inner_rows, ld, ld_outer, 0}, ids, log_probs, id_bytes, teacher_dtype, kept, 1, temperature, 1.f / temperature, weight, nullptr, 1.f,
+                    nullptr, reinterpret_cast<Norm *>(const_cast<float *>(norm)), upstream, reduction != NMG_REDUCE_NONE, skip_if_one, d_logits, ld_d, ld_d_outer};
+    int rc;
+    if ((rc = check_distill(p, vocab, dtype, remainder))) return rc;
+    if (reduction != NMG_REDUCE_NONE && reduction != NMG_REDUCE_SUM && reduction != NMG_REDUCE_MEAN) NMG_FAIL(NMG_ERR_INVALID, "unknown reduction %d", reduction);
+    if (!upstream || !d_logits || (reduction == NMG_REDUCE_MEAN && weight && !total)) NMG_FAIL(NMG_ERR_INVALID, "upstream, d_logits and, for a weighted mean, total must be non-NULL");
+    if (skip_if_one && reduction == NMG_REDUCE_NONE) NMG_FAIL(NMG_ERR_INVALID, "skip_if_one goes with the gradient of one loss");
+    if (reduction == NMG_REDUCE_MEAN) {
+        p.divisor = (float)rows;
+        p.total = weight ? total : nullptr;
+    }
+    return launch_distill_any<false, true>(p, dtype, remainder != 0, (cudaStream_t)stream);
+}

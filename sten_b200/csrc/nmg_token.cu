@@ -1,0 +1,386 @@
+// Log-probabilities of given tokens, entropy, log-sum-exp and the top alternatives of rows of logits, and their gradient.
+//
+//   token_kernel<T, TOP>      one pass over a row for the statistics (nmg_vocab.cuh) and, with TOP, the selection below
+//   token_grad_kernel<T, E>   dx_j = (p_j (A + B log p_j) + g_log_prob [j = target] + g_top,i [j = id_i]) / tau  with
+//                             A = g_lse - g_log_prob - sum g_top - g_entropy H,  B = -g_entropy  (E: there is an entropy gradient)
+//
+// The top k of a row, ordered by value and among equal values by column: every thread keeps the largest logit of its vectors
+// while it sums.  The k-th largest of those 512 maxima is no larger than the k-th largest logit, so only the threads whose maximum
+// reaches it can hold one of the top k: about k of 512.  Their vectors are read again, from L2, by all threads, and what reaches the
+// bound is a candidate (on random rows little more than k).  A candidate's place is the number of candidates before it.  The
+// buffer overflows where very many logits are equal or one thread's vectors hold most of the large ones: the bound is then
+// raised to the k-th largest of those buffered and the reading repeated, and where that is the bound itself, the logits above it
+// are collected and the places left are filled with equal ones in the order of their columns.  The CTAs of a cluster select
+// from their own slices and the first one merges their sorted lists.
+#include "nmg_vocab.cuh"
+
+namespace nmg {
+
+constexpr int TOP_MAX = 128, CANDIDATES = 2048;
+
+struct TokenParams {
+    Logits x;
+    const int64_t *targets;
+    int64_t ignore;
+    float tau, inv_tau;
+    int top, parts;
+    float *log_prob, *entropy, *lse, *top_log_prob;
+    int64_t *top_ids;
+    Norm *norm;
+};
+
+struct TokenGradParams {
+    Logits x;
+    const int64_t *targets;
+    int64_t ignore;
+    float inv_tau;
+    int top, parts;
+    const int64_t *top_ids;
+    const Norm *norm;
+    const float *entropy, *g_log_prob, *g_entropy, *g_lse, *g_top;
+    void *dx;
+    int64_t ld_dx, ld_dx_outer;
+};
+
+// Larger logits have larger keys, NaN the largest; -0 and 0 have the same.  No logit has key 0.
+__device__ __forceinline__ uint32_t order_key(float x) {
+    if (x != x) return 0xffffffffu;
+    const uint32_t u = __float_as_uint(x + 0.f);
+    return u >> 31 ? ~u : u | 0x80000000u;
+}
+__device__ __forceinline__ float key_value(uint32_t key) { return __uint_as_float(key == 0xffffffffu ? 0x7fffffffu : key >> 31 ? key & 0x7fffffffu : ~key); }
+// ... and of equal ones the smaller column comes first
+__device__ __forceinline__ uint64_t candidate(uint32_t key, int col) { return (uint64_t)key << 32 | (0xffffffffu - (uint32_t)col); }
+__device__ __forceinline__ int candidate_col(uint64_t c) { return (int)(0xffffffffu - (uint32_t)c); }
+
+struct TopShared {
+    uint64_t cand[CANDIDATES], top[TOP_MAX];
+    uint32_t keys[VT];
+    uint16_t hot[VT];
+    int scan[VT / 32];
+    uint32_t bound;
+    int n_cand, n_hot;
+};
+
+// exclusive prefix sum over the CTA and the total
+__device__ __forceinline__ int block_scan(int n, int *warps, int *total) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    int inc = n;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int other = __shfl_up_sync(FULL, inc, o);
+        if (lane >= o) inc += other;
+    }
+    __syncthreads();
+    if (lane == 31) warps[warp] = inc;
+    __syncthreads();
+    int before = 0, all = 0;
+#pragma unroll
+    for (int i = 0; i < VT / 32; i++) {
+        const int c = warps[i];
+        before += i < warp ? c : 0;
+        all += c;
+    }
+    *total = all;
+    return before + inc - n;
+}
+
+// sh.top[0 .. k): the slice's top k, sorted; 0 past its end.  `best`: the largest logit of this thread's vectors, NaN where one is.
+template <typename T> __device__ void select_top(const Slice<T> &sl, int k, float best, TopShared &sh) {
+    const int tid = (int)threadIdx.x, lane = tid & 31;
+    const uint32_t key = sl.v0 + tid < sl.v1 ? order_key(best) : 0u;
+    sh.keys[tid] = key;
+    if (tid == 0) sh.n_cand = sh.n_hot = 0;
+    __syncthreads();
+    if (tid < 32) {
+        uint32_t mine[VT / 32];
+#pragma unroll
+        for (int i = 0; i < VT / 32; i++) mine[i] = sh.keys[lane + 32 * i];
+        // the low bits are left zero, which only lowers the bound: bf16 keys have 16 bits, those of fp16 19
+        constexpr int LAST = DT<T>::id == NMG_BF16 ? 16 : DT<T>::id == NMG_F16 ? 13 : 12;
+        uint32_t bound = 0;
+        for (int bit = 31; bit >= LAST; bit--) {
+            const uint32_t next = bound | 1u << bit;
+            int c = 0;
+#pragma unroll
+            for (int i = 0; i < VT / 32; i++) c += mine[i] >= next;
+            if (__reduce_add_sync(FULL, c) >= k) bound = next;
+        }
+        if (lane == 0) sh.bound = bound;
+    }
+    __syncthreads();
+    uint32_t bound = sh.bound;
+    bool above = false;  // collect what is above the bound, not what is equal to it
+    const int rounds = (sl.v1 - sl.v0 + VT - 1) / VT, held = sl.count(), want = k < held ? k : held;
+    auto wanted = [&](uint32_t q) { return above ? q > bound : q >= bound; };
+    auto push = [&](uint32_t q, int col) {
+        const int at = atomicAdd(&sh.n_cand, 1);
+        if (at < CANDIDATES) sh.cand[at] = candidate(q, col);
+    };
+    for (;;) {
+        if (wanted(key) && key) sh.hot[atomicAdd(&sh.n_hot, 1)] = (uint16_t)tid;
+        __syncthreads();
+        const int n_hot = sh.n_hot, items = n_hot * rounds;
+        for (int i = tid; i < items; i += VT) {
+            const int v = sl.v0 + sh.hot[i % n_hot] + i / n_hot * VT;
+            if (v >= sl.v1) continue;
+            float x[VEC<T>];
+            unpack<T>(sl.vec(v), x);
+#pragma unroll
+            for (int u = 0; u < VEC<T>; u++)
+                if (const uint32_t q = order_key(x[u]); wanted(q)) push(q, sl.lead + v * VEC<T> + u);
+        }
+        if (const int col = sl.single(tid); col >= 0)
+            if (const uint32_t q = order_key(sl.at(col)); wanted(q)) push(q, col);
+        __syncthreads();
+        if (sh.n_cand <= CANDIDATES) break;
+        for (int i = tid; i < CANDIDATES; i += VT) {
+            const uint64_t c = sh.cand[i];
+            int place = 0;
+            for (int j = 0; j < CANDIDATES; j++) place += sh.cand[j] > c;
+            if (place == k - 1) sh.bound = (uint32_t)(c >> 32);
+        }
+        __syncthreads();
+        above = sh.bound == bound;  // a raised bound is above the last one, so this ends
+        bound = sh.bound;
+        if (tid == 0) sh.n_cand = sh.n_hot = 0;
+        __syncthreads();
+    }
+    int n = sh.n_cand;
+    if (above && n < want) {  // equal ones, in the order of their columns
+        for (int r = -1, found = 0; r <= rounds && n + found < want; r++) {
+            int col = -1, elems = 0;
+            uint32_t equal = 0;
+            if (r >= 0 && r < rounds) {
+                const int v = sl.v0 + r * VT + tid;
+                if (v < sl.v1) {
+                    float x[VEC<T>];
+                    unpack<T>(sl.vec(v), x);
+#pragma unroll
+                    for (int u = 0; u < VEC<T>; u++) equal |= order_key(x[u]) == bound ? 1u << u : 0u;
+                    col = sl.lead + v * VEC<T>;
+                    elems = VEC<T>;
+                }
+            } else if (const int c = r < 0 ? tid : sl.tail_at + tid; r < 0 ? tid < sl.lead_n : tid < sl.tail_n) {
+                equal = order_key(sl.at(c)) == bound;
+                col = c;
+                elems = 1;
+            }
+            int total;
+            int at = n + found + block_scan(__popc(equal), sh.scan, &total);
+            for (int u = 0; u < elems; u++)
+                if (equal >> u & 1) {
+                    if (at < want) sh.cand[at] = candidate(bound, col + u);
+                    at++;
+                }
+            found += total;
+        }
+        n = want;
+        __syncthreads();
+    }
+    for (int i = tid; i < n; i += VT) {
+        const uint64_t c = sh.cand[i];
+        int place = 0;
+        for (int j = 0; j < n; j++) place += sh.cand[j] > c;
+        if (place < want) sh.top[place] = c;
+    }
+    if (tid >= want && tid < k) sh.top[tid] = 0;
+    __syncthreads();
+}
+
+// sh.top of the cluster's CTAs into the first one's.  Between two barriers of the cluster; called by the first one only.
+__device__ __forceinline__ void merge_top(int k, int parts, TopShared &sh) {
+    const int tid = (int)threadIdx.x;
+    for (int e = tid; e < parts * k; e += VT) sh.cand[e] = peer_load_u64(peer_smem(&sh.top[e % k], e / k));
+    __syncthreads();
+    for (int e = tid; e < parts * k; e += VT) {
+        const uint64_t c = sh.cand[e];
+        int place = e % k;
+        for (int b = 0; b < parts; b++) {
+            if (b == e / k) continue;
+            int lo = 0, hi = k;  // how many of list b come first
+            while (lo < hi) {
+                const int mid = (lo + hi) >> 1;
+                if (sh.cand[b * k + mid] > c) lo = mid + 1;
+                else hi = mid;
+            }
+            place += lo;
+        }
+        if (c != 0 && place < k) sh.top[place] = c;
+    }
+    __syncthreads();
+}
+
+template <typename T, bool TOP> __global__ void __launch_bounds__(VT, VOCAB_CTAS) token_kernel(TokenParams p) {
+    __shared__ Stats red[VT / 32], part;
+    __shared__ __align__(16) unsigned char top_smem[TOP ? sizeof(TopShared) : 16];
+    TopShared &sh = *reinterpret_cast<TopShared *>(top_smem);
+    const int tid = (int)threadIdx.x, rank = p.parts > 1 ? cluster_rank() : 0;
+    const int64_t r = blockIdx.x / (unsigned)p.parts;
+    const Slice<T> sl(static_cast<const T *>(p.x.x) + row_offset(r, p.x.inner, p.x.ld, p.x.ld_outer), p.x.vocab, rank, p.parts);
+    const float a = LOG2E * p.inv_tau, slack = 8.f * p.tau;
+    int64_t target = p.ignore;
+    float target_x = 0.f;
+    if (rank == 0 && tid == 0 && p.targets) {
+        target = p.targets[r];
+        if (target >= 0 && target < p.x.vocab) target_x = sl.at((int)target);
+    }
+    Stats st = Stats::none();
+    float best = neg_inf();
+    for_vectors<4>(sl, [&](const uint4 *q, int, int) {
+        float x[4 * VEC<T>], top = neg_inf();
+#pragma unroll
+        for (int u = 0; u < 4; u++) unpack<T>(q[u], x + u * VEC<T>);
+#pragma unroll
+        for (int i = 0; i < 4 * VEC<T>; i++) top = fmaxf(top, x[i]);
+        if constexpr (TOP) best = fmaxf(best, top);
+        st.add<4 * VEC<T>, true>(x, a, slack, top);
+    });
+    if constexpr (TOP) {
+        if (st.s != st.s)  // NaN, or +inf: only the first has to be found
+            for (int v = sl.v0 + tid; v < sl.v1; v += VT) {
+                float x[VEC<T>];
+                unpack<T>(sl.vec(v), x);
+#pragma unroll
+                for (int u = 0; u < VEC<T>; u++) best = x[u] != x[u] ? x[u] : best;
+            }
+    }
+    if (const int col = sl.single(tid); col >= 0) {
+        const float x = sl.at(col);
+        st.add<1, true>(&x, a, slack, x);
+    }
+    st = block_merge(st, a, red);
+    if constexpr (TOP) select_top<T>(sl, p.top, best, sh);
+    if (p.parts > 1) {
+        if (tid == 0) part = st;
+        cluster_barrier_arrive();
+        cluster_barrier_wait();
+        if (rank == 0) {
+            st = peer_stats(&part, 0);
+            for (int i = 1; i < p.parts; i++) st.merge(peer_stats(&part, i), a);
+            if constexpr (TOP) merge_top(p.top, p.parts, sh);
+        }
+        cluster_barrier_arrive();  // shared memory of all CTAs stays until the first one has read it
+        cluster_barrier_wait();
+        if (rank != 0) return;
+    }
+    const Norm norm = norm_of(st);
+    if (tid == 0) {
+        if (p.log_prob) {
+            const bool ours = target >= 0 && target < p.x.vocab;
+            p.log_prob[r] = target == p.ignore ? 0.f : ours ? norm.log_prob(target_x, p.inv_tau) : __int_as_float(0x7fffffff);
+        }
+        p.entropy[r] = st.entropy(p.inv_tau);
+        p.lse[r] = norm.lse(p.inv_tau);
+        if (p.norm) p.norm[r] = norm;
+    }
+    if constexpr (TOP) {
+        if (tid < p.top) {
+            const uint64_t c = sh.top[tid];
+            p.top_ids[r * p.top + tid] = candidate_col(c);
+            p.top_log_prob[r * p.top + tid] = norm.log_prob(key_value((uint32_t)(c >> 32)), p.inv_tau);
+        }
+    }
+}
+
+template <typename T, bool E> __global__ void __launch_bounds__(VT, VOCAB_CTAS) token_grad_kernel(TokenGradParams p) {
+    const int tid = (int)threadIdx.x, lane = tid & 31, rank = (int)(blockIdx.x % (unsigned)p.parts);
+    const int64_t r = blockIdx.x / (unsigned)p.parts;
+    const Slice<T> sl(static_cast<const T *>(p.x.x) + row_offset(r, p.x.inner, p.x.ld, p.x.ld_outer), p.x.vocab, rank, p.parts);
+    T *dx = static_cast<T *>(p.dx) + row_offset(r, p.x.inner, p.ld_dx, p.ld_dx_outer);
+    const int64_t target = p.targets && p.g_log_prob ? p.targets[r] : p.ignore;
+    const bool in_row = target >= 0 && target < p.x.vocab && target != p.ignore;
+    const float g_lp = in_row ? p.g_log_prob[r] : 0.f, g_h = E ? p.g_entropy[r] : 0.f;
+    const Norm norm = p.norm[r];
+    float g_top = 0.f;
+    if (p.g_top) {
+        for (int i = lane; i < p.top; i += 32) g_top += p.g_top[r * p.top + i];
+#pragma unroll
+        for (int o = 16; o; o >>= 1) g_top += __shfl_xor_sync(FULL, g_top, o);
+    }
+    float A = (p.g_lse ? p.g_lse[r] : 0.f) - g_lp - g_top - (E ? g_h * p.entropy[r] : 0.f), B = -g_h;
+    if (!in_row && target != p.ignore) A = __int_as_float(0x7fffffff);  // no such token
+    const bool empty = norm.empty();
+    const float m = empty ? 0.f : norm.m, ln = norm.ln, a = LOG2E * p.inv_tau, ln2 = ln * LOG2E;  // nothing but -inf: p = 0 below
+    A *= p.inv_tau;
+    B *= p.inv_tau;
+    auto grad = [&](float x) {
+        const float d = x - m, e = exp2_fast(fmaf(d, a, -ln2));
+        return E ? e * (A + B * fmaf(fmaxf(d, -1e30f), p.inv_tau, -ln)) : e * A;  // 0 * -inf is not a part of it
+    };
+    grad_pass<4>(sl, dx, grad);
+    __syncthreads();  // the entries below replace what other threads wrote
+    if (empty) return;
+    if (tid < p.top && p.g_top) {
+        const int64_t id = p.top_ids[r * p.top + tid];
+        if (id >= 0 && id < p.x.vocab && !(in_row && id == target) && sl.holds((int)id))
+            dx[id] = DT<T>::from_f32(grad(sl.at((int)id)) + p.g_top[r * p.top + tid] * p.inv_tau);
+    }
+    if (tid == TOP_MAX && in_row && sl.holds((int)target)) {
+        float g = g_lp;
+        if (p.g_top)
+            for (int i = 0; i < p.top; i++)
+                if (p.top_ids[r * p.top + i] == target) g += p.g_top[r * p.top + i];
+        dx[target] = DT<T>::from_f32(grad(sl.at((int)target)) + g * p.inv_tau);
+    }
+}
+
+int check_logits(const Logits &x, int dtype, float temperature) {
+    if (dtype != NMG_F32 && dtype != NMG_F16 && dtype != NMG_BF16) NMG_FAIL(NMG_ERR_INVALID, "dtype must be NMG_F32, NMG_F16 or NMG_BF16, got %d", dtype);
+    if (!x.x) NMG_FAIL(NMG_ERR_INVALID, "logits must be non-NULL");
+    if (x.rows < 1 || x.inner < 1 || x.vocab < 1) NMG_FAIL(NMG_ERR_INVALID, "rows, inner_rows and vocab must be positive");
+    if (reinterpret_cast<uintptr_t>(x.x) % dtype_size(dtype)) NMG_FAIL(NMG_ERR_INVALID, "logits must be aligned to their elements");
+    if (!(temperature > 0.f) || temperature > 1e30f || temperature < 1e-30f) NMG_FAIL(NMG_ERR_INVALID, "temperature must be positive and finite, got %g", (double)temperature);
+    return NMG_OK;
+}
+
+static int check_top(int top, int vocab) {
+    if (top < 0 || top > TOP_MAX) NMG_FAIL(top < 0 ? NMG_ERR_INVALID : NMG_ERR_UNSUPPORTED, "top must be 0 .. %d, got %d", TOP_MAX, top);
+    if (top > vocab) NMG_FAIL(NMG_ERR_INVALID, "top = %d alternatives of %d tokens", top, vocab);
+    return NMG_OK;
+}
+static int check_vocab(int64_t vocab, int *out) {
+    if (vocab < 1 || vocab > INT32_MAX - 64) NMG_FAIL(NMG_ERR_INVALID, "vocab must be 1 .. 2^31 - 65, got %lld", (long long)vocab);
+    *out = (int)vocab;
+    return NMG_OK;
+}
+
+}  // namespace nmg
+
+using namespace nmg;
+
+extern "C" int nmg_token_log_probs(const void *logits, int64_t rows, int64_t inner_rows, int64_t ld, int64_t ld_outer, int64_t vocab, int dtype,
+                                   const int64_t *targets, int64_t ignore_index, float temperature, int top, float *log_prob, float *entropy,
+                                   float *lse, float *top_log_prob, int64_t *top_ids, float *norm, void *stream) {
+    TokenParams p{{logits, rows, inner_rows, ld, ld_outer, 0}, targets, ignore_index, temperature, 1.f / temperature, top, 1, log_prob, entropy, lse, top_log_prob, top_ids, reinterpret_cast<Norm *>(norm)};
+    int rc, sms;
+    if ((rc = check_vocab(vocab, &p.x.vocab)) || (rc = check_logits(p.x, dtype, temperature)) || (rc = check_top(top, p.x.vocab))) return rc;
+    if (!entropy || !lse || !log_prob != !targets) NMG_FAIL(NMG_ERR_INVALID, "entropy and lse must be non-NULL, and log_prob where there are targets");
+    if (reinterpret_cast<uintptr_t>(norm) % 8) NMG_FAIL(NMG_ERR_INVALID, "norm must be 8-byte aligned");
+    if (top && (!top_log_prob || !top_ids)) NMG_FAIL(NMG_ERR_INVALID, "top_log_prob and top_ids must be non-NULL when top > 0");
+    if ((rc = device_sms(&sms))) return rc;
+    p.parts = row_parts(rows, p.x.vocab, dtype, sms, false);
+    cudaStream_t st = (cudaStream_t)stream;
+    NMG_DISPATCH_DTYPE(dtype, T, { return top ? launch_rows(token_kernel<T, true>, rows, p.parts, 0, st, p) : launch_rows(token_kernel<T, false>, rows, p.parts, 0, st, p); });
+    return NMG_OK;
+}
+
+extern "C" int nmg_token_log_probs_backward(const void *logits, int64_t rows, int64_t inner_rows, int64_t ld, int64_t ld_outer, int64_t vocab, int dtype,
+                                            const int64_t *targets, int64_t ignore_index, float temperature, int top, const int64_t *top_ids,
+                                            const float *norm, const float *entropy, const float *g_log_prob, const float *g_entropy,
+                                            const float *g_lse, const float *g_top, void *d_logits, int64_t ld_d, int64_t ld_d_outer, void *stream) {
+    TokenGradParams p{{logits, rows, inner_rows, ld, ld_outer, 0}, targets, ignore_index, 1.f / temperature, top, 1, top_ids, reinterpret_cast<const Norm *>(norm), entropy, g_log_prob, g_entropy, g_lse, g_top, d_logits, ld_d, ld_d_outer};
+    int rc, sms;
+    if ((rc = check_vocab(vocab, &p.x.vocab)) || (rc = check_logits(p.x, dtype, temperature)) || (rc = check_top(top, p.x.vocab))) return rc;
+    if (!norm || !d_logits || (g_entropy && !entropy) || (g_log_prob && !targets) || (g_top && (!top_ids || !top)))
+        NMG_FAIL(NMG_ERR_INVALID, "a gradient needs what its output was computed from: norm and d_logits always, entropy, targets, top_ids");
+    if (reinterpret_cast<uintptr_t>(norm) % 8) NMG_FAIL(NMG_ERR_INVALID, "norm must be 8-byte aligned");
+    if (reinterpret_cast<uintptr_t>(d_logits) % dtype_size(dtype)) NMG_FAIL(NMG_ERR_INVALID, "d_logits must be aligned to its elements");
+    if ((rc = device_sms(&sms))) return rc;
+    p.parts = row_parts(rows, p.x.vocab, dtype, sms, false);
+    cudaStream_t st = (cudaStream_t)stream;
+    NMG_DISPATCH_DTYPE(dtype, T, {
+        return g_entropy ? launch_rows(token_grad_kernel<T, true>, rows, p.parts, 0, st, p) : launch_rows(token_grad_kernel<T, false>, rows, p.parts, 0, st, p);
+    });
+    return NMG_OK;
+}

@@ -1,0 +1,270 @@
+// Rows of logits over a vocabulary: how a row is cut over threads and CTAs, and the statistics of a softmax that one pass over it
+// collects.  Shared by the token log-probabilities and the distillation loss.
+//
+// A row of any length at any element-aligned address is `lead` elements up to the first 16-byte boundary, whole 16-byte vectors,
+// and a tail.  The CTAs of a cluster share a row: each takes a contiguous range of the vectors, the first the lead and the last
+// the tail (fewer than 16 elements together, one thread each).
+//
+// Statistics of a set of logits x at temperature tau, a = log2(e) / tau:  m >= max x - 8 tau,  s = sum 2^((x - m) a),
+// w = sum 2^((x - m) a) (x - m), all in 32 bits.  m follows the running maximum only once that is 8 tau above it: s then holds terms up to
+// e^8, which costs no precision, and the rescaling leaves the inner loop.  From them
+//   log-sum-exp of x / tau = m / tau + ln s,    entropy = ln s - (w / tau) / s.
+// A set that holds nothing but -inf has m = -inf and s = 0; NaN and +inf make s NaN.
+#pragma once
+
+#include "nmg_common.cuh"
+
+namespace nmg {
+
+constexpr int VT = 512;       // threads of a CTA
+constexpr int VOCAB_CTAS = 2; // CTAs of the row kernels that an SM holds at once
+
+struct Logits {
+    const void *x;
+    int64_t rows, inner, ld, ld_outer;  // row r begins at element (r / inner) * ld_outer + (r % inner) * ld
+    int vocab;
+};
+__host__ __device__ __forceinline__ int64_t row_offset(int64_t r, int64_t inner, int64_t ld, int64_t ld_outer) {
+    return r / inner * ld_outer + r % inner * ld;
+}
+
+#ifdef __CUDACC__
+constexpr unsigned FULL = 0xffffffffu;
+__device__ __forceinline__ float neg_inf() { return __int_as_float(0xff800000); }
+__device__ __forceinline__ float exp2_fast(float x) {  // results below 2^-126 are zero
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+constexpr float LOG2E = 1.4426950408889634f;
+
+template <typename T> constexpr int VEC = 16 / (int)sizeof(T);
+template <typename T> __device__ __forceinline__ uint32_t neg_inf_word();
+template <> __device__ __forceinline__ uint32_t neg_inf_word<float>() { return 0xff800000u; }
+template <> __device__ __forceinline__ uint32_t neg_inf_word<__half>() { return 0xfc00fc00u; }
+template <> __device__ __forceinline__ uint32_t neg_inf_word<__nv_bfloat16>() { return 0xff80ff80u; }
+
+template <typename T> __device__ __forceinline__ void unpack(const uint4 &v, float *x) {
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        if constexpr (sizeof(T) == 4) {
+            x[i] = __uint_as_float(w[i]);
+        } else if constexpr (DT<T>::id == NMG_BF16) {
+            x[2 * i] = __uint_as_float(w[i] << 16);
+            x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+        } else {
+            const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&w[i]));
+            x[2 * i] = f.x;
+            x[2 * i + 1] = f.y;
+        }
+    }
+}
+template <typename T> __device__ __forceinline__ uint4 pack(const float *x) {
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        if constexpr (sizeof(T) == 4) {
+            w[i] = __float_as_uint(x[i]);
+        } else if constexpr (DT<T>::id == NMG_BF16) {
+            const __nv_bfloat162 h = __floats2bfloat162_rn(x[2 * i], x[2 * i + 1]);
+            w[i] = *reinterpret_cast<const uint32_t *>(&h);
+        } else {
+            const __half2 h = __floats2half2_rn(x[2 * i], x[2 * i + 1]);
+            w[i] = *reinterpret_cast<const uint32_t *>(&h);
+        }
+    }
+    return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// This CTA's share of a row.
+template <typename T> struct Slice {
+    const T *row;
+    int lead, v0, v1;              // vector v holds columns lead + v * VEC ...
+    int lead_n, tail_at, tail_n;   // elements outside the vectors that are this CTA's
+    __device__ __forceinline__ Slice(const T *row_, int vocab, int part, int parts) : row(row_) {
+        const int to16 = (int)((16 - (reinterpret_cast<uintptr_t>(row_) & 15)) & 15) / (int)sizeof(T);
+        lead = to16 < vocab ? to16 : vocab;
+        const int nvec = (vocab - lead) / VEC<T>;
+        v0 = (int)((int64_t)nvec * part / parts);
+        v1 = (int)((int64_t)nvec * (part + 1) / parts);
+        lead_n = part == 0 ? lead : 0;
+        tail_at = lead + nvec * VEC<T>;
+        tail_n = part == parts - 1 ? vocab - tail_at : 0;
+    }
+    __device__ __forceinline__ int single(int t) const {  // column of the t-th element outside the vectors, or -1
+        return t < lead_n ? t : t - lead_n < tail_n ? tail_at + t - lead_n : -1;
+    }
+    __device__ __forceinline__ int count() const { return lead_n + tail_n + (v1 - v0) * VEC<T>; }
+    __device__ __forceinline__ bool holds(int col) const {
+        if (col < lead) return lead_n > 0;
+        if (col >= tail_at) return tail_n > 0;
+        const int v = (col - lead) / VEC<T>;
+        return v >= v0 && v < v1;
+    }
+    __device__ __forceinline__ uint4 vec(int v) const { return *reinterpret_cast<const uint4 *>(row + lead + (int64_t)v * VEC<T>); }
+    __device__ __forceinline__ float at(int col) const { return DT<T>::to_f32(row[col]); }
+};
+
+struct Stats {
+    float m, s, w;
+    static __device__ __forceinline__ Stats none() { return Stats{neg_inf(), 0.f, 0.f}; }
+
+    // N more logits; W: the entropy is wanted
+    template <int N, bool W> __device__ __forceinline__ void add(const float *x, float a, float slack, float top) {
+        if (top > m + slack) {
+            const float d = m - top, f = exp2_fast(d * a);
+            if constexpr (W) w = f == 0.f ? 0.f : f * (w + d * s);  // d * s may be -inf
+            s *= f;
+            m = top;
+        }
+        const float ref = m == neg_inf() ? 0.f : m;
+        float ps[2] = {0.f, 0.f}, pw[2] = {0.f, 0.f};
+#pragma unroll
+        for (int i = 0; i < N; i++) {
+            const float d = x[i] - ref, e = exp2_fast(d * a);
+            ps[i & 1] += e;
+            if constexpr (W) pw[i & 1] += e * fmaxf(d, -1e30f);  // 0 * -inf is not a part of the sum
+        }
+        s += ps[0] + ps[1];
+        if constexpr (W) w += pw[0] + pw[1];
+    }
+    __device__ __forceinline__ void merge(const Stats &o, float a) {
+        const float top = fmaxf(m, o.m), ref = top == neg_inf() ? 0.f : top;
+        const float d0 = m - ref, d1 = o.m - ref, f0 = exp2_fast(d0 * a), f1 = exp2_fast(d1 * a);
+        w = (f0 == 0.f ? 0.f : f0 * (w + d0 * s)) + (f1 == 0.f ? 0.f : f1 * (o.w + d1 * o.s));
+        s = s * f0 + o.s * f1;
+        m = top;
+    }
+    __device__ __forceinline__ bool empty() const { return m == neg_inf() && s == 0.f; }
+    __device__ __forceinline__ float entropy(float inv_tau) const { return empty() ? 0.f : logf(s) - w * inv_tau / s; }
+};
+
+// Normaliser of a set: log-sum-exp = m / tau + ln.  The two stay apart, also between the forward and the backward pass: where all that
+// is left of a row are masks of the type's lowest value, their sum has no room for ln.
+struct Norm {
+    float m, ln;  // nothing but -inf: m = -inf, ln = 0
+    __device__ __forceinline__ bool empty() const { return m == neg_inf() && ln == 0.f; }
+    __device__ __forceinline__ float lse(float inv_tau) const { return fmaf(m, inv_tau, ln); }
+    __device__ __forceinline__ float log_prob(float x, float inv_tau) const { return empty() ? neg_inf() : fmaf(x - m, inv_tau, -ln); }
+};
+__device__ __forceinline__ Norm norm_of(const Stats &st) { return st.empty() ? Norm{neg_inf(), 0.f} : Norm{st.m, logf(st.s)}; }
+
+// Everybody's statistics merged in one order; every thread of the warp gets the same.
+__device__ __forceinline__ Stats warp_merge(Stats st, float a, int lanes = 32) {
+    for (int o = lanes >> 1; o; o >>= 1) {
+        const Stats other{__shfl_xor_sync(FULL, st.m, o), __shfl_xor_sync(FULL, st.s, o), __shfl_xor_sync(FULL, st.w, o)};
+        st.merge(other, a);
+    }
+    return Stats{__shfl_sync(FULL, st.m, 0), __shfl_sync(FULL, st.s, 0), __shfl_sync(FULL, st.w, 0)};
+}
+// The CTA's; `red` holds one entry per warp and is free again after the next __syncthreads.
+__device__ __forceinline__ Stats block_merge(Stats st, float a, Stats *red) {
+    static_assert(VT == 512, "sixteen warps meet in half a warp");
+    st = warp_merge(st, a);
+    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = st;
+    __syncthreads();
+    return warp_merge(red[threadIdx.x & 15], a, 16);
+}
+
+// ---- clusters: the CTAs that share a row
+__device__ __forceinline__ int cluster_rank() {
+    uint32_t r;
+    asm volatile("mov.u32 %0, %cluster_ctarank;" : "=r"(r));
+    return (int)r;
+}
+__device__ __forceinline__ void cluster_barrier_arrive() { asm volatile("barrier.cluster.arrive;" ::: "memory"); }
+__device__ __forceinline__ void cluster_barrier_wait() { asm volatile("barrier.cluster.wait;" ::: "memory"); }
+// shared memory of CTA `rank` of the cluster, by this CTA's address of the same variable
+__device__ __forceinline__ uint32_t peer_smem(const void *p, int rank) {
+    uint32_t a;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_u32(p)), "r"(rank));
+    return a;
+}
+__device__ __forceinline__ float peer_load_f32(uint32_t a) {
+    float v;
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(a) : "memory");
+    return v;
+}
+__device__ __forceinline__ uint64_t peer_load_u64(uint32_t a) {
+    uint64_t v;
+    asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(v) : "r"(a) : "memory");
+    return v;
+}
+__device__ __forceinline__ Stats peer_stats(const Stats *mine, int rank) {
+    const uint32_t a = peer_smem(mine, rank);
+    return Stats{peer_load_f32(a), peer_load_f32(a + 4), peer_load_f32(a + 8)};
+}
+
+// One pass over the vectors of a slice, U of them in flight a thread: f(vectors, first vector's number, how many hold anything).
+template <int U, typename T, typename F> __device__ __forceinline__ void for_vectors(const Slice<T> &sl, F f) {
+    for (int v = sl.v0 + (int)threadIdx.x; v < sl.v1; v += U * VT) {
+        uint4 q[U];
+        const int left = (sl.v1 - v + VT - 1) / VT;
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            const uint32_t none = neg_inf_word<T>();
+            q[u] = u < left ? sl.vec(v + u * VT) : make_uint4(none, none, none, none);
+        }
+        f(q, v, left < U ? left : U);
+    }
+}
+
+// out[column] = f(logit) over the slice.  `out` is where the row's gradient begins; vectors are stored whole where its 16-byte
+// boundaries are those of the logits.
+template <int U, typename T, typename F> __device__ __forceinline__ void grad_pass(const Slice<T> &sl, T *out, F f) {
+    const bool whole = (reinterpret_cast<uintptr_t>(out + sl.lead) & 15) == 0;
+    for_vectors<U>(sl, [&](const uint4 *q, int v, int n) {
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            if (u >= n) break;
+            float x[VEC<T>];
+            unpack<T>(q[u], x);
+#pragma unroll
+            for (int i = 0; i < VEC<T>; i++) x[i] = f(x[i]);
+            T *dst = out + sl.lead + (int64_t)(v + u * VT) * VEC<T>;
+            if (whole) {
+                __stcs(reinterpret_cast<uint4 *>(dst), pack<T>(x));
+            } else {
+#pragma unroll
+                for (int i = 0; i < VEC<T>; i++) dst[i] = DT<T>::from_f32(x[i]);
+            }
+        }
+    });
+    if (const int col = sl.single((int)threadIdx.x); col >= 0) out[col] = DT<T>::from_f32(f(sl.at(col)));
+}
+#endif
+
+// CTAs that share a row: enough to fill the chip where there are few rows, as long as every thread has a vector to read; and, where rows
+// are visited twice, enough that the second visit finds the rows in flight in L2 (126 MB, of which they may take half).
+inline int row_parts(int64_t rows, int vocab, int dtype, int sms, bool twice) {
+    const int64_t bytes = (int64_t)vocab * (int64_t)dtype_size(dtype), slots = (int64_t)VOCAB_CTAS * sms;
+    int parts = 1;
+    while (parts < 8 && rows * parts * 2 <= slots && bytes >= (int64_t)parts * 2 * VT * 16) parts *= 2;
+    while (twice && parts < 8 && (rows < slots / parts ? rows : slots / parts) * bytes > (int64_t)64 << 20) parts *= 2;
+    return parts;
+}
+
+// rows x parts CTAs, the parts of a row in one cluster
+template <typename... P, typename... A>
+inline int launch_rows(void (*kernel)(P...), int64_t rows, int parts, size_t smem, cudaStream_t st, A... args) {
+    if (rows > INT32_MAX / parts) NMG_FAIL(NMG_ERR_UNSUPPORTED, "%lld rows are more than one launch takes", (long long)rows);
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(rows * parts));
+    cfg.blockDim = dim3(VT);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = (unsigned)parts;
+    attr.val.clusterDim.y = 1;
+    attr.val.clusterDim.z = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    NMG_CUDA(cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...));
+    return NMG_OK;
+}
+
+int check_logits(const Logits &x, int dtype, float temperature);
+
+}  // namespace nmg
