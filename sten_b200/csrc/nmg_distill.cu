@@ -64,6 +64,17 @@ __device__ __forceinline__ float warp_sum(float v) {
     return v;
 }
 
+// the elements of a vector whose bits are set become -inf
+template <typename T> __device__ __forceinline__ uint4 leave_out(uint4 q, uint32_t out) {
+    uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const uint32_t mask = sizeof(T) == 4 ? (out >> i & 1 ? FULL : 0u) : (out >> 2 * i & 1 ? 0xffffu : 0u) | (out >> (2 * i + 1) & 1 ? 0xffff0000u : 0u);
+        w[i] = (w[i] & ~mask) | (neg_inf_word<T>() & mask);
+    }
+    return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
 template <typename T, bool REST, bool STATS, bool GRAD> __global__ void __launch_bounds__(VT, VOCAB_CTAS) distill_kernel(DistillParams p) {
     extern __shared__ __align__(16) uint32_t bits[];
     __shared__ Stats red[VT / 32], part;
@@ -153,30 +164,17 @@ template <typename T, bool REST, bool STATS, bool GRAD> __global__ void __launch
     Norm all, rest;
     if constexpr (STATS) {
         Stats st = Stats::none();
-        constexpr int U = 4, N = U * VEC<T>;
+        constexpr int U = 4;
         auto marked = [&](int bit) { return bits[bit >> 5] >> (bit & 31); };
-        for_vectors<U>(sl, [&](const uint4 *q, int v, int n) {
-            float x[N], top = neg_inf();
+        for_vectors<U>(sl, [&](uint4 *q, int v, int n) {
+            if constexpr (REST) {
 #pragma unroll
-            for (int u = 0; u < U; u++) {
-                unpack<T>(q[u], x + u * VEC<T>);
-                if constexpr (REST) {
-                    const uint32_t out = u < n ? marked(BIT0 + (v + u * VT) * VEC<T>) & ((1u << VEC<T>) - 1) : 0u;
-                    if (out) {
-#pragma unroll
-                        for (int i = 0; i < VEC<T>; i++)
-                            if (out >> i & 1) x[u * VEC<T> + i] = neg_inf();
-                    }
-                }
+                for (int u = 0; u < U; u++)
+                    if (const uint32_t out = u < n ? marked(BIT0 + (v + u * VT) * VEC<T>) & ((1u << VEC<T>) - 1) : 0u) q[u] = leave_out<T>(q[u], out);
             }
-#pragma unroll
-            for (int i = 0; i < N; i++) top = fmaxf(top, x[i]);
-            st.add<N, false>(x, a, slack, top);
+            st.add<T, U, false>(q, a, slack, group_pick<T, true, U>(q));
         });
-        if (const int col = sl.single(tid); col >= 0) {
-            const float x = REST && (marked(bit_of(col)) & 1) ? neg_inf() : sl.at(col);
-            st.add<1, false>(&x, a, slack, x);
-        }
+        if (const int col = sl.single(tid); col >= 0) st.add_one<false>(REST && (marked(bit_of(col)) & 1) ? neg_inf() : sl.at(col), a, slack);
         st = block_merge(st, a, red);
         if (p.parts > 1) {
             if (tid == 0) part = st;

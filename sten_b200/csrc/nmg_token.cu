@@ -228,13 +228,9 @@ template <typename T, bool TOP> __global__ void __launch_bounds__(VT, VOCAB_CTAS
     Stats st = Stats::none();
     float best = neg_inf();
     for_vectors<4>(sl, [&](const uint4 *q, int, int) {
-        float x[4 * VEC<T>], top = neg_inf();
-#pragma unroll
-        for (int u = 0; u < 4; u++) unpack<T>(q[u], x + u * VEC<T>);
-#pragma unroll
-        for (int i = 0; i < 4 * VEC<T>; i++) top = fmaxf(top, x[i]);
+        const float top = group_pick<T, true, 4>(q);
         if constexpr (TOP) best = fmaxf(best, top);
-        st.add<4 * VEC<T>, true>(x, a, slack, top);
+        st.add<T, 4, true>(q, a, slack, top);
     });
     if constexpr (TOP) {
         if (st.s != st.s)  // NaN, or +inf: only the first has to be found
@@ -245,10 +241,7 @@ template <typename T, bool TOP> __global__ void __launch_bounds__(VT, VOCAB_CTAS
                 for (int u = 0; u < VEC<T>; u++) best = x[u] != x[u] ? x[u] : best;
             }
     }
-    if (const int col = sl.single(tid); col >= 0) {
-        const float x = sl.at(col);
-        st.add<1, true>(&x, a, slack, x);
-    }
+    if (const int col = sl.single(tid); col >= 0) st.add_one<true>(sl.at(col), a, slack);
     st = block_merge(st, a, red);
     if constexpr (TOP) select_top<T>(sl, p.top, best, sh);
     if (p.parts > 1) {

@@ -12,6 +12,8 @@
 // A set that holds nothing but -inf has m = -inf and s = 0; NaN and +inf make s NaN.
 #pragma once
 
+#include <type_traits>
+
 #include "nmg_common.cuh"
 
 namespace nmg {
@@ -106,35 +108,102 @@ template <typename T> struct Slice {
     __device__ __forceinline__ float at(int col) const { return DT<T>::to_f32(row[col]); }
 };
 
+// Largest and smallest of a group of vectors, NaN left aside; 16-bit logits are compared two at a time as they are.
+template <typename T, bool MAX> __device__ __forceinline__ uint32_t pick2(uint32_t a, uint32_t b) {
+    if constexpr (sizeof(T) == 4) {
+        const float x = __uint_as_float(a), y = __uint_as_float(b);
+        return __float_as_uint(MAX ? fmaxf(x, y) : fminf(x, y));
+    } else {
+        using T2 = std::conditional_t<DT<T>::id == NMG_BF16, __nv_bfloat162, __half2>;
+        const T2 x = *reinterpret_cast<const T2 *>(&a), y = *reinterpret_cast<const T2 *>(&b), r = MAX ? __hmax2(x, y) : __hmin2(x, y);
+        return *reinterpret_cast<const uint32_t *>(&r);
+    }
+}
+template <typename T, bool MAX, int U> __device__ __forceinline__ float group_pick(const uint4 *q) {
+    uint32_t r = pick2<T, MAX>(pick2<T, MAX>(q[0].x, q[0].y), pick2<T, MAX>(q[0].z, q[0].w));
+#pragma unroll
+    for (int u = 1; u < U; u++) r = pick2<T, MAX>(r, pick2<T, MAX>(pick2<T, MAX>(q[u].x, q[u].y), pick2<T, MAX>(q[u].z, q[u].w)));
+    if constexpr (sizeof(T) == 4) return __uint_as_float(r);
+    else if constexpr (DT<T>::id == NMG_BF16) return MAX ? fmaxf(__uint_as_float(r << 16), __uint_as_float(r & 0xffff0000u)) : fminf(__uint_as_float(r << 16), __uint_as_float(r & 0xffff0000u));
+    else {
+        const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&r));
+        return MAX ? fmaxf(f.x, f.y) : fminf(f.x, f.y);
+    }
+}
+__device__ __forceinline__ float warp_pick_max(float v) {  // NaN left aside
+    float r;
+    asm("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
+    return r;
+}
+__device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
+
 struct Stats {
     float m, s, w;
     static __device__ __forceinline__ Stats none() { return Stats{neg_inf(), 0.f, 0.f}; }
 
-    // N more logits; W: the entropy is wanted
-    template <int N, bool W> __device__ __forceinline__ void add(const float *x, float a, float slack, float top) {
+    // the reference follows a maximum of `top`
+    template <bool W> __device__ __forceinline__ void raise(float top, float a, float slack) {
         if (top > m + slack) {
             const float d = m - top, f = exp2_fast(d * a);
             if constexpr (W) w = f == 0.f ? 0.f : f * (w + d * s);  // d * s may be -inf
             s *= f;
             m = top;
         }
-        const float ref = m == neg_inf() ? 0.f : m;
-        float ps[2] = {0.f, 0.f}, pw[2] = {0.f, 0.f};
-#pragma unroll
-        for (int i = 0; i < N; i++) {
-            const float d = x[i] - ref, e = exp2_fast(d * a);
-            ps[i & 1] += e;
-            if constexpr (W) pw[i & 1] += e * fmaxf(d, -1e30f);  // 0 * -inf is not a part of the sum
-        }
-        s += ps[0] + ps[1];
-        if constexpr (W) w += pw[0] + pw[1];
     }
-    __device__ __forceinline__ void merge(const Stats &o, float a) {
-        const float top = fmaxf(m, o.m), ref = top == neg_inf() ? 0.f : top;
-        const float d0 = m - ref, d1 = o.m - ref, f0 = exp2_fast(d0 * a), f1 = exp2_fast(d1 * a);
-        w = (f0 == 0.f ? 0.f : f0 * (w + d0 * s)) + (f1 == 0.f ? 0.f : f1 * (o.w + d1 * o.s));
-        s = s * f0 + o.s * f1;
+    // U vectors of logits of which `top` is the largest; W: the entropy is wanted.  Two logits an instruction (f32x2).
+    template <typename T, int U, bool W> __device__ __forceinline__ void add(const uint4 *q, float a, float slack, float top) {
+        raise<W>(top, a, slack);
+        const float ref = m == neg_inf() ? 0.f : m;
+        float2 ps = both(0.f), pw = both(0.f);
+        // masked logits have e = 0 and d = -inf, whose product is not a part of the sum: groups that hold some take the longer way
+        const bool plain = !W || (group_pick<T, false, U>(q) > -1e30f && ref < 1e30f);
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            float x[VEC<T>];
+            unpack<T>(q[u], x);
+#pragma unroll
+            for (int i = 0; i < VEC<T>; i += 2) {
+                const float2 d = __fadd2_rn(make_float2(x[i], x[i + 1]), both(-ref)), t = __fmul2_rn(d, both(a));
+                const float2 e = make_float2(exp2_fast(t.x), exp2_fast(t.y));
+                ps = __fadd2_rn(ps, e);
+                if constexpr (W)
+                    if (plain) pw = __ffma2_rn(e, d, pw);
+            }
+        }
+        if (W && !plain) {
+#pragma unroll
+            for (int u = 0; u < U; u++) {
+                float x[VEC<T>];
+                unpack<T>(q[u], x);
+#pragma unroll
+                for (int i = 0; i < VEC<T>; i++) {
+                    const float d = x[i] - ref;
+                    pw.x += exp2_fast(d * a) * fmaxf(d, -1e30f);
+                }
+            }
+        }
+        s += ps.x + ps.y;
+        if constexpr (W) w += pw.x + pw.y;
+    }
+    template <bool W> __device__ __forceinline__ void add_one(float x, float a, float slack) {
+        raise<W>(x, a, slack);
+        const float d = x - (m == neg_inf() ? 0.f : m), e = exp2_fast(d * a);
+        s += e;
+        if constexpr (W) w += e * fmaxf(d, -1e30f);
+    }
+    // relative to `top`, which is no smaller than any of the set
+    __device__ __forceinline__ void rebase(float top, float a) {
+        const float d = m - (top == neg_inf() ? 0.f : top), f = exp2_fast(d * a);
+        w = f == 0.f ? 0.f : f * (w + d * s);
+        s *= f;
         m = top;
+    }
+    __device__ __forceinline__ void merge(Stats o, float a) {
+        const float top = fmaxf(m, o.m);
+        rebase(top, a);
+        o.rebase(top, a);
+        s += o.s;
+        w += o.w;
     }
     __device__ __forceinline__ bool empty() const { return m == neg_inf() && s == 0.f; }
     __device__ __forceinline__ float entropy(float inv_tau) const { return empty() ? 0.f : logf(s) - w * inv_tau / s; }
@@ -150,13 +219,14 @@ struct Norm {
 };
 __device__ __forceinline__ Norm norm_of(const Stats &st) { return st.empty() ? Norm{neg_inf(), 0.f} : Norm{st.m, logf(st.s)}; }
 
-// Everybody's statistics merged in one order; every thread of the warp gets the same.
+// Statistics of all lanes (of every half warp, with `lanes` = 16 and the same in both), added in one order: every lane gets the same.
 __device__ __forceinline__ Stats warp_merge(Stats st, float a, int lanes = 32) {
+    st.rebase(warp_pick_max(st.m), a);
     for (int o = lanes >> 1; o; o >>= 1) {
-        const Stats other{__shfl_xor_sync(FULL, st.m, o), __shfl_xor_sync(FULL, st.s, o), __shfl_xor_sync(FULL, st.w, o)};
-        st.merge(other, a);
+        st.s += __shfl_xor_sync(FULL, st.s, o);
+        st.w += __shfl_xor_sync(FULL, st.w, o);
     }
-    return Stats{__shfl_sync(FULL, st.m, 0), __shfl_sync(FULL, st.s, 0), __shfl_sync(FULL, st.w, 0)};
+    return st;
 }
 // The CTA's; `red` holds one entry per warp and is free again after the next __syncthreads.
 __device__ __forceinline__ Stats block_merge(Stats st, float a, Stats *red) {
