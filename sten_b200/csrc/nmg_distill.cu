@@ -53,11 +53,6 @@ __device__ __forceinline__ float teacher_value(const void *p, int dtype, int64_t
     if (dtype == NMG_F16) return __half2float(static_cast<const __half *>(p)[i]);
     return __bfloat162float(static_cast<const __nv_bfloat16 *>(p)[i]);
 }
-__device__ __forceinline__ float warp_max(float v) {
-#pragma unroll
-    for (int o = 16; o; o >>= 1) v = fmaxf(v, __shfl_xor_sync(FULL, v, o));
-    return v;
-}
 __device__ __forceinline__ float warp_sum(float v) {
 #pragma unroll
     for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(FULL, v, o);
@@ -75,165 +70,181 @@ template <typename T> __device__ __forceinline__ uint4 leave_out(uint4 q, uint32
     return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-template <typename T, bool REST, bool STATS, bool GRAD> __global__ void __launch_bounds__(VT, VOCAB_CTAS) distill_kernel(DistillParams p) {
-    extern __shared__ __align__(16) uint32_t bits[];
-    __shared__ Stats red[VT / 32], part;
+template <typename T, int NT, bool REST, bool STATS, bool GRAD> __global__ void __launch_bounds__(NT, SM_THREADS / NT) distill_kernel(const __grid_constant__ DistillParams p) {
+    extern __shared__ __align__(16) unsigned char smem[];
+    __shared__ Stats red[NT / 32], part;
     __shared__ KeptShared sh;
+    uint32_t *bits = reinterpret_cast<uint32_t *>(smem + RING_BYTES<NT>);
     const int tid = (int)threadIdx.x, lane = tid & 31, warp = tid >> 5, rank = (int)(blockIdx.x % (unsigned)p.parts);
-    const int64_t r = blockIdx.x / (unsigned)p.parts;
-    const Slice<T> sl(static_cast<const T *>(p.x.x) + row_offset(r, p.x.inner, p.x.ld, p.x.ld_outer), p.x.vocab, rank, p.parts);
-    T *dx = GRAD ? static_cast<T *>(p.dx) + row_offset(r, p.x.inner, p.ld_dx, p.ld_dx_outer) : nullptr;
+    const unsigned first = blockIdx.x / (unsigned)p.parts, step = gridDim.x / (unsigned)p.parts;
     if (GRAD && !STATS && p.skip_if_one && *p.upstream == 1.f) return;  // the gradient that is there already is this one
-    const float weight = p.weight ? p.weight[r] : 1.f;
-    auto leave = [&] {  // a row that does not count
-        if constexpr (GRAD) grad_pass<4>(sl, dx, [](float) { return 0.f; });
-        if (STATS && rank == 0 && tid == 0) {
-            p.loss[r] = 0.f;
-            p.norm[2 * r] = p.norm[2 * r + 1] = Norm{neg_inf(), 0.f};
-        }
+    Stream<T, NT, STATS && GRAD ? 2 : 1> stream(p.x, smem, p.weight, first, step, rank, p.parts);
+    for (int i = tid; i < (REST ? (p.x.vocab + BIT0 + 31) / 32 : FILTER_BITS / 32); i += NT) bits[i] = 0u;
+    const float a = LOG2E * p.inv_tau, slack = 8.f * p.tau, total = p.total ? *p.total : p.divisor;
+
+    // the kept tokens of a row are fetched while the row before is worked on
+    int64_t next_id = -1;
+    float next_logq = neg_inf();
+    auto fetch = [&](unsigned r) {
+        if (tid >= p.kept || r >= p.x.rows) return;
+        const int64_t i = (int64_t)r * p.kept + tid;
+        next_id = p.id_bytes == 8 ? static_cast<const int64_t *>(p.ids)[i] : static_cast<const int *>(p.ids)[i];
+        next_logq = teacher_value(p.log_probs, p.teacher_dtype, i);
     };
-    if (weight == 0.f) return leave();  // whatever its logits are, they are not read for the loss
-
-    // the kept tokens
-    const int words = REST ? (p.x.vocab + BIT0 + 31) / 32 : FILTER_BITS / 32;
-    auto bit_of = [&](int col) { return REST ? col - sl.lead + BIT0 : col & (FILTER_BITS - 1); };
-    for (int i = tid; i < words; i += VT) bits[i] = 0u;
-    int id = -1;
-    bool none_such = false;
-    if (tid < p.kept) {
-        const int64_t raw = p.id_bytes == 8 ? static_cast<const int64_t *>(p.ids)[r * p.kept + tid] : static_cast<const int *>(p.ids)[r * p.kept + tid];
-        none_such = raw >= p.x.vocab;
-        id = raw < 0 || none_such ? -1 : (int)raw;
-        sh.id[tid] = id;
-        sh.logq[tid] = id < 0 ? neg_inf() : teacher_value(p.log_probs, p.teacher_dtype, r * p.kept + tid);
-        sh.x[tid] = id < 0 ? neg_inf() : sl.at(id);
-        sh.first[tid] = 0;
-    }
-    if (tid == 0) sh.twice = 0;
-    const bool bad = __syncthreads_or(none_such);
-    if (id >= 0) {
-        const uint32_t bit = 1u << (bit_of(id) & 31);
-        if (atomicOr(&bits[bit_of(id) >> 5], bit) & bit) sh.twice = 1;  // without remainder: perhaps
-    }
-    __syncthreads();
-    if (sh.twice) {  // an id that is there more than once counts as one token with the sum of its q
+    fetch(first);
+    float weight = p.weight ? p.weight[first] : 1.f;
+    for (unsigned r = first; r < p.x.rows; r += step) {
+        const Slice<T> sl(static_cast<const T *>(p.x.x) + p.x.offset(r), p.x.vocab, rank, p.parts);
+        T *dx = GRAD ? static_cast<T *>(p.dx) + p.x.offset(r, p.ld_dx, p.ld_dx_outer) : nullptr;
+        const float w = weight;
+        const int64_t raw = next_id;
+        const float logq = next_logq;
+        if (p.weight && r + step < p.x.rows) weight = p.weight[r + step];
+        if (w == 0.f) {  // whatever its logits are, they are not read
+            fetch(r + step);
+            if constexpr (GRAD) zero_pass<NT>(sl, dx);
+            if (STATS && rank == 0 && tid == 0) {
+                p.loss[r] = 0.f;
+                p.norm[2 * (int64_t)r] = p.norm[2 * (int64_t)r + 1] = Norm{neg_inf(), 0.f};
+            }
+            continue;
+        }
+        const int col = sl.single(tid);
+        const float single = STATS && col >= 0 ? sl.at(col) : 0.f;
+        auto bit_of = [&](int c) { return REST ? c - sl.lead + BIT0 : c & (FILTER_BITS - 1); };
+        const bool none_such = tid < p.kept && raw >= p.x.vocab;
+        const int id = tid >= p.kept || raw < 0 || none_such ? -1 : (int)raw;
+        __syncthreads();  // the row before is done with what is written now
+        if (tid < p.kept) {
+            sh.id[tid] = id;
+            sh.logq[tid] = id < 0 ? neg_inf() : logq;
+            sh.x[tid] = id < 0 ? neg_inf() : sl.at(id);
+            sh.first[tid] = 0;
+        }
+        if (tid == 0) sh.twice = 0;
+        fetch(r + step);
+        const bool bad = __syncthreads_or(none_such);
         if (id >= 0) {
-            bool first = true;
-            for (int i = 0; i < tid; i++) first = first && sh.id[i] != id;
-            sh.first[tid] = first;
+            const uint32_t bit = 1u << (bit_of(id) & 31);
+            if (atomicOr(&bits[bit_of(id) >> 5], bit) & bit) sh.twice = 1;  // without remainder: perhaps
         }
-    } else if (id >= 0) {
-        sh.first[tid] = 1;
-    }
-    __syncthreads();
-    const float a = LOG2E * p.inv_tau, slack = 8.f * p.tau;
-    if (warp == 0) {
-        float top = neg_inf(), sum = 0.f, max_x = neg_inf(), sum_x = 0.f;
-        for (int i = lane; i < p.kept; i += 32) {
-            top = fmaxf(top, sh.logq[i]);
-            if (sh.first[i]) max_x = fmaxf(max_x, sh.x[i]);
-        }
-        top = REST ? 0.f : warp_max(top);
-        max_x = warp_max(max_x);
-        const float ref = top == neg_inf() ? 0.f : top, ref_x = max_x == neg_inf() ? 0.f : max_x;
-        for (int i = lane; i < p.kept; i += 32) {
-            const float q = expf(sh.logq[i] - ref);
-            sh.q[i] = q;
-            sum += q;
-            if (sh.first[i]) sum_x += exp2_fast((sh.x[i] - ref_x) * a);
-        }
-        sum = warp_sum(sum);
-        sum_x = warp_sum(sum_x);
-        if (!REST) {
-            const float norm = ref + logf(sum), inv = 1.f / sum;
-            for (int i = lane; i < p.kept; i += 32) {
-                sh.logq[i] -= norm;
-                sh.q[i] *= inv;
-            }
-        }
-        if (lane == 0) {
-            sh.some = REST || sum != 0.f;
-            sh.mass = REST ? sum : 1.f;
-            sh.rest = REST ? fmaxf(1.f - sum, 0.f) : 0.f;
-            sh.max_x = max_x;
-            sh.sum_x = sum_x;
-        }
-    }
-
-    // the normalisers: of all tokens, and of those not kept
-    Norm all, rest;
-    if constexpr (STATS) {
-        Stats st = Stats::none();
-        constexpr int U = 4;
-        auto marked = [&](int bit) { return bits[bit >> 5] >> (bit & 31); };
-        for_vectors<U>(sl, [&](uint4 *q, int v, int n) {
-            if constexpr (REST) {
-#pragma unroll
-                for (int u = 0; u < U; u++)
-                    if (const uint32_t out = u < n ? marked(BIT0 + (v + u * VT) * VEC<T>) & ((1u << VEC<T>) - 1) : 0u) q[u] = leave_out<T>(q[u], out);
-            }
-            st.add<T, U, false>(q, a, slack, group_pick<T, true, U>(q));
-        });
-        if (const int col = sl.single(tid); col >= 0) st.add_one<false>(REST && (marked(bit_of(col)) & 1) ? neg_inf() : sl.at(col), a, slack);
-        st = block_merge(st, a, red);
-        if (p.parts > 1) {
-            if (tid == 0) part = st;
-            cluster_barrier_arrive();
-            cluster_barrier_wait();
-            st = peer_stats(&part, 0);
-            for (int i = 1; i < p.parts; i++) st.merge(peer_stats(&part, i), a);
-            cluster_barrier_arrive();  // waited for at the end: shared memory of all CTAs stays until then
-        }
-        rest = norm_of(st);
-        if constexpr (REST) st.merge(Stats{sh.max_x, sh.sum_x, 0.f}, a);
-        all = norm_of(st);
-    } else {
         __syncthreads();
-        all = p.norm[2 * r];
-        rest = p.norm[2 * r + 1];
-    }
-    const bool counts = sh.some && !all.empty();
-    const float q0 = REST && !rest.empty() ? sh.rest : 0.f, mass = sh.mass + q0;
-    const float log_p0 = fmaf(rest.m - all.m, p.inv_tau, rest.ln - all.ln);
-    if constexpr (STATS) {
-        if (rank == 0 && warp == 0) {
-            float loss = 0.f;
-            for (int i = lane; i < p.kept; i += 32) {
-                const float q = sh.q[i];
-                if (q != 0.f) loss += q * (sh.logq[i] - all.log_prob(sh.x[i], p.inv_tau));
+        if (sh.twice) {  // an id that is there more than once counts as one token with the sum of its q
+            if (id >= 0) {
+                bool earliest = true;
+                for (int i = 0; i < tid; i++) earliest = earliest && sh.id[i] != id;
+                sh.first[tid] = earliest;
             }
-            loss = warp_sum(loss);
+        } else if (id >= 0) {
+            sh.first[tid] = 1;
+        }
+        __syncthreads();
+        if (warp == 0) {
+            float top = neg_inf(), sum = 0.f, max_x = neg_inf(), sum_x = 0.f;
+            for (int i = lane; i < p.kept; i += 32) {
+                top = fmaxf(top, sh.logq[i]);
+                if (sh.first[i]) max_x = fmaxf(max_x, sh.x[i]);
+            }
+            top = REST ? 0.f : warp_pick_max(top);
+            max_x = warp_pick_max(max_x);
+            const float ref = top == neg_inf() ? 0.f : top, ref_x = max_x == neg_inf() ? 0.f : max_x;
+            for (int i = lane; i < p.kept; i += 32) {
+                const float q = expf(sh.logq[i] - ref);
+                sh.q[i] = q;
+                sum += q;
+                if (sh.first[i]) sum_x += exp2_fast((sh.x[i] - ref_x) * a);
+            }
+            sum = warp_sum(sum);
+            sum_x = warp_sum(sum_x);
+            if (!REST) {
+                const float norm = ref + logf(sum), inv = 1.f / sum;
+                for (int i = lane; i < p.kept; i += 32) {
+                    sh.logq[i] -= norm;
+                    sh.q[i] *= inv;
+                }
+            }
             if (lane == 0) {
-                if (q0 != 0.f) loss += q0 * (logf(q0) - log_p0);
-                p.loss[r] = bad ? __int_as_float(0x7fffffff) : counts ? p.tau * p.tau * weight * loss : 0.f;
-                p.norm[2 * r] = all;
-                p.norm[2 * r + 1] = rest;
+                sh.some = REST || sum != 0.f;
+                sh.mass = REST ? sum : 1.f;
+                sh.rest = REST ? fmaxf(1.f - sum, 0.f) : 0.f;
+                sh.max_x = max_x;
+                sh.sum_x = sum_x;
             }
         }
-    }
-    if constexpr (GRAD) {
-        const float total = p.total ? *p.total : p.divisor;
-        float scale = total == 0.f ? 0.f : p.tau * weight / total;
-        if constexpr (!STATS) scale *= p.upstream_one ? *p.upstream : p.upstream[r];
-        if (bad) scale = __int_as_float(0x7fffffff);
-        if (!counts && !bad) {
-            grad_pass<4>(sl, dx, [](float) { return 0.f; });
+
+        // the normalisers: of all tokens, and of those not kept
+        Norm all, rest;
+        if constexpr (STATS) {
+            Stats st = Stats::none();
+            auto marked = [&](int bit) { return bits[bit >> 5] >> (bit & 31); };
+            stream.pass(sl, [&](uint4 *q, int v, int n) {
+                if constexpr (REST) {
+#pragma unroll
+                    for (int u = 0; u < STEP; u++)
+                        if (const uint32_t out = u < n ? marked(BIT0 + (v + u * NT) * VEC<T>) & ((1u << VEC<T>) - 1) : 0u) q[u] = leave_out<T>(q[u], out);
+                }
+                st.add<T, STEP, false>(q, a, slack, group_pick<T, true, STEP>(q));
+            });
+            if (col >= 0) st.add_one<false>(REST && (marked(bit_of(col)) & 1) ? neg_inf() : single, a, slack);
+            leave_stats<NT>(st, a, red);
+            __syncthreads();
+            st = block_stats<NT>(red, a);
+            if (p.parts > 1) {
+                if (tid == 0) part = st;
+                cluster_barrier_arrive();
+                cluster_barrier_wait();
+                st = peer_stats(&part, 0);
+                for (int i = 1; i < p.parts; i++) st.merge(peer_stats(&part, i), a);
+                cluster_barrier_arrive();  // waited for at the end of the row: what the others read stays until then
+            }
+            rest = norm_of(st);
+            if constexpr (REST) st.merge(Stats{sh.max_x, sh.sum_x, 0.f}, a);
+            all = norm_of(st);
         } else {
+            __syncthreads();
+            all = p.norm[2 * (int64_t)r];
+            rest = p.norm[2 * (int64_t)r + 1];
+        }
+        if (id >= 0) bits[bit_of(id) >> 5] = 0u;  // nobody reads them any more
+        const bool counts = sh.some && !all.empty();
+        const float q0 = REST && !rest.empty() ? sh.rest : 0.f, mass = sh.mass + q0;
+        const float log_p0 = fmaf(rest.m - all.m, p.inv_tau, rest.ln - all.ln);
+        if constexpr (STATS) {
+            if (rank == 0 && warp == 0) {
+                float loss = 0.f;
+                for (int i = lane; i < p.kept; i += 32) {
+                    const float q = sh.q[i];
+                    if (q != 0.f) loss += q * (sh.logq[i] - all.log_prob(sh.x[i], p.inv_tau));
+                }
+                loss = warp_sum(loss);
+                if (lane == 0) {
+                    if (q0 != 0.f) loss += q0 * (logf(q0) - log_p0);
+                    p.loss[r] = bad ? __int_as_float(0x7fffffff) : counts ? p.tau * p.tau * w * loss : 0.f;
+                    p.norm[2 * (int64_t)r] = all;
+                    p.norm[2 * (int64_t)r + 1] = rest;
+                }
+            }
+        }
+        if constexpr (GRAD) {
+            float scale = total == 0.f ? 0.f : p.tau * w / total;
+            if constexpr (!STATS) scale *= p.upstream_one ? *p.upstream : p.upstream[r];
+            if (bad) scale = __int_as_float(0x7fffffff);
             // away from the kept tokens every element is a multiple of one exponential
             const Norm of = REST ? rest : all;
             const float m = of.empty() ? 0.f : of.m, ln2 = of.ln * LOG2E;
             const float others = scale * (REST ? (rest.empty() ? 0.f : mass * exp2_fast(log_p0 * LOG2E) - q0) : 1.f);
-            grad_pass<4>(sl, dx, [&](float x) { return others * exp2_fast(fmaf(x - m, a, -ln2)); });
+            const bool zero = !counts && !bad;
+            grad_pass<NT>(stream, sl, dx, [&](float x) { return zero ? 0.f : others * exp2_fast(fmaf(x - m, a, -ln2)); });
             __syncthreads();  // the entries below replace what other threads wrote
-            if (tid < p.kept && sh.first[tid] && sl.holds(id)) {
+            if (!zero && tid < p.kept && sh.first[tid] && sl.holds(id)) {
                 float q = sh.q[tid];
                 if (sh.twice)
                     for (int i = tid + 1; i < p.kept; i++) q += sh.id[i] == id ? sh.q[i] : 0.f;
                 dx[id] = DT<T>::from_f32(scale * ((REST ? mass : 1.f) * exp2_fast(all.log_prob(sh.x[tid], p.inv_tau) * LOG2E) - q));
             }
         }
+        if (STATS && p.parts > 1) cluster_barrier_wait();
     }
-    if (STATS && p.parts > 1) cluster_barrier_wait();
 }
 
 // out = sum of v (divided by *by, or by 1; 0 where that is 0), added in 64 bits in a fixed order
@@ -254,16 +265,19 @@ __global__ void __launch_bounds__(1024) ordered_sum_kernel(const float *v, int64
     }
 }
 
-template <typename T, bool REST, bool STATS, bool GRAD> static int launch_distill(DistillParams &p, int dtype, cudaStream_t st) {
-    int sms, rc;
-    if ((rc = device_sms(&sms))) return rc;
-    p.parts = row_parts(p.x.rows, p.x.vocab, dtype, sms, STATS && GRAD);
-    const size_t smem = (REST ? ((size_t)p.x.vocab + BIT0 + 31) / 32 : FILTER_BITS / 32) * 4;
-    NMG_ALLOW_SMEM(smem, distill_kernel<T, REST, STATS, GRAD>);
-    return launch_rows(distill_kernel<T, REST, STATS, GRAD>, p.x.rows, p.parts, smem, st, p);
+template <typename T, int NT, bool REST, bool STATS, bool GRAD> static int launch_distill(DistillParams &p, Deal deal, int sms, cudaStream_t st) {
+    const size_t smem = RING_BYTES<NT> + (REST ? ((size_t)p.x.vocab + BIT0 + 31) / 32 : FILTER_BITS / 32) * 4;
+    NMG_ALLOW_SMEM(smem, distill_kernel<T, NT, REST, STATS, GRAD>);
+    return launch_rows(distill_kernel<T, NT, REST, STATS, GRAD>, p.x.rows, deal, sms, smem, st, p);
 }
 template <bool STATS, bool GRAD> static int launch_distill_any(DistillParams &p, int dtype, bool rest, cudaStream_t st) {
-    NMG_DISPATCH_DTYPE(dtype, T, { return rest ? launch_distill<T, true, STATS, GRAD>(p, dtype, st) : launch_distill<T, false, STATS, GRAD>(p, dtype, st); });
+    int sms, rc;
+    if ((rc = device_sms(&sms))) return rc;
+    const Deal deal = deal_rows(p.x.rows, p.x.vocab, dtype, sms, STATS && GRAD, p.kept <= 128 ? 128 : 256);
+    p.parts = deal.parts;
+    NMG_DISPATCH_DTYPE(dtype, T, {
+        NMG_DISPATCH_THREADS(deal.threads, NT, return rest ? launch_distill<T, NT, true, STATS, GRAD>(p, deal, sms, st) : launch_distill<T, NT, false, STATS, GRAD>(p, deal, sms, st));
+    });
     return NMG_OK;
 }
 

@@ -16,7 +16,8 @@
 
 namespace nmg {
 
-constexpr int TOP_MAX = 128, CANDIDATES = 2048;
+constexpr int TOP_MAX = 128;
+template <int NT> constexpr int CANDIDATES = 2 * NT;
 
 struct TokenParams {
     Logits x;
@@ -53,17 +54,17 @@ __device__ __forceinline__ float key_value(uint32_t key) { return __uint_as_floa
 __device__ __forceinline__ uint64_t candidate(uint32_t key, int col) { return (uint64_t)key << 32 | (0xffffffffu - (uint32_t)col); }
 __device__ __forceinline__ int candidate_col(uint64_t c) { return (int)(0xffffffffu - (uint32_t)c); }
 
-struct TopShared {
-    uint64_t cand[CANDIDATES], top[TOP_MAX];
-    uint32_t keys[VT];
-    uint16_t hot[VT];
-    int scan[VT / 32];
+template <int NT> struct TopShared {
+    uint64_t cand[CANDIDATES<NT>], top[TOP_MAX];
+    uint32_t keys[NT];
+    uint16_t hot[NT];
+    int scan[NT / 32];
     uint32_t bound;
     int n_cand, n_hot;
 };
 
 // exclusive prefix sum over the CTA and the total
-__device__ __forceinline__ int block_scan(int n, int *warps, int *total) {
+template <int NT> __device__ __forceinline__ int block_scan(int n, int *warps, int *total) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     int inc = n;
 #pragma unroll
@@ -76,7 +77,7 @@ __device__ __forceinline__ int block_scan(int n, int *warps, int *total) {
     __syncthreads();
     int before = 0, all = 0;
 #pragma unroll
-    for (int i = 0; i < VT / 32; i++) {
+    for (int i = 0; i < NT / 32; i++) {
         const int c = warps[i];
         before += i < warp ? c : 0;
         all += c;
@@ -86,16 +87,16 @@ __device__ __forceinline__ int block_scan(int n, int *warps, int *total) {
 }
 
 // sh.top[0 .. k): the slice's top k, sorted; 0 past its end.  `best`: the largest logit of this thread's vectors, NaN where one is.
-template <typename T> __device__ void select_top(const Slice<T> &sl, int k, float best, TopShared &sh) {
+template <typename T, int NT> __device__ void select_top(const Slice<T> &sl, int k, float best, TopShared<NT> &sh) {
     const int tid = (int)threadIdx.x, lane = tid & 31;
     const uint32_t key = sl.v0 + tid < sl.v1 ? order_key(best) : 0u;
     sh.keys[tid] = key;
     if (tid == 0) sh.n_cand = sh.n_hot = 0;
     __syncthreads();
     if (tid < 32) {
-        uint32_t mine[VT / 32];
+        uint32_t mine[NT / 32];
 #pragma unroll
-        for (int i = 0; i < VT / 32; i++) mine[i] = sh.keys[lane + 32 * i];
+        for (int i = 0; i < NT / 32; i++) mine[i] = sh.keys[lane + 32 * i];
         // the low bits are left zero, which only lowers the bound: bf16 keys have 16 bits, those of fp16 19
         constexpr int LAST = DT<T>::id == NMG_BF16 ? 16 : DT<T>::id == NMG_F16 ? 13 : 12;
         uint32_t bound = 0;
@@ -103,7 +104,7 @@ template <typename T> __device__ void select_top(const Slice<T> &sl, int k, floa
             const uint32_t next = bound | 1u << bit;
             int c = 0;
 #pragma unroll
-            for (int i = 0; i < VT / 32; i++) c += mine[i] >= next;
+            for (int i = 0; i < NT / 32; i++) c += mine[i] >= next;
             if (__reduce_add_sync(FULL, c) >= k) bound = next;
         }
         if (lane == 0) sh.bound = bound;
@@ -111,18 +112,18 @@ template <typename T> __device__ void select_top(const Slice<T> &sl, int k, floa
     __syncthreads();
     uint32_t bound = sh.bound;
     bool above = false;  // collect what is above the bound, not what is equal to it
-    const int rounds = (sl.v1 - sl.v0 + VT - 1) / VT, held = sl.count(), want = k < held ? k : held;
+    const int rounds = (sl.v1 - sl.v0 + NT - 1) / NT, held = sl.count(), want = k < held ? k : held;
     auto wanted = [&](uint32_t q) { return above ? q > bound : q >= bound; };
     auto push = [&](uint32_t q, int col) {
         const int at = atomicAdd(&sh.n_cand, 1);
-        if (at < CANDIDATES) sh.cand[at] = candidate(q, col);
+        if (at < CANDIDATES<NT>) sh.cand[at] = candidate(q, col);
     };
     for (;;) {
         if (wanted(key) && key) sh.hot[atomicAdd(&sh.n_hot, 1)] = (uint16_t)tid;
         __syncthreads();
         const int n_hot = sh.n_hot, items = n_hot * rounds;
-        for (int i = tid; i < items; i += VT) {
-            const int v = sl.v0 + sh.hot[i % n_hot] + i / n_hot * VT;
+        for (int i = tid; i < items; i += NT) {
+            const int v = sl.v0 + sh.hot[i % n_hot] + i / n_hot * NT;
             if (v >= sl.v1) continue;
             float x[VEC<T>];
             unpack<T>(sl.vec(v), x);
@@ -133,11 +134,11 @@ template <typename T> __device__ void select_top(const Slice<T> &sl, int k, floa
         if (const int col = sl.single(tid); col >= 0)
             if (const uint32_t q = order_key(sl.at(col)); wanted(q)) push(q, col);
         __syncthreads();
-        if (sh.n_cand <= CANDIDATES) break;
-        for (int i = tid; i < CANDIDATES; i += VT) {
+        if (sh.n_cand <= CANDIDATES<NT>) break;
+        for (int i = tid; i < CANDIDATES<NT>; i += NT) {
             const uint64_t c = sh.cand[i];
             int place = 0;
-            for (int j = 0; j < CANDIDATES; j++) place += sh.cand[j] > c;
+            for (int j = 0; j < CANDIDATES<NT>; j++) place += sh.cand[j] > c;
             if (place == k - 1) sh.bound = (uint32_t)(c >> 32);
         }
         __syncthreads();
@@ -152,7 +153,7 @@ template <typename T> __device__ void select_top(const Slice<T> &sl, int k, floa
             int col = -1, elems = 0;
             uint32_t equal = 0;
             if (r >= 0 && r < rounds) {
-                const int v = sl.v0 + r * VT + tid;
+                const int v = sl.v0 + r * NT + tid;
                 if (v < sl.v1) {
                     float x[VEC<T>];
                     unpack<T>(sl.vec(v), x);
@@ -167,7 +168,7 @@ template <typename T> __device__ void select_top(const Slice<T> &sl, int k, floa
                 elems = 1;
             }
             int total;
-            int at = n + found + block_scan(__popc(equal), sh.scan, &total);
+            int at = n + found + block_scan<NT>(__popc(equal), sh.scan, &total);
             for (int u = 0; u < elems; u++)
                 if (equal >> u & 1) {
                     if (at < want) sh.cand[at] = candidate(bound, col + u);
@@ -178,7 +179,7 @@ template <typename T> __device__ void select_top(const Slice<T> &sl, int k, floa
         n = want;
         __syncthreads();
     }
-    for (int i = tid; i < n; i += VT) {
+    for (int i = tid; i < n; i += NT) {
         const uint64_t c = sh.cand[i];
         int place = 0;
         for (int j = 0; j < n; j++) place += sh.cand[j] > c;
@@ -189,11 +190,11 @@ template <typename T> __device__ void select_top(const Slice<T> &sl, int k, floa
 }
 
 // sh.top of the cluster's CTAs into the first one's.  Between two barriers of the cluster; called by the first one only.
-__device__ __forceinline__ void merge_top(int k, int parts, TopShared &sh) {
+template <int NT> __device__ __forceinline__ void merge_top(int k, int parts, TopShared<NT> &sh) {
     const int tid = (int)threadIdx.x;
-    for (int e = tid; e < parts * k; e += VT) sh.cand[e] = peer_load_u64(peer_smem(&sh.top[e % k], e / k));
+    for (int e = tid; e < parts * k; e += NT) sh.cand[e] = peer_load_u64(peer_smem(&sh.top[e % k], e / k));
     __syncthreads();
-    for (int e = tid; e < parts * k; e += VT) {
+    for (int e = tid; e < parts * k; e += NT) {
         const uint64_t c = sh.cand[e];
         int place = e % k;
         for (int b = 0; b < parts; b++) {
@@ -211,110 +212,124 @@ __device__ __forceinline__ void merge_top(int k, int parts, TopShared &sh) {
     __syncthreads();
 }
 
-template <typename T, bool TOP> __global__ void __launch_bounds__(VT, VOCAB_CTAS) token_kernel(TokenParams p) {
-    __shared__ Stats red[VT / 32], part;
-    __shared__ __align__(16) unsigned char top_smem[TOP ? sizeof(TopShared) : 16];
-    TopShared &sh = *reinterpret_cast<TopShared *>(top_smem);
+template <typename T, int NT, bool TOP> __global__ void __launch_bounds__(NT, SM_THREADS / NT) token_kernel(const __grid_constant__ TokenParams p) {
+    extern __shared__ __align__(16) unsigned char smem[];
+    __shared__ Stats red[2][NT / 32], part;
+    TopShared<NT> &sh = *reinterpret_cast<TopShared<NT> *>(smem + RING_BYTES<NT>);
     const int tid = (int)threadIdx.x, rank = p.parts > 1 ? cluster_rank() : 0;
-    const int64_t r = blockIdx.x / (unsigned)p.parts;
-    const Slice<T> sl(static_cast<const T *>(p.x.x) + row_offset(r, p.x.inner, p.x.ld, p.x.ld_outer), p.x.vocab, rank, p.parts);
+    const unsigned first = blockIdx.x / (unsigned)p.parts, step = gridDim.x / (unsigned)p.parts;
     const float a = LOG2E * p.inv_tau, slack = 8.f * p.tau;
-    int64_t target = p.ignore;
-    float target_x = 0.f;
-    if (rank == 0 && tid == 0 && p.targets) {
-        target = p.targets[r];
-        if (target >= 0 && target < p.x.vocab) target_x = sl.at((int)target);
-    }
-    Stats st = Stats::none();
-    float best = neg_inf();
-    for_vectors<4>(sl, [&](const uint4 *q, int, int) {
-        const float top = group_pick<T, true, 4>(q);
-        if constexpr (TOP) best = fmaxf(best, top);
-        st.add<T, 4, true>(q, a, slack, top);
-    });
-    if constexpr (TOP) {
-        if (st.s != st.s)  // NaN, or +inf: only the first has to be found
-            for (int v = sl.v0 + tid; v < sl.v1; v += VT) {
-                float x[VEC<T>];
-                unpack<T>(sl.vec(v), x);
+    Stream<T, NT, 1> stream(p.x, smem, nullptr, first, step, rank, p.parts);
+    for (unsigned r = first, turn = 0; r < p.x.rows; r += step, turn ^= 1) {
+        const Slice<T> sl(static_cast<const T *>(p.x.x) + p.x.offset(r), p.x.vocab, rank, p.parts);
+        const int col = tid < 32 ? sl.single(tid) : -1;
+        const float single = col >= 0 ? sl.at(col) : 0.f;
+        int64_t target = p.ignore;
+        float target_x = 0.f;
+        if (rank == 0 && tid == 0 && p.targets) {
+            target = p.targets[r];
+            if (target >= 0 && target < p.x.vocab) target_x = sl.at((int)target);
+        }
+        Stats st = Stats::none();
+        float best = neg_inf();
+        stream.pass(sl, [&](const uint4 *q, int, int) {
+            const float top = group_pick<T, true, STEP>(q);
+            if constexpr (TOP) best = fmaxf(best, top);
+            st.add<T, STEP, true>(q, a, slack, top);
+        });
+        if constexpr (TOP) {
+            if (st.s != st.s)  // NaN, or +inf: only the first has to be found
+                for (int v = sl.v0 + tid; v < sl.v1; v += NT) {
+                    float x[VEC<T>];
+                    unpack<T>(sl.vec(v), x);
 #pragma unroll
-                for (int u = 0; u < VEC<T>; u++) best = x[u] != x[u] ? x[u] : best;
+                    for (int u = 0; u < VEC<T>; u++) best = x[u] != x[u] ? x[u] : best;
+                }
+        }
+        if (col >= 0) st.add_one<true>(single, a, slack);
+        leave_stats<NT>(st, a, red[turn]);
+        __syncthreads();
+        if (!TOP && tid >= 32 && p.parts == 1) continue;  // the first warp finishes the row
+        st = block_stats<NT>(red[turn], a);
+        if constexpr (TOP) select_top<T, NT>(sl, p.top, best, sh);
+        if (p.parts > 1) {
+            if (tid == 0) part = st;
+            cluster_barrier_arrive();
+            cluster_barrier_wait();
+            if (rank == 0) {
+                st = peer_stats(&part, 0);
+                for (int i = 1; i < p.parts; i++) st.merge(peer_stats(&part, i), a);
+                if constexpr (TOP) merge_top<NT>(p.top, p.parts, sh);
             }
-    }
-    if (const int col = sl.single(tid); col >= 0) st.add_one<true>(sl.at(col), a, slack);
-    st = block_merge(st, a, red);
-    if constexpr (TOP) select_top<T>(sl, p.top, best, sh);
-    if (p.parts > 1) {
-        if (tid == 0) part = st;
-        cluster_barrier_arrive();
-        cluster_barrier_wait();
-        if (rank == 0) {
-            st = peer_stats(&part, 0);
-            for (int i = 1; i < p.parts; i++) st.merge(peer_stats(&part, i), a);
-            if constexpr (TOP) merge_top(p.top, p.parts, sh);
+            cluster_barrier_arrive();  // what the first CTA reads in the others stays until it has
+            cluster_barrier_wait();
+            if (rank != 0) continue;
         }
-        cluster_barrier_arrive();  // shared memory of all CTAs stays until the first one has read it
-        cluster_barrier_wait();
-        if (rank != 0) return;
-    }
-    const Norm norm = norm_of(st);
-    if (tid == 0) {
-        if (p.log_prob) {
-            const bool ours = target >= 0 && target < p.x.vocab;
-            p.log_prob[r] = target == p.ignore ? 0.f : ours ? norm.log_prob(target_x, p.inv_tau) : __int_as_float(0x7fffffff);
+        if (TOP ? tid >= p.top && tid > 0 : tid > 0) continue;
+        const Norm norm = norm_of(st);
+        if (tid == 0) {
+            if (p.log_prob) {
+                const bool ours = target >= 0 && target < p.x.vocab;
+                p.log_prob[r] = target == p.ignore ? 0.f : ours ? norm.log_prob(target_x, p.inv_tau) : __int_as_float(0x7fffffff);
+            }
+            p.entropy[r] = st.entropy(p.inv_tau);
+            p.lse[r] = norm.lse(p.inv_tau);
+            if (p.norm) p.norm[r] = norm;
         }
-        p.entropy[r] = st.entropy(p.inv_tau);
-        p.lse[r] = norm.lse(p.inv_tau);
-        if (p.norm) p.norm[r] = norm;
-    }
-    if constexpr (TOP) {
-        if (tid < p.top) {
-            const uint64_t c = sh.top[tid];
-            p.top_ids[r * p.top + tid] = candidate_col(c);
-            p.top_log_prob[r * p.top + tid] = norm.log_prob(key_value((uint32_t)(c >> 32)), p.inv_tau);
+        if constexpr (TOP) {
+            if (tid < p.top) {
+                const uint64_t c = sh.top[tid];
+                p.top_ids[(int64_t)r * p.top + tid] = candidate_col(c);
+                p.top_log_prob[(int64_t)r * p.top + tid] = norm.log_prob(key_value((uint32_t)(c >> 32)), p.inv_tau);
+            }
         }
     }
 }
 
-template <typename T, bool E> __global__ void __launch_bounds__(VT, VOCAB_CTAS) token_grad_kernel(TokenGradParams p) {
+template <typename T, int NT, bool E> __global__ void __launch_bounds__(NT, SM_THREADS / NT) token_grad_kernel(const __grid_constant__ TokenGradParams p) {
+    extern __shared__ __align__(16) unsigned char smem[];
     const int tid = (int)threadIdx.x, lane = tid & 31, rank = (int)(blockIdx.x % (unsigned)p.parts);
-    const int64_t r = blockIdx.x / (unsigned)p.parts;
-    const Slice<T> sl(static_cast<const T *>(p.x.x) + row_offset(r, p.x.inner, p.x.ld, p.x.ld_outer), p.x.vocab, rank, p.parts);
-    T *dx = static_cast<T *>(p.dx) + row_offset(r, p.x.inner, p.ld_dx, p.ld_dx_outer);
-    const int64_t target = p.targets && p.g_log_prob ? p.targets[r] : p.ignore;
-    const bool in_row = target >= 0 && target < p.x.vocab && target != p.ignore;
-    const float g_lp = in_row ? p.g_log_prob[r] : 0.f, g_h = E ? p.g_entropy[r] : 0.f;
-    const Norm norm = p.norm[r];
-    float g_top = 0.f;
-    if (p.g_top) {
-        for (int i = lane; i < p.top; i += 32) g_top += p.g_top[r * p.top + i];
+    const unsigned first = blockIdx.x / (unsigned)p.parts, step = gridDim.x / (unsigned)p.parts;
+    Stream<T, NT, 1> stream(p.x, smem, nullptr, first, step, rank, p.parts);
+    for (unsigned r = first; r < p.x.rows; r += step) {
+        const int64_t at = (int64_t)r * p.top;
+        const Slice<T> sl(static_cast<const T *>(p.x.x) + p.x.offset(r), p.x.vocab, rank, p.parts);
+        T *dx = static_cast<T *>(p.dx) + p.x.offset(r, p.ld_dx, p.ld_dx_outer);
+        const int64_t target = p.targets && p.g_log_prob ? p.targets[r] : p.ignore;
+        const bool in_row = target >= 0 && target < p.x.vocab && target != p.ignore;
+        const float g_lp = in_row ? p.g_log_prob[r] : 0.f, g_h = E ? p.g_entropy[r] : 0.f;
+        const Norm norm = p.norm[r];
+        float g_top = 0.f;
+        if (p.g_top) {
+            for (int i = lane; i < p.top; i += 32) g_top += p.g_top[at + i];
 #pragma unroll
-        for (int o = 16; o; o >>= 1) g_top += __shfl_xor_sync(FULL, g_top, o);
-    }
-    float A = (p.g_lse ? p.g_lse[r] : 0.f) - g_lp - g_top - (E ? g_h * p.entropy[r] : 0.f), B = -g_h;
-    if (!in_row && target != p.ignore) A = __int_as_float(0x7fffffff);  // no such token
-    const bool empty = norm.empty();
-    const float m = empty ? 0.f : norm.m, ln = norm.ln, a = LOG2E * p.inv_tau, ln2 = ln * LOG2E;  // nothing but -inf: p = 0 below
-    A *= p.inv_tau;
-    B *= p.inv_tau;
-    auto grad = [&](float x) {
-        const float d = x - m, e = exp2_fast(fmaf(d, a, -ln2));
-        return E ? e * (A + B * fmaf(fmaxf(d, -1e30f), p.inv_tau, -ln)) : e * A;  // 0 * -inf is not a part of it
-    };
-    grad_pass<4>(sl, dx, grad);
-    __syncthreads();  // the entries below replace what other threads wrote
-    if (empty) return;
-    if (tid < p.top && p.g_top) {
-        const int64_t id = p.top_ids[r * p.top + tid];
-        if (id >= 0 && id < p.x.vocab && !(in_row && id == target) && sl.holds((int)id))
-            dx[id] = DT<T>::from_f32(grad(sl.at((int)id)) + p.g_top[r * p.top + tid] * p.inv_tau);
-    }
-    if (tid == TOP_MAX && in_row && sl.holds((int)target)) {
-        float g = g_lp;
-        if (p.g_top)
-            for (int i = 0; i < p.top; i++)
-                if (p.top_ids[r * p.top + i] == target) g += p.g_top[r * p.top + i];
-        dx[target] = DT<T>::from_f32(grad(sl.at((int)target)) + g * p.inv_tau);
+            for (int o = 16; o; o >>= 1) g_top += __shfl_xor_sync(FULL, g_top, o);
+        }
+        float A = (p.g_lse ? p.g_lse[r] : 0.f) - g_lp - g_top - (E ? g_h * p.entropy[r] : 0.f), B = -g_h;
+        if (!in_row && target != p.ignore) A = __int_as_float(0x7fffffff);  // no such token
+        const bool empty = norm.empty();
+        const float m = empty ? 0.f : norm.m, ln = norm.ln, a = LOG2E * p.inv_tau, ln2 = ln * LOG2E;  // nothing but -inf: p = 0 below
+        A *= p.inv_tau;
+        B *= p.inv_tau;
+        auto grad = [&](float x) {
+            const float d = x - m, e = exp2_fast(fmaf(d, a, -ln2));
+            return E ? e * (A + B * fmaf(fmaxf(d, -1e30f), p.inv_tau, -ln)) : e * A;  // 0 * -inf is not a part of it
+        };
+        grad_pass<NT>(stream, sl, dx, grad);
+        __syncthreads();  // the entries below replace what other threads wrote
+        if (empty) continue;
+        if (tid < p.top && p.g_top) {
+            const int64_t id = p.top_ids[at + tid];
+            if (id >= 0 && id < p.x.vocab && !(in_row && id == target) && sl.holds((int)id))
+                dx[id] = DT<T>::from_f32(grad(sl.at((int)id)) + p.g_top[at + tid] * p.inv_tau);
+        }
+        if (tid == NT - 1 && in_row && sl.holds((int)target)) {
+            float g = g_lp;
+            if (p.g_top)
+                for (int i = 0; i < p.top; i++)
+                    if (p.top_ids[at + i] == target) g += p.g_top[at + i];
+            dx[target] = DT<T>::from_f32(grad(sl.at((int)target)) + g * p.inv_tau);
+        }
     }
 }
 
@@ -327,6 +342,15 @@ int check_logits(const Logits &x, int dtype, float temperature) {
     return NMG_OK;
 }
 
+template <typename T, int NT, bool TOP> static int launch_token(const TokenParams &p, Deal deal, int sms, cudaStream_t st) {
+    const size_t smem = RING_BYTES<NT> + (TOP ? sizeof(TopShared<NT>) : 0);
+    NMG_ALLOW_SMEM(smem, token_kernel<T, NT, TOP>);
+    return launch_rows(token_kernel<T, NT, TOP>, p.x.rows, deal, sms, smem, st, p);
+}
+template <typename T, int NT, bool E> static int launch_token_grad(const TokenGradParams &p, Deal deal, int sms, cudaStream_t st) {
+    NMG_ALLOW_SMEM(RING_BYTES<NT>, token_grad_kernel<T, NT, E>);
+    return launch_rows(token_grad_kernel<T, NT, E>, p.x.rows, deal, sms, RING_BYTES<NT>, st, p);
+}
 static int check_top(int top, int vocab) {
     if (top < 0 || top > TOP_MAX) NMG_FAIL(top < 0 ? NMG_ERR_INVALID : NMG_ERR_UNSUPPORTED, "top must be 0 .. %d, got %d", TOP_MAX, top);
     if (top > vocab) NMG_FAIL(NMG_ERR_INVALID, "top = %d alternatives of %d tokens", top, vocab);
@@ -352,9 +376,12 @@ extern "C" int nmg_token_log_probs(const void *logits, int64_t rows, int64_t inn
     if (reinterpret_cast<uintptr_t>(norm) % 8) NMG_FAIL(NMG_ERR_INVALID, "norm must be 8-byte aligned");
     if (top && (!top_log_prob || !top_ids)) NMG_FAIL(NMG_ERR_INVALID, "top_log_prob and top_ids must be non-NULL when top > 0");
     if ((rc = device_sms(&sms))) return rc;
-    p.parts = row_parts(rows, p.x.vocab, dtype, sms, false);
+    const Deal deal = deal_rows(rows, p.x.vocab, dtype, sms, false, top <= 32 ? 128 : top <= 64 ? 256 : 512);  // about a quarter of the threads holds the top
+    p.parts = deal.parts;
     cudaStream_t st = (cudaStream_t)stream;
-    NMG_DISPATCH_DTYPE(dtype, T, { return top ? launch_rows(token_kernel<T, true>, rows, p.parts, 0, st, p) : launch_rows(token_kernel<T, false>, rows, p.parts, 0, st, p); });
+    NMG_DISPATCH_DTYPE(dtype, T, {
+        NMG_DISPATCH_THREADS(deal.threads, NT, return top ? launch_token<T, NT, true>(p, deal, sms, st) : launch_token<T, NT, false>(p, deal, sms, st));
+    });
     return NMG_OK;
 }
 
@@ -370,10 +397,11 @@ extern "C" int nmg_token_log_probs_backward(const void *logits, int64_t rows, in
     if (reinterpret_cast<uintptr_t>(norm) % 8) NMG_FAIL(NMG_ERR_INVALID, "norm must be 8-byte aligned");
     if (reinterpret_cast<uintptr_t>(d_logits) % dtype_size(dtype)) NMG_FAIL(NMG_ERR_INVALID, "d_logits must be aligned to its elements");
     if ((rc = device_sms(&sms))) return rc;
-    p.parts = row_parts(rows, p.x.vocab, dtype, sms, false);
+    const Deal deal = deal_rows(rows, p.x.vocab, dtype, sms, false, 128);
+    p.parts = deal.parts;
     cudaStream_t st = (cudaStream_t)stream;
     NMG_DISPATCH_DTYPE(dtype, T, {
-        return g_entropy ? launch_rows(token_grad_kernel<T, true>, rows, p.parts, 0, st, p) : launch_rows(token_grad_kernel<T, false>, rows, p.parts, 0, st, p);
+        NMG_DISPATCH_THREADS(deal.threads, NT, return g_entropy ? launch_token_grad<T, NT, true>(p, deal, sms, st) : launch_token_grad<T, NT, false>(p, deal, sms, st));
     });
     return NMG_OK;
 }

@@ -18,18 +18,20 @@
 
 namespace nmg {
 
-constexpr int VT = 512;       // threads of a CTA
-constexpr int VOCAB_CTAS = 2; // CTAs of the row kernels that an SM holds at once
+// A row belongs to a CTA of NT threads (128, 256 or 512, template argument), or to a cluster of them; an SM holds SM_THREADS of them.
+constexpr int SM_THREADS = 1024;
 
 struct Logits {
     const void *x;
     int64_t rows, inner, ld, ld_outer;  // row r begins at element (r / inner) * ld_outer + (r % inner) * ld
     int vocab;
+    __host__ __device__ __forceinline__ int64_t offset(unsigned r) const { return offset(r, ld, ld_outer); }
+    __host__ __device__ __forceinline__ int64_t offset(unsigned r, int64_t pitch, int64_t pitch_outer) const {  // of the same row elsewhere
+        if (rows <= inner) return r * pitch;
+        const unsigned o = r / (unsigned)inner;  // fewer than 2^31 rows
+        return o * pitch_outer + (r - o * (unsigned)inner) * pitch;
+    }
 };
-__host__ __device__ __forceinline__ int64_t row_offset(int64_t r, int64_t inner, int64_t ld, int64_t ld_outer) {
-    return r / inner * ld_outer + r % inner * ld;
-}
-
 #ifdef __CUDACC__
 constexpr unsigned FULL = 0xffffffffu;
 __device__ __forceinline__ float neg_inf() { return __int_as_float(0xff800000); }
@@ -88,8 +90,8 @@ template <typename T> struct Slice {
         const int to16 = (int)((16 - (reinterpret_cast<uintptr_t>(row_) & 15)) & 15) / (int)sizeof(T);
         lead = to16 < vocab ? to16 : vocab;
         const int nvec = (vocab - lead) / VEC<T>;
-        v0 = (int)((int64_t)nvec * part / parts);
-        v1 = (int)((int64_t)nvec * (part + 1) / parts);
+        v0 = parts == 1 ? 0 : (int)((int64_t)nvec * part / parts);
+        v1 = parts == 1 ? nvec : (int)((int64_t)nvec * (part + 1) / parts);
         lead_n = part == 0 ? lead : 0;
         tail_at = lead + nvec * VEC<T>;
         tail_n = part == parts - 1 ? vocab - tail_at : 0;
@@ -228,14 +230,12 @@ __device__ __forceinline__ Stats warp_merge(Stats st, float a, int lanes = 32) {
     }
     return st;
 }
-// The CTA's; `red` holds one entry per warp and is free again after the next __syncthreads.
-__device__ __forceinline__ Stats block_merge(Stats st, float a, Stats *red) {
-    static_assert(VT == 512, "sixteen warps meet in half a warp");
+// The CTA's statistics: every warp leaves its own in `red`, and after a __syncthreads any warp may put them together.
+template <int NT> __device__ __forceinline__ void leave_stats(Stats st, float a, Stats *red) {
     st = warp_merge(st, a);
     if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = st;
-    __syncthreads();
-    return warp_merge(red[threadIdx.x & 15], a, 16);
 }
+template <int NT> __device__ __forceinline__ Stats block_stats(const Stats *red, float a) { return warp_merge(red[threadIdx.x & (NT / 32 - 1)], a, NT / 32); }
 
 // ---- clusters: the CTAs that share a row
 __device__ __forceinline__ int cluster_rank() {
@@ -266,33 +266,94 @@ __device__ __forceinline__ Stats peer_stats(const Stats *mine, int rank) {
     return Stats{peer_load_f32(a), peer_load_f32(a + 4), peer_load_f32(a + 8)};
 }
 
-// One pass over the vectors of a slice, U of them in flight a thread: f(vectors, first vector's number, how many hold anything).
-template <int U, typename T, typename F> __device__ __forceinline__ void for_vectors(const Slice<T> &sl, F f) {
-    for (int v = sl.v0 + (int)threadIdx.x; v < sl.v1; v += U * VT) {
-        uint4 q[U];
-        const int left = (sl.v1 - v + VT - 1) / VT;
-#pragma unroll
-        for (int u = 0; u < U; u++) {
-            const uint32_t none = neg_inf_word<T>();
-            q[u] = u < left ? sl.vec(v + u * VT) : make_uint4(none, none, none, none);
-        }
-        f(q, v, left < U ? left : U);
-    }
-}
+// The vectors of one row after another on their way from global memory.  Every thread copies its own vectors (v0 + thread + i * VT)
+// asynchronously into slots of its own in shared memory and keeps DEPTH steps of STEP vectors under way, across the ends of rows and of
+// passes: while a CTA finishes a row, the next rows' logits arrive.  No thread waits for another's copies.
+constexpr int STEP = 4, DEPTH = 2;
+template <int NT> constexpr int RING_BYTES = STEP * DEPTH * NT * 16;  // 128 KB of an SM
 
-// out[column] = f(logit) over the slice.  `out` is where the row's gradient begins; vectors are stored whole where its 16-byte
-// boundaries are those of the logits.
-template <int U, typename T, typename F> __device__ __forceinline__ void grad_pass(const Slice<T> &sl, T *out, F f) {
-    const bool whole = (reinterpret_cast<uintptr_t>(out + sl.lead) & 15) == 0;
-    for_vectors<U>(sl, [&](const uint4 *q, int v, int n) {
+template <typename T, int NT, int PASSES> struct Stream {
+    const Logits &x;
+    uint4 *ring;  // + slot * NT
+    const float *weight;  // rows of weight 0 are left out
+    unsigned row, row_step;
+    int part, parts;
+    // what is copied next
+    const uint4 *from;
+    int left, passes, length;  // vectors of this pass, from this thread's on; passes behind this one; vectors of a pass
+    float next_weight;
+    int put, get;  // slots
+
+    __device__ __forceinline__ Stream(const Logits &x_, void *smem, const float *weight_, unsigned first, unsigned step, int part_, int parts_)
+        : x(x_), ring(static_cast<uint4 *>(smem) + threadIdx.x), weight(weight_), row(first), row_step(step), part(part_), parts(parts_), from(nullptr), left(0), passes(0), length(0), put(0), get(0) {
+        next_weight = weight && row < x.rows ? weight[row] : 1.f;
+        row -= row_step;
+        for (int i = 0; i < DEPTH; i++) issue();
+    }
+    __device__ __forceinline__ void issue() {
+        while (left <= 0) {
+            if (passes > 0) {
+                passes--;
+                left = length;
+                if (left <= 0) passes = 0;
+            } else {
+                row += row_step;
+                if (row >= x.rows) {
+                    row -= row_step;  // stays past the end
+                    break;
+                }
+                const float w = next_weight;
+                if (weight) next_weight = row + row_step < x.rows ? weight[row + row_step] : 1.f;
+                if (w == 0.f) continue;
+                const Slice<T> sl(static_cast<const T *>(x.x) + x.offset(row), x.vocab, part, parts);
+                from = reinterpret_cast<const uint4 *>(sl.row + sl.lead) + sl.v0 + threadIdx.x;
+                left = length = sl.v1 - sl.v0 - (int)threadIdx.x;
+                passes = PASSES - 1;
+            }
+        }
+        if (left > 0) {
+            const uint4 *src = from + (length - left);
 #pragma unroll
-        for (int u = 0; u < U; u++) {
+            for (int u = 0; u < STEP; u++)
+                if (left > u * NT) cp_async_16(ring + (put + u) * NT, src + u * NT);
+            left -= STEP * NT;
+        }
+        cp_async_commit();
+        put = put + STEP == STEP * DEPTH ? 0 : put + STEP;
+    }
+    // f(vectors, number of the first, how many there are) over one pass of a row; the missing ones of the last step are -inf
+    template <typename F> __device__ __forceinline__ void pass(const Slice<T> &sl, F f) {
+        for (int v = sl.v0 + (int)threadIdx.x; v < sl.v1; v += STEP * NT) {
+            cp_async_wait<DEPTH - 1>();
+            uint4 q[STEP];
+            int n = 0;
+#pragma unroll
+            for (int u = 0; u < STEP; u++) {
+                const uint32_t none = neg_inf_word<T>();
+                const bool there = v + u * NT < sl.v1;
+                q[u] = there ? ring[(get + u) * NT] : make_uint4(none, none, none, none);
+                n += there;
+            }
+            get = get + STEP == STEP * DEPTH ? 0 : get + STEP;
+            f(q, v, n);
+            issue();  // into the slots just read
+        }
+    }
+};
+
+// out[column] = f(logit) over the slice, a pass of the stream.  `out` is where the row's gradient begins; vectors are stored whole where its
+// 16-byte boundaries are those of the logits.
+template <int NT, typename T, typename S, typename F> __device__ __forceinline__ void grad_pass(S &stream, const Slice<T> &sl, T *out, F f) {
+    const bool whole = (reinterpret_cast<uintptr_t>(out + sl.lead) & 15) == 0;
+    stream.pass(sl, [&](const uint4 *q, int v, int n) {
+#pragma unroll
+        for (int u = 0; u < STEP; u++) {
             if (u >= n) break;
             float x[VEC<T>];
             unpack<T>(q[u], x);
 #pragma unroll
             for (int i = 0; i < VEC<T>; i++) x[i] = f(x[i]);
-            T *dst = out + sl.lead + (int64_t)(v + u * VT) * VEC<T>;
+            T *dst = out + sl.lead + (int64_t)(v + u * NT) * VEC<T>;
             if (whole) {
                 __stcs(reinterpret_cast<uint4 *>(dst), pack<T>(x));
             } else {
@@ -303,30 +364,51 @@ template <int U, typename T, typename F> __device__ __forceinline__ void grad_pa
     });
     if (const int col = sl.single((int)threadIdx.x); col >= 0) out[col] = DT<T>::from_f32(f(sl.at(col)));
 }
+// the same for a row that is not read
+template <int NT, typename T> __device__ __forceinline__ void zero_pass(const Slice<T> &sl, T *out) {
+    const bool whole = (reinterpret_cast<uintptr_t>(out + sl.lead) & 15) == 0;
+    for (int v = sl.v0 + (int)threadIdx.x; v < sl.v1; v += NT) {
+        T *dst = out + sl.lead + (int64_t)v * VEC<T>;
+        if (whole) {
+            __stcs(reinterpret_cast<uint4 *>(dst), make_uint4(0u, 0u, 0u, 0u));
+        } else {
+#pragma unroll
+            for (int i = 0; i < VEC<T>; i++) dst[i] = DT<T>::from_f32(0.f);
+        }
+    }
+    if (const int col = sl.single((int)threadIdx.x); col >= 0) out[col] = DT<T>::from_f32(0.f);
+}
 #endif
 
-// CTAs that share a row: enough to fill the chip where there are few rows, as long as every thread has a vector to read; and, where rows
-// are visited twice, enough that the second visit finds the rows in flight in L2 (126 MB, of which they may take half).
-inline int row_parts(int64_t rows, int vocab, int dtype, int sms, bool twice) {
-    const int64_t bytes = (int64_t)vocab * (int64_t)dtype_size(dtype), slots = (int64_t)VOCAB_CTAS * sms;
-    int parts = 1;
-    while (parts < 8 && rows * parts * 2 <= slots && bytes >= (int64_t)parts * 2 * VT * 16) parts *= 2;
+// How rows are dealt out.  A row takes NT threads for some hundred instructions at its end, so NT is the smaller the shorter the rows, as
+// long as there are rows enough to fill the chip.  Few rows are shared by clusters of CTAs, as long as every thread has a vector to
+// read; rows that are visited twice also until the second visit finds those in flight in L2 (126 MB, of which they may take half).
+struct Deal { int threads, parts; };
+inline Deal deal_rows(int64_t rows, int vocab, int dtype, int sms, bool twice, int least) {
+    const int64_t bytes = (int64_t)vocab * (int64_t)dtype_size(dtype);
+    int nt = 512, parts = 1;
+    while (nt > 128 && nt / 2 >= least && bytes / 16 < (int64_t)nt * 24 && rows >= (int64_t)sms * (SM_THREADS / (nt / 2))) nt /= 2;
+    const int64_t slots = (int64_t)sms * (SM_THREADS / nt);
+    while (parts < 8 && rows * parts * 2 <= slots && bytes >= (int64_t)parts * 2 * nt * 16) parts *= 2;
     while (twice && parts < 8 && (rows < slots / parts ? rows : slots / parts) * bytes > (int64_t)64 << 20) parts *= 2;
-    return parts;
+    return Deal{nt, parts};
 }
 
-// rows x parts CTAs, the parts of a row in one cluster
+// CTAs that stay, as many as the SMs hold: each cluster of `parts` takes one row after another
 template <typename... P, typename... A>
-inline int launch_rows(void (*kernel)(P...), int64_t rows, int parts, size_t smem, cudaStream_t st, A... args) {
-    if (rows > INT32_MAX / parts) NMG_FAIL(NMG_ERR_UNSUPPORTED, "%lld rows are more than one launch takes", (long long)rows);
+inline int launch_rows(void (*kernel)(P...), int64_t rows, Deal deal, int sms, size_t smem, cudaStream_t st, A... args) {
+    if (rows > INT32_MAX) NMG_FAIL(NMG_ERR_UNSUPPORTED, "%lld rows are more than one launch takes", (long long)rows);
+    int per_sm = SM_THREADS / deal.threads;
+    while (per_sm > 1 && (smem + (6 << 10)) * per_sm > (size_t)228 << 10) per_sm--;  // with what is static and reserved
+    const int64_t clusters = (int64_t)sms * per_sm / deal.parts;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(rows * parts));
-    cfg.blockDim = dim3(VT);
+    cfg.gridDim = dim3((unsigned)((rows < clusters ? rows : clusters) * deal.parts));
+    cfg.blockDim = dim3((unsigned)deal.threads);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = st;
     cudaLaunchAttribute attr;
     attr.id = cudaLaunchAttributeClusterDimension;
-    attr.val.clusterDim.x = (unsigned)parts;
+    attr.val.clusterDim.x = (unsigned)deal.parts;
     attr.val.clusterDim.y = 1;
     attr.val.clusterDim.z = 1;
     cfg.attrs = &attr;
@@ -334,6 +416,12 @@ inline int launch_rows(void (*kernel)(P...), int64_t rows, int parts, size_t sme
     NMG_CUDA(cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...));
     return NMG_OK;
 }
+#define NMG_DISPATCH_THREADS(threads, NT, ...)                        \
+    do {                                                              \
+        if ((threads) == 128) { constexpr int NT = 128; __VA_ARGS__; } \
+        else if ((threads) == 256) { constexpr int NT = 256; __VA_ARGS__; } \
+        else { constexpr int NT = 512; __VA_ARGS__; }                  \
+    } while (0)
 
 int check_logits(const Logits &x, int dtype, float temperature);
 
