@@ -80,7 +80,7 @@ template <typename T, int NT, bool REST, bool STATS, bool GRAD> __global__ void 
     if (GRAD && !STATS && p.skip_if_one && *p.upstream == 1.f) return;  // the gradient that is there already is this one
     Stream<T, NT, STATS && GRAD ? 2 : 1> stream(p.x, smem, p.weight, first, step, rank, p.parts);
     for (int i = tid; i < (REST ? (p.x.vocab + BIT0 + 31) / 32 : FILTER_BITS / 32); i += NT) bits[i] = 0u;
-    const float a = LOG2E * p.inv_tau, slack = 8.f * p.tau, total = p.total ? *p.total : p.divisor;
+    const float a = LOG2E * p.inv_tau, total = p.total ? *p.total : p.divisor;
 
     // the kept tokens of a row are fetched while the row before is worked on
     int64_t next_id = -1;
@@ -183,9 +183,9 @@ template <typename T, int NT, bool REST, bool STATS, bool GRAD> __global__ void 
                     for (int u = 0; u < STEP; u++)
                         if (const uint32_t out = u < n ? marked(BIT0 + (v + u * NT) * VEC<T>) & ((1u << VEC<T>) - 1) : 0u) q[u] = leave_out<T>(q[u], out);
                 }
-                st.add<T, STEP, false>(q, a, slack, group_pick<T, true, STEP>(q));
+                st.add<T, false>(q, a);
             });
-            if (col >= 0) st.add_one<false>(REST && (marked(bit_of(col)) & 1) ? neg_inf() : single, a, slack);
+            if (col >= 0) st.add_one<false>(REST && (marked(bit_of(col)) & 1) ? neg_inf() : single, a);
             leave_stats<NT>(st, a, red);
             __syncthreads();
             st = block_stats<NT>(red, a);

@@ -5,9 +5,9 @@
 //                             A = g_lse - g_log_prob - sum g_top - g_entropy H,  B = -g_entropy  (E: there is an entropy gradient)
 //
 // The top k of a row, ordered by value and among equal values by column: every thread keeps the largest logit of its vectors
-// while it sums.  The k-th largest of those 512 maxima is no larger than the k-th largest logit, so only the threads whose maximum
-// reaches it can hold one of the top k: about k of 512.  Their vectors are read again, from L2, by all threads, and what reaches the
-// bound is a candidate (on random rows little more than k).  A candidate's place is the number of candidates before it.  The
+// while it sums, and of each of up to SEGMENTS ranges of them.  The k-th largest of the threads' maxima is no larger than the k-th
+// largest logit, so only ranges whose maximum reaches it can hold one of the top k: about k of some thousand.  Their vectors are
+// read again, from L2, by all threads, and what reaches the bound is a candidate (on random rows little more than k).  A candidate's place is the number of candidates before it.  The
 // buffer overflows where very many logits are equal or one thread's vectors hold most of the large ones: the bound is then
 // raised to the k-th largest of those buffered and the reading repeated, and where that is the bound itself, the logits above it
 // are collected and the places left are filled with equal ones in the order of their columns.  The CTAs of a cluster select
@@ -16,7 +16,7 @@
 
 namespace nmg {
 
-constexpr int TOP_MAX = 128;
+constexpr int TOP_MAX = 128, SEGMENTS = 8;
 template <int NT> constexpr int CANDIDATES = 2 * NT;
 
 struct TokenParams {
@@ -56,8 +56,9 @@ __device__ __forceinline__ int candidate_col(uint64_t c) { return (int)(0xffffff
 
 template <int NT> struct TopShared {
     uint64_t cand[CANDIDATES<NT>], top[TOP_MAX];
+    float seg[SEGMENTS][NT];  // largest logit of each range of a thread's steps
     uint32_t keys[NT];
-    uint16_t hot[NT];
+    uint16_t hot[SEGMENTS * NT];
     int scan[NT / 32];
     uint32_t bound;
     int n_cand, n_hot;
@@ -86,8 +87,9 @@ template <int NT> __device__ __forceinline__ int block_scan(int n, int *warps, i
     return before + inc - n;
 }
 
-// sh.top[0 .. k): the slice's top k, sorted; 0 past its end.  `best`: the largest logit of this thread's vectors, NaN where one is.
-template <typename T, int NT> __device__ void select_top(const Slice<T> &sl, int k, float best, TopShared<NT> &sh) {
+// sh.top[0 .. k): the slice's top k, sorted; 0 past its end.  `best`: the largest logit of this thread's vectors, NaN where one is; it has
+// `segs` ranges of 2^shift steps.
+template <typename T, int NT> __device__ void select_top(const Slice<T> &sl, int k, float best, int segs, int shift, TopShared<NT> &sh) {
     const int tid = (int)threadIdx.x, lane = tid & 31;
     const uint32_t key = sl.v0 + tid < sl.v1 ? order_key(best) : 0u;
     sh.keys[tid] = key;
@@ -119,11 +121,14 @@ template <typename T, int NT> __device__ void select_top(const Slice<T> &sl, int
         if (at < CANDIDATES<NT>) sh.cand[at] = candidate(q, col);
     };
     for (;;) {
-        if (wanted(key) && key) sh.hot[atomicAdd(&sh.n_hot, 1)] = (uint16_t)tid;
+        if (key && wanted(key))
+            for (int g = 0; g < segs; g++)
+                if (key == 0xffffffffu || wanted(order_key(sh.seg[g][tid]))) sh.hot[atomicAdd(&sh.n_hot, 1)] = (uint16_t)(g * NT + tid);
         __syncthreads();
-        const int n_hot = sh.n_hot, items = n_hot * rounds;
+        static_assert(1 << STEP_BITS == STEP && SEGMENTS * NT <= 65536, "");
+        const int per = shift + STEP_BITS, items = sh.n_hot << per;
         for (int i = tid; i < items; i += NT) {
-            const int v = sl.v0 + sh.hot[i % n_hot] + i / n_hot * NT;
+            const int hot = sh.hot[i >> per], v = sl.v0 + hot % NT + ((hot / NT << per) + (i & ((1 << per) - 1))) * NT;
             if (v >= sl.v1) continue;
             float x[VEC<T>];
             unpack<T>(sl.vec(v), x);
@@ -218,7 +223,7 @@ template <typename T, int NT, bool TOP> __global__ void __launch_bounds__(NT, SM
     TopShared<NT> &sh = *reinterpret_cast<TopShared<NT> *>(smem + RING_BYTES<NT>);
     const int tid = (int)threadIdx.x, rank = p.parts > 1 ? cluster_rank() : 0;
     const unsigned first = blockIdx.x / (unsigned)p.parts, step = gridDim.x / (unsigned)p.parts;
-    const float a = LOG2E * p.inv_tau, slack = 8.f * p.tau;
+    const float a = LOG2E * p.inv_tau;
     Stream<T, NT, 1> stream(p.x, smem, nullptr, first, step, rank, p.parts);
     for (unsigned r = first, turn = 0; r < p.x.rows; r += step, turn ^= 1) {
         const Slice<T> sl(static_cast<const T *>(p.x.x) + p.x.offset(r), p.x.vocab, rank, p.parts);
@@ -232,12 +237,28 @@ template <typename T, int NT, bool TOP> __global__ void __launch_bounds__(NT, SM
         }
         Stats st = Stats::none();
         float best = neg_inf();
+        int steps = 0, shift = 0;
+        float segment = neg_inf();
+        if constexpr (TOP)
+            while (((sl.v1 - sl.v0 + STEP * NT - 1) / (STEP * NT) - 1) >> shift >= SEGMENTS) shift++;
         stream.pass(sl, [&](const uint4 *q, int, int) {
-            const float top = group_pick<T, true, STEP>(q);
-            if constexpr (TOP) best = fmaxf(best, top);
-            st.add<T, STEP, true>(q, a, slack, top);
+            if constexpr (TOP) {
+                segment = fmaxf(segment, group_pick_max<T>(q));
+                if ((++steps & ((1 << shift) - 1)) == 0) {
+                    sh.seg[(steps - 1) >> shift][tid] = segment;
+                    best = fmaxf(best, segment);
+                    segment = neg_inf();
+                }
+            }
+            st.add<T, true>(q, a);
         });
         if constexpr (TOP) {
+            const int open = steps & ((1 << shift) - 1);
+            if (open) {
+                sh.seg[steps >> shift][tid] = segment;
+                best = fmaxf(best, segment);
+                steps += (1 << shift) - open;
+            }
             if (st.s != st.s)  // NaN, or +inf: only the first has to be found
                 for (int v = sl.v0 + tid; v < sl.v1; v += NT) {
                     float x[VEC<T>];
@@ -246,12 +267,12 @@ template <typename T, int NT, bool TOP> __global__ void __launch_bounds__(NT, SM
                     for (int u = 0; u < VEC<T>; u++) best = x[u] != x[u] ? x[u] : best;
                 }
         }
-        if (col >= 0) st.add_one<true>(single, a, slack);
+        if (col >= 0) st.add_one<true>(single, a);
         leave_stats<NT>(st, a, red[turn]);
         __syncthreads();
         if (!TOP && tid >= 32 && p.parts == 1) continue;  // the first warp finishes the row
         st = block_stats<NT>(red[turn], a);
-        if constexpr (TOP) select_top<T, NT>(sl, p.top, best, sh);
+        if constexpr (TOP) select_top<T, NT>(sl, p.top, best, steps >> shift, shift, sh);
         if (p.parts > 1) {
             if (tid == 0) part = st;
             cluster_barrier_arrive();

@@ -5,9 +5,10 @@
 // and a tail.  The CTAs of a cluster share a row: each takes a contiguous range of the vectors, the first the lead and the last
 // the tail (fewer than 16 elements together, one thread each).
 //
-// Statistics of a set of logits x at temperature tau, a = log2(e) / tau:  m >= max x - 8 tau,  s = sum 2^((x - m) a),
-// w = sum 2^((x - m) a) (x - m), all in 32 bits.  m follows the running maximum only once that is 8 tau above it: s then holds terms up to
-// e^8, which costs no precision, and the rescaling leaves the inner loop.  From them
+// Statistics of a set of logits x at temperature tau, a = log2(e) / tau:  s = sum 2^((x - m) a),  w = sum 2^((x - m) a) (x - m), all
+// in 32 bits.  m is a reference that the maximum may exceed: it begins as the maximum of the thread's first vectors and is raised
+// to that of later ones only when their sum shows terms of some hundred, which costs s no precision and w some 6 units in the last
+// place of ln s.  So neither the maximum nor the rescaling is part of the inner loop.  From them
 //   log-sum-exp of x / tau = m / tau + ln s,    entropy = ln s - (w / tau) / s.
 // A set that holds nothing but -inf has m = -inf and s = 0; NaN and +inf make s NaN.
 #pragma once
@@ -110,26 +111,25 @@ template <typename T> struct Slice {
     __device__ __forceinline__ float at(int col) const { return DT<T>::to_f32(row[col]); }
 };
 
-// Largest and smallest of a group of vectors, NaN left aside; 16-bit logits are compared two at a time as they are.
-template <typename T, bool MAX> __device__ __forceinline__ uint32_t pick2(uint32_t a, uint32_t b) {
+// Largest of four vectors, NaN left aside; 16-bit logits are compared two at a time as they are.
+template <typename T> __device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b) {
     if constexpr (sizeof(T) == 4) {
-        const float x = __uint_as_float(a), y = __uint_as_float(b);
-        return __float_as_uint(MAX ? fmaxf(x, y) : fminf(x, y));
+        return __float_as_uint(fmaxf(__uint_as_float(a), __uint_as_float(b)));
     } else {
         using T2 = std::conditional_t<DT<T>::id == NMG_BF16, __nv_bfloat162, __half2>;
-        const T2 x = *reinterpret_cast<const T2 *>(&a), y = *reinterpret_cast<const T2 *>(&b), r = MAX ? __hmax2(x, y) : __hmin2(x, y);
+        const T2 r = __hmax2(*reinterpret_cast<const T2 *>(&a), *reinterpret_cast<const T2 *>(&b));
         return *reinterpret_cast<const uint32_t *>(&r);
     }
 }
-template <typename T, bool MAX, int U> __device__ __forceinline__ float group_pick(const uint4 *q) {
-    uint32_t r = pick2<T, MAX>(pick2<T, MAX>(q[0].x, q[0].y), pick2<T, MAX>(q[0].z, q[0].w));
+template <typename T> __device__ __forceinline__ float group_pick_max(const uint4 *q) {
+    uint32_t r = max2<T>(max2<T>(q[0].x, q[0].y), max2<T>(q[0].z, q[0].w));
 #pragma unroll
-    for (int u = 1; u < U; u++) r = pick2<T, MAX>(r, pick2<T, MAX>(pick2<T, MAX>(q[u].x, q[u].y), pick2<T, MAX>(q[u].z, q[u].w)));
+    for (int u = 1; u < 4; u++) r = max2<T>(r, max2<T>(max2<T>(q[u].x, q[u].y), max2<T>(q[u].z, q[u].w)));
     if constexpr (sizeof(T) == 4) return __uint_as_float(r);
-    else if constexpr (DT<T>::id == NMG_BF16) return MAX ? fmaxf(__uint_as_float(r << 16), __uint_as_float(r & 0xffff0000u)) : fminf(__uint_as_float(r << 16), __uint_as_float(r & 0xffff0000u));
+    else if constexpr (DT<T>::id == NMG_BF16) return fmaxf(__uint_as_float(r << 16), __uint_as_float(r & 0xffff0000u));
     else {
         const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&r));
-        return MAX ? fmaxf(f.x, f.y) : fminf(f.x, f.y);
+        return fmaxf(f.x, f.y);
     }
 }
 __device__ __forceinline__ float warp_pick_max(float v) {  // NaN left aside
@@ -143,24 +143,13 @@ struct Stats {
     float m, s, w;
     static __device__ __forceinline__ Stats none() { return Stats{neg_inf(), 0.f, 0.f}; }
 
-    // the reference follows a maximum of `top`
-    template <bool W> __device__ __forceinline__ void raise(float top, float a, float slack) {
-        if (top > m + slack) {
-            const float d = m - top, f = exp2_fast(d * a);
-            if constexpr (W) w = f == 0.f ? 0.f : f * (w + d * s);  // d * s may be -inf
-            s *= f;
-            m = top;
-        }
-    }
-    // U vectors of logits of which `top` is the largest; W: the entropy is wanted.  Two logits an instruction (f32x2).
-    template <typename T, int U, bool W> __device__ __forceinline__ void add(const uint4 *q, float a, float slack, float top) {
-        raise<W>(top, a, slack);
+    // Four vectors of logits; W: the entropy is wanted.  Two logits an instruction (f32x2).
+    template <typename T, bool W> __device__ __forceinline__ void add(const uint4 *q, float a) {
+        if (m == neg_inf()) m = group_pick_max<T>(q);
         const float ref = m == neg_inf() ? 0.f : m;
         float2 ps = both(0.f), pw = both(0.f);
-        // masked logits have e = 0 and d = -inf, whose product is not a part of the sum: groups that hold some take the longer way
-        const bool plain = !W || (group_pick<T, false, U>(q) > -1e30f && ref < 1e30f);
 #pragma unroll
-        for (int u = 0; u < U; u++) {
+        for (int u = 0; u < 4; u++) {
             float x[VEC<T>];
             unpack<T>(q[u], x);
 #pragma unroll
@@ -168,32 +157,47 @@ struct Stats {
                 const float2 d = __fadd2_rn(make_float2(x[i], x[i + 1]), both(-ref)), t = __fmul2_rn(d, both(a));
                 const float2 e = make_float2(exp2_fast(t.x), exp2_fast(t.y));
                 ps = __fadd2_rn(ps, e);
-                if constexpr (W)
-                    if (plain) pw = __ffma2_rn(e, d, pw);
+                if constexpr (W) pw = __ffma2_rn(e, d, pw);
             }
         }
-        if (W && !plain) {
-#pragma unroll
-            for (int u = 0; u < U; u++) {
-                float x[VEC<T>];
-                unpack<T>(q[u], x);
-#pragma unroll
-                for (int i = 0; i < VEC<T>; i++) {
-                    const float d = x[i] - ref;
-                    pw.x += exp2_fast(d * a) * fmaxf(d, -1e30f);
-                }
-            }
+        ps.x += ps.y;
+        pw.x += pw.y;
+        // the reference is too low; or masked logits: they have e = 0 and d = -inf, whose product is not a part of the sum; or a NaN
+        if (ps.x > 128.f * VEC<T> || (W && pw.x != pw.x)) {
+            *this = with_care<T>(*this, q[0], q[1], q[2], q[3], a);
+        } else {
+            s += ps.x;
+            if constexpr (W) w += pw.x;
         }
-        s += ps.x + ps.y;
-        if constexpr (W) w += pw.x + pw.y;
     }
-    template <bool W> __device__ __forceinline__ void add_one(float x, float a, float slack) {
-        raise<W>(x, a, slack);
+    template <typename T> static __device__ __noinline__ Stats with_care(Stats st, uint4 q0, uint4 q1, uint4 q2, uint4 q3, float a) {
+        const uint4 q[4] = {q0, q1, q2, q3};
+        const float top = group_pick_max<T>(q);
+        if (top > st.m) st.rebase(top, a);
+        const float ref = st.m == neg_inf() ? 0.f : st.m;
+        float ps = 0.f, pw = 0.f;
+#pragma unroll
+        for (int u = 0; u < 4; u++) {
+            float x[VEC<T>];
+            unpack<T>(q[u], x);
+#pragma unroll
+            for (int i = 0; i < VEC<T>; i++) {
+                const float d = x[i] - ref, e = exp2_fast(d * a);
+                ps += e;
+                pw += e * fmaxf(d, -1e30f);
+            }
+        }
+        st.s += ps;
+        st.w += pw;
+        return st;
+    }
+    template <bool W> __device__ __forceinline__ void add_one(float x, float a) {
+        if (x > m) rebase(x, a);
         const float d = x - (m == neg_inf() ? 0.f : m), e = exp2_fast(d * a);
         s += e;
         if constexpr (W) w += e * fmaxf(d, -1e30f);
     }
-    // relative to `top`, which is no smaller than any of the set
+    // relative to `top`; d * s may be -inf
     __device__ __forceinline__ void rebase(float top, float a) {
         const float d = m - (top == neg_inf() ? 0.f : top), f = exp2_fast(d * a);
         w = f == 0.f ? 0.f : f * (w + d * s);
@@ -269,7 +273,7 @@ __device__ __forceinline__ Stats peer_stats(const Stats *mine, int rank) {
 // The vectors of one row after another on their way from global memory.  Every thread copies its own vectors (v0 + thread + i * VT)
 // asynchronously into slots of its own in shared memory and keeps DEPTH steps of STEP vectors under way, across the ends of rows and of
 // passes: while a CTA finishes a row, the next rows' logits arrive.  No thread waits for another's copies.
-constexpr int STEP = 4, DEPTH = 2;
+constexpr int STEP = 4, STEP_BITS = 2, DEPTH = 2;
 template <int NT> constexpr int RING_BYTES = STEP * DEPTH * NT * 16;  // 128 KB of an SM
 
 template <typename T, int NT, int PASSES> struct Stream {
@@ -279,64 +283,77 @@ template <typename T, int NT, int PASSES> struct Stream {
     unsigned row, row_step;
     int part, parts;
     // what is copied next
-    const uint4 *from;
-    int left, passes, length;  // vectors of this pass, from this thread's on; passes behind this one; vectors of a pass
+    const uint4 *from, *begin;
+    int left, length, passes;  // vectors of this pass, from this thread's on; of every pass of the row; passes behind this one
     float next_weight;
     int put, get;  // slots
 
     __device__ __forceinline__ Stream(const Logits &x_, void *smem, const float *weight_, unsigned first, unsigned step, int part_, int parts_)
-        : x(x_), ring(static_cast<uint4 *>(smem) + threadIdx.x), weight(weight_), row(first), row_step(step), part(part_), parts(parts_), from(nullptr), left(0), passes(0), length(0), put(0), get(0) {
+        : x(x_), ring(static_cast<uint4 *>(smem) + threadIdx.x), weight(weight_), row(first), row_step(step), part(part_), parts(parts_), from(nullptr), begin(nullptr), left(0), length(0), passes(0), put(0), get(0) {
         next_weight = weight && row < x.rows ? weight[row] : 1.f;
         row -= row_step;
         for (int i = 0; i < DEPTH; i++) issue();
     }
-    __device__ __forceinline__ void issue() {
-        while (left <= 0) {
-            if (passes > 0) {
-                passes--;
-                left = length;
-                if (left <= 0) passes = 0;
-            } else {
+    __device__ __forceinline__ bool next_pass() {
+        if (passes > 0 && length > 0) {
+            passes--;
+        } else {
+            for (;;) {
+                if (row + row_step >= x.rows && row + row_step >= row_step) return false;  // no row left (the sum wraps before the first one)
                 row += row_step;
-                if (row >= x.rows) {
-                    row -= row_step;  // stays past the end
-                    break;
-                }
                 const float w = next_weight;
                 if (weight) next_weight = row + row_step < x.rows ? weight[row + row_step] : 1.f;
                 if (w == 0.f) continue;
                 const Slice<T> sl(static_cast<const T *>(x.x) + x.offset(row), x.vocab, part, parts);
-                from = reinterpret_cast<const uint4 *>(sl.row + sl.lead) + sl.v0 + threadIdx.x;
-                left = length = sl.v1 - sl.v0 - (int)threadIdx.x;
+                length = sl.v1 - sl.v0 - (int)threadIdx.x;
+                if (length <= 0) continue;
+                begin = reinterpret_cast<const uint4 *>(sl.row + sl.lead) + sl.v0 + threadIdx.x;
                 passes = PASSES - 1;
+                break;
             }
         }
-        if (left > 0) {
-            const uint4 *src = from + (length - left);
+        from = begin;
+        left = length;
+        return true;
+    }
+    __device__ __forceinline__ void issue() {
+        uint4 *to = ring + put * NT;
+        if (left > (STEP - 1) * NT || (left <= 0 && next_pass() && left > (STEP - 1) * NT)) {
+#pragma unroll
+            for (int u = 0; u < STEP; u++) cp_async_16(to + u * NT, from + u * NT);
+        } else {
 #pragma unroll
             for (int u = 0; u < STEP; u++)
-                if (left > u * NT) cp_async_16(ring + (put + u) * NT, src + u * NT);
-            left -= STEP * NT;
+                if (left > u * NT) cp_async_16(to + u * NT, from + u * NT);
         }
         cp_async_commit();
+        from += STEP * NT;
+        left -= STEP * NT;
         put = put + STEP == STEP * DEPTH ? 0 : put + STEP;
     }
     // f(vectors, number of the first, how many there are) over one pass of a row; the missing ones of the last step are -inf
     template <typename F> __device__ __forceinline__ void pass(const Slice<T> &sl, F f) {
-        for (int v = sl.v0 + (int)threadIdx.x; v < sl.v1; v += STEP * NT) {
+        int v = sl.v0 + (int)threadIdx.x;
+        uint4 q[STEP];
+        for (; v + (STEP - 1) * NT < sl.v1; v += STEP * NT) {
             cp_async_wait<DEPTH - 1>();
-            uint4 q[STEP];
-            int n = 0;
+#pragma unroll
+            for (int u = 0; u < STEP; u++) q[u] = ring[(get + u) * NT];
+            get = get + STEP == STEP * DEPTH ? 0 : get + STEP;
+            f(q, v, STEP);
+            issue();  // into the slots just read
+        }
+        if (v < sl.v1) {
+            cp_async_wait<DEPTH - 1>();
+            const int n = (sl.v1 - v + NT - 1) / NT;
 #pragma unroll
             for (int u = 0; u < STEP; u++) {
                 const uint32_t none = neg_inf_word<T>();
-                const bool there = v + u * NT < sl.v1;
-                q[u] = there ? ring[(get + u) * NT] : make_uint4(none, none, none, none);
-                n += there;
+                q[u] = u < n ? ring[(get + u) * NT] : make_uint4(none, none, none, none);
             }
             get = get + STEP == STEP * DEPTH ? 0 : get + STEP;
             f(q, v, n);
-            issue();  // into the slots just read
+            issue();
         }
     }
 };
