@@ -42,10 +42,10 @@ struct DistillParams {
 
 struct KeptShared {
     float q[KEPT_MAX], logq[KEPT_MAX], x[KEPT_MAX];
-    int id[KEPT_MAX];      // -1: padding
-    uint8_t first[KEPT_MAX];
+    int id[KEPT_MAX];  // -1: padding
+    uint8_t later[KEPT_MAX];  // where an id is there twice: this is not its first entry
     float mass, rest, max_x, sum_x;  // S, q_0, and the statistics of the kept logits
-    int some, twice;
+    int some;
 };
 
 __device__ __forceinline__ float teacher_value(const void *p, int dtype, int64_t i) {
@@ -73,35 +73,44 @@ template <typename T> __device__ __forceinline__ uint4 leave_out(uint4 q, uint32
 template <typename T, int NT, bool REST, bool STATS, bool GRAD> __global__ void __launch_bounds__(NT, SM_THREADS / NT) distill_kernel(const __grid_constant__ DistillParams p) {
     extern __shared__ __align__(16) unsigned char smem[];
     __shared__ Stats red[NT / 32], part;
-    __shared__ KeptShared sh;
+    __shared__ KeptShared kept_rows[2];  // of this row and of the one before
+    __shared__ int twice_rows[2];
     uint32_t *bits = reinterpret_cast<uint32_t *>(smem + RING_BYTES<NT>);
+    __shared__ uint32_t steps_marked[NT];  // bit s: a kept token is among step s (modulo 32) of the thread's vectors
     const int tid = (int)threadIdx.x, lane = tid & 31, warp = tid >> 5, rank = (int)(blockIdx.x % (unsigned)p.parts);
     const unsigned first = blockIdx.x / (unsigned)p.parts, step = gridDim.x / (unsigned)p.parts;
     if (GRAD && !STATS && p.skip_if_one && *p.upstream == 1.f) return;  // the gradient that is there already is this one
     Stream<T, NT, STATS && GRAD ? 2 : 1> stream(p.x, smem, p.weight, first, step, rank, p.parts);
     for (int i = tid; i < (REST ? (p.x.vocab + BIT0 + 31) / 32 : FILTER_BITS / 32); i += NT) bits[i] = 0u;
+    steps_marked[tid] = 0u;
+    if (tid < 2) twice_rows[tid] = 0;
     const float a = LOG2E * p.inv_tau, total = p.total ? *p.total : p.divisor;
 
-    // the kept tokens of a row are fetched while the row before is worked on
+    // the kept tokens of a row and their logits are fetched while the row before is worked on
     int64_t next_id = -1;
-    float next_logq = neg_inf();
+    float next_logq = neg_inf(), next_x = neg_inf();
     auto fetch = [&](unsigned r) {
         if (tid >= p.kept || r >= p.x.rows) return;
         const int64_t i = (int64_t)r * p.kept + tid;
         next_id = p.id_bytes == 8 ? static_cast<const int64_t *>(p.ids)[i] : static_cast<const int *>(p.ids)[i];
         next_logq = teacher_value(p.log_probs, p.teacher_dtype, i);
     };
+    auto fetch_x = [&](unsigned r) {
+        if (tid < p.kept && r < p.x.rows && next_id >= 0 && next_id < p.x.vocab) next_x = DT<T>::to_f32(static_cast<const T *>(p.x.x)[p.x.offset(r) + next_id]);
+    };
     fetch(first);
+    fetch_x(first);
     float weight = p.weight ? p.weight[first] : 1.f;
-    for (unsigned r = first; r < p.x.rows; r += step) {
+    __syncthreads();
+    for (unsigned r = first, turn = 0; r < p.x.rows; r += step) {
         const Slice<T> sl(static_cast<const T *>(p.x.x) + p.x.offset(r), p.x.vocab, rank, p.parts);
         T *dx = GRAD ? static_cast<T *>(p.dx) + p.x.offset(r, p.ld_dx, p.ld_dx_outer) : nullptr;
-        const float w = weight;
+        const float w = weight, logq = next_logq, kept_x = next_x;
         const int64_t raw = next_id;
-        const float logq = next_logq;
         if (p.weight && r + step < p.x.rows) weight = p.weight[r + step];
+        fetch(r + step);
         if (w == 0.f) {  // whatever its logits are, they are not read
-            fetch(r + step);
+            fetch_x(r + step);
             if constexpr (GRAD) zero_pass<NT>(sl, dx);
             if (STATS && rank == 0 && tid == 0) {
                 p.loss[r] = 0.f;
@@ -109,41 +118,42 @@ template <typename T, int NT, bool REST, bool STATS, bool GRAD> __global__ void 
             }
             continue;
         }
-        const int col = sl.single(tid);
+        KeptShared &sh = kept_rows[turn];
+        int &twice = twice_rows[turn];
+        turn ^= 1;
+        const int col = tid < 32 ? sl.single(tid) : -1;
         const float single = STATS && col >= 0 ? sl.at(col) : 0.f;
         auto bit_of = [&](int c) { return REST ? c - sl.lead + BIT0 : c & (FILTER_BITS - 1); };
         const bool none_such = tid < p.kept && raw >= p.x.vocab;
         const int id = tid >= p.kept || raw < 0 || none_such ? -1 : (int)raw;
-        __syncthreads();  // the row before is done with what is written now
         if (tid < p.kept) {
             sh.id[tid] = id;
             sh.logq[tid] = id < 0 ? neg_inf() : logq;
-            sh.x[tid] = id < 0 ? neg_inf() : sl.at(id);
-            sh.first[tid] = 0;
+            sh.x[tid] = id < 0 ? neg_inf() : kept_x;
+            sh.later[tid] = 0;
         }
-        if (tid == 0) sh.twice = 0;
-        fetch(r + step);
-        const bool bad = __syncthreads_or(none_such);
+        if (!GRAD) __syncthreads();  // the marks of the row before have been taken away (with GRAD: before its last entries)
         if (id >= 0) {
             const uint32_t bit = 1u << (bit_of(id) & 31);
-            if (atomicOr(&bits[bit_of(id) >> 5], bit) & bit) sh.twice = 1;  // without remainder: perhaps
-        }
-        __syncthreads();
-        if (sh.twice) {  // an id that is there more than once counts as one token with the sum of its q
-            if (id >= 0) {
-                bool earliest = true;
-                for (int i = 0; i < tid; i++) earliest = earliest && sh.id[i] != id;
-                sh.first[tid] = earliest;
+            if (atomicOr(&bits[bit_of(id) >> 5], bit) & bit) twice = 1;  // without remainder: perhaps
+            if (REST && STATS && id >= sl.lead && id < sl.tail_at) {
+                const int v = (id - sl.lead) / VEC<T> - sl.v0;
+                if (v >= 0) atomicOr(&steps_marked[v % NT], 1u << (v / (NT * STEP) & 31));
             }
-        } else if (id >= 0) {
-            sh.first[tid] = 1;
         }
-        __syncthreads();
+        const bool bad = __syncthreads_or(none_such);
+        if (twice) {  // an id that is there more than once counts as one token with the sum of its q
+            if (id >= 0)
+                for (int i = 0; i < tid; i++)
+                    if (sh.id[i] == id) sh.later[tid] = 1;
+            __syncthreads();
+        }
+        if (tid == 0) twice_rows[turn] = 0;  // of the next row
         if (warp == 0) {
             float top = neg_inf(), sum = 0.f, max_x = neg_inf(), sum_x = 0.f;
             for (int i = lane; i < p.kept; i += 32) {
                 top = fmaxf(top, sh.logq[i]);
-                if (sh.first[i]) max_x = fmaxf(max_x, sh.x[i]);
+                if (!sh.later[i]) max_x = fmaxf(max_x, sh.x[i]);
             }
             top = REST ? 0.f : warp_pick_max(top);
             max_x = warp_pick_max(max_x);
@@ -152,7 +162,7 @@ template <typename T, int NT, bool REST, bool STATS, bool GRAD> __global__ void 
                 const float q = expf(sh.logq[i] - ref);
                 sh.q[i] = q;
                 sum += q;
-                if (sh.first[i]) sum_x += exp2_fast((sh.x[i] - ref_x) * a);
+                if (!sh.later[i]) sum_x += exp2_fast((sh.x[i] - ref_x) * a);
             }
             sum = warp_sum(sum);
             sum_x = warp_sum(sum_x);
@@ -177,8 +187,11 @@ template <typename T, int NT, bool REST, bool STATS, bool GRAD> __global__ void 
         if constexpr (STATS) {
             Stats st = Stats::none();
             auto marked = [&](int bit) { return bits[bit >> 5] >> (bit & 31); };
+            uint32_t mine = REST ? steps_marked[tid] : 0u;
             stream.pass(sl, [&](uint4 *q, int v, int n) {
-                if constexpr (REST) {
+                const bool look = REST && (mine & 1);
+                mine = __funnelshift_r(mine, mine, 1);
+                if (look) {
 #pragma unroll
                     for (int u = 0; u < STEP; u++)
                         if (const uint32_t out = u < n ? marked(BIT0 + (v + u * NT) * VEC<T>) & ((1u << VEC<T>) - 1) : 0u) q[u] = leave_out<T>(q[u], out);
@@ -206,6 +219,8 @@ template <typename T, int NT, bool REST, bool STATS, bool GRAD> __global__ void 
             rest = p.norm[2 * (int64_t)r + 1];
         }
         if (id >= 0) bits[bit_of(id) >> 5] = 0u;  // nobody reads them any more
+        if (REST && STATS) steps_marked[tid] = 0u;
+        fetch_x(r + step);
         const bool counts = sh.some && !all.empty();
         const float q0 = REST && !rest.empty() ? sh.rest : 0.f, mass = sh.mass + q0;
         const float log_p0 = fmaf(rest.m - all.m, p.inv_tau, rest.ln - all.ln);
@@ -234,11 +249,18 @@ template <typename T, int NT, bool REST, bool STATS, bool GRAD> __global__ void 
             const float m = of.empty() ? 0.f : of.m, ln2 = of.ln * LOG2E;
             const float others = scale * (REST ? (rest.empty() ? 0.f : mass * exp2_fast(log_p0 * LOG2E) - q0) : 1.f);
             const bool zero = !counts && !bad;
-            grad_pass<NT>(stream, sl, dx, [&](float x) { return zero ? 0.f : others * exp2_fast(fmaf(x - m, a, -ln2)); });
+            if (zero) {  // of a row that may hold anything
+                grad_pass<NT>(stream, sl, dx, [](float2) { return both(0.f); });
+            } else {
+                grad_pass<NT>(stream, sl, dx, [&](float2 x) {
+                    const float2 t = __ffma2_rn(__fadd2_rn(x, both(-m)), both(a), both(-ln2));
+                    return __fmul2_rn(make_float2(exp2_fast(t.x), exp2_fast(t.y)), both(others));
+                });
+            }
             __syncthreads();  // the entries below replace what other threads wrote
-            if (!zero && tid < p.kept && sh.first[tid] && sl.holds(id)) {
+            if (!zero && id >= 0 && !sh.later[tid] && sl.holds(id)) {
                 float q = sh.q[tid];
-                if (sh.twice)
+                if (twice)
                     for (int i = tid + 1; i < p.kept; i++) q += sh.id[i] == id ? sh.q[i] : 0.f;
                 dx[id] = DT<T>::from_f32(scale * ((REST ? mass : 1.f) * exp2_fast(all.log_prob(sh.x[tid], p.inv_tau) * LOG2E) - q));
             }

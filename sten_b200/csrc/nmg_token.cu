@@ -332,9 +332,14 @@ template <typename T, int NT, bool E> __global__ void __launch_bounds__(NT, SM_T
         const float m = empty ? 0.f : norm.m, ln = norm.ln, a = LOG2E * p.inv_tau, ln2 = ln * LOG2E;  // nothing but -inf: p = 0 below
         A *= p.inv_tau;
         B *= p.inv_tau;
-        auto grad = [&](float x) {
-            const float d = x - m, e = exp2_fast(fmaf(d, a, -ln2));
-            return E ? e * (A + B * fmaf(fmaxf(d, -1e30f), p.inv_tau, -ln)) : e * A;  // 0 * -inf is not a part of it
+        const float lin = A - B * ln;  // A + B log p = lin + B (x - m) / tau
+        B *= p.inv_tau;
+        auto grad = [&](float2 x) {
+            const float2 d = __fadd2_rn(x, both(-m)), t = __ffma2_rn(d, both(a), both(-ln2)), e = make_float2(exp2_fast(t.x), exp2_fast(t.y));
+            if constexpr (!E) return __fmul2_rn(e, both(A));
+            float2 y = __fmul2_rn(e, __ffma2_rn(d, both(B), both(lin)));
+            if (y.x != y.x || y.y != y.y) y = make_float2(e.x * (lin + B * fmaxf(d.x, -1e30f)), e.y * (lin + B * fmaxf(d.y, -1e30f)));  // masked: 0 * -inf is not a part of it
+            return y;
         };
         grad_pass<NT>(stream, sl, dx, grad);
         __syncthreads();  // the entries below replace what other threads wrote
@@ -342,14 +347,14 @@ template <typename T, int NT, bool E> __global__ void __launch_bounds__(NT, SM_T
         if (tid < p.top && p.g_top) {
             const int64_t id = p.top_ids[at + tid];
             if (id >= 0 && id < p.x.vocab && !(in_row && id == target) && sl.holds((int)id))
-                dx[id] = DT<T>::from_f32(grad(sl.at((int)id)) + p.g_top[at + tid] * p.inv_tau);
+                dx[id] = DT<T>::from_f32(grad(both(sl.at((int)id))).x + p.g_top[at + tid] * p.inv_tau);
         }
         if (tid == NT - 1 && in_row && sl.holds((int)target)) {
             float g = g_lp;
             if (p.g_top)
                 for (int i = 0; i < p.top; i++)
                     if (p.top_ids[at + i] == target) g += p.g_top[at + i];
-            dx[target] = DT<T>::from_f32(grad(sl.at((int)target)) + g * p.inv_tau);
+            dx[target] = DT<T>::from_f32(grad(both(sl.at((int)target))).x + g * p.inv_tau);
         }
     }
 }

@@ -358,28 +358,32 @@ template <typename T, int NT, int PASSES> struct Stream {
     }
 };
 
-// out[column] = f(logit) over the slice, a pass of the stream.  `out` is where the row's gradient begins; vectors are stored whole where its
-// 16-byte boundaries are those of the logits.
+// out[column] = f(logit) over the slice, a pass of the stream; f takes two logits at a time.  `out` is where the row's gradient begins;
+// vectors are stored whole where its 16-byte boundaries are those of the logits.
 template <int NT, typename T, typename S, typename F> __device__ __forceinline__ void grad_pass(S &stream, const Slice<T> &sl, T *out, F f) {
     const bool whole = (reinterpret_cast<uintptr_t>(out + sl.lead) & 15) == 0;
     stream.pass(sl, [&](const uint4 *q, int v, int n) {
+        T *dst = out + sl.lead + (int64_t)v * VEC<T>;
 #pragma unroll
         for (int u = 0; u < STEP; u++) {
             if (u >= n) break;
             float x[VEC<T>];
             unpack<T>(q[u], x);
 #pragma unroll
-            for (int i = 0; i < VEC<T>; i++) x[i] = f(x[i]);
-            T *dst = out + sl.lead + (int64_t)(v + u * NT) * VEC<T>;
+            for (int i = 0; i < VEC<T>; i += 2) {
+                const float2 y = f(make_float2(x[i], x[i + 1]));
+                x[i] = y.x;
+                x[i + 1] = y.y;
+            }
             if (whole) {
-                __stcs(reinterpret_cast<uint4 *>(dst), pack<T>(x));
+                __stcs(reinterpret_cast<uint4 *>(dst + u * NT * VEC<T>), pack<T>(x));
             } else {
 #pragma unroll
-                for (int i = 0; i < VEC<T>; i++) dst[i] = DT<T>::from_f32(x[i]);
+                for (int i = 0; i < VEC<T>; i++) dst[u * NT * VEC<T> + i] = DT<T>::from_f32(x[i]);
             }
         }
     });
-    if (const int col = sl.single((int)threadIdx.x); col >= 0) out[col] = DT<T>::from_f32(f(sl.at(col)));
+    if (const int col = sl.single((int)threadIdx.x); col >= 0) out[col] = DT<T>::from_f32(f(both(sl.at(col))).x);
 }
 // the same for a row that is not read
 template <int NT, typename T> __device__ __forceinline__ void zero_pass(const Slice<T> &sl, T *out) {
