@@ -5,13 +5,14 @@
 //                             A = g_lse - g_log_prob - sum g_top - g_entropy H,  B = -g_entropy  (E: there is an entropy gradient)
 //
 // The top k of a row, ordered by value and among equal values by column: every thread keeps the largest logit of its vectors
-// while it sums, and of each of up to SEGMENTS ranges of them.  The k-th largest of the threads' maxima is no larger than the k-th
-// largest logit, so only ranges whose maximum reaches it can hold one of the top k: about k of some thousand.  Their vectors are
-// read again, from L2, by all threads, and what reaches the bound is a candidate (on random rows little more than k).  A candidate's place is the number of candidates before it.  The
-// buffer overflows where very many logits are equal or one thread's vectors hold most of the large ones: the bound is then
-// raised to the k-th largest of those buffered and the reading repeated, and where that is the bound itself, the logits above it
-// are collected and the places left are filled with equal ones in the order of their columns.  The CTAs of a cluster select
-// from their own slices and the first one merges their sorted lists.
+// while it sums, and of each of up to SEGMENTS ranges of them.  Every warp finds the j-th largest of its lanes' maxima, j = k / warps
+// rounded up; the smallest of these is no larger than k of the maxima, and so no larger than the k-th largest logit: a bound.
+// Only ranges whose maximum reaches it can hold one of the top k, some two per alternative; they are read again, from L2, by all
+// threads, and what reaches the bound is a candidate.  A candidate's place is the number of candidates before it.  The buffer overflows where
+// very many logits are equal or a few ranges hold most of the large ones: the bound is then raised to the k-th largest of those
+// buffered and the reading repeated, and where that is the bound itself, the logits above it are collected and the places left
+// are filled with equal ones in the order of their columns.  The CTAs of a cluster select from their own slices and the first one
+// merges their sorted lists.
 #include "nmg_vocab.cuh"
 
 namespace nmg {
@@ -54,14 +55,14 @@ __device__ __forceinline__ float key_value(uint32_t key) { return __uint_as_floa
 __device__ __forceinline__ uint64_t candidate(uint32_t key, int col) { return (uint64_t)key << 32 | (0xffffffffu - (uint32_t)col); }
 __device__ __forceinline__ int candidate_col(uint64_t c) { return (int)(0xffffffffu - (uint32_t)c); }
 
-template <int NT> struct TopShared {
-    uint64_t cand[CANDIDATES<NT>], top[TOP_MAX];
+template <int NT> struct __align__(16) TopShared {
+    uint64_t cand[CANDIDATES<NT>];
     float seg[SEGMENTS][NT];  // largest logit of each range of a thread's steps
-    uint32_t keys[NT];
     uint16_t hot[SEGMENTS * NT];
+    uint32_t bounds[2][NT / 32];
+    int n_hot[2], n_cand[2];  // of this row and of the one before
     int scan[NT / 32];
     uint32_t bound;
-    int n_cand, n_hot;
 };
 
 // exclusive prefix sum over the CTA and the total
@@ -87,59 +88,69 @@ template <int NT> __device__ __forceinline__ int block_scan(int n, int *warps, i
     return before + inc - n;
 }
 
-// sh.top[0 .. k): the slice's top k, sorted; 0 past its end.  `best`: the largest logit of this thread's vectors, NaN where one is; it has
-// `segs` ranges of 2^shift steps.
-template <typename T, int NT> __device__ void select_top(const Slice<T> &sl, int k, float best, int segs, int shift, TopShared<NT> &sh) {
-    const int tid = (int)threadIdx.x, lane = tid & 31;
-    const uint32_t key = sl.v0 + tid < sl.v1 ? order_key(best) : 0u;
-    sh.keys[tid] = key;
-    if (tid == 0) sh.n_cand = sh.n_hot = 0;
-    __syncthreads();
-    if (tid < 32) {
-        uint32_t mine[NT / 32];
-#pragma unroll
-        for (int i = 0; i < NT / 32; i++) mine[i] = sh.keys[lane + 32 * i];
-        // the low bits are left zero, which only lowers the bound: bf16 keys have 16 bits, those of fp16 19
-        constexpr int LAST = DT<T>::id == NMG_BF16 ? 16 : DT<T>::id == NMG_F16 ? 13 : 12;
-        uint32_t bound = 0;
-        for (int bit = 31; bit >= LAST; bit--) {
-            const uint32_t next = bound | 1u << bit;
-            int c = 0;
-#pragma unroll
-            for (int i = 0; i < NT / 32; i++) c += mine[i] >= next;
-            if (__reduce_add_sync(FULL, c) >= k) bound = next;
-        }
-        if (lane == 0) sh.bound = bound;
+// f(place, candidate) for each of the n candidates; GROUP threads count those before one
+template <int NT, typename F> __device__ __forceinline__ void rank_candidates(const uint64_t *cand, int n, F f) {
+    const int tid = (int)threadIdx.x;
+    int bits = 0;
+    while (bits < 5 && n << (bits + 1) <= NT) bits++;
+    const int group = 1 << bits, sub = tid & (group - 1);
+    for (int i = tid >> bits; i - (tid >> bits) < n; i += NT >> bits) {  // all lanes of a warp come round as often
+        const uint64_t c = i < n ? cand[i] : 0;
+        int place = 0;
+#pragma unroll 4
+        for (int j = sub; j < n; j += group) place += cand[j] > c;
+        for (int o = group >> 1; o; o >>= 1) place += __shfl_xor_sync(FULL, place, o);
+        if (i < n && sub == 0) f(place, c);
     }
-    __syncthreads();
-    uint32_t bound = sh.bound;
-    bool above = false;  // collect what is above the bound, not what is equal to it
-    const int rounds = (sl.v1 - sl.v0 + NT - 1) / NT, held = sl.count(), want = k < held ? k : held;
+}
+
+// This warp's bound: the j-th largest of its lanes' keys (0 where a lane has no vectors)
+__device__ __forceinline__ uint32_t warp_bound(uint32_t key, int j) {
+    uint32_t bound = 0;
+    for (int i = 0; i < j; i++) {
+        bound = __reduce_max_sync(FULL, key);
+        const unsigned who = __ballot_sync(FULL, key == bound);
+        if ((int)(threadIdx.x & 31) == __ffs(who) - 1) key = 0u;
+    }
+    return bound;
+}
+
+// Candidates of the slice: every logit whose key reaches the bound (is above it, with `above`).  `key`: of the largest of this thread's
+// vectors, which are `segs` ranges of 2^shift steps.  `held`: the slice's vectors in shared memory, or NULL where they are not all there any
+// more.  `single`: this thread's logit outside the vectors.  n_hot and n_cand are 0 when the CTA comes here; n_cand is to be read after a
+// __syncthreads.
+template <typename T, int NT> __device__ __forceinline__ void collect(const Slice<T> &sl, const uint4 *held, uint32_t key, float single, int segs, int shift, uint32_t bound, bool above, TopShared<NT> &sh, int &n_hot, int &n_cand) {
+    const int tid = (int)threadIdx.x;
     auto wanted = [&](uint32_t q) { return above ? q > bound : q >= bound; };
     auto push = [&](uint32_t q, int col) {
-        const int at = atomicAdd(&sh.n_cand, 1);
+        const int at = atomicAdd(&n_cand, 1);
         if (at < CANDIDATES<NT>) sh.cand[at] = candidate(q, col);
     };
-    for (;;) {
-        if (key && wanted(key))
-            for (int g = 0; g < segs; g++)
-                if (key == 0xffffffffu || wanted(order_key(sh.seg[g][tid]))) sh.hot[atomicAdd(&sh.n_hot, 1)] = (uint16_t)(g * NT + tid);
-        __syncthreads();
-        static_assert(1 << STEP_BITS == STEP && SEGMENTS * NT <= 65536, "");
-        const int per = shift + STEP_BITS, items = sh.n_hot << per;
-        for (int i = tid; i < items; i += NT) {
-            const int hot = sh.hot[i >> per], v = sl.v0 + hot % NT + ((hot / NT << per) + (i & ((1 << per) - 1))) * NT;
-            if (v >= sl.v1) continue;
-            float x[VEC<T>];
-            unpack<T>(sl.vec(v), x);
+    if (key && wanted(key))
+        for (int g = 0; g < segs; g++)
+            if (key == 0xffffffffu || wanted(order_key(sh.seg[g][tid]))) sh.hot[atomicAdd(&n_hot, 1)] = (uint16_t)(g * NT + tid);
+    __syncthreads();
+    static_assert(1 << STEP_BITS == STEP && SEGMENTS * NT <= 65536, "");
+    const int per = shift + STEP_BITS, items = n_hot << per;
+    for (int i = tid; i < items; i += NT) {
+        const int hot = sh.hot[i >> per], v = sl.v0 + hot % NT + ((hot / NT << per) + (i & ((1 << per) - 1))) * NT;
+        if (v >= sl.v1) continue;
+        float x[VEC<T>];
+        unpack<T>(held ? held[v - sl.v0] : sl.vec(v), x);
 #pragma unroll
-            for (int u = 0; u < VEC<T>; u++)
-                if (const uint32_t q = order_key(x[u]); wanted(q)) push(q, sl.lead + v * VEC<T> + u);
-        }
+        for (int u = 0; u < VEC<T>; u++)
+            if (const uint32_t q = order_key(x[u]); wanted(q)) push(q, sl.lead + v * VEC<T> + u);
+    }
+    if (tid < 32)
         if (const int col = sl.single(tid); col >= 0)
-            if (const uint32_t q = order_key(sl.at(col)); wanted(q)) push(q, col);
-        __syncthreads();
-        if (sh.n_cand <= CANDIDATES<NT>) break;
+            if (const uint32_t q = order_key(single); wanted(q)) push(q, col);
+}
+
+// The longer way of select_top: raises the bound until the candidates fit.  Returns how many there are, all in sh.cand.
+template <typename T, int NT> __device__ __noinline__ int select_again(const Slice<T> &sl, int k, uint32_t key, float single, int segs, int shift, uint32_t bound, TopShared<NT> &sh, int &n_hot, int &n_cand) {
+    const int tid = (int)threadIdx.x, rounds = (sl.v1 - sl.v0 + NT - 1) / NT, held = sl.count(), want = k < held ? k : held;
+    bool above = false;
+    while (n_cand > CANDIDATES<NT>) {
         for (int i = tid; i < CANDIDATES<NT>; i += NT) {
             const uint64_t c = sh.cand[i];
             int place = 0;
@@ -149,10 +160,12 @@ template <typename T, int NT> __device__ void select_top(const Slice<T> &sl, int
         __syncthreads();
         above = sh.bound == bound;  // a raised bound is above the last one, so this ends
         bound = sh.bound;
-        if (tid == 0) sh.n_cand = sh.n_hot = 0;
+        if (tid == 0) n_hot = n_cand = 0;
+        __syncthreads();
+        collect<T, NT>(sl, nullptr, key, single, segs, shift, bound, above, sh, n_hot, n_cand);
         __syncthreads();
     }
-    int n = sh.n_cand;
+    int n = n_cand;
     if (above && n < want) {  // equal ones, in the order of their columns
         for (int r = -1, found = 0; r <= rounds && n + found < want; r++) {
             int col = -1, elems = 0;
@@ -184,57 +197,51 @@ template <typename T, int NT> __device__ void select_top(const Slice<T> &sl, int
         n = want;
         __syncthreads();
     }
-    for (int i = tid; i < n; i += NT) {
-        const uint64_t c = sh.cand[i];
-        int place = 0;
-        for (int j = 0; j < n; j++) place += sh.cand[j] > c;
-        if (place < want) sh.top[place] = c;
-    }
-    if (tid >= want && tid < k) sh.top[tid] = 0;
-    __syncthreads();
+    return n;
 }
 
-// sh.top of the cluster's CTAs into the first one's.  Between two barriers of the cluster; called by the first one only.
-template <int NT> __device__ __forceinline__ void merge_top(int k, int parts, TopShared<NT> &sh) {
-    const int tid = (int)threadIdx.x;
-    for (int e = tid; e < parts * k; e += NT) sh.cand[e] = peer_load_u64(peer_smem(&sh.top[e % k], e / k));
-    __syncthreads();
-    for (int e = tid; e < parts * k; e += NT) {
-        const uint64_t c = sh.cand[e];
-        int place = e % k;
-        for (int b = 0; b < parts; b++) {
-            if (b == e / k) continue;
-            int lo = 0, hi = k;  // how many of list b come first
-            while (lo < hi) {
-                const int mid = (lo + hi) >> 1;
-                if (sh.cand[b * k + mid] > c) lo = mid + 1;
-                else hi = mid;
-            }
-            place += lo;
+// f(place, candidate) for the first k of `parts` sorted lists of k (0 past their ends)
+template <int NT, typename F> __device__ __forceinline__ void merge_top(const uint64_t *lists, int k, int parts, F f) {
+    for (int e = (int)threadIdx.x; e < parts * k; e += NT) {
+        const uint64_t c = lists[e];
+        int lo[8], hi[8], place = 0;  // how many of each list come first; all lists are searched at once
+#pragma unroll
+        for (int b = 0; b < 8; b++) lo[b] = 0, hi[b] = b < parts ? k : 0;
+        for (int n = k; n > 0; n >>= 1) {
+#pragma unroll
+            for (int b = 0; b < 8; b++)
+                if (lo[b] < hi[b]) {
+                    const int mid = (lo[b] + hi[b]) >> 1;
+                    if (lists[b * k + mid] > c) lo[b] = mid + 1;
+                    else hi[b] = mid;
+                }
         }
-        if (c != 0 && place < k) sh.top[place] = c;
+#pragma unroll
+        for (int b = 0; b < 8; b++) place += lo[b];
+        if (c != 0 && place < k) f(place, c);
     }
-    __syncthreads();
 }
 
 template <typename T, int NT, bool TOP> __global__ void __launch_bounds__(NT, SM_THREADS / NT) token_kernel(const __grid_constant__ TokenParams p) {
     extern __shared__ __align__(16) unsigned char smem[];
-    __shared__ Stats red[2][NT / 32], part;
+    __shared__ Stats red[2][NT / 32], told[2][8];
     TopShared<NT> &sh = *reinterpret_cast<TopShared<NT> *>(smem + RING_BYTES<NT>);
+    uint64_t *lists = reinterpret_cast<uint64_t *>(smem + RING_BYTES<NT> + sizeof(TopShared<NT>));  // [2 rows][parts][top], told by the cluster's CTAs to the first one
     const int tid = (int)threadIdx.x, rank = p.parts > 1 ? cluster_rank() : 0;
     const unsigned first = blockIdx.x / (unsigned)p.parts, step = gridDim.x / (unsigned)p.parts;
     const float a = LOG2E * p.inv_tau;
+    bool met = false;  // all CTAs of the cluster have begun
+    if (p.parts > 1) cluster_barrier_arrive();
+    const int each = (p.top + NT / 32 - 1) / (NT / 32);
     Stream<T, NT, 1> stream(p.x, smem, nullptr, first, step, rank, p.parts);
+    if constexpr (TOP) {
+        if (tid < 2) sh.n_hot[tid] = sh.n_cand[tid] = 0;
+    }
     for (unsigned r = first, turn = 0; r < p.x.rows; r += step, turn ^= 1) {
         const Slice<T> sl(static_cast<const T *>(p.x.x) + p.x.offset(r), p.x.vocab, rank, p.parts);
         const int col = tid < 32 ? sl.single(tid) : -1;
         const float single = col >= 0 ? sl.at(col) : 0.f;
-        int64_t target = p.ignore;
-        float target_x = 0.f;
-        if (rank == 0 && tid == 0 && p.targets) {
-            target = p.targets[r];
-            if (target >= 0 && target < p.x.vocab) target_x = sl.at((int)target);
-        }
+        const int64_t target = rank == 0 && tid == 0 && p.targets ? p.targets[r] : p.ignore;
         Stats st = Stats::none();
         float best = neg_inf();
         int steps = 0, shift = 0;
@@ -269,41 +276,60 @@ template <typename T, int NT, bool TOP> __global__ void __launch_bounds__(NT, SM
         }
         if (col >= 0) st.add_one<true>(single, a);
         leave_stats<NT>(st, a, red[turn]);
+        uint32_t key = 0;
+        if constexpr (TOP) {
+            key = sl.v0 + tid < sl.v1 ? order_key(best) : 0u;
+            const int warps = sl.v1 - sl.v0 >= NT ? NT / 32 : (sl.v1 - sl.v0) / 32;  // those all of whose lanes have a vector
+            const int j = warps == NT / 32 ? each : warps ? (p.top + warps - 1) / warps : 33;
+            const uint32_t bound = j > 32 ? 0u : tid >> 5 < warps ? warp_bound(key, j) : FULL;  // 0: too few vectors, everything is a candidate
+            if ((tid & 31) == 0) sh.bounds[turn][tid >> 5] = bound;
+        }
         __syncthreads();
         if (!TOP && tid >= 32 && p.parts == 1) continue;  // the first warp finishes the row
         st = block_stats<NT>(red[turn], a);
-        if constexpr (TOP) select_top<T, NT>(sl, p.top, best, steps >> shift, shift, sh);
+        Norm norm = norm_of(st);
+        auto put = [&](int place, uint64_t c) {
+            p.top_ids[(int64_t)r * p.top + place] = candidate_col(c);
+            p.top_log_prob[(int64_t)r * p.top + place] = norm.log_prob(key_value((uint32_t)(c >> 32)), p.inv_tau);
+        };
+        const bool ours = target >= 0 && target < p.x.vocab && target != p.ignore;
+        const float target_x = ours ? sl.at((int)target) : 0.f;
+        if constexpr (TOP) {
+            const uint32_t bound = __reduce_min_sync(FULL, sh.bounds[turn][tid & (NT / 32 - 1)]);
+            int &n_hot = sh.n_hot[turn], &n_cand = sh.n_cand[turn];
+            // a short slice that is this CTA's only one is still in the ring, in its order
+            const uint4 *held = r == first && r + step >= p.x.rows && sl.v1 - sl.v0 <= STEP * DEPTH * NT ? reinterpret_cast<const uint4 *>(smem) : nullptr;
+            collect<T, NT>(sl, held, key, single, steps >> shift, shift, bound, false, sh, n_hot, n_cand);
+            __syncthreads();
+            int n = n_cand;
+            if (n > CANDIDATES<NT>) n = select_again<T, NT>(sl, p.top, key, single, steps >> shift, shift, bound, sh, n_hot, n_cand);
+            if (tid == 0) sh.n_hot[turn ^ 1] = sh.n_cand[turn ^ 1] = 0;
+            if (p.parts == 1) {
+                rank_candidates<NT>(sh.cand, n, [&](int place, uint64_t c) { if (place < p.top) put(place, c); });
+            } else {
+                if (!met) cluster_barrier_wait();
+                met = true;
+                uint64_t *list = lists + (turn * p.parts + rank) * p.top;
+                rank_candidates<NT>(sh.cand, n, [&](int place, uint64_t c) { if (place < p.top) peer_store(peer_smem(list + place, 0), c); });
+                if (tid >= n && tid < p.top) peer_store(peer_smem(list + tid, 0), (uint64_t)0);  // a slice of fewer
+            }
+        }
         if (p.parts > 1) {
-            if (tid == 0) part = st;
+            if (!met) cluster_barrier_wait();
+            met = true;
+            if (tid == 0) tell_stats(st, &told[turn][rank], 0);
             cluster_barrier_arrive();
             cluster_barrier_wait();
-            if (rank == 0) {
-                st = peer_stats(&part, 0);
-                for (int i = 1; i < p.parts; i++) st.merge(peer_stats(&part, i), a);
-                if constexpr (TOP) merge_top<NT>(p.top, p.parts, sh);
-            }
-            cluster_barrier_arrive();  // what the first CTA reads in the others stays until it has
-            cluster_barrier_wait();
             if (rank != 0) continue;
+            st = told_stats(told[turn], p.parts, a);
+            norm = norm_of(st);
+            if constexpr (TOP) merge_top<NT>(lists + turn * p.parts * p.top, p.top, p.parts, put);
         }
-        if (TOP ? tid >= p.top && tid > 0 : tid > 0) continue;
-        const Norm norm = norm_of(st);
-        if (tid == 0) {
-            if (p.log_prob) {
-                const bool ours = target >= 0 && target < p.x.vocab;
-                p.log_prob[r] = target == p.ignore ? 0.f : ours ? norm.log_prob(target_x, p.inv_tau) : __int_as_float(0x7fffffff);
-            }
-            p.entropy[r] = st.entropy(p.inv_tau);
-            p.lse[r] = norm.lse(p.inv_tau);
-            if (p.norm) p.norm[r] = norm;
-        }
-        if constexpr (TOP) {
-            if (tid < p.top) {
-                const uint64_t c = sh.top[tid];
-                p.top_ids[(int64_t)r * p.top + tid] = candidate_col(c);
-                p.top_log_prob[(int64_t)r * p.top + tid] = norm.log_prob(key_value((uint32_t)(c >> 32)), p.inv_tau);
-            }
-        }
+        if (rank != 0 || tid != 0) continue;
+        if (p.log_prob) p.log_prob[r] = ours ? norm.log_prob(target_x, p.inv_tau) : target == p.ignore ? 0.f : __int_as_float(0x7fffffff);
+        p.entropy[r] = st.entropy(p.inv_tau);
+        p.lse[r] = norm.lse(p.inv_tau);
+        if (p.norm) p.norm[r] = norm;
     }
 }
 
@@ -369,7 +395,7 @@ int check_logits(const Logits &x, int dtype, float temperature) {
 }
 
 template <typename T, int NT, bool TOP> static int launch_token(const TokenParams &p, Deal deal, int sms, cudaStream_t st) {
-    const size_t smem = RING_BYTES<NT> + (TOP ? sizeof(TopShared<NT>) : 0);
+    const size_t smem = RING_BYTES<NT> + (TOP ? sizeof(TopShared<NT>) + (deal.parts > 1 ? (size_t)2 * deal.parts * p.top * 8 : 0) : 0);
     NMG_ALLOW_SMEM(smem, token_kernel<T, NT, TOP>);
     return launch_rows(token_kernel<T, NT, TOP>, p.x.rows, deal, sms, smem, st, p);
 }
@@ -402,7 +428,7 @@ extern "C" int nmg_token_log_probs(const void *logits, int64_t rows, int64_t inn
     if (reinterpret_cast<uintptr_t>(norm) % 8) NMG_FAIL(NMG_ERR_INVALID, "norm must be 8-byte aligned");
     if (top && (!top_log_prob || !top_ids)) NMG_FAIL(NMG_ERR_INVALID, "top_log_prob and top_ids must be non-NULL when top > 0");
     if ((rc = device_sms(&sms))) return rc;
-    const Deal deal = deal_rows(rows, p.x.vocab, dtype, sms, false, top <= 32 ? 128 : top <= 64 ? 256 : 512);  // about a quarter of the threads holds the top
+    const Deal deal = deal_rows(rows, p.x.vocab, dtype, sms, false, top <= 32 ? 128 : top <= 64 ? 256 : 512);  // the bound comes from maxima of far more ranges than there are alternatives
     p.parts = deal.parts;
     cudaStream_t st = (cudaStream_t)stream;
     NMG_DISPATCH_DTYPE(dtype, T, {

@@ -255,20 +255,18 @@ __device__ __forceinline__ uint32_t peer_smem(const void *p, int rank) {
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_u32(p)), "r"(rank));
     return a;
 }
-__device__ __forceinline__ float peer_load_f32(uint32_t a) {
-    float v;
-    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(a) : "memory");
-    return v;
+__device__ __forceinline__ void peer_store(uint32_t a, float v) { asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(a), "f"(v) : "memory"); }
+__device__ __forceinline__ void peer_store(uint32_t a, uint64_t v) { asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(a), "l"(v) : "memory"); }
+// What a CTA has to say to another is stored there before a barrier of the cluster, and read by the other after it: one barrier a row.
+// The places are of two rows in turn, so nothing is overwritten before its reader comes to the next barrier.
+__device__ __forceinline__ void tell_stats(const Stats &st, Stats *place, int rank) {
+    const uint32_t at = peer_smem(place, rank);
+    peer_store(at, st.m);
+    peer_store(at + 4, st.s);
+    peer_store(at + 8, st.w);
 }
-__device__ __forceinline__ uint64_t peer_load_u64(uint32_t a) {
-    uint64_t v;
-    asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(v) : "r"(a) : "memory");
-    return v;
-}
-__device__ __forceinline__ Stats peer_stats(const Stats *mine, int rank) {
-    const uint32_t a = peer_smem(mine, rank);
-    return Stats{peer_load_f32(a), peer_load_f32(a + 4), peer_load_f32(a + 8)};
-}
+// The statistics that `parts` CTAs (a power of two up to 8) told this one, put together in every warp that asks.
+__device__ __forceinline__ Stats told_stats(const Stats *places, int parts, float a) { return warp_merge(places[threadIdx.x & (parts - 1)], a, parts); }
 
 // The vectors of one row after another on their way from global memory.  Every thread copies its own vectors (v0 + thread + i * VT)
 // asynchronously into slots of its own in shared memory and keeps DEPTH steps of STEP vectors under way, across the ends of rows and of
@@ -433,7 +431,7 @@ inline int launch_rows(void (*kernel)(P...), int64_t rows, Deal deal, int sms, s
     attr.val.clusterDim.y = 1;
     attr.val.clusterDim.z = 1;
     cfg.attrs = &attr;
-    cfg.numAttrs = 1;
+    cfg.numAttrs = deal.parts > 1 ? 1 : 0;
     NMG_CUDA(cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...));
     return NMG_OK;
 }
