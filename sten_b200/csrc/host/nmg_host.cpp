@@ -14,6 +14,8 @@
 #include <c10/cuda/CUDAStream.h>
 #include <pybind11/pybind11.h>
 #include <torch/csrc/Exceptions.h>
+#include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <algorithm>
@@ -25,6 +27,8 @@
 #include "../../../include/nmg_b200.h"
 
 namespace {
+
+using torch::autograd::variable_list;
 
 PyObject *g_error_class = nullptr;  // sten_b200._native.NmgError(status, message)
 PyObject *g_s_val, *g_s_idx, *g_s_packed, *g_s_packed_sp24, *g_zero;
@@ -881,10 +885,10 @@ PyObject *handle_gather(PyObject *self, PyObject *const *a, Py_ssize_t nargs) {
 }
 
 // ------------------------------------------------------------------------------------------------ rows of logits
-float float_arg(PyObject *o) {
+double double_arg(PyObject *o) {
     const double v = PyFloat_AsDouble(o);
     if (v == -1.0 && PyErr_Occurred()) throw PyRaised();
-    return (float)v;
+    return v;
 }
 
 int float_code(const at::Tensor &t, const char *what) {
@@ -956,91 +960,132 @@ void check_lead(const at::Tensor &t, const at::Tensor &logits, const char *what)
     if (t.sizes() != logits.sizes().slice(0, logits.dim() - 1))
         py_raise(PyExc_ValueError, std::string(what) + " must have one entry per row of the logits: expected shape " + shape_str(logits.sizes().slice(0, logits.dim() - 1)) + ", got " + shape_str(t.sizes()));
 }
-const int64_t *targets_ptr(const at::Tensor &targets) { return targets.defined() ? static_cast<const int64_t *>(targets.const_data_ptr()) : nullptr; }
-at::Tensor checked_targets(PyObject *o, const at::Tensor &logits) {
-    const at::Tensor t = optional_tensor(o);
+at::Tensor checked_targets(const at::Tensor &t, const at::Tensor &logits) {
     if (!t.defined()) return t;
     if (t.scalar_type() != at::kLong) py_raise(PyExc_TypeError, std::string("targets must be int64, got ") + c10::toString(t.scalar_type()));
+    if (logits.dim() < 1) py_raise(PyExc_ValueError, "logits must have a last dimension");
     check_lead(t, logits, "targets");
     return packed_rows(t);
 }
+const int64_t *i64_ptr(const at::Tensor &t) { return t.defined() ? static_cast<const int64_t *>(t.const_data_ptr()) : nullptr; }
 const float *f32_ptr(const at::Tensor &t) { return t.defined() ? static_cast<const float *>(t.const_data_ptr()) : nullptr; }
-// gradient of an fp32 output, as the kernels read it
-at::Tensor upstream_arg(PyObject *o) {
-    const at::Tensor t = optional_tensor(o);
-    if (!t.defined()) return t;
-    if (t.scalar_type() != at::kFloat) py_raise(PyExc_TypeError, std::string("gradients of float32 outputs must be float32, got ") + c10::toString(t.scalar_type()));
-    return packed_rows(t);
-}
+float *f32_out(const at::Tensor &t) { return t.defined() ? static_cast<float *>(t.mutable_data_ptr()) : nullptr; }
+// gradient of an fp32 output, as the kernels read it (autograd has checked its type)
+at::Tensor f32_rows(const at::Tensor &t) { return t.defined() ? packed_rows(t) : t; }
 void set_item(PyObject *tuple, Py_ssize_t i, const at::Tensor &t) { PyTuple_SET_ITEM(tuple, i, t.defined() ? THPVariable_Wrap(t) : Py_NewRef(Py_None)); }
 
-// token_log_probs(logits, targets, ignore_index, temperature, top, with_norm) -> (log_prob, entropy, lse, top_log_prob, top_ids, norm)
+// A library call that failed where no interpreter is at hand: in the backward pass, on one of autograd's threads.
+void check_backward(int status) { TORCH_CHECK(status == NMG_OK, "nmg_b200 status ", status, ": ", nmg_last_error()); }
+
+// A backward pass that is recorded itself (create_graph): its result can be had, and what differentiates it again is told that it cannot.
+variable_list differentiable_once(const at::Tensor &d, const char *what, size_t inputs) {
+    variable_list out(inputs);
+    out[0] = d;
+    if (c10::GradMode::is_enabled()) {
+        at::Tensor fake = d.detach();
+        fake.set_requires_grad(true);
+        out[0] = (*std::make_shared<torch::autograd::DelayedError>(std::string(what) + " is differentiable once", 1))({fake})[0];
+    }
+    return out;
+}
+
+std::optional<at::Tensor> maybe(const at::Tensor &t) { return t.defined() ? std::optional<at::Tensor>(t) : std::nullopt; }  // autograd takes no undefined inputs
+
+struct TokenOut { at::Tensor log_prob, entropy, lse, top_log_prob, top_ids, norm; };
+TokenOut token_forward(const at::Tensor &logits, const at::Tensor &targets, int64_t ignore, float temperature, int64_t top, bool with_norm) {
+    const c10::Device dev = logits.device();
+    const int code = float_code(logits, "logits");
+    const LogitRows x = logit_rows(logits);
+    if (top < 0 || top > x.vocab) py_raise(PyExc_ValueError, "top must be between 0 and the vocabulary's " + std::to_string(x.vocab) + " tokens, got " + std::to_string(top));
+    const std::vector<int64_t> lead = lead_shape(logits);
+    TokenOut o;
+    o.entropy = new_empty(lead, at::kFloat);
+    o.lse = new_empty(lead, at::kFloat);
+    if (targets.defined()) o.log_prob = new_empty(lead, at::kFloat);
+    if (with_norm) o.norm = new_empty({x.rows, 2}, at::kFloat);
+    if (top > 0) {
+        std::vector<int64_t> many = lead;
+        many.push_back(top);
+        o.top_log_prob = new_empty(many, at::kFloat);
+        o.top_ids = new_empty(many, at::kLong);
+    }
+    if (x.rows > 0) {
+        void *st = stream_of(dev);
+        PyThreadState *save = PyEval_SaveThread();
+        const int rc = nmg_token_log_probs(x.t.const_data_ptr(), x.rows, x.inner, x.ld, x.ld_outer, x.vocab, code, i64_ptr(targets), ignore, temperature, (int)std::min<int64_t>(top, 1 << 30),
+                                           f32_out(o.log_prob), f32_out(o.entropy), f32_out(o.lse), f32_out(o.top_log_prob), top > 0 ? static_cast<int64_t *>(o.top_ids.mutable_data_ptr()) : nullptr,
+                                           f32_out(o.norm), st);
+        PyEval_RestoreThread(save);
+        check(rc);
+    }
+    return o;
+}
+
+// The operator for autograd: an interpreter's Function costs some 30 us of host time for a forward and a backward pass.
+struct TokenLogProbs : torch::autograd::Function<TokenLogProbs> {
+    static variable_list forward(torch::autograd::AutogradContext *ctx, const at::Tensor &logits, const std::optional<at::Tensor> &given_targets, int64_t ignore, double temperature, int64_t top) {
+        const at::Tensor targets = given_targets.value_or(at::Tensor());
+        const TokenOut o = token_forward(logits, targets, ignore, (float)temperature, top, true);
+        ctx->save_for_backward({logits, targets, o.entropy, o.norm, o.top_ids});
+        ctx->saved_data["ignore"] = ignore;
+        ctx->saved_data["temperature"] = temperature;
+        ctx->set_materialize_grads(false);
+        variable_list out{o.entropy, o.lse};  // those that there are, in this order
+        if (targets.defined()) out.push_back(o.log_prob);
+        if (top > 0) {
+            out.push_back(o.top_log_prob);
+            out.push_back(o.top_ids);
+            ctx->mark_non_differentiable({o.top_ids});
+        }
+        return out;
+    }
+    static variable_list backward(torch::autograd::AutogradContext *ctx, variable_list g) {
+        const variable_list saved = ctx->get_saved_variables();
+        const at::Tensor &logits = saved[0], &targets = saved[1], &entropy = saved[2], &norm = saved[3], &top_ids = saved[4];
+        size_t next = 2;
+        const at::Tensor g_entropy = f32_rows(g[0]), g_lse = f32_rows(g[1]), g_log_prob = targets.defined() ? f32_rows(g[next++]) : at::Tensor(), g_top = top_ids.defined() ? f32_rows(g[next]) : at::Tensor();
+        const c10::cuda::CUDAGuard guard(logits.device());
+        const LogitRows x = logit_rows(logits), d = gradient_of(x);
+        if (x.rows > 0)
+            check_backward(nmg_token_log_probs_backward(x.t.const_data_ptr(), x.rows, x.inner, x.ld, x.ld_outer, x.vocab, float_code(logits, "logits"), i64_ptr(targets), ctx->saved_data["ignore"].toInt(),
+                                                        (float)ctx->saved_data["temperature"].toDouble(), top_ids.defined() ? (int)top_ids.size(-1) : 0, i64_ptr(top_ids), f32_ptr(norm), f32_ptr(entropy),
+                                                        f32_ptr(g_log_prob), f32_ptr(g_entropy), f32_ptr(g_lse), f32_ptr(g_top), d.t.mutable_data_ptr(), d.ld, d.ld_outer, stream_of(logits.device())));
+        return differentiable_once(d.t, "token_log_probs", 5);
+    }
+};
+
+// token_log_probs(logits, targets, ignore_index, temperature, top) -> (log_prob, entropy, lse, top_log_prob, top_ids)
 PyObject *py_token_log_probs(PyObject *, PyObject *const *a, Py_ssize_t nargs) {
-    NMG_PY_BEGIN(6)
+    NMG_PY_BEGIN(5)
     const at::Tensor &logits = tensor_arg(a[0]);
     const at::Tensor raw = optional_tensor(a[1]);
     const c10::Device dev = device_of({&logits, &raw});
-    const int code = float_code(logits, "logits");
+    float_code(logits, "logits");
     const c10::cuda::CUDAGuard guard(dev);
-    const LogitRows x = logit_rows(logits);
-    const at::Tensor targets = checked_targets(a[1], logits);
+    const at::Tensor targets = checked_targets(raw, logits);
     const int64_t ignore = int_arg(a[2]), top = int_arg(a[4]);
-    const float temperature = float_arg(a[3]);
-    if (top < 0 || top > x.vocab) py_raise(PyExc_ValueError, "top must be between 0 and the vocabulary's " + std::to_string(x.vocab) + " tokens, got " + std::to_string(top));
-    const std::vector<int64_t> lead = lead_shape(logits);
-    std::vector<int64_t> many = lead;
-    many.push_back(top);
-    at::Tensor log_prob, top_log_prob, top_ids, norm;
-    const at::Tensor entropy = new_empty(lead, at::kFloat), lse = new_empty(lead, at::kFloat);
-    if (targets.defined()) log_prob = new_empty(lead, at::kFloat);
-    if (int_arg(a[5]) != 0) norm = new_empty({x.rows, 2}, at::kFloat);
-    if (top > 0) {
-        top_log_prob = new_empty(many, at::kFloat);
-        top_ids = new_empty(many, at::kLong);
+    const double temperature = double_arg(a[3]);
+    TokenOut o;
+    if (c10::GradMode::is_enabled() && logits.requires_grad()) {
+        const variable_list v = TokenLogProbs::apply(logits, maybe(targets), ignore, temperature, top);
+        size_t next = 2;
+        o.entropy = v[0];
+        o.lse = v[1];
+        if (targets.defined()) o.log_prob = v[next++];
+        if (top > 0) {
+            o.top_log_prob = v[next];
+            o.top_ids = v[next + 1];
+        }
+    } else {
+        o = token_forward(logits, targets, ignore, (float)temperature, top, false);
     }
-    if (x.rows > 0) {
-        void *st = stream_of(dev);
-        auto f32 = [](const at::Tensor &t) { return t.defined() ? static_cast<float *>(t.mutable_data_ptr()) : nullptr; };
-        PyThreadState *save = PyEval_SaveThread();
-        const int rc = nmg_token_log_probs(x.t.const_data_ptr(), x.rows, x.inner, x.ld, x.ld_outer, x.vocab, code, targets_ptr(targets), ignore, temperature, (int)std::min<int64_t>(top, 1 << 30),
-                                           f32(log_prob), f32(entropy), f32(lse), f32(top_log_prob), top > 0 ? static_cast<int64_t *>(top_ids.mutable_data_ptr()) : nullptr, f32(norm), st);
-        PyEval_RestoreThread(save);
-        check(rc);
-    }
-    PyObject *r = PyTuple_New(6);
-    set_item(r, 0, log_prob);
-    set_item(r, 1, entropy);
-    set_item(r, 2, lse);
-    set_item(r, 3, top_log_prob);
-    set_item(r, 4, top_ids);
-    set_item(r, 5, norm);
+    PyObject *r = PyTuple_New(5);
+    set_item(r, 0, o.log_prob);
+    set_item(r, 1, o.entropy);
+    set_item(r, 2, o.lse);
+    set_item(r, 3, o.top_log_prob);
+    set_item(r, 4, o.top_ids);
     return r;
-    NMG_PY_END
-}
-
-// token_log_probs_backward(logits, targets, ignore_index, temperature, top_ids, norm, entropy, g_log_prob, g_entropy, g_lse, g_top) -> d_logits
-PyObject *py_token_log_probs_backward(PyObject *, PyObject *const *a, Py_ssize_t nargs) {
-    NMG_PY_BEGIN(11)
-    const at::Tensor &logits = tensor_arg(a[0]);
-    const c10::Device dev = device_of({&logits});
-    const int code = float_code(logits, "logits");
-    const c10::cuda::CUDAGuard guard(dev);
-    const LogitRows x = logit_rows(logits);
-    const at::Tensor targets = checked_targets(a[1], logits), top_ids = optional_tensor(a[4]), norm = tensor_arg(a[5]), entropy = optional_tensor(a[6]);
-    const at::Tensor g_log_prob = upstream_arg(a[7]), g_entropy = upstream_arg(a[8]), g_lse = upstream_arg(a[9]), g_top = upstream_arg(a[10]);
-    const LogitRows d = gradient_of(x);
-    if (x.rows > 0) {
-        void *st = stream_of(dev);
-        const int64_t ignore = int_arg(a[2]);
-        const float temperature = float_arg(a[3]);
-        PyThreadState *save = PyEval_SaveThread();
-        const int rc = nmg_token_log_probs_backward(x.t.const_data_ptr(), x.rows, x.inner, x.ld, x.ld_outer, x.vocab, code, targets_ptr(targets), ignore, temperature,
-                                                    top_ids.defined() ? (int)top_ids.size(-1) : 0, targets_ptr(top_ids), f32_ptr(norm), f32_ptr(entropy), f32_ptr(g_log_prob),
-                                                    f32_ptr(g_entropy), f32_ptr(g_lse), f32_ptr(g_top), d.t.mutable_data_ptr(), d.ld, d.ld_outer, st);
-        PyEval_RestoreThread(save);
-        check(rc);
-    }
-    return THPVariable_Wrap(d.t);
     NMG_PY_END
 }
 
@@ -1049,12 +1094,10 @@ struct Teacher {
     int id_bytes, code;
     int64_t kept;
 };
-Teacher teacher_args(PyObject *ids_, PyObject *log_probs_, PyObject *weight_, const at::Tensor &logits) {
-    const at::Tensor &ids = tensor_arg(ids_), &log_probs = tensor_arg(log_probs_);
-    const at::Tensor weight = optional_tensor(weight_);
+Teacher teacher_of(const at::Tensor &ids, const at::Tensor &log_probs, const at::Tensor &weight, const at::Tensor &logits) {
     if (ids.scalar_type() != at::kLong && ids.scalar_type() != at::kInt) py_raise(PyExc_TypeError, std::string("teacher_ids must be int64 or int32, got ") + c10::toString(ids.scalar_type()));
     const int code = float_code(log_probs, "teacher_log_probs");
-    if (ids.dim() != logits.dim() || ids.sizes().slice(0, ids.dim() - 1) != logits.sizes().slice(0, logits.dim() - 1) || ids.size(-1) < 1)
+    if (ids.dim() != logits.dim() || ids.dim() < 1 || ids.sizes().slice(0, ids.dim() - 1) != logits.sizes().slice(0, logits.dim() - 1) || ids.size(-1) < 1)
         py_raise(PyExc_ValueError, "teacher_ids must hold at least one token per row of the logits: logits " + shape_str(logits.sizes()) + ", teacher_ids " + shape_str(ids.sizes()));
     if (log_probs.sizes() != ids.sizes()) py_raise(PyExc_ValueError, "teacher_log_probs must have the shape of teacher_ids " + shape_str(ids.sizes()) + ", got " + shape_str(log_probs.sizes()));
     if (weight.defined()) {
@@ -1064,77 +1107,87 @@ Teacher teacher_args(PyObject *ids_, PyObject *log_probs_, PyObject *weight_, co
     return Teacher{packed_rows(ids), packed_rows(log_probs), weight.defined() ? packed_rows(weight) : weight, ids.scalar_type() == at::kLong ? 8 : 4, code, ids.size(-1)};
 }
 
-// distill(logits, ids, log_probs, weight, remainder, temperature, reduction, with_gradient) -> (loss, norm, total, d_logits)
-PyObject *py_distill(PyObject *, PyObject *const *a, Py_ssize_t nargs) {
-    NMG_PY_BEGIN(8)
-    const at::Tensor &logits = tensor_arg(a[0]), &ids = tensor_arg(a[1]), &log_probs = tensor_arg(a[2]);
-    const at::Tensor weight = optional_tensor(a[3]);
-    const c10::Device dev = device_of({&logits, &ids, &log_probs, &weight});
-    const int code = float_code(logits, "logits");
-    const c10::cuda::CUDAGuard guard(dev);
+struct DistillOut { at::Tensor loss, norm, total, d_logits; };
+DistillOut distill_forward(const at::Tensor &logits, const Teacher &t, int remainder, float temperature, int reduction, bool with_gradient) {
     const LogitRows x = logit_rows(logits);
-    const Teacher t = teacher_args(a[1], a[2], a[3], logits);
-    const int remainder = int_arg(a[4]) != 0, reduction = (int)int_arg(a[6]);
-    const float temperature = float_arg(a[5]);
-    const std::vector<int64_t> lead = lead_shape(logits);
-    const at::Tensor row_loss = new_empty(lead, at::kFloat), norm = new_empty({x.rows, 4}, at::kFloat);
-    at::Tensor loss, total;
-    if (reduction != NMG_REDUCE_NONE) loss = new_empty({}, at::kFloat);
-    if (reduction == NMG_REDUCE_MEAN && t.weight.defined()) total = new_empty({1}, at::kFloat);
+    const at::Tensor row_loss = new_empty(lead_shape(logits), at::kFloat);
+    DistillOut o;
+    o.norm = new_empty({x.rows, 4}, at::kFloat);
+    o.loss = reduction != NMG_REDUCE_NONE ? new_empty({}, at::kFloat) : row_loss;
+    if (reduction == NMG_REDUCE_MEAN && t.weight.defined()) o.total = new_empty({1}, at::kFloat);
     LogitRows d{at::Tensor(), 0, 1, 0, 0, 0, true};
-    if (int_arg(a[7]) != 0) d = gradient_of(x);
+    if (with_gradient) d = gradient_of(x);
+    o.d_logits = d.t;
     if (x.rows > 0) {
-        void *st = stream_of(dev);
-        auto f32 = [](const at::Tensor &v) { return v.defined() ? static_cast<float *>(v.mutable_data_ptr()) : nullptr; };
+        void *st = stream_of(logits.device());
         PyThreadState *save = PyEval_SaveThread();
-        const int rc = nmg_distill(x.t.const_data_ptr(), x.rows, x.inner, x.ld, x.ld_outer, x.vocab, code, t.ids.const_data_ptr(), t.id_bytes, t.log_probs.const_data_ptr(), t.code,
-                                   (int)std::min<int64_t>(t.kept, 1 << 30), remainder, temperature, f32_ptr(t.weight), reduction, f32(row_loss), f32(norm), f32(total), f32(loss),
-                                   d.t.defined() ? d.t.mutable_data_ptr() : nullptr, d.ld, d.ld_outer, st);
+        const int rc = nmg_distill(x.t.const_data_ptr(), x.rows, x.inner, x.ld, x.ld_outer, x.vocab, float_code(logits, "logits"), t.ids.const_data_ptr(), t.id_bytes, t.log_probs.const_data_ptr(), t.code,
+                                   (int)std::min<int64_t>(t.kept, 1 << 30), remainder, temperature, f32_ptr(t.weight), reduction, f32_out(row_loss), f32_out(o.norm), f32_out(o.total),
+                                   reduction != NMG_REDUCE_NONE ? f32_out(o.loss) : nullptr, with_gradient ? d.t.mutable_data_ptr() : nullptr, d.ld, d.ld_outer, st);
         PyEval_RestoreThread(save);
         check(rc);
-    } else if (loss.defined()) {
-        loss.zero_();
+    } else if (reduction != NMG_REDUCE_NONE) {
+        o.loss.zero_();
     }
-    PyObject *r = PyTuple_New(4);
-    set_item(r, 0, reduction == NMG_REDUCE_NONE ? row_loss : loss);
-    set_item(r, 1, norm);
-    set_item(r, 2, total);
-    set_item(r, 3, d.t);
-    return r;
-    NMG_PY_END
+    return o;
 }
 
-// distill_backward(logits, ids, log_probs, weight, remainder, temperature, reduction, norm, total, upstream, d_logits) -> d_logits;
-// a d_logits that distill() wrote stays as it is where upstream is 1, and is written again where it is not
-PyObject *py_distill_backward(PyObject *, PyObject *const *a, Py_ssize_t nargs) {
-    NMG_PY_BEGIN(11)
-    const at::Tensor &logits = tensor_arg(a[0]);
-    const c10::Device dev = device_of({&logits});
-    const int code = float_code(logits, "logits");
-    const c10::cuda::CUDAGuard guard(dev);
-    const LogitRows x = logit_rows(logits);
-    const Teacher t = teacher_args(a[1], a[2], a[3], logits);
-    const int remainder = int_arg(a[4]) != 0, reduction = (int)int_arg(a[6]);
-    const float temperature = float_arg(a[5]);
-    const at::Tensor norm = tensor_arg(a[7]), total = optional_tensor(a[8]), upstream = upstream_arg(a[9]), made = optional_tensor(a[10]);
-    LogitRows d = gradient_of(x);
-    if (made.defined()) {
-        d = logit_rows(made);
-        if (d.inner != x.inner) {  // rows that collapse to one level here and to two there
+// A reduced loss is most often the root of the backward pass, or scaled after it: its gradient for an upstream of 1 is written while
+// the row is still in L2, and the backward pass writes it again, from the logits and rounded once, only where the upstream turns out to
+// be another number (a loss scale).  That costs such a step the writing of one gradient and saves all others the reading of the logits.
+struct Distill : torch::autograd::Function<Distill> {
+    static at::Tensor forward(torch::autograd::AutogradContext *ctx, const at::Tensor &logits, const at::Tensor &ids, const at::Tensor &log_probs, const std::optional<at::Tensor> &given_weight, int64_t remainder, double temperature, int64_t reduction) {
+        const at::Tensor weight = given_weight.value_or(at::Tensor());
+        const DistillOut o = distill_forward(logits, teacher_of(ids, log_probs, weight, logits), (int)remainder, (float)temperature, (int)reduction, reduction != NMG_REDUCE_NONE);
+        ctx->save_for_backward({logits, ids, log_probs, weight, o.norm, o.total});
+        ctx->saved_data["remainder"] = remainder;
+        ctx->saved_data["temperature"] = temperature;
+        ctx->saved_data["reduction"] = reduction;
+        if (o.d_logits.defined()) ctx->saved_data["made"] = o.d_logits;
+        return o.loss;
+    }
+    static variable_list backward(torch::autograd::AutogradContext *ctx, variable_list g) {
+        const variable_list saved = ctx->get_saved_variables();
+        const at::Tensor &logits = saved[0];
+        const at::Tensor upstream = f32_rows(g[0]);
+        at::Tensor made;
+        if (const auto it = ctx->saved_data.find("made"); it != ctx->saved_data.end()) {  // it becomes the caller's: a second backward pass makes its own
+            made = it->second.toTensor();
+            ctx->saved_data.erase(it);
+        }
+        const c10::cuda::CUDAGuard guard(logits.device());
+        const Teacher t = teacher_of(saved[1], saved[2], saved[3], logits);
+        const int reduction = (int)ctx->saved_data["reduction"].toInt();
+        const LogitRows x = logit_rows(logits);
+        LogitRows d = made.defined() ? logit_rows(made) : gradient_of(x);
+        if (d.inner != x.inner) {  // rows that are one level there and two in the logits
             d.inner = x.inner;
             d.ld_outer = x.inner * d.ld;
         }
+        if (x.rows > 0)
+            check_backward(nmg_distill_backward(x.t.const_data_ptr(), x.rows, x.inner, x.ld, x.ld_outer, x.vocab, float_code(logits, "logits"), t.ids.const_data_ptr(), t.id_bytes, t.log_probs.const_data_ptr(),
+                                                t.code, (int)t.kept, (int)ctx->saved_data["remainder"].toInt(), (float)ctx->saved_data["temperature"].toDouble(), f32_ptr(t.weight), reduction, f32_ptr(saved[4]),
+                                                f32_ptr(saved[5]), f32_ptr(upstream), made.defined(), d.t.mutable_data_ptr(), d.ld, d.ld_outer, stream_of(logits.device())));
+        return differentiable_once(d.t, "distillation_loss", 7);
     }
-    if (x.rows > 0) {
-        void *st = stream_of(dev);
-        PyThreadState *save = PyEval_SaveThread();
-        const int rc = nmg_distill_backward(x.t.const_data_ptr(), x.rows, x.inner, x.ld, x.ld_outer, x.vocab, code, t.ids.const_data_ptr(), t.id_bytes, t.log_probs.const_data_ptr(), t.code,
-                                            (int)std::min<int64_t>(t.kept, 1 << 30), remainder, temperature, f32_ptr(t.weight), reduction, f32_ptr(norm), f32_ptr(total),
-                                            f32_ptr(upstream), made.defined(), d.t.mutable_data_ptr(), d.ld, d.ld_outer, st);
-        PyEval_RestoreThread(save);
-        check(rc);
+};
+
+// distill(logits, ids, log_probs, weight, remainder, temperature, reduction) -> loss
+PyObject *py_distill(PyObject *, PyObject *const *a, Py_ssize_t nargs) {
+    NMG_PY_BEGIN(7)
+    const at::Tensor &logits = tensor_arg(a[0]), &ids = tensor_arg(a[1]), &log_probs = tensor_arg(a[2]);
+    const at::Tensor weight = optional_tensor(a[3]);
+    const c10::Device dev = device_of({&logits, &ids, &log_probs, &weight});
+    float_code(logits, "logits");
+    const int64_t remainder = int_arg(a[4]) != 0, reduction = int_arg(a[6]);
+    const double temperature = double_arg(a[5]);
+    const c10::cuda::CUDAGuard guard(dev);
+    if (c10::GradMode::is_enabled()) {
+        if (log_probs.requires_grad()) py_raise(PyExc_ValueError, "teacher_log_probs gets no gradient: detach it");
+        if (weight.defined() && weight.requires_grad()) py_raise(PyExc_ValueError, "weight gets no gradient: detach it");
+        if (logits.requires_grad()) return THPVariable_Wrap(Distill::apply(logits, ids, log_probs, maybe(weight), remainder, temperature, reduction));
     }
-    return THPVariable_Wrap(d.t);
+    return THPVariable_Wrap(distill_forward(logits, teacher_of(ids, log_probs, weight, logits), (int)remainder, (float)temperature, (int)reduction, false).loss);
     NMG_PY_END
 }
 
@@ -1164,9 +1217,7 @@ PyMethodDef module_methods[] = {
     NMG_METHOD("column_sum", py_column_sum),
     NMG_METHOD("densify", py_densify),
     NMG_METHOD("token_log_probs", py_token_log_probs),
-    NMG_METHOD("token_log_probs_backward", py_token_log_probs_backward),
     NMG_METHOD("distill", py_distill),
-    NMG_METHOD("distill_backward", py_distill_backward),
     NMG_METHOD("capturing", py_capturing),
     NMG_METHOD("check_weight", py_check_weight),
     NMG_METHOD("set_dispatch", py_set_dispatch),

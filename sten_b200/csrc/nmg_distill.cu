@@ -40,14 +40,12 @@ struct DistillParams {
     int64_t ld_dx, ld_dx_outer;
 };
 
-// What the warps that hold kept tokens (a thread each) leave for all, of two rows in turn
 struct KeptShared {
-    float top[KEPT_MAX / 32], sum[KEPT_MAX / 32];      // of the teacher's: maximum, and sum of exponentials relative to it
-    float max_x[KEPT_MAX / 32], sum_x[KEPT_MAX / 32];  // statistics of the student's kept logits
-    float loss[KEPT_MAX / 32];
-    float q[KEPT_MAX];
+    float q[KEPT_MAX], logq[KEPT_MAX], x[KEPT_MAX];
     int id[KEPT_MAX];  // -1: padding
-    int twice, bad;
+    uint8_t later[KEPT_MAX];  // where an id is there twice: this is not its first entry
+    float mass, rest, max_x, sum_x;  // S, q_0, and the statistics of the kept logits
+    int some;
 };
 
 __device__ __forceinline__ float teacher_value(const void *p, int dtype, int64_t i) {
@@ -74,8 +72,9 @@ template <typename T> __device__ __forceinline__ uint4 leave_out(uint4 q, uint32
 
 template <typename T, int NT, bool REST, bool STATS, bool GRAD> __global__ void __launch_bounds__(NT, SM_THREADS / NT) distill_kernel(const __grid_constant__ DistillParams p) {
     extern __shared__ __align__(16) unsigned char smem[];
-    __shared__ Stats red[NT / 32], told[2][8];
-    __shared__ KeptShared kept_rows[2];
+    __shared__ Stats red[NT / 32], part;
+    __shared__ KeptShared kept_rows[2];  // of this row and of the one before
+    __shared__ int twice_rows[2];
     uint32_t *bits = reinterpret_cast<uint32_t *>(smem + RING_BYTES<NT>);
     __shared__ uint32_t steps_marked[NT];  // bit s: a kept token is among step s (modulo 32) of the thread's vectors
     const int tid = (int)threadIdx.x, lane = tid & 31, warp = tid >> 5, rank = (int)(blockIdx.x % (unsigned)p.parts);
@@ -83,12 +82,9 @@ template <typename T, int NT, bool REST, bool STATS, bool GRAD> __global__ void 
     if (GRAD && !STATS && p.skip_if_one && *p.upstream == 1.f) return;  // the gradient that is there already is this one
     Stream<T, NT, STATS && GRAD ? 2 : 1> stream(p.x, smem, p.weight, first, step, rank, p.parts);
     for (int i = tid; i < (REST ? (p.x.vocab + BIT0 + 31) / 32 : FILTER_BITS / 32); i += NT) bits[i] = 0u;
-    bool met = false;  // all CTAs of the cluster have begun
-    if (STATS && p.parts > 1) cluster_barrier_arrive();
     steps_marked[tid] = 0u;
-    if (tid < 2) kept_rows[tid].twice = kept_rows[tid].bad = 0;
-    const int kept_warps = (p.kept + 31) / 32;
-    const float a = LOG2E * p.inv_tau, total = p.total ? *p.total : p.divisor, per_weight = total == 0.f ? 0.f : p.tau / total;
+    if (tid < 2) twice_rows[tid] = 0;
+    const float a = LOG2E * p.inv_tau, total = p.total ? *p.total : p.divisor;
 
     // the kept tokens of a row and their logits are fetched while the row before is worked on
     int64_t next_id = -1;
@@ -123,44 +119,66 @@ template <typename T, int NT, bool REST, bool STATS, bool GRAD> __global__ void 
             continue;
         }
         KeptShared &sh = kept_rows[turn];
+        int &twice = twice_rows[turn];
         turn ^= 1;
         const int col = tid < 32 ? sl.single(tid) : -1;
         const float single = STATS && col >= 0 ? sl.at(col) : 0.f;
         auto bit_of = [&](int c) { return REST ? c - sl.lead + BIT0 : c & (FILTER_BITS - 1); };
         const bool none_such = tid < p.kept && raw >= p.x.vocab;
         const int id = tid >= p.kept || raw < 0 || none_such ? -1 : (int)raw;
-        if (none_such) sh.bad = 1;
-        if (tid < p.kept) sh.id[tid] = id;
-        if ((REST || GRAD) && id >= 0) {
+        if (tid < p.kept) {
+            sh.id[tid] = id;
+            sh.logq[tid] = id < 0 ? neg_inf() : logq;
+            sh.x[tid] = id < 0 ? neg_inf() : kept_x;
+            sh.later[tid] = 0;
+        }
+        if (!GRAD) __syncthreads();  // the marks of the row before have been taken away (with GRAD: before its last entries)
+        if (id >= 0) {
             const uint32_t bit = 1u << (bit_of(id) & 31);
-            if (atomicOr(&bits[bit_of(id) >> 5], bit) & bit) sh.twice = 1;  // without remainder: perhaps
+            if (atomicOr(&bits[bit_of(id) >> 5], bit) & bit) twice = 1;  // without remainder: perhaps
             if (REST && STATS && id >= sl.lead && id < sl.tail_at) {
                 const int v = (id - sl.lead) / VEC<T> - sl.v0;
                 if (v >= 0) atomicOr(&steps_marked[v % NT], 1u << (v / (NT * STEP) & 31));
             }
         }
-        bool later = false;  // where an id is there more than once it counts as one token with the sum of its q: not its first entry
-        if constexpr (REST) {
+        const bool bad = __syncthreads_or(none_such);
+        if (twice) {  // an id that is there more than once counts as one token with the sum of its q
+            if (id >= 0)
+                for (int i = 0; i < tid; i++)
+                    if (sh.id[i] == id) sh.later[tid] = 1;
             __syncthreads();
-            if (sh.twice)
-                for (int i = 0; i < tid && id >= 0; i++) later = later || sh.id[i] == id;
         }
-        float q = 0.f, l = id < 0 ? neg_inf() : logq;
-        if (warp < kept_warps) {
-            const float top = REST ? 0.f : warp_pick_max(l);
-            q = expf(l - (top == neg_inf() ? 0.f : top));
-            const float sum = warp_sum(q);
-            float max_x = 0.f, sum_x = 0.f;
-            if constexpr (REST) {
-                const float x = id < 0 || later ? neg_inf() : kept_x;
-                max_x = warp_pick_max(x);
-                sum_x = warp_sum(exp2_fast((x - (max_x == neg_inf() ? 0.f : max_x)) * a));
+        if (tid == 0) twice_rows[turn] = 0;  // of the next row
+        if (warp == 0) {
+            float top = neg_inf(), sum = 0.f, max_x = neg_inf(), sum_x = 0.f;
+            for (int i = lane; i < p.kept; i += 32) {
+                top = fmaxf(top, sh.logq[i]);
+                if (!sh.later[i]) max_x = fmaxf(max_x, sh.x[i]);
+            }
+            top = REST ? 0.f : warp_pick_max(top);
+            max_x = warp_pick_max(max_x);
+            const float ref = top == neg_inf() ? 0.f : top, ref_x = max_x == neg_inf() ? 0.f : max_x;
+            for (int i = lane; i < p.kept; i += 32) {
+                const float q = expf(sh.logq[i] - ref);
+                sh.q[i] = q;
+                sum += q;
+                if (!sh.later[i]) sum_x += exp2_fast((sh.x[i] - ref_x) * a);
+            }
+            sum = warp_sum(sum);
+            sum_x = warp_sum(sum_x);
+            if (!REST) {
+                const float norm = ref + logf(sum), inv = 1.f / sum;
+                for (int i = lane; i < p.kept; i += 32) {
+                    sh.logq[i] -= norm;
+                    sh.q[i] *= inv;
+                }
             }
             if (lane == 0) {
-                sh.top[warp] = top;
-                sh.sum[warp] = sum;
-                sh.max_x[warp] = max_x;
-                sh.sum_x[warp] = sum_x;
+                sh.some = REST || sum != 0.f;
+                sh.mass = REST ? sum : 1.f;
+                sh.rest = REST ? fmaxf(1.f - sum, 0.f) : 0.f;
+                sh.max_x = max_x;
+                sh.sum_x = sum_x;
             }
         }
 
@@ -185,91 +203,69 @@ template <typename T, int NT, bool REST, bool STATS, bool GRAD> __global__ void 
             __syncthreads();
             st = block_stats<NT>(red, a);
             if (p.parts > 1) {
-                if (!met) cluster_barrier_wait();
-                met = true;
-                if (tid < p.parts) tell_stats(st, &told[turn][rank], tid);
+                if (tid == 0) part = st;
                 cluster_barrier_arrive();
                 cluster_barrier_wait();
-                st = told_stats(told[turn], p.parts, a);
+                st = cluster_stats(&part, p.parts, a);
+                cluster_barrier_arrive();  // waited for at the end of the row: what the others read stays until then
             }
             rest = norm_of(st);
-            if constexpr (REST) {
-                for (int i = 0; i < kept_warps; i++) st.merge(Stats{sh.max_x[i], sh.sum_x[i], 0.f}, a);
-                all = norm_of(st);
-            } else {
-                all = rest;
-            }
+            if constexpr (REST) st.merge(Stats{sh.max_x, sh.sum_x, 0.f}, a);
+            all = norm_of(st);
         } else {
             __syncthreads();
             all = p.norm[2 * (int64_t)r];
             rest = p.norm[2 * (int64_t)r + 1];
         }
-        if ((REST || GRAD) && id >= 0) bits[bit_of(id) >> 5] = 0u;  // nobody reads them any more
+        if (id >= 0) bits[bit_of(id) >> 5] = 0u;  // nobody reads them any more
         if (REST && STATS) steps_marked[tid] = 0u;
-        if (tid == 0) kept_rows[turn].twice = kept_rows[turn].bad = 0;  // of the next row
         fetch_x(r + step);
-
-        // the teacher's distribution
-        float top = sh.top[0], sum = sh.sum[0];
-        for (int i = 1; i < kept_warps; i++) {
-            const float t = fmaxf(top, sh.top[i]), ref = t == neg_inf() ? 0.f : t;
-            sum = sum * exp2_fast((top - ref) * LOG2E) + sh.sum[i] * exp2_fast((sh.top[i] - ref) * LOG2E);
-            top = t;
-        }
-        const bool bad = sh.bad, counts = (REST || sum != 0.f) && !all.empty();
-        const float q0 = REST && !rest.empty() ? fmaxf(1.f - sum, 0.f) : 0.f, mass = REST ? sum + q0 : 1.f;
+        const bool counts = sh.some && !all.empty();
+        const float q0 = REST && !rest.empty() ? sh.rest : 0.f, mass = sh.mass + q0;
         const float log_p0 = fmaf(rest.m - all.m, p.inv_tau, rest.ln - all.ln);
-        if (!REST && tid < p.kept) {
-            const float ln = logf(sum);
-            l -= top + ln;
-            q = expf(l);
-        }
         if constexpr (STATS) {
-            if (warp < kept_warps) {
-                const float term = warp_sum(q != 0.f && id >= 0 ? q * (l - all.log_prob(kept_x, p.inv_tau)) : 0.f);
-                if (lane == 0) sh.loss[warp] = term;
+            if (rank == 0 && warp == 0) {
+                float loss = 0.f;
+                for (int i = lane; i < p.kept; i += 32) {
+                    const float q = sh.q[i];
+                    if (q != 0.f) loss += q * (sh.logq[i] - all.log_prob(sh.x[i], p.inv_tau));
+                }
+                loss = warp_sum(loss);
+                if (lane == 0) {
+                    if (q0 != 0.f) loss += q0 * (logf(q0) - log_p0);
+                    p.loss[r] = bad ? __int_as_float(0x7fffffff) : counts ? p.tau * p.tau * w * loss : 0.f;
+                    p.norm[2 * (int64_t)r] = all;
+                    p.norm[2 * (int64_t)r + 1] = rest;
+                }
             }
         }
-        if (GRAD && tid < p.kept) sh.q[tid] = q;
         if constexpr (GRAD) {
-            float scale = per_weight * w;
+            float scale = total == 0.f ? 0.f : p.tau * w / total;
             if constexpr (!STATS) scale *= p.upstream_one ? *p.upstream : p.upstream[r];
             if (bad) scale = __int_as_float(0x7fffffff);
+            // away from the kept tokens every element is a multiple of one exponential
+            const Norm of = REST ? rest : all;
+            const float m = of.empty() ? 0.f : of.m, ln2 = of.ln * LOG2E;
+            const float others = scale * (REST ? (rest.empty() ? 0.f : mass * exp2_fast(log_p0 * LOG2E) - q0) : 1.f);
             const bool zero = !counts && !bad;
             if (zero) {  // of a row that may hold anything
                 grad_pass<NT>(stream, sl, dx, [](float2) { return both(0.f); });
             } else {
-                // away from the kept tokens every element is a multiple of one exponential
-                const Norm of = REST ? rest : all;
-                const float m = of.empty() ? 0.f : of.m, ln2 = of.ln * LOG2E;
-                const float others = scale * (REST ? (rest.empty() ? 0.f : mass * exp2_fast(log_p0 * LOG2E) - q0) : 1.f);
                 grad_pass<NT>(stream, sl, dx, [&](float2 x) {
                     const float2 t = __ffma2_rn(__fadd2_rn(x, both(-m)), both(a), both(-ln2));
                     return __fmul2_rn(make_float2(exp2_fast(t.x), exp2_fast(t.y)), both(others));
                 });
             }
             __syncthreads();  // the entries below replace what other threads wrote
-            if (!zero && id >= 0 && sl.holds(id)) {
-                if (sh.twice) {
-                    later = false;
-                    for (int i = 0; i < tid; i++) later = later || sh.id[i] == id;
+            if (!zero && id >= 0 && !sh.later[tid] && sl.holds(id)) {
+                float q = sh.q[tid];
+                if (twice)
                     for (int i = tid + 1; i < p.kept; i++) q += sh.id[i] == id ? sh.q[i] : 0.f;
-                }
-                if (!later) dx[id] = DT<T>::from_f32(scale * (mass * exp2_fast(all.log_prob(kept_x, p.inv_tau) * LOG2E) - q));
+                dx[id] = DT<T>::from_f32(scale * ((REST ? mass : 1.f) * exp2_fast(all.log_prob(sh.x[tid], p.inv_tau) * LOG2E) - q));
             }
-        } else {
-            __syncthreads();  // the terms are there; and what was marked for this row is gone
         }
-        if (STATS && rank == 0 && tid == 0) {
-            float loss = 0.f;
-            for (int i = 0; i < kept_warps; i++) loss += sh.loss[i];
-            if (q0 != 0.f) loss += q0 * (logf(q0) - log_p0);
-            p.loss[r] = bad ? __int_as_float(0x7fffffff) : counts ? p.tau * p.tau * w * loss : 0.f;
-            p.norm[2 * (int64_t)r] = all;
-            p.norm[2 * (int64_t)r + 1] = rest;
-        }
+        if (STATS && p.parts > 1) cluster_barrier_wait();
     }
-    if (STATS && p.parts > 1 && !met) cluster_barrier_wait();
 }
 
 // out = sum of v (divided by *by, or by 1; 0 where that is 0), added in 64 bits in a fixed order
@@ -298,10 +294,12 @@ template <typename T, int NT, bool REST, bool STATS, bool GRAD> static int launc
 template <bool STATS, bool GRAD> static int launch_distill_any(DistillParams &p, int dtype, bool rest, cudaStream_t st) {
     int sms, rc;
     if ((rc = device_sms(&sms))) return rc;
-    const Deal deal = deal_rows(p.x.rows, p.x.vocab, dtype, sms, STATS && GRAD, p.kept <= 128 ? 128 : 256);
+    const Deal deal = deal_rows(p.x.rows, p.x.vocab, dtype, sms, STATS && GRAD, p.kept <= 32 ? 128 : 256, 0);  // the first warp's work on the kept tokens is a part of a larger CTA's
     p.parts = deal.parts;
     NMG_DISPATCH_DTYPE(dtype, T, {
-        NMG_DISPATCH_THREADS(deal.threads, NT, return rest ? launch_distill<T, NT, true, STATS, GRAD>(p, deal, sms, st) : launch_distill<T, NT, false, STATS, GRAD>(p, deal, sms, st));
+        NMG_DISPATCH_THREADS(deal.threads, NT, {
+            if constexpr (NT >= 128) return rest ? launch_distill<T, NT, true, STATS, GRAD>(p, deal, sms, st) : launch_distill<T, NT, false, STATS, GRAD>(p, deal, sms, st);
+        });
     });
     return NMG_OK;
 }

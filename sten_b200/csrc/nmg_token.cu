@@ -56,7 +56,7 @@ __device__ __forceinline__ uint64_t candidate(uint32_t key, int col) { return (u
 __device__ __forceinline__ int candidate_col(uint64_t c) { return (int)(0xffffffffu - (uint32_t)c); }
 
 template <int NT> struct __align__(16) TopShared {
-    uint64_t cand[CANDIDATES<NT>];
+    uint64_t cand[CANDIDATES<NT>], top[TOP_MAX];
     float seg[SEGMENTS][NT];  // largest logit of each range of a thread's steps
     uint16_t hot[SEGMENTS * NT];
     uint32_t bounds[2][NT / 32];
@@ -224,14 +224,11 @@ template <int NT, typename F> __device__ __forceinline__ void merge_top(const ui
 
 template <typename T, int NT, bool TOP> __global__ void __launch_bounds__(NT, SM_THREADS / NT) token_kernel(const __grid_constant__ TokenParams p) {
     extern __shared__ __align__(16) unsigned char smem[];
-    __shared__ Stats red[2][NT / 32], told[2][8];
+    __shared__ Stats red[2][NT / 32], part;
     TopShared<NT> &sh = *reinterpret_cast<TopShared<NT> *>(smem + RING_BYTES<NT>);
-    uint64_t *lists = reinterpret_cast<uint64_t *>(smem + RING_BYTES<NT> + sizeof(TopShared<NT>));  // [2 rows][parts][top], told by the cluster's CTAs to the first one
     const int tid = (int)threadIdx.x, rank = p.parts > 1 ? cluster_rank() : 0;
     const unsigned first = blockIdx.x / (unsigned)p.parts, step = gridDim.x / (unsigned)p.parts;
     const float a = LOG2E * p.inv_tau;
-    bool met = false;  // all CTAs of the cluster have begun
-    if (p.parts > 1) cluster_barrier_arrive();
     const int each = (p.top + NT / 32 - 1) / (NT / 32);
     Stream<T, NT, 1> stream(p.x, smem, nullptr, first, step, rank, p.parts);
     if constexpr (TOP) {
@@ -307,23 +304,28 @@ template <typename T, int NT, bool TOP> __global__ void __launch_bounds__(NT, SM
             if (p.parts == 1) {
                 rank_candidates<NT>(sh.cand, n, [&](int place, uint64_t c) { if (place < p.top) put(place, c); });
             } else {
-                if (!met) cluster_barrier_wait();
-                met = true;
-                uint64_t *list = lists + (turn * p.parts + rank) * p.top;
-                rank_candidates<NT>(sh.cand, n, [&](int place, uint64_t c) { if (place < p.top) peer_store(peer_smem(list + place, 0), c); });
-                if (tid >= n && tid < p.top) peer_store(peer_smem(list + tid, 0), (uint64_t)0);  // a slice of fewer
+                rank_candidates<NT>(sh.cand, n, [&](int place, uint64_t c) { if (place < p.top) sh.top[place] = c; });
+                if (tid >= n && tid < p.top) sh.top[tid] = 0;  // a slice of fewer
             }
         }
         if (p.parts > 1) {
-            if (!met) cluster_barrier_wait();
-            met = true;
-            if (tid == 0) tell_stats(st, &told[turn][rank], 0);
+            if (tid == 0) part = st;
             cluster_barrier_arrive();
             cluster_barrier_wait();
-            if (rank != 0) continue;
-            st = told_stats(told[turn], p.parts, a);
-            norm = norm_of(st);
-            if constexpr (TOP) merge_top<NT>(lists + turn * p.parts * p.top, p.top, p.parts, put);
+            if (rank == 0) {
+                if constexpr (TOP)
+                    for (int e = tid; e < p.parts * p.top; e += NT) sh.cand[e] = peer_load_u64(peer_smem(&sh.top[e % p.top], e / p.top));
+                st = cluster_stats(&part, p.parts, a);
+                norm = norm_of(st);
+            }
+            cluster_barrier_arrive();  // what the first CTA has read in the others may be written again
+            if constexpr (TOP) {
+                if (rank == 0) {
+                    __syncthreads();
+                    merge_top<NT>(sh.cand, p.top, p.parts, put);
+                }
+            }
+            cluster_barrier_wait();
         }
         if (rank != 0 || tid != 0) continue;
         if (p.log_prob) p.log_prob[r] = ours ? norm.log_prob(target_x, p.inv_tau) : target == p.ignore ? 0.f : __int_as_float(0x7fffffff);
@@ -395,7 +397,7 @@ int check_logits(const Logits &x, int dtype, float temperature) {
 }
 
 template <typename T, int NT, bool TOP> static int launch_token(const TokenParams &p, Deal deal, int sms, cudaStream_t st) {
-    const size_t smem = RING_BYTES<NT> + (TOP ? sizeof(TopShared<NT>) + (deal.parts > 1 ? (size_t)2 * deal.parts * p.top * 8 : 0) : 0);
+    const size_t smem = RING_BYTES<NT> + (TOP ? sizeof(TopShared<NT>) : 0);
     NMG_ALLOW_SMEM(smem, token_kernel<T, NT, TOP>);
     return launch_rows(token_kernel<T, NT, TOP>, p.x.rows, deal, sms, smem, st, p);
 }
@@ -428,11 +430,14 @@ extern "C" int nmg_token_log_probs(const void *logits, int64_t rows, int64_t inn
     if (reinterpret_cast<uintptr_t>(norm) % 8) NMG_FAIL(NMG_ERR_INVALID, "norm must be 8-byte aligned");
     if (top && (!top_log_prob || !top_ids)) NMG_FAIL(NMG_ERR_INVALID, "top_log_prob and top_ids must be non-NULL when top > 0");
     if ((rc = device_sms(&sms))) return rc;
-    const Deal deal = deal_rows(rows, p.x.vocab, dtype, sms, false, top <= 32 ? 128 : top <= 64 ? 256 : 512);  // the bound comes from maxima of far more ranges than there are alternatives
+    const Deal deal = deal_rows(rows, p.x.vocab, dtype, sms, false, top == 0 ? 64 : top <= 32 ? 128 : top <= 64 ? 256 : 512, top ? 6 : 0);  // the bound comes from maxima of far more ranges than there are alternatives
     p.parts = deal.parts;
     cudaStream_t st = (cudaStream_t)stream;
     NMG_DISPATCH_DTYPE(dtype, T, {
-        NMG_DISPATCH_THREADS(deal.threads, NT, return top ? launch_token<T, NT, true>(p, deal, sms, st) : launch_token<T, NT, false>(p, deal, sms, st));
+        NMG_DISPATCH_THREADS(deal.threads, NT, {
+            if constexpr (NT >= 128) if (top) return launch_token<T, NT, true>(p, deal, sms, st);
+            return launch_token<T, NT, false>(p, deal, sms, st);
+        });
     });
     return NMG_OK;
 }
@@ -449,7 +454,7 @@ extern "C" int nmg_token_log_probs_backward(const void *logits, int64_t rows, in
     if (reinterpret_cast<uintptr_t>(norm) % 8) NMG_FAIL(NMG_ERR_INVALID, "norm must be 8-byte aligned");
     if (reinterpret_cast<uintptr_t>(d_logits) % dtype_size(dtype)) NMG_FAIL(NMG_ERR_INVALID, "d_logits must be aligned to its elements");
     if ((rc = device_sms(&sms))) return rc;
-    const Deal deal = deal_rows(rows, p.x.vocab, dtype, sms, false, 128);
+    const Deal deal = deal_rows(rows, p.x.vocab, dtype, sms, false, 64, 0);
     p.parts = deal.parts;
     cudaStream_t st = (cudaStream_t)stream;
     NMG_DISPATCH_DTYPE(dtype, T, {

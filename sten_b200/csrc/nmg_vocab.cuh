@@ -19,7 +19,7 @@
 
 namespace nmg {
 
-// A row belongs to a CTA of NT threads (128, 256 or 512, template argument), or to a cluster of them; an SM holds SM_THREADS of them.
+// A row belongs to a CTA of NT threads (64 to 512, template argument), or to a cluster of them; an SM holds SM_THREADS of them.
 constexpr int SM_THREADS = 1024;
 
 struct Logits {
@@ -255,18 +255,23 @@ __device__ __forceinline__ uint32_t peer_smem(const void *p, int rank) {
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_u32(p)), "r"(rank));
     return a;
 }
-__device__ __forceinline__ void peer_store(uint32_t a, float v) { asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(a), "f"(v) : "memory"); }
-__device__ __forceinline__ void peer_store(uint32_t a, uint64_t v) { asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(a), "l"(v) : "memory"); }
-// What a CTA has to say to another is stored there before a barrier of the cluster, and read by the other after it: one barrier a row.
-// The places are of two rows in turn, so nothing is overwritten before its reader comes to the next barrier.
-__device__ __forceinline__ void tell_stats(const Stats &st, Stats *place, int rank) {
-    const uint32_t at = peer_smem(place, rank);
-    peer_store(at, st.m);
-    peer_store(at + 4, st.s);
-    peer_store(at + 8, st.w);
+__device__ __forceinline__ float peer_load_f32(uint32_t a) {
+    float v;
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(a) : "memory");
+    return v;
 }
-// The statistics that `parts` CTAs (a power of two up to 8) told this one, put together in every warp that asks.
-__device__ __forceinline__ Stats told_stats(const Stats *places, int parts, float a) { return warp_merge(places[threadIdx.x & (parts - 1)], a, parts); }
+__device__ __forceinline__ uint64_t peer_load_u64(uint32_t a) {
+    uint64_t v;
+    asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(v) : "r"(a) : "memory");
+    return v;
+}
+// The statistics of the cluster's `parts` CTAs (a power of two up to 8) put together, in every warp that asks: a lane reads each.  Read
+// between two barriers of the cluster.  (Stored into each other's shared memory before one barrier, they cost more: 8192 rows of 131072
+// bf16 with their gradient 1020 us instead of 910.)
+__device__ __forceinline__ Stats cluster_stats(const Stats *mine, int parts, float a) {
+    const uint32_t at = peer_smem(mine, threadIdx.x & (parts - 1));
+    return warp_merge(Stats{peer_load_f32(at), peer_load_f32(at + 4), peer_load_f32(at + 8)}, a, parts);
+}
 
 // The vectors of one row after another on their way from global memory.  Every thread copies its own vectors (v0 + thread + i * VT)
 // asynchronously into slots of its own in shared memory and keeps DEPTH steps of STEP vectors under way, across the ends of rows and of
@@ -399,18 +404,30 @@ template <int NT, typename T> __device__ __forceinline__ void zero_pass(const Sl
 }
 #endif
 
-// How rows are dealt out.  A row takes NT threads for some hundred instructions at its end, so NT is the smaller the shorter the rows, as
-// long as there are rows enough to fill the chip.  Few rows are shared by clusters of CTAs, as long as every thread has a vector to
-// read; rows that are visited twice also until the second visit finds those in flight in L2 (126 MB, of which they may take half).
+// How rows are dealt out: NT threads a CTA and `parts` CTAs a row, by the least estimated time in units of a vector a thread on a full SM.
+// A row's end and beginning cost a thread about as much as ten vectors, the meetings of a cluster's CTAs ten more; the rounds are whole.
+// Where one round does, what counts is latency: larger CTAs take longer to meet, and a half-empty SM is faster, up to twice.  `meeting`:
+// what a cluster has to do beyond its statistics.  Measured (us, NT = 64 / 128 / 256 / 512): 12288 rows of 30522 fp16 133 / 143 / 168 /
+// 206; 777 rows of 32003 fp32 39 / 32 / 37 / 41; 4096 rows of 131072 bf16 with 64 alternatives - / 311 / 268 / 283; 64 such rows with 20,
+// 1 / 2 / 4 / 8 CTAs of 256: 19.1 / 15.8 / 14.6 / 17.8.  Rows that are visited twice are found in L2 (126 MB) the second time as long as
+// those in flight take half of it (8192 rows of 131072 bf16, CTAs of 512, one a row 1010, two 910).
 struct Deal { int threads, parts; };
-inline Deal deal_rows(int64_t rows, int vocab, int dtype, int sms, bool twice, int least) {
+inline Deal deal_rows(int64_t rows, int vocab, int dtype, int sms, bool twice, int least, int meeting) {
     const int64_t bytes = (int64_t)vocab * (int64_t)dtype_size(dtype);
-    int nt = 512, parts = 1;
-    while (nt > 128 && nt / 2 >= least && bytes / 16 < (int64_t)nt * 24 && rows >= (int64_t)sms * (SM_THREADS / (nt / 2))) nt /= 2;
-    const int64_t slots = (int64_t)sms * (SM_THREADS / nt);
-    while (parts < 8 && rows * parts * 2 <= slots && bytes >= (int64_t)parts * 2 * nt * 16) parts *= 2;
-    while (twice && parts < 8 && (rows < slots / parts ? rows : slots / parts) * bytes > (int64_t)64 << 20) parts *= 2;
-    return Deal{nt, parts};
+    const double vectors = (double)(bytes / 16);
+    Deal best{512, 1};
+    double best_time = 1e300;
+    for (int nt = 512; nt >= least; nt /= 2)
+        for (int parts = 1; parts <= 8; parts *= 2) {
+            const int64_t slots = (int64_t)sms * (SM_THREADS / nt) / parts, rounds = (rows + slots - 1) / slots, in_flight = rows < slots ? rows : slots;
+            if (parts > 1 && vectors < (double)parts * nt) continue;
+            if (twice && in_flight * bytes > (int64_t)64 << 20 && parts < 8) continue;
+            const double x = vectors / ((double)nt * parts), filled = (double)((rows * parts + sms - 1) / sms * nt) / SM_THREADS;
+            const double time = rounds > 1 ? (double)rounds * (x + (parts > 1 ? 20 : 10))
+                                           : (x + 6 + nt / 64 + (parts > 1 ? 2 + 2 * parts + meeting : 0)) * (filled < 0.5 ? 0.5 : filled > 1 ? 1 : filled);
+            if (time < best_time) best_time = time, best = Deal{nt, parts};
+        }
+    return best;
 }
 
 // CTAs that stay, as many as the SMs hold: each cluster of `parts` takes one row after another
@@ -425,19 +442,20 @@ inline int launch_rows(void (*kernel)(P...), int64_t rows, Deal deal, int sms, s
     cfg.blockDim = dim3((unsigned)deal.threads);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = st;
-    cudaLaunchAttribute attr;
+    cudaLaunchAttribute attr;  // clusters of one too: placed like this the CTAs are some 8 % faster than without the attribute (2048 rows of 131072 bf16, gradient: 169 us, 187)
     attr.id = cudaLaunchAttributeClusterDimension;
     attr.val.clusterDim.x = (unsigned)deal.parts;
     attr.val.clusterDim.y = 1;
     attr.val.clusterDim.z = 1;
     cfg.attrs = &attr;
-    cfg.numAttrs = deal.parts > 1 ? 1 : 0;
+    cfg.numAttrs = 1;
     NMG_CUDA(cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...));
     return NMG_OK;
 }
 #define NMG_DISPATCH_THREADS(threads, NT, ...)                        \
     do {                                                              \
-        if ((threads) == 128) { constexpr int NT = 128; __VA_ARGS__; } \
+        if ((threads) == 64) { constexpr int NT = 64; __VA_ARGS__; }  \
+        else if ((threads) == 128) { constexpr int NT = 128; __VA_ARGS__; } \
         else if ((threads) == 256) { constexpr int NT = 256; __VA_ARGS__; } \
         else { constexpr int NT = 512; __VA_ARGS__; }                  \
     } while (0)

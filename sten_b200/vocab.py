@@ -14,7 +14,6 @@ logits (once).  The reference has no counterpart: it leaves every loss to the mo
 from typing import NamedTuple, Optional
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _native as nat
 from .dispatch import SparseTensorWrapper
@@ -36,25 +35,6 @@ def _dense(logits):
     return logits
 
 
-class _TokenLogProbs(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, logits, targets, ignore_index, temperature, top):
-        *out, norm = nat.host().token_log_probs(logits, targets, ignore_index, temperature, top, True)
-        ctx.save_for_backward(logits, targets, out[1], norm, out[4])
-        ctx.arguments = ignore_index, temperature
-        ctx.set_materialize_grads(False)
-        if out[4] is not None:
-            ctx.mark_non_differentiable(out[4])
-        return tuple(out)
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, g_log_prob, g_entropy, g_lse, g_top, _):
-        logits, targets, entropy, norm, top_ids = ctx.saved_tensors
-        d = nat.host().token_log_probs_backward(logits, targets, *ctx.arguments, top_ids, norm, entropy, g_log_prob, g_entropy, g_lse, g_top)
-        return d, None, None, None, None
-
-
 def token_log_probs(logits, targets=None, *, temperature=1.0, top=0, ignore_index=-100):
     """Log-probabilities under ``softmax(logits / temperature)`` along the last dimension.
 
@@ -65,35 +45,10 @@ def token_log_probs(logits, targets=None, *, temperature=1.0, top=0, ignore_inde
 
     A row that is -inf throughout has log-probabilities and log-sum-exp -inf, entropy 0 and no gradient; a row that holds NaN or +inf
     gives NaN."""
-    _dense(logits)
-    if torch.is_grad_enabled() and isinstance(logits, torch.Tensor) and logits.requires_grad:
-        return TokenLogProbs(*_TokenLogProbs.apply(logits, targets, ignore_index, temperature, top))
-    return TokenLogProbs(*nat.host().token_log_probs(logits, targets, ignore_index, temperature, top, False)[:5])
+    return TokenLogProbs(*nat.host().token_log_probs(_dense(logits), targets, ignore_index, temperature, top))
 
 
 _REDUCTIONS = {"none": nat.NMG_REDUCE_NONE, "sum": nat.NMG_REDUCE_SUM, "mean": nat.NMG_REDUCE_MEAN}
-
-
-class _Distill(torch.autograd.Function):
-    # A reduced loss is most often the root of the backward pass, or scaled after it: its gradient for an upstream of 1 is written
-    # while the row is still in L2, and the backward pass writes it again, from the logits and rounded once, only where the upstream
-    # turns out to be another number (a loss scale).  That costs such a step the writing of one gradient and saves all others the
-    # reading of the logits.
-    @staticmethod
-    def forward(ctx, logits, ids, log_probs, weight, remainder, temperature, reduction):
-        out = nat.host().distill(logits, ids, log_probs, weight, remainder, temperature, reduction, reduction != nat.NMG_REDUCE_NONE)
-        ctx.save_for_backward(logits, ids, log_probs, weight, *out[1:3])
-        ctx.arguments = remainder, temperature, reduction
-        ctx.made = out[3]
-        return out[0]
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, upstream):
-        logits, ids, log_probs, weight, norm, total = ctx.saved_tensors
-        made, ctx.made = ctx.made, None  # it becomes the caller's: a second backward pass makes its own
-        d = nat.host().distill_backward(logits, ids, log_probs, weight, *ctx.arguments, norm, total, upstream, made)
-        return d, None, None, None, None, None, None
 
 
 def distillation_loss(logits, teacher_ids, teacher_log_probs, *, remainder=False, weight=None, temperature=1.0, reduction="mean"):
@@ -109,11 +64,4 @@ def distillation_loss(logits, teacher_ids, teacher_log_probs, *, remainder=False
     Gradients go to the logits only.  Rows of which the mask (or the padding) leaves nothing have loss 0 and gradient 0."""
     if reduction not in _REDUCTIONS:
         raise ValueError(f"reduction must be 'none', 'sum' or 'mean', got {reduction!r}")
-    _dense(logits)
-    for name, t in (("teacher_log_probs", teacher_log_probs), ("weight", weight)):
-        if torch.is_grad_enabled() and isinstance(t, torch.Tensor) and t.requires_grad:
-            raise ValueError(f"{name} gets no gradient: detach it")
-    args = logits, teacher_ids, teacher_log_probs, weight, bool(remainder), temperature, _REDUCTIONS[reduction]
-    if torch.is_grad_enabled() and isinstance(logits, torch.Tensor) and logits.requires_grad:
-        return _Distill.apply(*args)
-    return nat.host().distill(*args, False)[0]
+    return nat.host().distill(_dense(logits), teacher_ids, teacher_log_probs, weight, remainder, temperature, _REDUCTIONS[reduction])
