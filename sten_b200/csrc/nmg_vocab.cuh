@@ -279,6 +279,21 @@ __device__ __forceinline__ Stats cluster_stats(const Stats *mine, int parts, flo
 constexpr int STEP = 4, STEP_BITS = 2, DEPTH = 2;
 template <int NT> constexpr int RING_BYTES = STEP * DEPTH * NT * 16;  // 128 KB of an SM
 
+// What L2 should do with a line: one that is read again soon is kept, one that has been read for the last time goes first.
+__device__ __forceinline__ uint64_t l2_keep() {
+    uint64_t p;
+    asm("createpolicy.fractional.L2::evict_last.b64 %0, 1.0;" : "=l"(p));
+    return p;
+}
+__device__ __forceinline__ uint64_t l2_drop() {
+    uint64_t p;
+    asm("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(p));
+    return p;
+}
+__device__ __forceinline__ void cp_async_16_hint(void *smem_dst, const void *gsrc, uint64_t policy) {
+    asm volatile("cp.async.cg.shared.global.L2::cache_hint [%0], [%1], 16, %2;" ::"r"(smem_u32(smem_dst)), "l"(gsrc), "l"(policy) : "memory");
+}
+
 template <typename T, int NT, int PASSES> struct Stream {
     const Logits &x;
     uint4 *ring;  // + slot * NT
@@ -288,6 +303,7 @@ template <typename T, int NT, int PASSES> struct Stream {
     // what is copied next
     const uint4 *from, *begin;
     int left, length, passes;  // vectors of this pass, from this thread's on; of every pass of the row; passes behind this one
+    uint64_t policy = 0;
     float next_weight;
     int put, get;  // slots
 
@@ -317,17 +333,23 @@ template <typename T, int NT, int PASSES> struct Stream {
         }
         from = begin;
         left = length;
+        if constexpr (PASSES > 1) policy = passes ? l2_keep() : l2_drop();
         return true;
     }
     __device__ __forceinline__ void issue() {
         uint4 *to = ring + put * NT;
-        if (left > (STEP - 1) * NT || (left <= 0 && next_pass() && left > (STEP - 1) * NT)) {
+        const bool whole = left > (STEP - 1) * NT || (left <= 0 && next_pass() && left > (STEP - 1) * NT);
+        auto copy = [&](int u) {
+            if constexpr (PASSES == 1) cp_async_16(to + u * NT, from + u * NT);
+            else cp_async_16_hint(to + u * NT, from + u * NT, policy);
+        };
+        if (whole) {
 #pragma unroll
-            for (int u = 0; u < STEP; u++) cp_async_16(to + u * NT, from + u * NT);
+            for (int u = 0; u < STEP; u++) copy(u);
         } else {
 #pragma unroll
             for (int u = 0; u < STEP; u++)
-                if (left > u * NT) cp_async_16(to + u * NT, from + u * NT);
+                if (left > u * NT) copy(u);
         }
         cp_async_commit();
         from += STEP * NT;
@@ -410,7 +432,8 @@ template <int NT, typename T> __device__ __forceinline__ void zero_pass(const Sl
 // what a cluster has to do beyond its statistics.  Measured (us, NT = 64 / 128 / 256 / 512): 12288 rows of 30522 fp16 133 / 143 / 168 /
 // 206; 777 rows of 32003 fp32 39 / 32 / 37 / 41; 4096 rows of 131072 bf16 with 64 alternatives - / 311 / 268 / 283; 64 such rows with 20,
 // 1 / 2 / 4 / 8 CTAs of 256: 19.1 / 15.8 / 14.6 / 17.8.  Rows that are visited twice are found in L2 (126 MB) the second time as long as
-// those in flight take half of it (8192 rows of 131072 bf16, CTAs of 512, one a row 1010, two 910).
+// those in flight take no more than 80 MB of it, better 40, and what has been read for the last time or written goes first (8192 rows of 131072
+// bf16, CTAs of 512 / 256: 829 / 1047; without the hints to L2 1010 / 1130).
 struct Deal { int threads, parts; };
 inline Deal deal_rows(int64_t rows, int vocab, int dtype, int sms, bool twice, int least, int meeting) {
     const int64_t bytes = (int64_t)vocab * (int64_t)dtype_size(dtype);
@@ -421,10 +444,11 @@ inline Deal deal_rows(int64_t rows, int vocab, int dtype, int sms, bool twice, i
         for (int parts = 1; parts <= 8; parts *= 2) {
             const int64_t slots = (int64_t)sms * (SM_THREADS / nt) / parts, rounds = (rows + slots - 1) / slots, in_flight = rows < slots ? rows : slots;
             if (parts > 1 && vectors < (double)parts * nt) continue;
-            if (twice && in_flight * bytes > (int64_t)64 << 20 && parts < 8) continue;
+            if (twice && in_flight * bytes > (int64_t)80 << 20 && parts < 8) continue;
             const double x = vectors / ((double)nt * parts), filled = (double)((rows * parts + sms - 1) / sms * nt) / SM_THREADS;
-            const double time = rounds > 1 ? (double)rounds * (x + (parts > 1 ? 20 : 10))
-                                           : (x + 6 + nt / 64 + (parts > 1 ? 2 + 2 * parts + meeting : 0)) * (filled < 0.5 ? 0.5 : filled > 1 ? 1 : filled);
+            double time = rounds > 1 ? (double)rounds * (x + (parts > 1 ? 20 : 10))
+                                           : (x + 4 + nt / 40 + (parts > 1 ? 2 + 2 * parts + meeting : 0)) * (filled < 0.5 ? 0.5 : filled > 1 ? 1 : filled);
+            if (twice && in_flight * bytes > (int64_t)40 << 20) time *= 1.2;
             if (time < best_time) best_time = time, best = Deal{nt, parts};
         }
     return best;
