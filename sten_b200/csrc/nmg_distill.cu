@@ -289,7 +289,7 @@ __global__ void __launch_bounds__(1024) ordered_sum_kernel(const float *v, int64
 template <typename T, int NT, bool REST, bool STATS, bool GRAD> static int launch_distill(DistillParams &p, Deal deal, int sms, cudaStream_t st) {
     const size_t smem = RING_BYTES<NT> + (REST ? ((size_t)p.x.vocab + BIT0 + 31) / 32 : FILTER_BITS / 32) * 4;
     NMG_ALLOW_SMEM(smem, distill_kernel<T, NT, REST, STATS, GRAD>);
-    return launch_rows(distill_kernel<T, NT, REST, STATS, GRAD>, p.x.rows, deal, sms, smem, st, p);
+    return launch_rows(distill_kernel<T, NT, REST, STATS, GRAD>, p.x.rows, deal, sms, smem, sizeof(KeptShared) * 2 + (3 << 10), st, p);
 }
 template <bool STATS, bool GRAD> static int launch_distill_any(DistillParams &p, int dtype, bool rest, cudaStream_t st) {
     int sms, rc;

@@ -5,7 +5,7 @@
 //                             A = g_lse - g_log_prob - sum g_top - g_entropy H,  B = -g_entropy  (E: there is an entropy gradient)
 //
 // The top k of a row, ordered by value and among equal values by column: every thread keeps the largest logit of its vectors
-// while it sums, and of each of up to SEGMENTS ranges of them.  Every warp finds the j-th largest of its lanes' maxima, j = k / warps
+// while it sums, and of each of up to 16 ranges of them (8 in fp32).  Every warp finds the j-th largest of its lanes' maxima, j = k / warps
 // rounded up; the smallest of these is no larger than k of the maxima, and so no larger than the k-th largest logit: a bound.
 // Only ranges whose maximum reaches it can hold one of the top k, some two per alternative; they are read again, from L2, by all
 // threads, and what reaches the bound is a candidate.  A candidate's place is the number of candidates before it.  The buffer overflows where
@@ -17,7 +17,8 @@
 
 namespace nmg {
 
-constexpr int TOP_MAX = 128, SEGMENTS = 8;
+constexpr int TOP_MAX = 128;
+template <typename T> constexpr int SEGMENTS = 32 / (int)sizeof(T);  // ranges of a thread's vectors
 template <int NT> constexpr int CANDIDATES = 2 * NT;
 
 struct TokenParams {
@@ -55,10 +56,10 @@ __device__ __forceinline__ float key_value(uint32_t key) { return __uint_as_floa
 __device__ __forceinline__ uint64_t candidate(uint32_t key, int col) { return (uint64_t)key << 32 | (0xffffffffu - (uint32_t)col); }
 __device__ __forceinline__ int candidate_col(uint64_t c) { return (int)(0xffffffffu - (uint32_t)c); }
 
-template <int NT> struct __align__(16) TopShared {
+template <typename T, int NT> struct __align__(16) TopShared {
     uint64_t cand[CANDIDATES<NT>], top[TOP_MAX];
-    float seg[SEGMENTS][NT];  // largest logit of each range of a thread's steps
-    uint16_t hot[SEGMENTS * NT];
+    T seg[SEGMENTS<T>][NT];  // largest logit of each range of a thread's steps
+    uint16_t hot[SEGMENTS<T> * NT];
     uint32_t bounds[2][NT / 32];
     int n_hot[2], n_cand[2];  // of this row and of the one before
     int scan[NT / 32];
@@ -89,16 +90,21 @@ template <int NT> __device__ __forceinline__ int block_scan(int n, int *warps, i
 }
 
 // f(place, candidate) for each of the n candidates; GROUP threads count those before one
-template <int NT, typename F> __device__ __forceinline__ void rank_candidates(const uint64_t *cand, int n, F f) {
+template <int NT, typename F> __device__ __forceinline__ void rank_candidates(uint64_t *cand, int n, F f) {
     const int tid = (int)threadIdx.x;
     int bits = 0;
     while (bits < 5 && n << (bits + 1) <= NT) bits++;
     const int group = 1 << bits, sub = tid & (group - 1);
+    const ulonglong2 *pairs = reinterpret_cast<const ulonglong2 *>(cand);
     for (int i = tid >> bits; i - (tid >> bits) < n; i += NT >> bits) {  // all lanes of a warp come round as often
         const uint64_t c = i < n ? cand[i] : 0;
         int place = 0;
 #pragma unroll 4
-        for (int j = sub; j < n; j += group) place += cand[j] > c;
+        for (int j = i < n ? sub : n; j < n >> 1; j += group) {
+            const ulonglong2 two = pairs[j];
+            place += (two.x > c) + (two.y > c);
+        }
+        if ((n & 1) && sub == 0) place += cand[n - 1] > c;
         for (int o = group >> 1; o; o >>= 1) place += __shfl_xor_sync(FULL, place, o);
         if (i < n && sub == 0) f(place, c);
     }
@@ -119,18 +125,20 @@ __device__ __forceinline__ uint32_t warp_bound(uint32_t key, int j) {
 // vectors, which are `segs` ranges of 2^shift steps.  `held`: the slice's vectors in shared memory, or NULL where they are not all there any
 // more.  `single`: this thread's logit outside the vectors.  n_hot and n_cand are 0 when the CTA comes here; n_cand is to be read after a
 // __syncthreads.
-template <typename T, int NT> __device__ __forceinline__ void collect(const Slice<T> &sl, const uint4 *held, uint32_t key, float single, int segs, int shift, uint32_t bound, bool above, TopShared<NT> &sh, int &n_hot, int &n_cand) {
+template <typename T, int NT> __device__ __forceinline__ void collect(const Slice<T> &sl, const uint4 *held, uint32_t key, float single, int segs, int shift, uint32_t bound, bool above, TopShared<T, NT> &sh, int &n_hot, int &n_cand) {
     const int tid = (int)threadIdx.x;
-    auto wanted = [&](uint32_t q) { return above ? q > bound : q >= bound; };
-    auto push = [&](uint32_t q, int col) {
+    // of no bound (0): NaN, which nothing is below; where the bound itself is NaN only NaN reaches it, and nothing is above it
+    const float least = key_value(bound);
+    auto wanted = [&](float x) { return bound == 0xffffffffu ? x != x && !above : !(above ? x <= least : x < least); };
+    auto push = [&](float x, int col) {
         const int at = atomicAdd(&n_cand, 1);
-        if (at < CANDIDATES<NT>) sh.cand[at] = candidate(q, col);
+        if (at < CANDIDATES<NT>) sh.cand[at] = candidate(order_key(x), col);
     };
-    if (key && wanted(key))
+    if (key && (above ? key > bound : key >= bound))
         for (int g = 0; g < segs; g++)
-            if (key == 0xffffffffu || wanted(order_key(sh.seg[g][tid]))) sh.hot[atomicAdd(&n_hot, 1)] = (uint16_t)(g * NT + tid);
+            if (key == 0xffffffffu || wanted(DT<T>::to_f32(sh.seg[g][tid]))) sh.hot[atomicAdd(&n_hot, 1)] = (uint16_t)(g * NT + tid);
     __syncthreads();
-    static_assert(1 << STEP_BITS == STEP && SEGMENTS * NT <= 65536, "");
+    static_assert(1 << STEP_BITS == STEP && SEGMENTS<T> * NT <= 65536, "");
     const int per = shift + STEP_BITS, items = n_hot << per;
     for (int i = tid; i < items; i += NT) {
         const int hot = sh.hot[i >> per], v = sl.v0 + hot % NT + ((hot / NT << per) + (i & ((1 << per) - 1))) * NT;
@@ -139,15 +147,14 @@ template <typename T, int NT> __device__ __forceinline__ void collect(const Slic
         unpack<T>(held ? held[v - sl.v0] : sl.vec(v), x);
 #pragma unroll
         for (int u = 0; u < VEC<T>; u++)
-            if (const uint32_t q = order_key(x[u]); wanted(q)) push(q, sl.lead + v * VEC<T> + u);
+            if (wanted(x[u])) push(x[u], sl.lead + v * VEC<T> + u);
     }
     if (tid < 32)
-        if (const int col = sl.single(tid); col >= 0)
-            if (const uint32_t q = order_key(single); wanted(q)) push(q, col);
+        if (const int col = sl.single(tid); col >= 0 && wanted(single)) push(single, col);
 }
 
 // The longer way of select_top: raises the bound until the candidates fit.  Returns how many there are, all in sh.cand.
-template <typename T, int NT> __device__ __noinline__ int select_again(const Slice<T> &sl, int k, uint32_t key, float single, int segs, int shift, uint32_t bound, TopShared<NT> &sh, int &n_hot, int &n_cand) {
+template <typename T, int NT> __device__ __noinline__ int select_again(const Slice<T> &sl, int k, uint32_t key, float single, int segs, int shift, uint32_t bound, TopShared<T, NT> &sh, int &n_hot, int &n_cand) {
     const int tid = (int)threadIdx.x, rounds = (sl.v1 - sl.v0 + NT - 1) / NT, held = sl.count(), want = k < held ? k : held;
     bool above = false;
     while (n_cand > CANDIDATES<NT>) {
@@ -225,7 +232,7 @@ template <int NT, typename F> __device__ __forceinline__ void merge_top(const ui
 template <typename T, int NT, bool TOP> __global__ void __launch_bounds__(NT, SM_THREADS / NT) token_kernel(const __grid_constant__ TokenParams p) {
     extern __shared__ __align__(16) unsigned char smem[];
     __shared__ Stats red[2][NT / 32], part;
-    TopShared<NT> &sh = *reinterpret_cast<TopShared<NT> *>(smem + RING_BYTES<NT>);
+    TopShared<T, NT> &sh = *reinterpret_cast<TopShared<T, NT> *>(smem + RING_BYTES<NT>);
     const int tid = (int)threadIdx.x, rank = p.parts > 1 ? cluster_rank() : 0;
     const unsigned first = blockIdx.x / (unsigned)p.parts, step = gridDim.x / (unsigned)p.parts;
     const float a = LOG2E * p.inv_tau;
@@ -244,12 +251,12 @@ template <typename T, int NT, bool TOP> __global__ void __launch_bounds__(NT, SM
         int steps = 0, shift = 0;
         float segment = neg_inf();
         if constexpr (TOP)
-            while (((sl.v1 - sl.v0 + STEP * NT - 1) / (STEP * NT) - 1) >> shift >= SEGMENTS) shift++;
+            while (((sl.v1 - sl.v0 + STEP * NT - 1) / (STEP * NT) - 1) >> shift >= SEGMENTS<T>) shift++;
         stream.pass(sl, [&](const uint4 *q, int, int) {
             if constexpr (TOP) {
                 segment = fmaxf(segment, group_pick_max<T>(q));
                 if ((++steps & ((1 << shift) - 1)) == 0) {
-                    sh.seg[(steps - 1) >> shift][tid] = segment;
+                    sh.seg[(steps - 1) >> shift][tid] = DT<T>::from_f32(segment);
                     best = fmaxf(best, segment);
                     segment = neg_inf();
                 }
@@ -259,7 +266,7 @@ template <typename T, int NT, bool TOP> __global__ void __launch_bounds__(NT, SM
         if constexpr (TOP) {
             const int open = steps & ((1 << shift) - 1);
             if (open) {
-                sh.seg[steps >> shift][tid] = segment;
+                sh.seg[steps >> shift][tid] = DT<T>::from_f32(segment);
                 best = fmaxf(best, segment);
                 steps += (1 << shift) - open;
             }
@@ -397,13 +404,13 @@ int check_logits(const Logits &x, int dtype, float temperature) {
 }
 
 template <typename T, int NT, bool TOP> static int launch_token(const TokenParams &p, Deal deal, int sms, cudaStream_t st) {
-    const size_t smem = RING_BYTES<NT> + (TOP ? sizeof(TopShared<NT>) : 0);
+    const size_t smem = RING_BYTES<NT> + (TOP ? sizeof(TopShared<T, NT>) : 0);
     NMG_ALLOW_SMEM(smem, token_kernel<T, NT, TOP>);
-    return launch_rows(token_kernel<T, NT, TOP>, p.x.rows, deal, sms, smem, st, p);
+    return launch_rows(token_kernel<T, NT, TOP>, p.x.rows, deal, sms, smem, 2 << 10, st, p);
 }
 template <typename T, int NT, bool E> static int launch_token_grad(const TokenGradParams &p, Deal deal, int sms, cudaStream_t st) {
     NMG_ALLOW_SMEM(RING_BYTES<NT>, token_grad_kernel<T, NT, E>);
-    return launch_rows(token_grad_kernel<T, NT, E>, p.x.rows, deal, sms, RING_BYTES<NT>, st, p);
+    return launch_rows(token_grad_kernel<T, NT, E>, p.x.rows, deal, sms, RING_BYTES<NT>, 2 << 10, st, p);
 }
 static int check_top(int top, int vocab) {
     if (top < 0 || top > TOP_MAX) NMG_FAIL(top < 0 ? NMG_ERR_INVALID : NMG_ERR_UNSUPPORTED, "top must be 0 .. %d, got %d", TOP_MAX, top);

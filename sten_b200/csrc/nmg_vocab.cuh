@@ -454,12 +454,13 @@ inline Deal deal_rows(int64_t rows, int vocab, int dtype, int sms, bool twice, i
     return best;
 }
 
-// CTAs that stay, as many as the SMs hold: each cluster of `parts` takes one row after another
+// CTAs that stay, as many as the SMs hold: each cluster of `parts` takes one row after another.  smem_beside: no less than what a CTA
+// has in static shared memory and the 1 KB that is reserved.
 template <typename... P, typename... A>
-inline int launch_rows(void (*kernel)(P...), int64_t rows, Deal deal, int sms, size_t smem, cudaStream_t st, A... args) {
+inline int launch_rows(void (*kernel)(P...), int64_t rows, Deal deal, int sms, size_t smem, size_t smem_beside, cudaStream_t st, A... args) {
     if (rows > INT32_MAX) NMG_FAIL(NMG_ERR_UNSUPPORTED, "%lld rows are more than one launch takes", (long long)rows);
     int per_sm = SM_THREADS / deal.threads;
-    while (per_sm > 1 && (smem + (6 << 10)) * per_sm > (size_t)228 << 10) per_sm--;  // with what is static and reserved
+    while (per_sm > 1 && (smem + smem_beside) * per_sm > (size_t)228 << 10) per_sm--;
     const int64_t clusters = (int64_t)sms * per_sm / deal.parts;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)((rows < clusters ? rows : clusters) * deal.parts));
