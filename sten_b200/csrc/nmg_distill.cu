@@ -185,7 +185,7 @@ template <typename T, int NT, bool REST, bool STATS, bool GRAD> __global__ void 
         // the normalisers: of all tokens, and of those not kept
         Norm all, rest;
         if constexpr (STATS) {
-            Stats st = Stats::none();
+            RunningStats<T, false> running;
             auto marked = [&](int bit) { return bits[bit >> 5] >> (bit & 31); };
             uint32_t mine = REST ? steps_marked[tid] : 0u;
             stream.pass(sl, [&](uint4 *q, int v, int n) {
@@ -196,8 +196,9 @@ template <typename T, int NT, bool REST, bool STATS, bool GRAD> __global__ void 
                     for (int u = 0; u < STEP; u++)
                         if (const uint32_t out = u < n ? marked(BIT0 + (v + u * NT) * VEC<T>) & ((1u << VEC<T>) - 1) : 0u) q[u] = leave_out<T>(q[u], out);
                 }
-                st.add<T, false>(q, a);
+                running.add(q, a);
             });
+            Stats st = running.st;
             if (col >= 0) st.add_one<false>(REST && (marked(bit_of(col)) & 1) ? neg_inf() : single, a);
             leave_stats<NT>(st, a, red);
             __syncthreads();
@@ -250,6 +251,12 @@ template <typename T, int NT, bool REST, bool STATS, bool GRAD> __global__ void 
             const bool zero = !counts && !bad;
             if (zero) {  // of a row that may hold anything
                 grad_pass<NT>(stream, sl, dx, [](float2) { return both(0.f); });
+            } else if (const Exponent ex(m, a, ln2); ex.c == ex.c) {
+                const float factor = others * exp2_fast(-ex.off);
+                grad_pass<NT>(stream, sl, dx, [&](float2 x) {
+                    const float2 t = __ffma2_rn(x, both(a), both(ex.c));
+                    return __fmul2_rn(make_float2(exp2_fast(t.x), exp2_fast(t.y)), both(factor));
+                });
             } else {
                 grad_pass<NT>(stream, sl, dx, [&](float2 x) {
                     const float2 t = __ffma2_rn(__fadd2_rn(x, both(-m)), both(a), both(-ln2));

@@ -246,7 +246,7 @@ template <typename T, int NT, bool TOP> __global__ void __launch_bounds__(NT, SM
         const int col = tid < 32 ? sl.single(tid) : -1;
         const float single = col >= 0 ? sl.at(col) : 0.f;
         const int64_t target = rank == 0 && tid == 0 && p.targets ? p.targets[r] : p.ignore;
-        Stats st = Stats::none();
+        RunningStats<T, true> running;
         float best = neg_inf();
         int steps = 0, shift = 0;
         float segment = neg_inf();
@@ -261,8 +261,10 @@ template <typename T, int NT, bool TOP> __global__ void __launch_bounds__(NT, SM
                     segment = neg_inf();
                 }
             }
-            st.add<T, true>(q, a);
+            running.add(q, a);
         });
+        running.settle(a);
+        Stats st = running.st;
         if constexpr (TOP) {
             const int open = steps & ((1 << shift) - 1);
             if (open) {
@@ -336,7 +338,7 @@ template <typename T, int NT, bool TOP> __global__ void __launch_bounds__(NT, SM
         }
         if (rank != 0 || tid != 0) continue;
         if (p.log_prob) p.log_prob[r] = ours ? norm.log_prob(target_x, p.inv_tau) : target == p.ignore ? 0.f : __int_as_float(0x7fffffff);
-        p.entropy[r] = st.entropy(p.inv_tau);
+        p.entropy[r] = st.entropy();
         p.lse[r] = norm.lse(p.inv_tau);
         if (p.norm) p.norm[r] = norm;
     }
@@ -367,16 +369,28 @@ template <typename T, int NT, bool E> __global__ void __launch_bounds__(NT, SM_T
         const float m = empty ? 0.f : norm.m, ln = norm.ln, a = LOG2E * p.inv_tau, ln2 = ln * LOG2E;  // nothing but -inf: p = 0 below
         A *= p.inv_tau;
         B *= p.inv_tau;
-        const float lin = A - B * ln;  // A + B log p = lin + B (x - m) / tau
-        B *= p.inv_tau;
+        const float lin = A - B * ln, B_x = B * p.inv_tau;  // A + B log p = lin + B (x - m) / tau
         auto grad = [&](float2 x) {
             const float2 d = __fadd2_rn(x, both(-m)), t = __ffma2_rn(d, both(a), both(-ln2)), e = make_float2(exp2_fast(t.x), exp2_fast(t.y));
             if constexpr (!E) return __fmul2_rn(e, both(A));
-            float2 y = __fmul2_rn(e, __ffma2_rn(d, both(B), both(lin)));
-            if (y.x != y.x || y.y != y.y) y = make_float2(e.x * (lin + B * fmaxf(d.x, -1e30f)), e.y * (lin + B * fmaxf(d.y, -1e30f)));  // masked: 0 * -inf is not a part of it
+            float2 y = __fmul2_rn(e, __ffma2_rn(d, both(B_x), both(lin)));
+            if (y.x != y.x || y.y != y.y) y = make_float2(e.x * (lin + B_x * fmaxf(d.x, -1e30f)), e.y * (lin + B_x * fmaxf(d.y, -1e30f)));  // masked: 0 * -inf is not a part of it
             return y;
         };
-        grad_pass<NT>(stream, sl, dx, grad);
+        // t = log2 p in one instruction, off by `off`, which goes into the factors: A + B log p = A + B ln 2 (t - off)
+        const Exponent ex(m, a, ln2);
+        if (ex.c == ex.c) {
+            const float factor = exp2_fast(-ex.off), A_t = (A - B * LN2 * ex.off) * factor, B_t = B * LN2 * factor;
+            grad_pass<NT>(stream, sl, dx, [&](float2 x) {
+                const float2 t = __ffma2_rn(x, both(a), both(ex.c)), e = make_float2(exp2_fast(t.x), exp2_fast(t.y));
+                if constexpr (!E) return __fmul2_rn(e, both(A_t));
+                float2 y = __fmul2_rn(e, __ffma2_rn(t, both(B_t), both(A_t)));
+                if (y.x != y.x || y.y != y.y) y = make_float2(e.x * (A_t + B_t * fmaxf(t.x, -1e30f)), e.y * (A_t + B_t * fmaxf(t.y, -1e30f)));
+                return y;
+            });
+        } else {
+            grad_pass<NT>(stream, sl, dx, grad);
+        }
         __syncthreads();  // the entries below replace what other threads wrote
         if (empty) continue;
         if (tid < p.top && p.g_top) {

@@ -5,11 +5,12 @@
 // and a tail.  The CTAs of a cluster share a row: each takes a contiguous range of the vectors, the first the lead and the last
 // the tail (fewer than 16 elements together, one thread each).
 //
-// Statistics of a set of logits x at temperature tau, a = log2(e) / tau:  s = sum 2^((x - m) a),  w = sum 2^((x - m) a) (x - m), all
-// in 32 bits.  m is a reference that the maximum may exceed: it begins as the maximum of the thread's first vectors and is raised
-// to that of later ones only when their sum shows terms of some hundred, which costs s no precision and w some 6 units in the last
-// place of ln s.  So neither the maximum nor the rescaling is part of the inner loop.  From them
-//   log-sum-exp of x / tau = m / tau + ln s,    entropy = ln s - (w / tau) / s.
+// Statistics of a set of logits x at temperature tau, a = log2(e) / tau, t = (x - m) a:  s = sum 2^t,  w = sum 2^t t, all in 32 bits.
+// m is a reference that the maximum may exceed: it begins as the maximum of the thread's first vectors and is raised to that of later
+// ones only when their sum shows terms of some hundred, which costs s no precision and w some 6 units in the last place of ln s.  So
+// neither the maximum nor the rescaling is part of the inner loop.  t takes one instruction, x a + c with c = -m a rounded; what c was
+// rounded by, r = m a + c (exact in one fma), is taken off the sums: as a factor 2^-r and as r s.  From them
+//   log-sum-exp of x / tau = m / tau + ln s,    entropy = ln s - ln 2 w / s.
 // A set that holds nothing but -inf has m = -inf and s = 0; NaN and +inf make s NaN.
 #pragma once
 
@@ -41,7 +42,7 @@ __device__ __forceinline__ float exp2_fast(float x) {  // results below 2^-126 a
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
-constexpr float LOG2E = 1.4426950408889634f;
+constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.69314718055994531f;
 
 template <typename T> constexpr int VEC = 16 / (int)sizeof(T);
 template <typename T> __device__ __forceinline__ uint32_t neg_inf_word();
@@ -143,33 +144,6 @@ struct Stats {
     float m, s, w;
     static __device__ __forceinline__ Stats none() { return Stats{neg_inf(), 0.f, 0.f}; }
 
-    // Four vectors of logits; W: the entropy is wanted.  Two logits an instruction (f32x2).
-    template <typename T, bool W> __device__ __forceinline__ void add(const uint4 *q, float a) {
-        if (m == neg_inf()) m = group_pick_max<T>(q);
-        const float ref = m == neg_inf() ? 0.f : m;
-        float2 ps = both(0.f), pw = both(0.f);
-#pragma unroll
-        for (int u = 0; u < 4; u++) {
-            float x[VEC<T>];
-            unpack<T>(q[u], x);
-#pragma unroll
-            for (int i = 0; i < VEC<T>; i += 2) {
-                const float2 d = __fadd2_rn(make_float2(x[i], x[i + 1]), both(-ref)), t = __fmul2_rn(d, both(a));
-                const float2 e = make_float2(exp2_fast(t.x), exp2_fast(t.y));
-                ps = __fadd2_rn(ps, e);
-                if constexpr (W) pw = __ffma2_rn(e, d, pw);
-            }
-        }
-        ps.x += ps.y;
-        pw.x += pw.y;
-        // the reference is too low; or masked logits: they have e = 0 and d = -inf, whose product is not a part of the sum; or a NaN
-        if (ps.x > 128.f * VEC<T> || (W && pw.x != pw.x)) {
-            *this = with_care<T>(*this, q[0], q[1], q[2], q[3], a);
-        } else {
-            s += ps.x;
-            if constexpr (W) w += pw.x;
-        }
-    }
     template <typename T> static __device__ __noinline__ Stats with_care(Stats st, uint4 q0, uint4 q1, uint4 q2, uint4 q3, float a) {
         const uint4 q[4] = {q0, q1, q2, q3};
         const float top = group_pick_max<T>(q);
@@ -182,9 +156,9 @@ struct Stats {
             unpack<T>(q[u], x);
 #pragma unroll
             for (int i = 0; i < VEC<T>; i++) {
-                const float d = x[i] - ref, e = exp2_fast(d * a);
+                const float t = (x[i] - ref) * a, e = exp2_fast(t);
                 ps += e;
-                pw += e * fmaxf(d, -1e30f);
+                pw += e * fmaxf(t, -1e30f);
             }
         }
         st.s += ps;
@@ -193,13 +167,13 @@ struct Stats {
     }
     template <bool W> __device__ __forceinline__ void add_one(float x, float a) {
         if (x > m) rebase(x, a);
-        const float d = x - (m == neg_inf() ? 0.f : m), e = exp2_fast(d * a);
+        const float t = (x - (m == neg_inf() ? 0.f : m)) * a, e = exp2_fast(t);
         s += e;
-        if constexpr (W) w += e * fmaxf(d, -1e30f);
+        if constexpr (W) w += e * fmaxf(t, -1e30f);
     }
     // relative to `top`; d * s may be -inf
     __device__ __forceinline__ void rebase(float top, float a) {
-        const float d = m - (top == neg_inf() ? 0.f : top), f = exp2_fast(d * a);
+        const float d = (m - (top == neg_inf() ? 0.f : top)) * a, f = exp2_fast(d);
         w = f == 0.f ? 0.f : f * (w + d * s);
         s *= f;
         m = top;
@@ -212,7 +186,75 @@ struct Stats {
         w += o.w;
     }
     __device__ __forceinline__ bool empty() const { return m == neg_inf() && s == 0.f; }
-    __device__ __forceinline__ float entropy(float inv_tau) const { return empty() ? 0.f : logf(s) - w * inv_tau / s; }
+    __device__ __forceinline__ float entropy() const { return empty() ? 0.f : logf(s) - w * LN2 / s; }
+};
+
+// x a + c as the exponent 2^((x - m) a) asks for it, and what it is off by.  Beyond 2^22 (logits of some millions, or masks of the type's
+// lowest value that are all there is) c has no place for it: c is then NaN, and so is what is computed with it.
+struct Reference {
+    float c, r;
+    __device__ __forceinline__ Reference(float m, float a) {
+        c = -m * a;
+        r = fmaf(m, a, c);
+        if (!(fabsf(c) < 4194304.f)) c = __int_as_float(0x7fffffff);
+    }
+};
+
+// x a + c as the exponent of a probability, 2^((x - m) a - ln2) with ln2 the normaliser's log2, and what it is off by.
+struct Exponent {
+    float c, off;
+    __device__ __forceinline__ Exponent(float m, float a, float ln2) {
+        const Reference ref(m, a);
+        c = ref.c - ln2;
+        off = ref.r - ((ref.c - c) - ln2);
+    }
+};
+
+// A thread's statistics while it goes over its vectors; W: the entropy is wanted.
+template <typename T, bool W> struct RunningStats {
+    Stats st = Stats::none();
+    float c = 0.f, factor = 1.f, s_before = 0.f;  // of the reference st.m; what st.s held when it was taken
+
+    __device__ __forceinline__ void refer(float a) {
+        const Reference ref(st.m, a);
+        c = ref.c;
+        factor = exp2_fast(-ref.r);
+        s_before = st.s;
+    }
+    __device__ __forceinline__ void settle(float a) {  // st as it is defined
+        if (W && c == c && st.m != neg_inf()) st.w -= Reference(st.m, a).r * (st.s - s_before);
+    }
+    // Four vectors of logits, two logits an instruction (f32x2)
+    __device__ __forceinline__ void add(const uint4 *q, float a) {
+        if (st.m == neg_inf()) {
+            st.m = group_pick_max<T>(q);
+            refer(a);
+        }
+        float2 ps = both(0.f), pw = both(0.f);
+#pragma unroll
+        for (int u = 0; u < 4; u++) {
+            float x[VEC<T>];
+            unpack<T>(q[u], x);
+#pragma unroll
+            for (int i = 0; i < VEC<T>; i += 2) {
+                const float2 t = __ffma2_rn(make_float2(x[i], x[i + 1]), both(a), both(c));
+                const float2 e = make_float2(exp2_fast(t.x), exp2_fast(t.y));
+                ps = __fadd2_rn(ps, e);
+                if constexpr (W) pw = __ffma2_rn(e, t, pw);
+            }
+        }
+        ps.x += ps.y;
+        pw.x += pw.y;
+        // the reference is too low, or none; or masked logits: they have e = 0 and t = -inf, whose product is not a part of the sum; or a NaN
+        if (!(ps.x <= 128.f * VEC<T>) || (W && pw.x != pw.x)) {
+            settle(a);
+            st = Stats::with_care<T>(st, q[0], q[1], q[2], q[3], a);
+            refer(a);
+        } else {
+            st.s = fmaf(ps.x, factor, st.s);
+            if constexpr (W) st.w = fmaf(pw.x, factor, st.w);
+        }
+    }
 };
 
 // Normaliser of a set: log-sum-exp = m / tau + ln.  The two stay apart, also between the forward and the backward pass: where all that
