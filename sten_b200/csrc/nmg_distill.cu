@@ -29,7 +29,7 @@ struct DistillParams {
     Logits x;
     const void *ids, *log_probs;
     int id_bytes, teacher_dtype, kept, parts;
-    float tau, inv_tau;
+    float tau, a;
     const float *weight, *total;  // total: what the losses are divided by, NULL for `divisor`
     float divisor;
     float *loss;                  // per row
@@ -84,7 +84,7 @@ template <typename T, int NT, bool REST, bool STATS, bool GRAD> __global__ void 
     for (int i = tid; i < (REST ? (p.x.vocab + BIT0 + 31) / 32 : FILTER_BITS / 32); i += NT) bits[i] = 0u;
     steps_marked[tid] = 0u;
     if (tid < 2) twice_rows[tid] = 0;
-    const float a = LOG2E * p.inv_tau, total = p.total ? *p.total : p.divisor;
+    const float a = p.a, total = p.total ? *p.total : p.divisor;
 
     // the kept tokens of a row and their logits are fetched while the row before is worked on
     int64_t next_id = -1;
@@ -211,7 +211,13 @@ template <typename T, int NT, bool REST, bool STATS, bool GRAD> __global__ void 
                 cluster_barrier_arrive();  // waited for at the end of the row: what the others read stays until then
             }
             rest = norm_of(st);
-            if constexpr (REST) st.merge(Stats{sh.max_x, sh.sum_x, 0.f}, a);
+            if constexpr (REST) {
+                const Stats others = st;
+                st.merge(Stats{sh.max_x, sh.sum_x, 0.f}, a);
+                // the sum's own share of the tokens not kept, so that log p_0 has no part of what ex2.approx made of their factor
+                const float below = (others.m - st.m) * a, share = others.s * exp2_fast(below);
+                if (share > 1e-30f) rest.ln = logf(share) - below * LN2;
+            }
             all = norm_of(st);
         } else {
             __syncthreads();
@@ -223,13 +229,13 @@ template <typename T, int NT, bool REST, bool STATS, bool GRAD> __global__ void 
         fetch_x(r + step);
         const bool counts = sh.some && !all.empty();
         const float q0 = REST && !rest.empty() ? sh.rest : 0.f, mass = sh.mass + q0;
-        const float log_p0 = fmaf(rest.m - all.m, p.inv_tau, rest.ln - all.ln);
+        const float below = (rest.m - all.m) * a, log_p0 = (below > -100.f ? below * LN2 : (rest.m - all.m) / p.tau) + (rest.ln - all.ln);
         if constexpr (STATS) {
             if (rank == 0 && warp == 0) {
                 float loss = 0.f;
                 for (int i = lane; i < p.kept; i += 32) {
                     const float q = sh.q[i];
-                    if (q != 0.f) loss += q * (sh.logq[i] - all.log_prob(sh.x[i], p.inv_tau));
+                    if (q != 0.f) loss += q * (sh.logq[i] - all.log_prob_as_summed(sh.x[i], a, p.tau));
                 }
                 loss = warp_sum(loss);
                 if (lane == 0) {
@@ -252,7 +258,7 @@ template <typename T, int NT, bool REST, bool STATS, bool GRAD> __global__ void 
             if (zero) {  // of a row that may hold anything
                 grad_pass<NT>(stream, sl, dx, [](float2) { return both(0.f); });
             } else if (const Exponent ex(m, a, ln2); ex.c == ex.c) {
-                const float factor = others * exp2_fast(-ex.off);
+                const float factor = others * exp2_small(-ex.off);
                 grad_pass<NT>(stream, sl, dx, [&](float2 x) {
                     const float2 t = __ffma2_rn(x, both(a), both(ex.c));
                     return __fmul2_rn(make_float2(exp2_fast(t.x), exp2_fast(t.y)), both(factor));
@@ -268,7 +274,7 @@ template <typename T, int NT, bool REST, bool STATS, bool GRAD> __global__ void 
                 float q = sh.q[tid];
                 if (twice)
                     for (int i = tid + 1; i < p.kept; i++) q += sh.id[i] == id ? sh.q[i] : 0.f;
-                dx[id] = DT<T>::from_f32(scale * ((REST ? mass : 1.f) * exp2_fast(all.log_prob(sh.x[tid], p.inv_tau) * LOG2E) - q));
+                dx[id] = DT<T>::from_f32(scale * ((REST ? mass : 1.f) * exp2_fast(all.log_prob_as_summed(sh.x[tid], a, p.tau) * LOG2E) - q));
             }
         }
         if (STATS && p.parts > 1) cluster_barrier_wait();
@@ -335,7 +341,7 @@ extern "C" int nmg_distill(const void *logits, int64_t rows, int64_t inner_rows,
                            const void *ids, int id_bytes, const void *log_probs, int teacher_dtype, int kept, int remainder,
                            float temperature, const float *weight, int reduction, float *row_loss, float *norm, float *total,
                            float *loss, void *d_logits, int64_t ld_d, int64_t ld_d_outer, void *stream) {
-    DistillParams p{{logits, rows, inner_rows, ld, ld_outer, 0}, ids, log_probs, id_bytes, teacher_dtype, kept, 1, temperature, 1.f / temperature, weight, nullptr, 1.f,
+    DistillParams p{{logits, rows, inner_rows, ld, ld_outer, 0}, ids, log_probs, id_bytes, teacher_dtype, kept, 1, temperature, exponent_scale(temperature), weight, nullptr, 1.f,
                     row_loss, reinterpret_cast<Norm *>(norm), nullptr, 0, 0, d_logits, ld_d, ld_d_outer};
     int rc;
     if ((rc = check_distill(p, vocab, dtype, remainder))) return rc;
@@ -363,7 +369,7 @@ extern "C" int nmg_distill_backward(const void *logits, int64_t rows, int64_t in
                                     const void *ids, int id_bytes, const void *log_probs, int teacher_dtype, int kept, int remainder,
                                     float temperature, const float *weight, int reduction, const float *norm, const float *total, const float *upstream, int skip_if_one, void *d_logits, int64_t ld_d,
                                     int64_t ld_d_outer, void *stream) {
-    DistillParams p{{logits, rows, inner_rows, ld, ld_outer, 0}, ids, log_probs, id_bytes, teacher_dtype, kept, 1, temperature, 1.f / temperature, weight, nullptr, 1.f,
+    DistillParams p{{logits, rows, inner_rows, ld, ld_outer, 0}, ids, log_probs, id_bytes, teacher_dtype, kept, 1, temperature, exponent_scale(temperature), weight, nullptr, 1.f,
                     nullptr, reinterpret_cast<Norm *>(const_cast<float *>(norm)), upstream, reduction != NMG_REDUCE_NONE, skip_if_one, d_logits, ld_d, ld_d_outer};
     int rc;
     if ((rc = check_distill(p, vocab, dtype, remainder))) return rc;

@@ -25,7 +25,7 @@ struct TokenParams {
     Logits x;
     const int64_t *targets;
     int64_t ignore;
-    float tau, inv_tau;
+    float tau, a;
     int top, parts;
     float *log_prob, *entropy, *lse, *top_log_prob;
     int64_t *top_ids;
@@ -36,7 +36,7 @@ struct TokenGradParams {
     Logits x;
     const int64_t *targets;
     int64_t ignore;
-    float inv_tau;
+    float inv_tau, a;
     int top, parts;
     const int64_t *top_ids;
     const Norm *norm;
@@ -235,7 +235,7 @@ template <typename T, int NT, bool TOP> __global__ void __launch_bounds__(NT, SM
     TopShared<T, NT> &sh = *reinterpret_cast<TopShared<T, NT> *>(smem + RING_BYTES<NT>);
     const int tid = (int)threadIdx.x, rank = p.parts > 1 ? cluster_rank() : 0;
     const unsigned first = blockIdx.x / (unsigned)p.parts, step = gridDim.x / (unsigned)p.parts;
-    const float a = LOG2E * p.inv_tau;
+    const float a = p.a;
     const int each = (p.top + NT / 32 - 1) / (NT / 32);
     Stream<T, NT, 1> stream(p.x, smem, nullptr, first, step, rank, p.parts);
     if constexpr (TOP) {
@@ -296,7 +296,7 @@ template <typename T, int NT, bool TOP> __global__ void __launch_bounds__(NT, SM
         Norm norm = norm_of(st);
         auto put = [&](int place, uint64_t c) {
             p.top_ids[(int64_t)r * p.top + place] = candidate_col(c);
-            p.top_log_prob[(int64_t)r * p.top + place] = norm.log_prob(key_value((uint32_t)(c >> 32)), p.inv_tau);
+            p.top_log_prob[(int64_t)r * p.top + place] = norm.log_prob(key_value((uint32_t)(c >> 32)), p.tau);
         };
         const bool ours = target >= 0 && target < p.x.vocab && target != p.ignore;
         const float target_x = ours ? sl.at((int)target) : 0.f;
@@ -337,9 +337,9 @@ template <typename T, int NT, bool TOP> __global__ void __launch_bounds__(NT, SM
             cluster_barrier_wait();
         }
         if (rank != 0 || tid != 0) continue;
-        if (p.log_prob) p.log_prob[r] = ours ? norm.log_prob(target_x, p.inv_tau) : target == p.ignore ? 0.f : __int_as_float(0x7fffffff);
+        if (p.log_prob) p.log_prob[r] = ours ? norm.log_prob(target_x, p.tau) : target == p.ignore ? 0.f : __int_as_float(0x7fffffff);
         p.entropy[r] = st.entropy();
-        p.lse[r] = norm.lse(p.inv_tau);
+        p.lse[r] = norm.lse(p.tau);
         if (p.norm) p.norm[r] = norm;
     }
 }
@@ -366,7 +366,7 @@ template <typename T, int NT, bool E> __global__ void __launch_bounds__(NT, SM_T
         float A = (p.g_lse ? p.g_lse[r] : 0.f) - g_lp - g_top - (E ? g_h * p.entropy[r] : 0.f), B = -g_h;
         if (!in_row && target != p.ignore) A = __int_as_float(0x7fffffff);  // no such token
         const bool empty = norm.empty();
-        const float m = empty ? 0.f : norm.m, ln = norm.ln, a = LOG2E * p.inv_tau, ln2 = ln * LOG2E;  // nothing but -inf: p = 0 below
+        const float m = empty ? 0.f : norm.m, ln = norm.ln, a = p.a, ln2 = ln * LOG2E;  // nothing but -inf: p = 0 below
         A *= p.inv_tau;
         B *= p.inv_tau;
         const float lin = A - B * ln, B_x = B * p.inv_tau;  // A + B log p = lin + B (x - m) / tau
@@ -380,7 +380,7 @@ template <typename T, int NT, bool E> __global__ void __launch_bounds__(NT, SM_T
         // t = log2 p in one instruction, off by `off`, which goes into the factors: A + B log p = A + B ln 2 (t - off)
         const Exponent ex(m, a, ln2);
         if (ex.c == ex.c) {
-            const float factor = exp2_fast(-ex.off), A_t = (A - B * LN2 * ex.off) * factor, B_t = B * LN2 * factor;
+            const float factor = exp2_small(-ex.off), A_t = (A - B * LN2 * ex.off) * factor, B_t = B * LN2 * factor;
             grad_pass<NT>(stream, sl, dx, [&](float2 x) {
                 const float2 t = __ffma2_rn(x, both(a), both(ex.c)), e = make_float2(exp2_fast(t.x), exp2_fast(t.y));
                 if constexpr (!E) return __fmul2_rn(e, both(A_t));
@@ -444,7 +444,7 @@ using namespace nmg;
 extern "C" int nmg_token_log_probs(const void *logits, int64_t rows, int64_t inner_rows, int64_t ld, int64_t ld_outer, int64_t vocab, int dtype,
                                    const int64_t *targets, int64_t ignore_index, float temperature, int top, float *log_prob, float *entropy,
                                    float *lse, float *top_log_prob, int64_t *top_ids, float *norm, void *stream) {
-    TokenParams p{{logits, rows, inner_rows, ld, ld_outer, 0}, targets, ignore_index, temperature, 1.f / temperature, top, 1, log_prob, entropy, lse, top_log_prob, top_ids, reinterpret_cast<Norm *>(norm)};
+    TokenParams p{{logits, rows, inner_rows, ld, ld_outer, 0}, targets, ignore_index, temperature, exponent_scale(temperature), top, 1, log_prob, entropy, lse, top_log_prob, top_ids, reinterpret_cast<Norm *>(norm)};
     int rc, sms;
     if ((rc = check_vocab(vocab, &p.x.vocab)) || (rc = check_logits(p.x, dtype, temperature)) || (rc = check_top(top, p.x.vocab))) return rc;
     if (!entropy || !lse || !log_prob != !targets) NMG_FAIL(NMG_ERR_INVALID, "entropy and lse must be non-NULL, and log_prob where there are targets");
@@ -467,7 +467,7 @@ extern "C" int nmg_token_log_probs_backward(const void *logits, int64_t rows, in
                                             const int64_t *targets, int64_t ignore_index, float temperature, int top, const int64_t *top_ids,
                                             const float *norm, const float *entropy, const float *g_log_prob, const float *g_entropy,
                                             const float *g_lse, const float *g_top, void *d_logits, int64_t ld_d, int64_t ld_d_outer, void *stream) {
-    TokenGradParams p{{logits, rows, inner_rows, ld, ld_outer, 0}, targets, ignore_index, 1.f / temperature, top, 1, top_ids, reinterpret_cast<const Norm *>(norm), entropy, g_log_prob, g_entropy, g_lse, g_top, d_logits, ld_d, ld_d_outer};
+    TokenGradParams p{{logits, rows, inner_rows, ld, ld_outer, 0}, targets, ignore_index, 1.f / temperature, exponent_scale(temperature), top, 1, top_ids, reinterpret_cast<const Norm *>(norm), entropy, g_log_prob, g_entropy, g_lse, g_top, d_logits, ld_d, ld_d_outer};
     int rc, sms;
     if ((rc = check_vocab(vocab, &p.x.vocab)) || (rc = check_logits(p.x, dtype, temperature)) || (rc = check_top(top, p.x.vocab))) return rc;
     if (!norm || !d_logits || (g_entropy && !entropy) || (g_log_prob && !targets) || (g_top && (!top_ids || !top)))

@@ -189,6 +189,12 @@ struct Stats {
     __device__ __forceinline__ float entropy() const { return empty() ? 0.f : logf(s) - w * LN2 / s; }
 };
 
+// 2^x of a small x, a rounding error's size most often: there ex2.approx is off by more than x makes out
+__device__ __forceinline__ float exp2_small(float x) {
+    const float u = x * LN2;
+    return fabsf(u) < 1e-3f ? fmaf(u, fmaf(u, 0.5f, 1.f), 1.f) : exp2_fast(x);
+}
+
 // x a + c as the exponent 2^((x - m) a) asks for it, and what it is off by.  Beyond 2^22 (logits of some millions, or masks of the type's
 // lowest value that are all there is) c has no place for it: c is then NaN, and so is what is computed with it.
 struct Reference {
@@ -218,7 +224,7 @@ template <typename T, bool W> struct RunningStats {
     __device__ __forceinline__ void refer(float a) {
         const Reference ref(st.m, a);
         c = ref.c;
-        factor = exp2_fast(-ref.r);
+        factor = exp2_small(-ref.r);
         s_before = st.s;
     }
     __device__ __forceinline__ void settle(float a) {  // st as it is defined
@@ -262,8 +268,14 @@ template <typename T, bool W> struct RunningStats {
 struct Norm {
     float m, ln;  // nothing but -inf: m = -inf, ln = 0
     __device__ __forceinline__ bool empty() const { return m == neg_inf() && ln == 0.f; }
-    __device__ __forceinline__ float lse(float inv_tau) const { return fmaf(m, inv_tau, ln); }
-    __device__ __forceinline__ float log_prob(float x, float inv_tau) const { return empty() ? neg_inf() : fmaf(x - m, inv_tau, -ln); }
+    __device__ __forceinline__ float lse(float tau) const { return m / tau + ln; }
+    __device__ __forceinline__ float log_prob(float x, float tau) const { return empty() ? neg_inf() : (x - m) / tau - ln; }
+    // The same, from the term that the sum has of x: what ex2.approx is off by on the average (some -6e-8) and what a was rounded by are
+    // in both and cancel.  A divergence, a small difference of such logarithms, would show them.
+    __device__ __forceinline__ float log_prob_as_summed(float x, float a, float tau) const {
+        const float t = (x - m) * a;
+        return empty() ? neg_inf() : t > -100.f ? logf(exp2_fast(t)) - ln : (x - m) / tau - ln;
+    }
 };
 __device__ __forceinline__ Norm norm_of(const Stats &st) { return st.empty() ? Norm{neg_inf(), 0.f} : Norm{st.m, logf(st.s)}; }
 
@@ -528,5 +540,6 @@ inline int launch_rows(void (*kernel)(P...), int64_t rows, Deal deal, int sms, s
     } while (0)
 
 int check_logits(const Logits &x, int dtype, float temperature);
+inline float exponent_scale(float temperature) { return (float)(1.4426950408889634 / (double)temperature); }  // a: rounded once
 
 }  // namespace nmg

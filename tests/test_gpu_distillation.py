@@ -250,6 +250,18 @@ def test_differences(remainder):
     assert abs(slope - float((g * v).sum())) < 2e-3  # third derivative along v below 1, values off by less than 3e-5
 
 
+@pytest.mark.parametrize("remainder", [False, True])
+@pytest.mark.parametrize("tau", [1.0, 1.5])
+def test_no_part_of_the_error_is_the_same_in_every_row(remainder, tau):
+    """A student near its teacher: the loss is a small difference, and a bias of the exponentials (ex2.approx has one of half a unit
+    in the last place, 6e-8) would be a large part of it.  Allowed on the average of 2000 rows, in units of tau^2: that bias once, and
+    four standard errors of single errors of 6e-7."""
+    x, ids, lp, _ = problem(2000, 20011, 17, torch.float32, 4, temperature=tau)
+    got = sten.distillation_loss(x, ids, lp, remainder=remainder, temperature=tau, reduction="none")
+    want = parts(x.double(), ids, lp, remainder, None, tau)[0]
+    assert abs(float((got.double() - want).mean())) <= tau * tau * (6e-8 + 4 * 6e-7 / 2000 ** 0.5)
+
+
 def test_no_rows_streams_and_graphs():
     e = torch.empty(0, 100, device="cuda", requires_grad=True)
     none = torch.empty(0, 4, device="cuda")
