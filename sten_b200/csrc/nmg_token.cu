@@ -4,6 +4,11 @@
 //   token_grad_kernel<T, E>   dx_j = (p_j (A + B log p_j) + g_log_prob [j = target] + g_top,i [j = id_i]) / tau  with
 //                             A = g_lse - g_log_prob - sum g_top - g_entropy H,  B = -g_entropy  (E: there is an entropy gradient)
 //
+// What bounds them: HBM, and for 16-bit logits nearly as much the special-function unit (an exponential per element).  12288 x 30522
+// fp16: 137 us, 5.5 TB/s of 6.5, special-function unit 69 % busy.  4088 x 30522 fp32: 86 us, 5.8 TB/s.  Gradient of 2048 x 131072 bf16,
+// with the entropy's: 169 us, 6.4 TB/s.  With 64 alternatives 4096 x 131072 bf16: 256 us, 4.2 TB/s, issue slots 63 % busy (1.5
+// instructions per element for the ranges' maxima, 10 000 warp instructions a row for the selection).  One row of 30522 with five: 8.6 us.
+//
 // The top k of a row, ordered by value and among equal values by column: every thread keeps the largest logit of its vectors
 // while it sums, and of each of up to 16 ranges of them (8 in fp32).  Every warp finds the j-th largest of its lanes' maxima, j = k / warps
 // rounded up; the smallest of these is no larger than k of the maxima, and so no larger than the k-th largest logit: a bound.

@@ -327,7 +327,7 @@ __device__ __forceinline__ Stats cluster_stats(const Stats *mine, int parts, flo
     return warp_merge(Stats{peer_load_f32(at), peer_load_f32(at + 4), peer_load_f32(at + 8)}, a, parts);
 }
 
-// The vectors of one row after another on their way from global memory.  Every thread copies its own vectors (v0 + thread + i * VT)
+// The vectors of one row after another on their way from global memory.  Every thread copies its own vectors (v0 + thread + i * NT)
 // asynchronously into slots of its own in shared memory and keeps DEPTH steps of STEP vectors under way, across the ends of rows and of
 // passes: while a CTA finishes a row, the next rows' logits arrive.  No thread waits for another's copies.
 constexpr int STEP = 4, STEP_BITS = 2, DEPTH = 2;
