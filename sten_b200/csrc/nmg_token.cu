@@ -398,11 +398,12 @@ template <typename T, int NT, bool E> __global__ void __launch_bounds__(NT, SM_T
         }
         __syncthreads();  // the entries below replace what other threads wrote
         if (empty) continue;
-        if (tid < p.top && p.g_top) {
-            const int64_t id = p.top_ids[at + tid];
-            if (id >= 0 && id < p.x.vocab && !(in_row && id == target) && sl.holds((int)id))
-                dx[id] = DT<T>::from_f32(grad(both(sl.at((int)id))).x + p.g_top[at + tid] * p.inv_tau);
-        }
+        if (p.g_top)
+            for (int i = tid; i < p.top; i += NT) {  // there may be more alternatives than threads
+                const int64_t id = p.top_ids[at + i];
+                if (id >= 0 && id < p.x.vocab && !(in_row && id == target) && sl.holds((int)id))
+                    dx[id] = DT<T>::from_f32(grad(both(sl.at((int)id))).x + p.g_top[at + i] * p.inv_tau);
+            }
         if (tid == NT - 1 && in_row && sl.holds((int)target)) {
             float g = g_lp;
             if (p.g_top)
