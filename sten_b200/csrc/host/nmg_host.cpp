@@ -956,6 +956,18 @@ LogitRows gradient_of(const LogitRows &x) {
     return g;
 }
 
+// The library takes one cut into two levels for the logits and their gradient.  Rows of one level can be cut as the other's are; the two
+// may differ although the gradient was laid out by the logits: hooks on saved tensors (offloading) may return the logits in other strides.
+bool same_levels(LogitRows &a, LogitRows &b) {
+    auto cut = [](LogitRows &r, int64_t inner) {
+        if (r.rows > r.inner) return false;
+        r.inner = inner;
+        r.ld_outer = inner * r.ld;
+        return true;
+    };
+    return a.inner == b.inner || cut(b, a.inner) || cut(a, b.inner);
+}
+
 void check_lead(const at::Tensor &t, const at::Tensor &logits, const char *what) {
     if (t.sizes() != logits.sizes().slice(0, logits.dim() - 1))
         py_raise(PyExc_ValueError, std::string(what) + " must have one entry per row of the logits: expected shape " + shape_str(logits.sizes().slice(0, logits.dim() - 1)) + ", got " + shape_str(t.sizes()));
@@ -1158,12 +1170,12 @@ struct Distill : torch::autograd::Function<Distill> {
         const c10::cuda::CUDAGuard guard(logits.device());
         const Teacher t = teacher_of(saved[1], saved[2], saved[3], logits);
         const int reduction = (int)ctx->saved_data["reduction"].toInt();
-        const LogitRows x = logit_rows(logits);
-        LogitRows d = made.defined() ? logit_rows(made) : gradient_of(x);
-        if (d.inner != x.inner) {  // rows that are one level there and two in the logits
-            d.inner = x.inner;
-            d.ld_outer = x.inner * d.ld;
+        LogitRows x = logit_rows(logits), d = x;
+        if (made.defined()) {
+            d = logit_rows(made);
+            if (!same_levels(x, d)) made = at::Tensor();  // what it holds is of no use then, not even where the upstream is 1
         }
+        if (!made.defined()) d = gradient_of(x);
         if (x.rows > 0)
             check_backward(nmg_distill_backward(x.t.const_data_ptr(), x.rows, x.inner, x.ld, x.ld_outer, x.vocab, float_code(logits, "logits"), t.ids.const_data_ptr(), t.id_bytes, t.log_probs.const_data_ptr(),
                                                 t.code, (int)t.kept, (int)ctx->saved_data["remainder"].toInt(), (float)ctx->saved_data["temperature"].toDouble(), f32_ptr(t.weight), reduction, f32_ptr(saved[4]),

@@ -61,6 +61,9 @@ def distillation_loss(logits, teacher_ids, teacher_log_probs, *, remainder=False
     and the mass they leave over is held against the student's probability of all other tokens together.  ``weight``: float32 of
     the leading shape; rows of weight 0 are not read.  ``reduction``: "none", "sum", or "mean" over the rows' weights.
 
+    A reduced loss of logits that require a gradient keeps, beside them, a tensor of their size with their gradient until its backward
+    pass.  That tensor is not among the saved ones: hooks on those (``save_on_cpu``, checkpointing) leave it on the device.
+
     Gradients go to the logits only.  Rows of which the mask (or the padding) leaves nothing have loss 0 and gradient 0."""
     if reduction not in _REDUCTIONS:
         raise ValueError(f"reduction must be 'none', 'sum' or 'mean', got {reduction!r}")
