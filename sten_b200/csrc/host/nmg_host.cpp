@@ -47,6 +47,16 @@ struct Ref {  // owned reference
     throw PyRaised();
 }
 
+// What call() returns, other threads running beside it.  The interpreter is back when it throws, too: a tensor without memory of its own
+// (one of torch.func's, a sparse one) throws where its address is asked for.
+template <typename F> auto without_interpreter(F call) {
+    struct Released {
+        PyThreadState *state = PyEval_SaveThread();
+        ~Released() { PyEval_RestoreThread(state); }
+    } released;
+    return call();
+}
+
 void check(int status) {
     if (status == NMG_OK) return;
     PyObject *args = Py_BuildValue("(is)", status, nmg_last_error());
@@ -190,16 +200,14 @@ void call_spmm(const Geo &geo, int code, c10::Device dev, const at::Tensor &val,
     const void *pk = packed.defined() ? packed.const_data_ptr() : nullptr;
     const void *bp = b.defined() ? b.const_data_ptr() : nullptr;
     const int16_t *ip = static_cast<const int16_t *>(i.const_data_ptr());
-    int rc;
-    PyThreadState *save = PyEval_SaveThread();
-    if (epi.act != NMG_EPI_NONE || epi.residual.defined())
-        rc = nmg_spmm_fused(v.const_data_ptr(), ip, pk, geo.M, geo.K, geo.n, geo.m, geo.g, code, act.t.const_data_ptr(), act.ld, tokens, bp, epi.act,
-                            epi.residual.defined() ? epi.residual.const_data_ptr() : nullptr, epi.ld, out.mutable_data_ptr(), ld_out, layout, algo, wsp,
-                            nbytes, st);
-    else
-        rc = nmg_spmm(v.const_data_ptr(), ip, pk, geo.M, geo.K, geo.n, geo.m, geo.g, code, act.t.const_data_ptr(), act.ld, tokens, bp,
-                      out.mutable_data_ptr(), ld_out, layout, algo, wsp, nbytes, st);
-    PyEval_RestoreThread(save);
+    const int rc = without_interpreter([&] {
+        if (epi.act != NMG_EPI_NONE || epi.residual.defined())
+            return nmg_spmm_fused(v.const_data_ptr(), ip, pk, geo.M, geo.K, geo.n, geo.m, geo.g, code, act.t.const_data_ptr(), act.ld, tokens, bp, epi.act,
+                                  epi.residual.defined() ? epi.residual.const_data_ptr() : nullptr, epi.ld, out.mutable_data_ptr(), ld_out, layout, algo, wsp,
+                                  nbytes, st);
+        return nmg_spmm(v.const_data_ptr(), ip, pk, geo.M, geo.K, geo.n, geo.m, geo.g, code, act.t.const_data_ptr(), act.ld, tokens, bp,
+                        out.mutable_data_ptr(), ld_out, layout, algo, wsp, nbytes, st);
+    });
     check(rc);
 }
 
@@ -214,16 +222,14 @@ void call_spmm_t(const Geo &geo, int code, c10::Device dev, const at::Tensor &va
         nbytes = nmg_spmm_t_workspace_bytes(geo.M, geo.K, dy.rows, geo.n, geo.m, geo.g, code, algo, given(packed, dy));
         if (nbytes) ws = new_empty({(int64_t)nbytes}, at::kByte);
     }
-    int rc;
-    PyThreadState *save = PyEval_SaveThread();
-    if (sp24.defined())
-        rc = nmg_spmm_t_sp24(sp24.const_data_ptr(), geo.M, geo.K, geo.n, geo.m, geo.g, code, dy.t.const_data_ptr(), dy.ld, dy.rows, dx.mutable_data_ptr(),
-                             geo.K, st);
-    else
-        rc = nmg_spmm_t(v.const_data_ptr(), static_cast<const int16_t *>(i.const_data_ptr()), packed.defined() ? packed.const_data_ptr() : nullptr, geo.M,
-                        geo.K, geo.n, geo.m, geo.g, code, dy.t.const_data_ptr(), dy.ld, dy.rows, dx.mutable_data_ptr(), geo.K, algo,
-                        nbytes ? ws.mutable_data_ptr() : nullptr, nbytes, st);
-    PyEval_RestoreThread(save);
+    const int rc = without_interpreter([&] {
+        if (sp24.defined())
+            return nmg_spmm_t_sp24(sp24.const_data_ptr(), geo.M, geo.K, geo.n, geo.m, geo.g, code, dy.t.const_data_ptr(), dy.ld, dy.rows, dx.mutable_data_ptr(),
+                                   geo.K, st);
+        return nmg_spmm_t(v.const_data_ptr(), static_cast<const int16_t *>(i.const_data_ptr()), packed.defined() ? packed.const_data_ptr() : nullptr, geo.M,
+                          geo.K, geo.n, geo.m, geo.g, code, dy.t.const_data_ptr(), dy.ld, dy.rows, dx.mutable_data_ptr(), geo.K, algo,
+                          nbytes ? ws.mutable_data_ptr() : nullptr, nbytes, st);
+    });
     check(rc);
 }
 
@@ -340,10 +346,10 @@ PyObject *py_sparsify(PyObject *, PyObject *const *a, Py_ssize_t nargs) {
     const Tiles t = tiles_of(d.B, d.M, d.K, n, m, g);
     const at::Tensor val = new_empty({t.count, t.C, g, n}, w.scalar_type()), idx = new_empty({t.count, t.C, g, 1}, at::kShort);
     void *st = stream_of(dev);
-    PyThreadState *save = PyEval_SaveThread();
-    const int rc = nmg_sparsify(d.t.const_data_ptr(), d.B, d.M, d.K, d.ld, d.bs, n, m, g, code, val.mutable_data_ptr(),
-                                static_cast<int16_t *>(idx.mutable_data_ptr()), st);
-    PyEval_RestoreThread(save);
+    const int rc = without_interpreter([&] {
+        return nmg_sparsify(d.t.const_data_ptr(), d.B, d.M, d.K, d.ld, d.bs, n, m, g, code, val.mutable_data_ptr(),
+                            static_cast<int16_t *>(idx.mutable_data_ptr()), st);
+    });
     check(rc);
     PyObject *v = THPVariable_Wrap(val), *i = THPVariable_Wrap(idx);
     PyObject *r = PyTuple_New(2);
@@ -360,10 +366,10 @@ PyObject *gather_values(const Dense3 &d, const at::Tensor &idx0, int n, int m, i
     if (idx.scalar_type() != at::kShort || idx.numel() != t.count * t.cc) py_raise(PyExc_ValueError, "idx does not belong to a layout of this shape");
     const at::Tensor val = new_empty({t.count, t.C, g, n}, w.scalar_type());
     void *st = stream_of(dev);
-    PyThreadState *save = PyEval_SaveThread();
-    const int rc = nmg_gather(d.t.const_data_ptr(), static_cast<const int16_t *>(idx.const_data_ptr()), d.B, d.M, d.K, d.ld, d.bs, n, m, g, code,
-                              val.mutable_data_ptr(), st);
-    PyEval_RestoreThread(save);
+    const int rc = without_interpreter([&] {
+        return nmg_gather(d.t.const_data_ptr(), static_cast<const int16_t *>(idx.const_data_ptr()), d.B, d.M, d.K, d.ld, d.bs, n, m, g, code,
+                          val.mutable_data_ptr(), st);
+    });
     check(rc);
     return THPVariable_Wrap(val);
 }
@@ -392,10 +398,10 @@ PyObject *py_densify(PyObject *, PyObject *const *a, Py_ssize_t nargs) {
     const at::Tensor val = packed_rows(val0), idx = packed_rows(idx0);
     const at::Tensor out = new_empty({B, geo.M, geo.K}, val.scalar_type());
     void *st = stream_of(dev);
-    PyThreadState *save = PyEval_SaveThread();
-    const int rc = nmg_densify(val.const_data_ptr(), static_cast<const int16_t *>(idx.const_data_ptr()), B, geo.M, geo.K, geo.n, geo.m, geo.g, code,
-                               out.mutable_data_ptr(), geo.K, geo.M * geo.K, st);
-    PyEval_RestoreThread(save);
+    const int rc = without_interpreter([&] {
+        return nmg_densify(val.const_data_ptr(), static_cast<const int16_t *>(idx.const_data_ptr()), B, geo.M, geo.K, geo.n, geo.m, geo.g, code,
+                           out.mutable_data_ptr(), geo.K, geo.M * geo.K, st);
+    });
     check(rc);
     return THPVariable_Wrap(out);
     NMG_PY_END
@@ -715,9 +721,9 @@ at::Tensor column_sums(const Rows &x, int code, c10::Device dev) {
     const size_t nbytes = nmg_column_sum_workspace_bytes(x.rows, x.cols);
     const at::Tensor ws = new_empty({(int64_t)nbytes}, at::kByte);
     void *st = stream_of(dev);
-    PyThreadState *save = PyEval_SaveThread();
-    const int rc = nmg_column_sum(x.t.const_data_ptr(), x.rows, x.cols, x.ld, code, out.mutable_data_ptr(), ws.mutable_data_ptr(), nbytes, st);
-    PyEval_RestoreThread(save);
+    const int rc = without_interpreter([&] {
+        return nmg_column_sum(x.t.const_data_ptr(), x.rows, x.cols, x.ld, code, out.mutable_data_ptr(), ws.mutable_data_ptr(), nbytes, st);
+    });
     check(rc);
     return out;
 }
@@ -1023,11 +1029,11 @@ TokenOut token_forward(const at::Tensor &logits, const at::Tensor &targets, int6
     }
     if (x.rows > 0) {
         void *st = stream_of(dev);
-        PyThreadState *save = PyEval_SaveThread();
-        const int rc = nmg_token_log_probs(x.t.const_data_ptr(), x.rows, x.inner, x.ld, x.ld_outer, x.vocab, code, i64_ptr(targets), ignore, temperature, (int)std::min<int64_t>(top, 1 << 30),
-                                           f32_out(o.log_prob), f32_out(o.entropy), f32_out(o.lse), f32_out(o.top_log_prob), top > 0 ? static_cast<int64_t *>(o.top_ids.mutable_data_ptr()) : nullptr,
-                                           f32_out(o.norm), st);
-        PyEval_RestoreThread(save);
+        const int rc = without_interpreter([&] {
+            return nmg_token_log_probs(x.t.const_data_ptr(), x.rows, x.inner, x.ld, x.ld_outer, x.vocab, code, i64_ptr(targets), ignore, temperature, (int)std::min<int64_t>(top, 1 << 30),
+                                       f32_out(o.log_prob), f32_out(o.entropy), f32_out(o.lse), f32_out(o.top_log_prob), top > 0 ? static_cast<int64_t *>(o.top_ids.mutable_data_ptr()) : nullptr,
+                                       f32_out(o.norm), st);
+        });
         check(rc);
     }
     return o;
@@ -1132,11 +1138,11 @@ DistillOut distill_forward(const at::Tensor &logits, const Teacher &t, int remai
     o.d_logits = d.t;
     if (x.rows > 0) {
         void *st = stream_of(logits.device());
-        PyThreadState *save = PyEval_SaveThread();
-        const int rc = nmg_distill(x.t.const_data_ptr(), x.rows, x.inner, x.ld, x.ld_outer, x.vocab, float_code(logits, "logits"), t.ids.const_data_ptr(), t.id_bytes, t.log_probs.const_data_ptr(), t.code,
-                                   (int)std::min<int64_t>(t.kept, 1 << 30), remainder, temperature, f32_ptr(t.weight), reduction, f32_out(row_loss), f32_out(o.norm), f32_out(o.total),
-                                   reduction != NMG_REDUCE_NONE ? f32_out(o.loss) : nullptr, with_gradient ? d.t.mutable_data_ptr() : nullptr, d.ld, d.ld_outer, st);
-        PyEval_RestoreThread(save);
+        const int rc = without_interpreter([&] {
+            return nmg_distill(x.t.const_data_ptr(), x.rows, x.inner, x.ld, x.ld_outer, x.vocab, float_code(logits, "logits"), t.ids.const_data_ptr(), t.id_bytes, t.log_probs.const_data_ptr(), t.code,
+                               (int)std::min<int64_t>(t.kept, 1 << 30), remainder, temperature, f32_ptr(t.weight), reduction, f32_out(row_loss), f32_out(o.norm), f32_out(o.total),
+                               reduction != NMG_REDUCE_NONE ? f32_out(o.loss) : nullptr, with_gradient ? d.t.mutable_data_ptr() : nullptr, d.ld, d.ld_outer, st);
+        });
         check(rc);
     } else if (reduction != NMG_REDUCE_NONE) {
         o.loss.zero_();
