@@ -995,6 +995,17 @@ void set_item(PyObject *tuple, Py_ssize_t i, const at::Tensor &t) { PyTuple_SET_
 // A library call that failed where no interpreter is at hand: in the backward pass, on one of autograd's threads.
 void check_backward(int status) { TORCH_CHECK(status == NMG_OK, "nmg_b200 status ", status, ": ", nmg_last_error()); }
 
+// Forward-mode derivatives: a tangent that is there must not be left out, which would read as a derivative of zero.
+bool has_tangent(const at::Tensor &t) { return t.defined() && t._fw_grad(/*level=*/0).defined(); }
+std::string no_forward_mode(const char *what) { return std::string(what) + " has no forward-mode derivative: its operands must not be dual tensors"; }
+void refuse_tangents(std::initializer_list<const at::Tensor *> ts, const char *what) {
+    for (const at::Tensor *t : ts)
+        if (has_tangent(*t)) py_raise(PyExc_NotImplementedError, no_forward_mode(what));
+}
+void check_no_tangents(const variable_list &gradients, const char *what) {
+    for (const at::Tensor &g : gradients) TORCH_CHECK_NOT_IMPLEMENTED(!has_tangent(g), no_forward_mode(what));
+}
+
 // A backward pass that is recorded itself (create_graph): its result can be had, and what differentiates it again is told that it cannot.
 variable_list differentiable_once(const at::Tensor &d, const char *what, size_t inputs) {
     variable_list out(inputs);
@@ -1058,6 +1069,7 @@ struct TokenLogProbs : torch::autograd::Function<TokenLogProbs> {
         return out;
     }
     static variable_list backward(torch::autograd::AutogradContext *ctx, variable_list g) {
+        check_no_tangents(g, "token_log_probs");
         const variable_list saved = ctx->get_saved_variables();
         const at::Tensor &logits = saved[0], &targets = saved[1], &entropy = saved[2], &norm = saved[3], &top_ids = saved[4];
         size_t next = 2;
@@ -1079,6 +1091,7 @@ PyObject *py_token_log_probs(PyObject *, PyObject *const *a, Py_ssize_t nargs) {
     const at::Tensor raw = optional_tensor(a[1]);
     const c10::Device dev = device_of({&logits, &raw});
     float_code(logits, "logits");
+    refuse_tangents({&logits}, "token_log_probs");
     const c10::cuda::CUDAGuard guard(dev);
     const at::Tensor targets = checked_targets(raw, logits);
     const int64_t ignore = int_arg(a[2]), top = int_arg(a[4]);
@@ -1165,6 +1178,7 @@ struct Distill : torch::autograd::Function<Distill> {
         return o.loss;
     }
     static variable_list backward(torch::autograd::AutogradContext *ctx, variable_list g) {
+        check_no_tangents(g, "distillation_loss");
         const variable_list saved = ctx->get_saved_variables();
         const at::Tensor &logits = saved[0];
         const at::Tensor upstream = f32_rows(g[0]);
@@ -1197,6 +1211,7 @@ PyObject *py_distill(PyObject *, PyObject *const *a, Py_ssize_t nargs) {
     const at::Tensor weight = optional_tensor(a[3]);
     const c10::Device dev = device_of({&logits, &ids, &log_probs, &weight});
     float_code(logits, "logits");
+    refuse_tangents({&logits, &log_probs, &weight}, "distillation_loss");
     const int64_t remainder = int_arg(a[4]) != 0, reduction = int_arg(a[6]);
     const double temperature = double_arg(a[5]);
     const c10::cuda::CUDAGuard guard(dev);

@@ -3,7 +3,7 @@
 ``token_log_probs`` reads logits once for the log-probabilities of given tokens, the entropy and the top alternatives of every
 row; ``distillation_loss`` holds a student against the top log-probabilities that ``token_log_probs`` kept of its teacher.  Both
 take fp32, fp16 and bf16 logits of any row length and alignment, compute in 32 bits, and differentiate with respect to the
-logits (once).  The reference has no counterpart: it leaves every loss to the model code.
+logits (once, in reverse mode; dual tensors are refused).  The reference has no counterpart: it leaves every loss to the model code.
 
     with torch.no_grad():                                               # the dense model, once per batch
         kept = sten.token_log_probs(teacher(x), top=64, temperature=2.0)
