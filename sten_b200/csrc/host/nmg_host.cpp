@@ -1006,6 +1006,15 @@ void check_no_tangents(const variable_list &gradients, const char *what) {
     for (const at::Tensor &g : gradients) TORCH_CHECK_NOT_IMPLEMENTED(!has_tangent(g), no_forward_mode(what));
 }
 
+// Saved tensors may come back as anything: from a user's hooks, or with `.data` of the user's own tensor replaced since.  The kernels take
+// addresses, so the backward passes look again at where a tensor is, its type and its shape, without the interpreter.
+bool is_float(const at::Tensor &t) { return t.scalar_type() == at::kFloat || t.scalar_type() == at::kHalf || t.scalar_type() == at::kBFloat16; }
+bool lives_with(const at::Tensor &t, const at::Tensor &logits) { return t.device() == logits.device() && t.has_storage(); }
+void check_saved(bool as_saved, const char *what) {
+    TORCH_CHECK(as_saved, what, ": a gradient or a tensor that was saved for the backward pass has another device, type or shape than it had, or no memory of its own");
+}
+void check_saved_logits(const at::Tensor &t, const char *what) { check_saved(t.is_cuda() && t.has_storage() && is_float(t) && t.dim() >= 1 && t.size(-1) >= 1, what); }
+
 // A backward pass that is recorded itself (create_graph): its result can be had, and what differentiates it again is told that it cannot.
 variable_list differentiable_once(const at::Tensor &d, const char *what, size_t inputs) {
     variable_list out(inputs);
@@ -1071,14 +1080,26 @@ struct TokenLogProbs : torch::autograd::Function<TokenLogProbs> {
     static variable_list backward(torch::autograd::AutogradContext *ctx, variable_list g) {
         check_no_tangents(g, "token_log_probs");
         const variable_list saved = ctx->get_saved_variables();
-        const at::Tensor &logits = saved[0], &targets = saved[1], &entropy = saved[2], &norm = saved[3], &top_ids = saved[4];
+        const at::Tensor &logits = saved[0];
+        const char *what = "token_log_probs";
+        check_saved_logits(logits, what);
+        const int64_t rows = logits.numel() / logits.size(-1);
+        auto packed = [&](const at::Tensor &t, at::ScalarType type, int64_t each) {
+            if (!t.defined()) return t;
+            check_saved(lives_with(t, logits) && t.scalar_type() == type && t.numel() == rows * each, what);
+            return packed_rows(t);
+        };
+        const int64_t top = saved[4].defined() && saved[4].dim() > 0 ? saved[4].size(-1) : 0;
+        const at::Tensor targets = packed(saved[1], at::kLong, 1), entropy = packed(saved[2], at::kFloat, 1), norm = packed(saved[3], at::kFloat, 2), top_ids = packed(saved[4], at::kLong, top);
         size_t next = 2;
         const at::Tensor g_entropy = f32_rows(g[0]), g_lse = f32_rows(g[1]), g_log_prob = targets.defined() ? f32_rows(g[next++]) : at::Tensor(), g_top = top_ids.defined() ? f32_rows(g[next]) : at::Tensor();
+        for (const at::Tensor *t : {&g_entropy, &g_lse, &g_log_prob}) check_saved(!t->defined() || (lives_with(*t, logits) && t->numel() == rows), what);
+        check_saved(!g_top.defined() || (lives_with(g_top, logits) && g_top.numel() == rows * top), what);
         const c10::cuda::CUDAGuard guard(logits.device());
         const LogitRows x = logit_rows(logits), d = gradient_of(x);
         if (x.rows > 0)
             check_backward(nmg_token_log_probs_backward(x.t.const_data_ptr(), x.rows, x.inner, x.ld, x.ld_outer, x.vocab, float_code(logits, "logits"), i64_ptr(targets), ctx->saved_data["ignore"].toInt(),
-                                                        (float)ctx->saved_data["temperature"].toDouble(), top_ids.defined() ? (int)top_ids.size(-1) : 0, i64_ptr(top_ids), f32_ptr(norm), f32_ptr(entropy),
+                                                        (float)ctx->saved_data["temperature"].toDouble(), (int)top, i64_ptr(top_ids), f32_ptr(norm), f32_ptr(entropy),
                                                         f32_ptr(g_log_prob), f32_ptr(g_entropy), f32_ptr(g_lse), f32_ptr(g_top), d.t.mutable_data_ptr(), d.ld, d.ld_outer, stream_of(logits.device())));
         return differentiable_once(d.t, "token_log_probs", 5);
     }
@@ -1180,16 +1201,27 @@ struct Distill : torch::autograd::Function<Distill> {
     static variable_list backward(torch::autograd::AutogradContext *ctx, variable_list g) {
         check_no_tangents(g, "distillation_loss");
         const variable_list saved = ctx->get_saved_variables();
-        const at::Tensor &logits = saved[0];
-        const at::Tensor upstream = f32_rows(g[0]);
+        const at::Tensor &logits = saved[0], &ids = saved[1], &log_probs = saved[2], &weight = saved[3], &norm = saved[4], &total = saved[5];
+        const char *what = "distillation_loss";
+        check_saved_logits(logits, what);
+        const int64_t rows = logits.numel() / logits.size(-1);
+        const int reduction = (int)ctx->saved_data["reduction"].toInt();
+        const c10::IntArrayRef lead = logits.sizes().slice(0, logits.dim() - 1);
+        check_saved(lives_with(ids, logits) && (ids.scalar_type() == at::kLong || ids.scalar_type() == at::kInt) && ids.dim() == logits.dim() && ids.size(-1) >= 1 && ids.sizes().slice(0, ids.dim() - 1) == lead, what);
+        check_saved(lives_with(log_probs, logits) && is_float(log_probs) && log_probs.sizes() == ids.sizes(), what);
+        check_saved(!weight.defined() || (lives_with(weight, logits) && weight.scalar_type() == at::kFloat && weight.sizes() == lead), what);
+        check_saved(lives_with(norm, logits) && norm.scalar_type() == at::kFloat && norm.numel() == 4 * rows, what);
+        check_saved(!total.defined() || (lives_with(total, logits) && total.scalar_type() == at::kFloat && total.numel() == 1), what);
+        const at::Tensor upstream = f32_rows(g[0]), norms = packed_rows(norm);
+        check_saved(lives_with(upstream, logits) && upstream.numel() == (reduction == NMG_REDUCE_NONE ? rows : 1), what);
         at::Tensor made;
         if (const auto it = ctx->saved_data.find("made"); it != ctx->saved_data.end()) {  // it becomes the caller's: a second backward pass makes its own
             made = it->second.toTensor();
             ctx->saved_data.erase(it);
+            check_saved(made.device() == logits.device() && made.scalar_type() == logits.scalar_type() && made.sizes() == logits.sizes(), what);
         }
         const c10::cuda::CUDAGuard guard(logits.device());
-        const Teacher t = teacher_of(saved[1], saved[2], saved[3], logits);
-        const int reduction = (int)ctx->saved_data["reduction"].toInt();
+        const Teacher t = teacher_of(ids, log_probs, weight, logits);
         LogitRows x = logit_rows(logits), d = x;
         if (made.defined()) {
             d = logit_rows(made);
@@ -1198,8 +1230,8 @@ struct Distill : torch::autograd::Function<Distill> {
         if (!made.defined()) d = gradient_of(x);
         if (x.rows > 0)
             check_backward(nmg_distill_backward(x.t.const_data_ptr(), x.rows, x.inner, x.ld, x.ld_outer, x.vocab, float_code(logits, "logits"), t.ids.const_data_ptr(), t.id_bytes, t.log_probs.const_data_ptr(),
-                                                t.code, (int)t.kept, (int)ctx->saved_data["remainder"].toInt(), (float)ctx->saved_data["temperature"].toDouble(), f32_ptr(t.weight), reduction, f32_ptr(saved[4]),
-                                                f32_ptr(saved[5]), f32_ptr(upstream), made.defined(), d.t.mutable_data_ptr(), d.ld, d.ld_outer, stream_of(logits.device())));
+                                                t.code, (int)t.kept, (int)ctx->saved_data["remainder"].toInt(), (float)ctx->saved_data["temperature"].toDouble(), f32_ptr(t.weight), reduction, f32_ptr(norms),
+                                                f32_ptr(total), f32_ptr(upstream), made.defined(), d.t.mutable_data_ptr(), d.ld, d.ld_outer, stream_of(logits.device())));
         return differentiable_once(d.t, "distillation_loss", 7);
     }
 };
