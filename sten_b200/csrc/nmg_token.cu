@@ -372,6 +372,7 @@ template <typename T, int NT, bool E> __global__ void __launch_bounds__(NT, SM_T
         if (!in_row && target != p.ignore) A = __int_as_float(0x7fffffff);  // no such token
         const bool empty = norm.empty();
         const float m = empty ? 0.f : norm.m, ln = norm.ln, a = p.a, ln2 = ln * LOG2E;  // nothing but -inf: p = 0 below
+        if (empty && (in_row || target == p.ignore)) A = B = 0.f;  // whatever the incoming gradients are
         A *= p.inv_tau;
         B *= p.inv_tau;
         const float lin = A - B * ln, B_x = B * p.inv_tau;  // A + B log p = lin + B (x - m) / tau
