@@ -376,11 +376,13 @@ template <typename T, int NT, bool E> __global__ void __launch_bounds__(NT, SM_T
         A *= p.inv_tau;
         B *= p.inv_tau;
         const float lin = A - B * ln, B_x = B * p.inv_tau;  // A + B log p = lin + B (x - m) / tau
+        // Below 2^-1000 a probability is 0 in 32 bits: further exponents (masks) give the same 0, and no product that overflows beside it
+        const float lowest = -1000.f / a;
         auto grad = [&](float2 x) {
             const float2 d = __fadd2_rn(x, both(-m)), t = __ffma2_rn(d, both(a), both(-ln2)), e = make_float2(exp2_fast(t.x), exp2_fast(t.y));
             if constexpr (!E) return __fmul2_rn(e, both(A));
             float2 y = __fmul2_rn(e, __ffma2_rn(d, both(B_x), both(lin)));
-            if (y.x != y.x || y.y != y.y) y = make_float2(e.x * (lin + B_x * fmaxf(d.x, -1e30f)), e.y * (lin + B_x * fmaxf(d.y, -1e30f)));  // masked: 0 * -inf is not a part of it
+            if (y.x != y.x || y.y != y.y) y = make_float2(e.x * (lin + B_x * fmaxf(d.x, lowest)), e.y * (lin + B_x * fmaxf(d.y, lowest)));  // masked: 0 * -inf is not a part of it
             return y;
         };
         // t = log2 p in one instruction, off by `off`, which goes into the factors: A + B log p = A + B ln 2 (t - off)
@@ -391,7 +393,7 @@ template <typename T, int NT, bool E> __global__ void __launch_bounds__(NT, SM_T
                 const float2 t = __ffma2_rn(x, both(a), both(ex.c)), e = make_float2(exp2_fast(t.x), exp2_fast(t.y));
                 if constexpr (!E) return __fmul2_rn(e, both(A_t));
                 float2 y = __fmul2_rn(e, __ffma2_rn(t, both(B_t), both(A_t)));
-                if (y.x != y.x || y.y != y.y) y = make_float2(e.x * (A_t + B_t * fmaxf(t.x, -1e30f)), e.y * (A_t + B_t * fmaxf(t.y, -1e30f)));
+                if (y.x != y.x || y.y != y.y) y = make_float2(e.x * (A_t + B_t * fmaxf(t.x, -1000.f)), e.y * (A_t + B_t * fmaxf(t.y, -1000.f)));
                 return y;
             });
         } else {
