@@ -272,7 +272,9 @@ int nmg_token_log_probs_backward(const void *logits, int64_t rows, int64_t inner
  *                  together (left out where the student has no finite logit among them); vocab at most 2^20
  *   row_loss = temperature^2 * weight[r] * sum q (log q - log softmax(z));  weight may be NULL (all 1)
  * A row of weight 0, without a kept token of non-zero q, or of logits -inf throughout has loss 0 and gradient 0.  An id of
- * vocab or more makes its row NaN; an id that occurs twice in a row stands for one token of the summed q.
+ * vocab or more makes its row NaN; an id that occurs twice in a row is one token to the gradient (that of
+ * the summed q) and to the remainder, while row_loss keeps a term q (log q - log softmax(z)) for each of its entries: it is lower than
+ * for the summed q by the entropy of the split, whatever the logits are, and may be below 0.
  * reduction: NMG_REDUCE_NONE row_loss is the result; NMG_REDUCE_SUM loss = sum row_loss; NMG_REDUCE_MEAN that divided by the sum of
  * the weights (by rows without weights; 0 where it is 0).  Sums over rows are added in 64 bits in a fixed order.
  * norm [rows][4] (8-byte aligned) and total [1] are written for nmg_distill_backward.  d_logits, where not NULL (a reduction only), receives

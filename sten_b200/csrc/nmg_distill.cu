@@ -146,7 +146,7 @@ template <typename T, int NT, bool REST, bool STATS, bool GRAD> __global__ void 
             }
         }
         const bool bad = __syncthreads_or(none_such);
-        if (twice) {  // an id that is there more than once counts as one token with the sum of its q
+        if (twice) {  // an id that is there more than once is one token, whose gradient has the sum of its q; the loss has a term for each entry
             if (id >= 0)
                 for (int i = 0; i < tid; i++)
                     if (sh.id[i] == id) sh.later[tid] = 1;

@@ -64,6 +64,9 @@ def distillation_loss(logits, teacher_ids, teacher_log_probs, *, remainder=False
     A reduced loss of logits that require a gradient keeps, beside them, a tensor of their size with their gradient until its backward
     pass.  That tensor is not among the saved ones: hooks on those (``save_on_cpu``, checkpointing) leave it on the device.
 
+    A token that occurs more than once among a row's ids has a term of its own in the loss for each occurrence, which lowers the loss by
+    a constant and may take it below 0; the gradient and the remainder are those of one token with the summed probability.
+
     Gradients go to the logits only.  Rows of which the mask (or the padding) leaves nothing have loss 0 and gradient 0."""
     if reduction not in _REDUCTIONS:
         raise ValueError(f"reduction must be 'none', 'sum' or 'mean', got {reduction!r}")
