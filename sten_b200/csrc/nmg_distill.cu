@@ -52,6 +52,13 @@ struct KeptShared {
     int some;
 };
 
+template <int NT> struct DistillShared {
+    KeptShared kept_rows[2];  // of this row and of the one before
+    Stats red[NT / 32], part;
+    int twice_rows[2];
+    uint32_t steps_marked[NT];  // bit s: a kept token is among step s (modulo 32) of the thread's vectors
+};
+
 __device__ __forceinline__ float teacher_value(const void *p, int dtype, int64_t i) {
     if (dtype == NMG_F32) return static_cast<const float *>(p)[i];
     if (dtype == NMG_F16) return __half2float(static_cast<const __half *>(p)[i]);
@@ -76,11 +83,9 @@ template <typename T> __device__ __forceinline__ uint4 leave_out(uint4 q, uint32
 
 template <typename T, int NT, bool REST, bool STATS, bool GRAD> __global__ void __launch_bounds__(NT, SM_THREADS / NT) distill_kernel(const __grid_constant__ DistillParams p) {
     extern __shared__ __align__(16) unsigned char smem[];
-    __shared__ Stats red[NT / 32], part;
-    __shared__ KeptShared kept_rows[2];  // of this row and of the one before
-    __shared__ int twice_rows[2];
+    __shared__ DistillShared<NT> fixed;
+    auto &[kept_rows, red, part, twice_rows, steps_marked] = fixed;
     uint32_t *bits = reinterpret_cast<uint32_t *>(smem + RING_BYTES<NT>);
-    __shared__ uint32_t steps_marked[NT];  // bit s: a kept token is among step s (modulo 32) of the thread's vectors
     const int tid = (int)threadIdx.x, lane = tid & 31, warp = tid >> 5, rank = (int)(blockIdx.x % (unsigned)p.parts);
     const unsigned first = blockIdx.x / (unsigned)p.parts, step = gridDim.x / (unsigned)p.parts;
     if (GRAD && !STATS && p.skip_if_one && *p.upstream == 1.f) return;  // the gradient that is there already is this one
@@ -306,7 +311,7 @@ __global__ void __launch_bounds__(1024) ordered_sum_kernel(const float *v, int64
 template <typename T, int NT, bool REST, bool STATS, bool GRAD> static int launch_distill(DistillParams &p, Deal deal, int sms, cudaStream_t st) {
     const size_t smem = RING_BYTES<NT> + (REST ? ((size_t)p.x.vocab + BIT0 + 31) / 32 : FILTER_BITS / 32) * 4;
     NMG_ALLOW_SMEM(smem, distill_kernel<T, NT, REST, STATS, GRAD>);
-    return launch_rows(distill_kernel<T, NT, REST, STATS, GRAD>, p.x.rows, deal, sms, smem, sizeof(KeptShared) * 2 + (3 << 10), st, p);
+    return launch_rows(distill_kernel<T, NT, REST, STATS, GRAD>, p.x.rows, deal, sms, smem, sizeof(DistillShared<NT>) + (1 << 10), st, p);
 }
 template <bool STATS, bool GRAD> static int launch_distill_any(DistillParams &p, int dtype, bool rest, cudaStream_t st) {
     int sms, rc;
