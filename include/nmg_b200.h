@@ -244,7 +244,7 @@ int nmg_spmm_noalloc(const void *val, const int16_t *idx, int64_t M, int64_t K, 
  * model code).  Row r < rows begins at element (r / inner_rows) * ld_outer + (r % inner_rows) * ld of `logits` and has `vocab`
  * consecutive elements of `dtype`; base and strides need no alignment beyond the element's.  z = x / temperature, everything
  * is computed in 32 bits.  Logits may be -inf (masked).  A row that is -inf throughout has no distribution: its log-sum-exp
- * and log-probabilities are -inf, its entropy, its divergence and its gradient 0.  A row that holds NaN or +inf gives NaN.
+ * and log-probabilities are -inf, its entropy, its divergence and its gradient 0 (whatever gradients come in).  A row that holds NaN or +inf gives NaN.
  *
  * nmg_token_log_probs writes, in fp32 and for every row,
  *   log_prob  log softmax(z) at targets[r]; 0 where that is ignore_index, NaN where there is no such token (targets and log_prob
@@ -255,7 +255,7 @@ int nmg_spmm_noalloc(const void *val, const int16_t *idx, int64_t M, int64_t K, 
  *   top_log_prob, top_ids   [rows][top] log-probabilities and columns of the `top` (0 .. 128) largest logits, largest first, equal
  *             ones in the order of their columns (-0 equals 0, NaN counts as larger than all)
  * nmg_token_log_probs_backward writes d_logits (row pitches ld_d, ld_d_outer) from the gradients of those outputs, any of which
- * may be NULL; it reads norm always, entropy with g_entropy, top_ids with g_top. */
+ * may be NULL; it reads norm always, entropy with g_entropy, top_ids with g_top.  d_logits, here and below, must not overlap the logits. */
 int nmg_token_log_probs(const void *logits, int64_t rows, int64_t inner_rows, int64_t ld, int64_t ld_outer, int64_t vocab, int dtype,
                         const int64_t *targets, int64_t ignore_index, float temperature, int top, float *log_prob, float *entropy,
                         float *lse, float *top_log_prob, int64_t *top_ids, float *norm, void *stream);
@@ -271,7 +271,7 @@ int nmg_token_log_probs_backward(const void *logits, int64_t rows, int64_t inner
  *   remainder = 1: q_i = exp(log_prob), and 1 - sum q (at least 0) is held against the student's probability of all other tokens
  *                  together (left out where the student has no finite logit among them); vocab at most 2^20
  *   row_loss = temperature^2 * weight[r] * sum q (log q - log softmax(z));  weight may be NULL (all 1)
- * A row of weight 0, without a kept token of non-zero q, or of logits -inf throughout has loss 0 and gradient 0.  An id of
+ * A row of weight 0, of logits -inf throughout, or (remainder = 0) without a kept token of non-zero q has loss 0 and gradient 0.  An id of
  * vocab or more makes its row NaN; an id that occurs twice in a row is one token to the gradient (that of
  * the summed q) and to the remainder, while row_loss keeps a term q (log q - log softmax(z)) for each of its entries: it is lower than
  * for the summed q by the entropy of the split, whatever the logits are, and may be below 0.

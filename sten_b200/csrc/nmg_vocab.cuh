@@ -20,7 +20,8 @@
 
 namespace nmg {
 
-// A row belongs to a CTA of NT threads (64 to 512, template argument), or to a cluster of them; an SM holds SM_THREADS of them.
+// A row belongs to a CTA of NT threads (64 to 512, template argument), or to a cluster of them; an SM holds SM_THREADS of them, or as many as
+// shared memory has room for (distillation: 6 of 8 CTAs of 128 threads).
 constexpr int SM_THREADS = 1024;
 
 struct Logits {
@@ -482,6 +483,7 @@ template <int NT, typename T> __device__ __forceinline__ void zero_pass(const Sl
 
 // How rows are dealt out: NT threads a CTA and `parts` CTAs a row, by the least estimated time in units of a vector a thread on a full SM.
 // A row's end and beginning cost a thread about as much as ten vectors, the meetings of a cluster's CTAs ten more; the rounds are whole.
+// SM_THREADS on every SM are taken for granted, whatever shared memory allows.
 // Where one round does, what counts is latency: larger CTAs take longer to meet, and a half-empty SM is faster, up to twice.  `meeting`:
 // what a cluster has to do beyond its statistics.  Measured (us, NT = 64 / 128 / 256 / 512): 12288 rows of 30522 fp16 133 / 143 / 168 /
 // 206; 777 rows of 32003 fp32 39 / 32 / 37 / 41; 4096 rows of 131072 bf16 with 64 alternatives - / 311 / 268 / 283; 64 such rows with 20,
