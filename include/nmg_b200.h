@@ -291,6 +291,31 @@ int nmg_distill_backward(const void *logits, int64_t rows, int64_t inner_rows, i
                          float temperature, const float *weight, int reduction, const float *norm, const float *total, const float *upstream, int skip_if_one, void *d_logits, int64_t ld_d,
                          int64_t ld_d_outer, void *stream);
 
+/* Layer norm (no counterpart in the reference, which leaves it to the model code).  Rows r < rows of `width` elements begin at element
+ * r * ld; y, sum and d_x are [rows][width] without gaps.  weight and bias: [width] of param_dtype (dtype or NMG_F32), NULL: ones, zeros.
+ *   h = x, or with a residual sum = x + residual rounded to dtype, which is written
+ *   y = (h - mean) rstd weight + bias,  rstd = 1 / sqrt(mean of (h - mean)^2 + eps);  stats [rows][2] (8-byte aligned, may be NULL): mean, rstd
+ * nmg_layer_norm_backward takes h (x or sum) and stats, the gradient of y and (or NULL) that of sum, and writes d_x, which is the residual's
+ * gradient too, d_weight and d_bias, each unless NULL.  The sums over rows are added in 32 bits in a fixed order.  The workspace (16-byte
+ * aligned) is needed for d_weight and d_bias only; its size depends on the current device.  No output may overlap an input. */
+int nmg_layer_norm(const void *x, int64_t ld_x, const void *residual, int64_t ld_residual, int64_t rows, int64_t width, int dtype,
+                   const void *weight, const void *bias, int param_dtype, float eps, void *y, void *sum, float *stats, void *stream);
+size_t nmg_layer_norm_backward_workspace_bytes(int64_t rows, int64_t width);
+int nmg_layer_norm_backward(const void *h, int64_t ld_h, int64_t rows, int64_t width, int dtype, const void *weight, int param_dtype,
+                            const float *stats, const void *g_y, int64_t ld_g_y, const void *g_sum, int64_t ld_g_sum, void *d_x,
+                            void *d_weight, void *d_bias, void *workspace, size_t workspace_bytes, void *stream);
+
+/* Embedding (no counterpart in the reference).  out[t] = scale * weight[ids[t]], [tokens][width] without gaps; the rows of weight[vocab][width]
+ * are ld elements apart, ids have id_bytes 4 or 8 each.  An id outside 0 .. vocab - 1 makes its row NaN and adds to no gradient.
+ * nmg_embedding_backward writes all of d_weight[vocab][width] (no gaps, 16-byte aligned): scale times the sum of the rows of g that
+ * belong to a row, in the order of their positions and in 32 bits, zero where there are none and in row `padding` (-1: no such row).
+ * workspace: 16-byte aligned. */
+int nmg_embedding(const void *weight, int64_t vocab, int64_t width, int64_t ld, int dtype, const void *ids, int id_bytes, int64_t tokens,
+                  float scale, void *out, void *stream);
+size_t nmg_embedding_backward_workspace_bytes(int64_t tokens, int64_t width);
+int nmg_embedding_backward(const void *g, int64_t ld_g, int64_t tokens, int64_t width, int dtype, const void *ids, int id_bytes, int64_t vocab,
+                           int64_t padding, float scale, void *d_weight, void *workspace, size_t workspace_bytes, void *stream);
+
 /* Measurement helpers (no counterpart in the reference; its profiling is wall-clock around whole operators,
  * src/sten/sten.py:30-49).
  * nmg_profile_next: the next nmg_spmm / nmg_spmm_t call made by this thread records `start_event` immediately before

@@ -58,6 +58,12 @@ SIGNATURES = {
     "nmg_distill": (_int, [_vp, _i64, _i64, _i64, _i64, _i64, _int, _vp, _int, _vp, _int, _int, _int, _f32, _vp, _int, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _vp]),
     "nmg_distill_backward": (_int, [_vp, _i64, _i64, _i64, _i64, _i64, _int, _vp, _int, _vp, _int, _int, _int, _f32, _vp, _int, _vp, _vp, _vp, _int, _vp, _i64, _i64,
                                     _vp]),
+    "nmg_layer_norm": (_int, [_vp, _i64, _vp, _i64, _i64, _i64, _int, _vp, _vp, _int, _f32, _vp, _vp, _vp, _vp]),
+    "nmg_layer_norm_backward_workspace_bytes": (_sz, [_i64, _i64]),
+    "nmg_layer_norm_backward": (_int, [_vp, _i64, _i64, _i64, _int, _vp, _int, _vp, _vp, _i64, _vp, _i64, _vp, _vp, _vp, _vp, _sz, _vp]),
+    "nmg_embedding": (_int, [_vp, _i64, _i64, _i64, _int, _vp, _int, _i64, _f32, _vp, _vp]),
+    "nmg_embedding_backward_workspace_bytes": (_sz, [_i64, _i64]),
+    "nmg_embedding_backward": (_int, [_vp, _i64, _i64, _i64, _int, _vp, _int, _i64, _i64, _f32, _vp, _vp, _sz, _vp]),
     "nmg_profile_next": (_int, [_vp, _vp]),
     "nmg_measure_fma_peak": (_int, [ctypes.POINTER(ctypes.c_double), _vp]),
     "nmg_memcpy_2d_async": (_int, [_vp, _sz, _vp, _sz, _sz, _sz, _vp]),

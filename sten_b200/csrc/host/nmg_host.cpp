@@ -1015,16 +1015,25 @@ void check_saved(bool as_saved, const char *what) {
 }
 void check_saved_logits(const at::Tensor &t, const char *what) { check_saved(t.is_cuda() && t.has_storage() && is_float(t) && t.dim() >= 1 && t.size(-1) >= 1, what); }
 
-// A backward pass that is recorded itself (create_graph): its result can be had, and what differentiates it again is told that it cannot.
+// A backward pass that is recorded itself (create_graph): its results can be had, and what differentiates them again is told that it cannot.
+variable_list differentiable_once(variable_list out, const char *what) {
+    if (!c10::GradMode::is_enabled()) return out;
+    variable_list fakes;
+    for (const at::Tensor &d : out)
+        if (d.defined()) {
+            fakes.push_back(d.detach());
+            fakes.back().set_requires_grad(true);
+        }
+    variable_list recorded = (*std::make_shared<torch::autograd::DelayedError>(std::string(what) + " is differentiable once", (int64_t)fakes.size()))(std::move(fakes));
+    size_t next = 0;
+    for (at::Tensor &d : out)
+        if (d.defined()) d = recorded[next++];
+    return out;
+}
 variable_list differentiable_once(const at::Tensor &d, const char *what, size_t inputs) {
     variable_list out(inputs);
     out[0] = d;
-    if (c10::GradMode::is_enabled()) {
-        at::Tensor fake = d.detach();
-        fake.set_requires_grad(true);
-        out[0] = (*std::make_shared<torch::autograd::DelayedError>(std::string(what) + " is differentiable once", 1))({fake})[0];
-    }
-    return out;
+    return differentiable_once(std::move(out), what);
 }
 
 std::optional<at::Tensor> maybe(const at::Tensor &t) { return t.defined() ? std::optional<at::Tensor>(t) : std::nullopt; }  // autograd takes no undefined inputs
@@ -1256,6 +1265,221 @@ PyObject *py_distill(PyObject *, PyObject *const *a, Py_ssize_t nargs) {
     NMG_PY_END
 }
 
+// ------------------------------------------------------------------------------------------------ between the products
+// A backward pass in a CUDA graph meets the node that accumulates a leaf's gradient.  One that an eager graph on the legacy default stream
+// keeps alive would have autograd wait for that stream, which no capture can do: the error comes on one of autograd's threads.
+void refuse_foreign_accumulators(std::initializer_list<const at::Tensor *> ts, c10::Device dev, const char *what) {
+    if (!capturing(dev)) return;
+    for (const at::Tensor *t : ts) {
+        if (!t->defined() || !t->requires_grad() || !t->is_leaf()) continue;
+        const auto node = torch::autograd::impl::try_get_grad_accumulator(*t);
+        if (!node) continue;
+        const std::optional<c10::Stream> made_on = node->stream();
+        if (made_on && c10::cuda::CUDAStream(*made_on) == c10::cuda::getDefaultCUDAStream(dev.index()))
+            py_raise(PyExc_RuntimeError, std::string(what) + ": a graph that was recorded outside of this capture on the default stream still holds a leaf of this call; "
+                                         "release its outputs before capturing, or record under torch.no_grad()");
+    }
+}
+
+// The rows of a tensor whose last dimension has been checked; without the interpreter.
+Rows hidden_rows(const at::Tensor &t, int64_t width) {
+    const int64_t rows = t.numel() / width;
+    at::Tensor r = t.dim() == 2 ? t : t.is_contiguous() ? t : t.reshape({rows, width});
+    if (r.dim() == 2 && !r.is_contiguous() && (r.stride(1) != 1 || r.stride(0) < width)) r = r.contiguous();
+    return Rows{r, rows, width, r.is_contiguous() || rows < 2 ? width : r.stride(0)};
+}
+const void *const_ptr(const at::Tensor &t) { return t.defined() ? t.const_data_ptr() : nullptr; }
+void *out_ptr(const at::Tensor &t) { return t.defined() ? t.mutable_data_ptr() : nullptr; }
+int type_code(const at::Tensor &t) { return t.scalar_type() == at::kFloat ? NMG_F32 : t.scalar_type() == at::kHalf ? NMG_F16 : NMG_BF16; }  // of a type that has been checked
+
+struct NormOut { at::Tensor y, sum, stats; };
+NormOut norm_forward(const at::Tensor &x, const at::Tensor &residual, const at::Tensor &weight, const at::Tensor &bias, float eps, bool with_stats) {
+    const int64_t width = x.size(-1);
+    const Rows rx = hidden_rows(x, width), rr = residual.defined() ? hidden_rows(residual, width) : Rows{at::Tensor(), 0, 0, 0};
+    const at::Tensor w = weight.defined() ? packed_rows(weight) : weight, b = bias.defined() ? packed_rows(bias) : bias;
+    NormOut o;
+    o.y = new_empty(x.sizes(), x.scalar_type());
+    if (residual.defined()) o.sum = new_empty(x.sizes(), x.scalar_type());
+    if (with_stats) o.stats = new_empty({rx.rows, 2}, at::kFloat);
+    if (rx.rows > 0) {
+        void *st = stream_of(x.device());
+        const int rc = without_interpreter([&] {
+            return nmg_layer_norm(rx.t.const_data_ptr(), rx.ld, const_ptr(rr.t), rr.ld, rx.rows, width, type_code(x), const_ptr(w), const_ptr(b),
+                                  w.defined() ? type_code(w) : b.defined() ? type_code(b) : type_code(x), eps, o.y.mutable_data_ptr(), out_ptr(o.sum), f32_out(o.stats), st);
+        });
+        check(rc);
+    }
+    return o;
+}
+
+struct LayerNorm : torch::autograd::Function<LayerNorm> {
+    static variable_list forward(torch::autograd::AutogradContext *ctx, const at::Tensor &x, const std::optional<at::Tensor> &given_residual, const std::optional<at::Tensor> &given_weight,
+                                 const std::optional<at::Tensor> &given_bias, double eps) {
+        const at::Tensor residual = given_residual.value_or(at::Tensor()), weight = given_weight.value_or(at::Tensor()), bias = given_bias.value_or(at::Tensor());
+        const NormOut o = norm_forward(x, residual, weight, bias, (float)eps, true);
+        ctx->save_for_backward({residual.defined() ? o.sum : x, weight, o.stats});
+        // the places of the tensors among the inputs that have a gradient, -1: not there
+        int64_t next = 1;
+        ctx->saved_data["residual"] = residual.defined() ? next++ : (int64_t)-1;
+        ctx->saved_data["weight"] = weight.defined() ? next++ : (int64_t)-1;
+        ctx->saved_data["bias"] = bias.defined() ? next++ : (int64_t)-1;
+        ctx->saved_data["param_type"] = (int64_t)(weight.defined() ? weight : bias.defined() ? bias : x).scalar_type();
+        ctx->set_materialize_grads(false);
+        return residual.defined() ? variable_list{o.y, o.sum} : variable_list{o.y};
+    }
+    static variable_list backward(torch::autograd::AutogradContext *ctx, variable_list g) {
+        const char *what = "layer_norm";
+        check_no_tangents(g, what);
+        const variable_list saved = ctx->get_saved_variables();
+        const at::Tensor &h = saved[0], &weight = saved[1], &stats = saved[2];
+        check_saved(h.is_cuda() && h.has_storage() && is_float(h) && h.dim() >= 1 && h.size(-1) >= 1, what);
+        const int64_t width = h.size(-1), rows = h.numel() / width;
+        const auto param_type = (at::ScalarType)ctx->saved_data["param_type"].toInt();
+        const int64_t at_residual = ctx->saved_data["residual"].toInt(), at_weight = ctx->saved_data["weight"].toInt(), at_bias = ctx->saved_data["bias"].toInt();
+        check_saved(param_type == h.scalar_type() || param_type == at::kFloat, what);
+        check_saved(weight.defined() == (at_weight >= 0) && (!weight.defined() || (lives_with(weight, h) && weight.scalar_type() == param_type && weight.numel() == width)), what);
+        check_saved(stats.defined() && lives_with(stats, h) && stats.scalar_type() == at::kFloat && stats.numel() == 2 * rows, what);
+        const at::Tensor &g_y = g[0], g_sum = g.size() > 1 ? g[1] : at::Tensor();
+        for (const at::Tensor *t : {&g_y, &g_sum}) check_saved(!t->defined() || (lives_with(*t, h) && t->scalar_type() == h.scalar_type() && t->sizes() == h.sizes()), what);
+        const bool need_x = ctx->needs_input_grad(0) || (at_residual >= 0 && ctx->needs_input_grad((size_t)at_residual));
+        const bool need_w = at_weight >= 0 && ctx->needs_input_grad((size_t)at_weight), need_b = at_bias >= 0 && ctx->needs_input_grad((size_t)at_bias);
+        const c10::cuda::CUDAGuard guard(h.device());
+        at::Tensor d, dw, db;
+        if (!g_y.defined()) {
+            d = g_sum;  // the norm has no part in it
+        } else {
+            if (need_x) d = new_empty(h.sizes(), h.scalar_type());
+            if (need_w) dw = new_empty({width}, param_type);
+            if (need_b) db = new_empty({width}, param_type);
+            if (rows < 1) {
+                for (at::Tensor *t : {&dw, &db})
+                    if (t->defined()) t->zero_();
+            } else if (need_x || need_w || need_b) {
+                const Rows rh = hidden_rows(h, width), ry = hidden_rows(g_y, width), rs = g_sum.defined() ? hidden_rows(g_sum, width) : Rows{at::Tensor(), 0, 0, 0};
+                const at::Tensor w = weight.defined() ? packed_rows(weight) : weight, st = packed_rows(stats);
+                const size_t nbytes = need_w || need_b ? nmg_layer_norm_backward_workspace_bytes(rows, width) : 0;
+                const at::Tensor ws = nbytes ? new_empty({(int64_t)nbytes}, at::kByte) : at::Tensor();
+                check_backward(nmg_layer_norm_backward(rh.t.const_data_ptr(), rh.ld, rows, width, type_code(h), const_ptr(w), param_type == at::kFloat ? NMG_F32 : type_code(h), f32_ptr(st),
+                                                       ry.t.const_data_ptr(), ry.ld, const_ptr(rs.t), rs.ld, out_ptr(d), out_ptr(dw), out_ptr(db), out_ptr(ws), nbytes, stream_of(h.device())));
+            }
+        }
+        return differentiable_once({d, at_residual >= 0 ? d : at::Tensor(), dw, db, at::Tensor()}, what);
+    }
+};
+
+// layer_norm(x, weight, bias, eps, residual) -> y, or (y, sum) where there is a residual
+PyObject *py_layer_norm(PyObject *, PyObject *const *a, Py_ssize_t nargs) {
+    NMG_PY_BEGIN(5)
+    const at::Tensor &x = tensor_arg(a[0]);
+    const at::Tensor weight = optional_tensor(a[1]), bias = optional_tensor(a[2]), residual = optional_tensor(a[4]);
+    const double eps = double_arg(a[3]);
+    const c10::Device dev = device_of({&x, &weight, &bias, &residual});
+    float_code(x, "x");
+    refuse_tangents({&x, &weight, &bias, &residual}, "layer_norm");
+    if (x.dim() < 1 || x.size(-1) < 1) py_raise(PyExc_ValueError, "x must have a last dimension of at least one feature, got shape " + shape_str(x.sizes()));
+    for (const at::Tensor *t : {&weight, &bias}) {
+        if (!t->defined()) continue;
+        const std::string name = t == &weight ? "weight" : "bias";
+        float_code(*t, name.c_str());
+        if (t->dim() != 1 || t->size(0) != x.size(-1)) py_raise(PyExc_ValueError, name + " must have one element per feature (" + std::to_string(x.size(-1)) + "), got shape " + shape_str(t->sizes()));
+        if (t->scalar_type() != x.scalar_type() && t->scalar_type() != at::kFloat) py_raise(PyExc_TypeError, name + " must be of x's type or float32, got " + c10::toString(t->scalar_type()));
+    }
+    if (weight.defined() && bias.defined() && weight.scalar_type() != bias.scalar_type()) py_raise(PyExc_TypeError, "weight and bias must be of one type");
+    if (residual.defined()) {
+        if (residual.scalar_type() != x.scalar_type()) py_raise(PyExc_TypeError, std::string("residual must be of x's type, got ") + c10::toString(residual.scalar_type()));
+        if (residual.sizes() != x.sizes()) py_raise(PyExc_ValueError, "residual must have the shape of x " + shape_str(x.sizes()) + ", got " + shape_str(residual.sizes()));
+    }
+    const c10::cuda::CUDAGuard guard(dev);
+    at::Tensor y, sum;
+    if (c10::GradMode::is_enabled() && (x.requires_grad() || (residual.defined() && residual.requires_grad()) || (weight.defined() && weight.requires_grad()) || (bias.defined() && bias.requires_grad()))) {
+        refuse_foreign_accumulators({&x, &residual, &weight, &bias}, dev, "layer_norm");
+        const variable_list v = LayerNorm::apply(x, maybe(residual), maybe(weight), maybe(bias), eps);
+        y = v[0];
+        if (residual.defined()) sum = v[1];
+    } else {
+        const NormOut o = norm_forward(x, residual, weight, bias, (float)eps, false);
+        y = o.y;
+        sum = o.sum;
+    }
+    if (!residual.defined()) return THPVariable_Wrap(y);
+    PyObject *r = PyTuple_New(2);
+    set_item(r, 0, y);
+    set_item(r, 1, sum);
+    return r;
+    NMG_PY_END
+}
+
+at::Tensor embed_forward(const at::Tensor &weight, const at::Tensor &ids, float scale) {
+    const Rows w = hidden_rows(weight, weight.size(1));
+    std::vector<int64_t> shape(ids.sizes().begin(), ids.sizes().end());
+    shape.push_back(w.cols);
+    const at::Tensor out = new_empty(shape, weight.scalar_type()), id = packed_rows(ids);
+    if (id.numel() > 0) {
+        void *st = stream_of(weight.device());
+        const int rc = without_interpreter([&] {
+            return nmg_embedding(w.t.const_data_ptr(), w.rows, w.cols, w.ld, type_code(weight), id.const_data_ptr(), (int)id.element_size(), id.numel(), scale, out.mutable_data_ptr(), st);
+        });
+        check(rc);
+    }
+    return out;
+}
+
+struct Embedding : torch::autograd::Function<Embedding> {
+    static at::Tensor forward(torch::autograd::AutogradContext *ctx, const at::Tensor &weight, const at::Tensor &ids, double scale, int64_t padding) {
+        ctx->save_for_backward({ids});
+        ctx->saved_data["scale"] = scale;
+        ctx->saved_data["padding"] = padding;
+        ctx->saved_data["vocab"] = weight.size(0);
+        ctx->saved_data["width"] = weight.size(1);
+        ctx->saved_data["tokens"] = ids.numel();
+        ctx->saved_data["id_bytes"] = (int64_t)ids.element_size();
+        return embed_forward(weight, ids, (float)scale);
+    }
+    static variable_list backward(torch::autograd::AutogradContext *ctx, variable_list g) {
+        const char *what = "embedding";
+        check_no_tangents(g, what);
+        const variable_list saved = ctx->get_saved_variables();
+        const at::Tensor &ids = saved[0], &up = g[0];
+        const int64_t vocab = ctx->saved_data["vocab"].toInt(), width = ctx->saved_data["width"].toInt(), tokens = ctx->saved_data["tokens"].toInt();
+        check_saved(up.defined() && up.is_cuda() && up.has_storage() && is_float(up) && up.numel() == tokens * width, what);
+        check_saved(lives_with(ids, up) && (ids.scalar_type() == at::kLong || ids.scalar_type() == at::kInt) && ids.numel() == tokens, what);
+        const c10::cuda::CUDAGuard guard(up.device());
+        const at::Tensor d = new_empty({vocab, width}, up.scalar_type());
+        if (tokens < 1) {
+            d.zero_();
+        } else {
+            const Rows r = hidden_rows(up, width);
+            const at::Tensor id = packed_rows(ids);
+            const size_t nbytes = nmg_embedding_backward_workspace_bytes(tokens, width);
+            const at::Tensor ws = new_empty({(int64_t)nbytes}, at::kByte);
+            check_backward(nmg_embedding_backward(r.t.const_data_ptr(), r.ld, tokens, width, type_code(up), id.const_data_ptr(), (int)id.element_size(), vocab, ctx->saved_data["padding"].toInt(),
+                                                  (float)ctx->saved_data["scale"].toDouble(), d.mutable_data_ptr(), ws.mutable_data_ptr(), nbytes, stream_of(up.device())));
+        }
+        return differentiable_once(d, what, 4);
+    }
+};
+
+// embedding(ids, weight, scale, padding) -> rows; padding: a row of the matrix that gets no gradient, or -1
+PyObject *py_embedding(PyObject *, PyObject *const *a, Py_ssize_t nargs) {
+    NMG_PY_BEGIN(4)
+    const at::Tensor &ids = tensor_arg(a[0]), &weight = tensor_arg(a[1]);
+    const double scale = double_arg(a[2]);
+    const int64_t padding = int_arg(a[3]);
+    const c10::Device dev = device_of({&ids, &weight});
+    float_code(weight, "weight");
+    if (ids.scalar_type() != at::kLong && ids.scalar_type() != at::kInt) py_raise(PyExc_TypeError, std::string("ids must be int64 or int32, got ") + c10::toString(ids.scalar_type()));
+    if (weight.dim() != 2 || weight.size(0) < 1 || weight.size(1) < 1) py_raise(PyExc_ValueError, "weight must be a matrix of at least one row and one column, got shape " + shape_str(weight.sizes()));
+    if (padding < -1 || padding >= weight.size(0)) py_raise(PyExc_ValueError, "padding_idx must be a row of the matrix of " + std::to_string(weight.size(0)) + " rows");
+    refuse_tangents({&weight}, "embedding");
+    const c10::cuda::CUDAGuard guard(dev);
+    if (c10::GradMode::is_enabled() && weight.requires_grad()) {
+        refuse_foreign_accumulators({&weight}, dev, "embedding");
+        return THPVariable_Wrap(Embedding::apply(weight, ids, scale, padding));
+    }
+    return THPVariable_Wrap(embed_forward(weight, ids, (float)scale));
+    NMG_PY_END
+}
+
 PyMethodDef handle_methods[] = {
     NMG_METHOD("gather", handle_gather),
     NMG_METHOD("linear", handle_linear),
@@ -1283,6 +1507,8 @@ PyMethodDef module_methods[] = {
     NMG_METHOD("densify", py_densify),
     NMG_METHOD("token_log_probs", py_token_log_probs),
     NMG_METHOD("distill", py_distill),
+    NMG_METHOD("layer_norm", py_layer_norm),
+    NMG_METHOD("embedding", py_embedding),
     NMG_METHOD("capturing", py_capturing),
     NMG_METHOD("check_weight", py_check_weight),
     NMG_METHOD("set_dispatch", py_set_dispatch),
