@@ -291,6 +291,21 @@ int nmg_distill_backward(const void *logits, int64_t rows, int64_t inner_rows, i
                          float temperature, const float *weight, int reduction, const float *norm, const float *total, const float *upstream, int skip_if_one, void *d_logits, int64_t ld_d,
                          int64_t ld_d_outer, void *stream);
 
+/* One token drawn from every row of logits by its uniform number u in [0, 1).  With z = logits / temperature, in this order:
+ *   top_k    the k largest logits (0, or no fewer than there are: all; equal ones in the order of their columns)
+ *   top_p    of these, largest first, the shortest run whose probabilities reach p of their sum, the largest one at least (1: all)
+ *   min_p    of these, the ones of at least min_p times the largest one's probability (0: all)
+ *   token    the first column, in their order, up to and including which the probabilities of what is left exceed u times their sum
+ *   log_prob its log-probability among what is left, in fp32
+ * Each setting is one number for all rows or, where its array is not NULL, one for each row (the number is then not looked at; values
+ * beyond a setting's range mean the nearest one in it).  A temperature of 0 takes the first of the largest logits, with log-probability 0;
+ * u >= 1 takes the last token that is left.  A row that holds NaN or +inf or nothing but -inf, or one with a temperature below 0 or above 1e30
+ * or a NaN among its settings has token -1 and log-probability NaN.  Tokens of less than 2^-(s+1) times the largest one's probability are never drawn (s =
+ * min(46, 62 - log2 vocab)). */
+int nmg_sample_tokens(const void *logits, int64_t rows, int64_t inner_rows, int64_t ld, int64_t ld_outer, int64_t vocab, int dtype,
+                      const float *uniform, const float *temperatures, double temperature, const int64_t *top_ks, int64_t top_k,
+                      const float *top_ps, double top_p, const float *min_ps, double min_p, int64_t *tokens, float *log_prob, void *stream);
+
 /* Layer norm (no counterpart in the reference, which leaves it to the model code).  Rows r < rows of `width` elements begin at element
  * r * ld; y, sum and d_x are [rows][width] without gaps.  weight and bias: [width] of param_dtype (dtype or NMG_F32), NULL: ones, zeros.
  *   h = x, or with a residual sum = x + residual rounded to dtype, which is written

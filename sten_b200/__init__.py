@@ -14,7 +14,7 @@ from .grouped_nm_tensor import GroupedNMTensor, PerfectNMTensor
 from .nmg_impls import GroupedNMSparsifier, WeightLayoutSparsifier
 from .fusion import fuse_linear_epilogues, sparse_linear_fused
 from .hidden import embedding, layer_norm
-from .vocab import TokenLogProbs, distillation_loss, token_log_probs
+from .vocab import SampledTokens, TokenLogProbs, distillation_loss, sample_tokens, token_log_probs
 from .patches import patch, patch_ddp, sparse_ddp_all_reduce_hook
 
 __version__ = "0.1.0"

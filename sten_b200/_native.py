@@ -58,6 +58,7 @@ SIGNATURES = {
     "nmg_distill": (_int, [_vp, _i64, _i64, _i64, _i64, _i64, _int, _vp, _int, _vp, _int, _int, _int, _f32, _vp, _int, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _vp]),
     "nmg_distill_backward": (_int, [_vp, _i64, _i64, _i64, _i64, _i64, _int, _vp, _int, _vp, _int, _int, _int, _f32, _vp, _int, _vp, _vp, _vp, _int, _vp, _i64, _i64,
                                     _vp]),
+    "nmg_sample_tokens": (_int, [_vp, _i64, _i64, _i64, _i64, _i64, _int, _vp, _vp, ctypes.c_double, _vp, _i64, _vp, ctypes.c_double, _vp, ctypes.c_double, _vp, _vp, _vp]),
     "nmg_layer_norm": (_int, [_vp, _i64, _vp, _i64, _i64, _i64, _int, _vp, _vp, _int, _f32, _vp, _vp, _vp, _vp]),
     "nmg_layer_norm_backward_workspace_bytes": (_sz, [_i64, _i64]),
     "nmg_layer_norm_backward": (_int, [_vp, _i64, _i64, _i64, _int, _vp, _int, _vp, _vp, _i64, _vp, _i64, _vp, _vp, _vp, _vp, _sz, _vp]),

@@ -1265,6 +1265,52 @@ PyObject *py_distill(PyObject *, PyObject *const *a, Py_ssize_t nargs) {
     NMG_PY_END
 }
 
+// A setting of sample_tokens: a number for all rows, or a tensor with one for each.
+struct Setting {
+    at::Tensor each;
+    PyObject *number;
+    Setting(PyObject *o, at::ScalarType type, const char *what, const at::Tensor &logits) : number(o) {
+        if (!THPVariable_Check(o)) return;
+        each = THPVariable_Unpack(o);
+        if (each.device() != logits.device()) py_raise(PyExc_RuntimeError, std::string(what) + " must be a number or a tensor on the logits' device");
+        if (each.scalar_type() != type) py_raise(PyExc_TypeError, std::string(what) + " must be " + c10::toString(type) + " where it is a tensor, got " + c10::toString(each.scalar_type()));
+        check_lead(each, logits, what);
+        each = packed_rows(each);
+    }
+};
+// sample_tokens(logits, uniform, temperature, top_k, top_p, min_p) -> (tokens, log_prob)
+PyObject *py_sample_tokens(PyObject *, PyObject *const *a, Py_ssize_t nargs) {
+    NMG_PY_BEGIN(6)
+    const at::Tensor &logits = tensor_arg(a[0]), &uniform0 = tensor_arg(a[1]);
+    const c10::Device dev = device_of({&logits, &uniform0});
+    const int code = float_code(logits, "logits");
+    refuse_tangents({&logits, &uniform0}, "sample_tokens");
+    const c10::cuda::CUDAGuard guard(dev);
+    const LogitRows x = logit_rows(logits);
+    if (uniform0.scalar_type() != at::kFloat) py_raise(PyExc_TypeError, std::string("uniform must be float32, got ") + c10::toString(uniform0.scalar_type()));
+    check_lead(uniform0, logits, "uniform");
+    const at::Tensor uniform = packed_rows(uniform0);
+    const Setting temperature(a[2], at::kFloat, "temperature", logits), top_k(a[3], at::kLong, "top_k", logits), top_p(a[4], at::kFloat, "top_p", logits), min_p(a[5], at::kFloat, "min_p", logits);
+    auto number = [](const Setting &s) { return s.each.defined() ? 0.0 : double_arg(s.number); };
+    const double tau = number(temperature), p = number(top_p), least = number(min_p);
+    const int64_t k = top_k.each.defined() ? 0 : int_arg(a[3]);
+    const std::vector<int64_t> lead = lead_shape(logits);
+    const at::Tensor tokens = new_empty(lead, at::kLong), log_prob = new_empty(lead, at::kFloat);
+    if (x.rows > 0) {
+        void *st = stream_of(dev);
+        const int rc = without_interpreter([&] {
+            return nmg_sample_tokens(x.t.const_data_ptr(), x.rows, x.inner, x.ld, x.ld_outer, x.vocab, code, f32_ptr(uniform), f32_ptr(temperature.each), tau, i64_ptr(top_k.each), k, f32_ptr(top_p.each), p,
+                                     f32_ptr(min_p.each), least, static_cast<int64_t *>(tokens.mutable_data_ptr()), f32_out(log_prob), st);
+        });
+        check(rc);
+    }
+    PyObject *r = PyTuple_New(2);
+    set_item(r, 0, tokens);
+    set_item(r, 1, log_prob);
+    return r;
+    NMG_PY_END
+}
+
 // ------------------------------------------------------------------------------------------------ between the products
 // A backward pass in a CUDA graph meets the node that accumulates a leaf's gradient.  One that an eager graph on the legacy default stream
 // keeps alive would have autograd wait for that stream, which no capture can do: the error comes on one of autograd's threads.
@@ -1507,6 +1553,7 @@ PyMethodDef module_methods[] = {
     NMG_METHOD("densify", py_densify),
     NMG_METHOD("token_log_probs", py_token_log_probs),
     NMG_METHOD("distill", py_distill),
+    NMG_METHOD("sample_tokens", py_sample_tokens),
     NMG_METHOD("layer_norm", py_layer_norm),
     NMG_METHOD("embedding", py_embedding),
     NMG_METHOD("capturing", py_capturing),

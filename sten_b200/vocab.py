@@ -48,6 +48,27 @@ def token_log_probs(logits, targets=None, *, temperature=1.0, top=0, ignore_inde
     return TokenLogProbs(*nat.host().token_log_probs(_dense(logits), targets, ignore_index, temperature, top))
 
 
+class SampledTokens(NamedTuple):
+    """What ``sample_tokens`` draws from every row: int64 and float32 tensors of the logits' leading shape."""
+
+    tokens: torch.Tensor
+    log_prob: torch.Tensor
+
+
+def sample_tokens(logits, uniform, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
+    """One token of every row of ``logits [..., vocab]`` by the row's number in ``uniform`` (float32 in [0, 1), the leading shape).
+
+    ``top_k`` keeps the k largest logits of a row (0: all; equal ones in the order of their ids), ``top_p`` of these the shortest run, largest first,
+    whose probabilities under ``softmax(logits / temperature)`` reach p of their sum (at least one token), ``min_p`` of these the ones of at
+    least min_p times the largest probability.  The token is the first, in the order of ids, where the probabilities of what is left
+    exceed ``uniform`` times their sum; ``log_prob`` is its log-probability among what is left.  Each setting is a number or a tensor with
+    one for each row (float32; ``top_k`` int64).  ``temperature`` 0 takes the first of the largest logits.
+
+    A row that holds NaN or +inf, or is -inf throughout, gives token -1 and log-probability NaN.  The same logits, number and settings give
+    the same token in every call, whatever else is in the batch.  Not differentiable: ``token_log_probs`` is."""
+    return SampledTokens(*nat.host().sample_tokens(_dense(logits), uniform, temperature, top_k, top_p, min_p))
+
+
 _REDUCTIONS = {"none": nat.NMG_REDUCE_NONE, "sum": nat.NMG_REDUCE_SUM, "mean": nat.NMG_REDUCE_MEAN}
 
 
