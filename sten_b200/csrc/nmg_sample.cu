@@ -17,7 +17,6 @@ namespace nmg {
 
 struct SampleParams {
     Logits x;
-    int parts;
     const float *uniform, *temperatures, *top_ps, *min_ps;  // a row each; NULL: the number below
     const int64_t *top_ks;
     double temperature, top_p, min_p;
@@ -27,19 +26,37 @@ struct SampleParams {
     float *log_prob;
 };
 
-constexpr int SAMPLE_THREADS = 512, SAMPLE_WARPS = SAMPLE_THREADS / 32, BINS = 2048;
+constexpr int SAMPLE_THREADS = 256, SAMPLE_WARPS = SAMPLE_THREADS / 32, BINS = 1024, LISTED = 448, FLAT = 4096;
 struct SampleShared {
-    unsigned long long bin[BINS];
-    double table[32];  // 2^(s + j / 32)
+    unsigned bin[2][BINS];  // low and high words: additions of 64 bits to shared memory are loops of compare-and-swap, which all lanes that add to one bin go through
+    double table[32];       // 2^(s + j / 32)
     unsigned long long scan[SAMPLE_WARPS];
-    // what the CTAs of a cluster tell each other
-    unsigned long long warp_weight[SAMPLE_WARPS];
-    unsigned warp_ties[SAMPLE_WARPS];
-    float warp_top[SAMPLE_WARPS], top;
-    unsigned first;
+    float3 scan3[SAMPLE_WARPS];
+    // what the CTAs of a cluster tell each other, a warp each
+    float warp_top[SAMPLE_WARPS];
+    Stats stats[SAMPLE_WARPS];
+    unsigned first[SAMPLE_WARPS];
+    unsigned long long weight[SAMPLE_WARPS], above[SAMPLE_WARPS], kept_weight[SAMPLE_WARPS];
+    unsigned count[SAMPLE_WARPS], listed[SAMPLE_WARPS], kept_ties[SAMPLE_WARPS];
+    // and the warps of a CTA
+    unsigned long long part_weight[SAMPLE_WARPS];
+    unsigned part_ties[SAMPLE_WARPS];
     // found by one thread
-    unsigned long long base, total;
-    int crossing;
+    unsigned long long base, before, seen;
+    int crossing, hit;
+    unsigned from, to;
+    float upto, lo, hi;
+    double log_all;
+    // found by the first CTA for all
+    float border;
+    unsigned long long border_ties;
+    union {
+        float flat[FLAT];                 // of the first CTA: all warps' lists
+        unsigned long long merged[BINS];  // bins of all CTAs
+    };
+    // a warp's logits between two borders, in the order of their columns
+    float list_x[SAMPLE_WARPS][LISTED];
+    int list_col[SAMPLE_WARPS][LISTED];
 };
 
 // Logits in their order as integers, equal ones equal (-0 is 0).  The low bits that no logit of the type has are left out.
@@ -87,25 +104,45 @@ template <typename T> __device__ __forceinline__ float vector_max(const uint4 &q
 }
 
 // w 2^s of a logit, rounded.  2^(t/32), t = k + r with |r| <= 1/2: a table of 2^(j/32) (256 bytes: lanes that read different entries do
-// not collide twice), 2^(k/32) - 1 as a polynomial of degree 4 that equals it at five points (error 2^-42.5), the exponent added as an integer.
+// not collide twice), 2^(r/32) - 1 as a polynomial of degree 4 that equals it at five points (error 2^-42.5), the exponent added as an integer.
+// 11 additions and products in 64 bits; what else there is to do is done on words.
 struct Weight {
-    double top, per_logit, lowest;  // M; 32 log2(e) / tau; t below which the rounded weight is zero
+    static constexpr double MAGIC = 6755399441055744.0;  // 1.5 2^52: what is added to it is rounded to an integer
+    static constexpr unsigned long long ONE = 0x4330000000000000ull;  // 2^52: the integer that is added to it is what stands behind the exponent
+    double top, per_logit;  // M 2^-896; 32 log2(e) / tau 2^896
+    unsigned least;         // first word of -32 (s + 2), where the rounded weight is zero
     const double *table;
-    __device__ __forceinline__ unsigned long long operator()(float x) const {
-        constexpr double MAGIC = 6755399441055744.0;  // 1.5 2^52: what is added to it is rounded to an integer
-        const double t = ((double)x - top) * per_logit;
-        if (!(t > lowest)) return 0;
+    __device__ __forceinline__ Weight(float m, double per_logit_, int scale_bits, const double *table_) {
+        top = widen(m);
+        per_logit = per_logit_ * 5.282945311356653e269;  // 2^896
+        least = (unsigned)__double2hiint(-32.0 * (scale_bits + 2));
+        table = table_;
+    }
+    // A float times 2^-896 in 64 bits, by words (the conversion instruction is slow, and the exponent's bias stays as it is; -inf becomes -2^-768)
+    static __device__ __forceinline__ double widen(float x) {
+        const int b = __float_as_int(x);
+        return __hiloint2double((b >> 3) & 0x8fffffff, b << 29);
+    }
+    __device__ __forceinline__ unsigned long long beside_one(float x) const {  // ONE + the weight
+        const double d = (widen(x) - top) * per_logit;
+        const double t = __hiloint2double((int)min((unsigned)__double2hiint(d), least), __double2loint(d));  // negative: the larger word is the lower number
         const double y = t + MAGIC, r = t - (y - MAGIC);
         const int k = __double2loint(y);
         double q = fma(r, 9.1725985660293348698e-9, 1.6938609067364199039e-6);
         q = fma(r, q, 0.0002345961982011260327);
         q = fma(r, q, 0.02166084939218784396);
         const double a = table[k & 31];
-        const double w = __hiloint2double(__double2hiint(a) + ((k >> 5) << 20), __double2loint(a));
-        return (unsigned long long)__double_as_longlong(fma(w, r * q, w) + 4503599627370496.0) & 0xfffffffffffffull;  // 2^52: the integer is what is behind the exponent
+        const double w = __hiloint2double(__double2hiint(a) + ((k & ~31) << 15), __double2loint(a));
+        return (unsigned long long)__double_as_longlong(fma(w, r * q, w) + 4503599627370496.0);
     }
+    __device__ __forceinline__ unsigned long long operator()(float x) const { return beside_one(x) - ONE; }
 };
 
+__device__ __forceinline__ float warp_sum(float v) {  // every lane gets the same
+#pragma unroll
+    for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(FULL, v, o);
+    return v;
+}
 __device__ __forceinline__ unsigned long long warp_sum_u64(unsigned long long v) {
 #pragma unroll
     for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(FULL, v, o);
@@ -119,17 +156,43 @@ __device__ __forceinline__ unsigned long long warp_scan_u64(unsigned long long v
     }
     return v;
 }
-__device__ __forceinline__ void meet(int parts) {  // the CTAs that share the row
-    if (parts == 1) __syncthreads();
+__device__ __forceinline__ unsigned warp_scan_u32(unsigned v, int lane) {
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const unsigned up = __shfl_up_sync(FULL, v, o);
+        if (lane >= o) v += up;
+    }
+    return v;
+}
+
+// ---- the CTAs that share a row.  Their number is a template argument, so that what is read from several of them is under way at the same time.
+template <int PARTS> __device__ __forceinline__ void meet() {
+    if constexpr (PARTS == 1) __syncthreads();
     else {
         cluster_barrier_arrive();
         cluster_barrier_wait();
     }
 }
-__device__ __forceinline__ uint32_t peer_u32(const void *p, int rank) {
-    uint32_t v;
+template <int PARTS> __device__ __forceinline__ unsigned peer_u32(const void *p, int rank) {
+    if constexpr (PARTS == 1) return *static_cast<const unsigned *>(p);
+    unsigned v;
     asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(peer_smem(p, rank)) : "memory");
     return v;
+}
+template <int PARTS> __device__ __forceinline__ unsigned long long peer_u64(const void *p, int rank) {
+    if constexpr (PARTS == 1) return *static_cast<const unsigned long long *>(p);
+    return peer_load_u64(peer_smem(p, rank));
+}
+template <int PARTS> __device__ __forceinline__ float peer_f32(const void *p, int rank) { return __uint_as_float(peer_u32<PARTS>(p, rank)); }
+// What the row's warps left, a lane each, in the order of their shares: f(rank, warp of it, whether there is one) for every 32 of them
+template <int PARTS, typename F> __device__ __forceinline__ void of_warps(F f) {
+    const int lane = (int)threadIdx.x & 31;
+#pragma unroll
+    for (int i = 0; i < (PARTS * SAMPLE_WARPS + 31) / 32; i++) {
+        const int w = i * 32 + lane;
+        const bool there = w < PARTS * SAMPLE_WARPS;
+        f(there ? w / SAMPLE_WARPS : 0, w % SAMPLE_WARPS, there);
+    }
 }
 
 // The share of one warp: a range of the row's vectors, the first warp's with the elements before them and the last's with those behind.
@@ -137,65 +200,114 @@ template <typename T> struct Share {
     Slice<T> sl;
     int lane;
     __device__ __forceinline__ Share(const T *row, int vocab, int warp, int warps) : sl(row, vocab, warp, warps), lane((int)threadIdx.x & 31) {}
+    __device__ __forceinline__ Share(const Share &of, int part, int parts) : sl(of.sl), lane(of.lane) {  // a part of it
+        const int n = of.sl.v1 - of.sl.v0;
+        sl.v0 = of.sl.v0 + (int)((int64_t)n * part / parts);
+        sl.v1 = of.sl.v0 + (int)((int64_t)n * (part + 1) / parts);
+        if (part) sl.lead_n = 0;
+        if (part + 1 < parts) sl.tail_n = 0;
+    }
+    __device__ __forceinline__ uint4 vector_or_none(int v) const {
+        const uint32_t none = neg_inf_word<T>();
+        return v < sl.v1 ? sl.vec(v) : make_uint4(none, none, none, none);
+    }
+    // f(N vectors a lane, number of the first) over the vectors; those that are not there are -inf
+    template <int N, typename F> __device__ __forceinline__ void steps(F f) const {
+        for (int v0 = sl.v0; v0 < sl.v1; v0 += 32 * N) {
+            const int v = v0 + lane;
+            uint4 q[N];
+            if (v0 + 32 * N <= sl.v1) {
+#pragma unroll
+                for (int u = 0; u < N; u++) q[u] = sl.vec(v + 32 * u);
+            } else {
+#pragma unroll
+                for (int u = 0; u < N; u++) q[u] = vector_or_none(v + 32 * u);
+            }
+            f(q, v);
+        }
+    }
+    // f(x, column of x[0]) for neighbouring elements a lane (a vector, or one element and -inf behind it) in the order of their columns: those of a lane,
+    // of the next lane, of the next call.  All lanes are there.
+    template <int N, typename F> __device__ __forceinline__ void walk(F f) const {
+        float x[VEC<T>];
+        auto single = [&](int col, bool in) {
+            x[0] = in ? sl.at(col) : neg_inf();
+#pragma unroll
+            for (int i = 1; i < VEC<T>; i++) x[i] = neg_inf();
+            f(x, col);
+        };
+        if (sl.lead_n) single(lane, lane < sl.lead_n);
+        steps<N>([&](const uint4 *q, int v) {
+#pragma unroll
+            for (int u = 0; u < N; u++) {
+                unpack<T>(q[u], x);
+                f(x, sl.lead + (v + 32 * u) * VEC<T>);
+            }
+        });
+        if (sl.tail_n) single(sl.tail_at + lane, lane < sl.tail_n);
+    }
     // each(logit) over elements above `above`, in no order
     template <typename F> __device__ __forceinline__ void over(float above, F each) const {
         if (const int c = sl.single(lane); c >= 0) {
             const float x = sl.at(c);
             if (x > above) each(x);
         }
-        int v = sl.v0 + lane;
-        auto one = [&](const uint4 &q) {
-            if (!(vector_max<T>(q) > above)) return;
-            float x[VEC<T>];
-            unpack<T>(q, x);
+        steps<4>([&](const uint4 *q, int) {
 #pragma unroll
-            for (int i = 0; i < VEC<T>; i++)
-                if (x[i] > above) each(x[i]);
-        };
-        for (; v + 96 < sl.v1; v += 128) {
-            uint4 q[4];
+            for (int u = 0; u < 4; u++) {
+                if (!(vector_max<T>(q[u]) > above)) continue;
+                float x[VEC<T>];
+                unpack<T>(q[u], x);
 #pragma unroll
-            for (int u = 0; u < 4; u++) q[u] = sl.vec(v + 32 * u);
-#pragma unroll
-            for (int u = 0; u < 4; u++) one(q[u]);
-        }
-        for (; v < sl.v1; v += 32) one(sl.vec(v));
+                for (int i = 0; i < VEC<T>; i++)
+                    if (x[i] > above) each(x[i]);
+            }
+        });
     }
-    __device__ __forceinline__ float top() const {  // NaN if there is one
+    // The largest (NaN if there is one) and, where `stats` is given, the lane's part of the softmax's sum.
+    template <typename R> __device__ __forceinline__ float top(R *stats, float a) const {
         float m = neg_inf();
-        if (const int c = sl.single(lane); c >= 0) m = sl.at(c);
-        int v = sl.v0 + lane;
-        for (; v + 96 < sl.v1; v += 128) {
-            uint4 q[4];
-#pragma unroll
-            for (int u = 0; u < 4; u++) q[u] = sl.vec(v + 32 * u);
+        if (const int c = sl.single(lane); c >= 0) {
+            m = sl.at(c);
+            if (stats) stats->st.template add_one<false>(m, a), stats->refer(a);
+        }
+        steps<4>([&](const uint4 *q, int) {
 #pragma unroll
             for (int u = 0; u < 4; u++) m = max_or_nan(m, vector_max_or_nan<T>(q[u]));
-        }
-        for (; v < sl.v1; v += 32) m = max_or_nan(m, vector_max_or_nan<T>(sl.vec(v)));
+            if (stats) stats->add(q, a);
+        });
 #pragma unroll
         for (int o = 16; o; o >>= 1) m = max_or_nan(m, __shfl_xor_sync(FULL, m, o));
         return m;
     }
-    // Groups of elements in the order of their columns, until f(group's lane values, first column, how many) says that it is done:
-    // a lane holds `n` neighbouring elements (one, or a vector), the next lane those behind.
-    template <typename F> __device__ __forceinline__ void in_order(F f) const {
-        float x[VEC<T>];
-        if (sl.lead_n) {
-            const bool in = lane < sl.lead_n;
-            x[0] = in ? sl.at(lane) : neg_inf();
-            if (f(x, lane, in ? 1 : 0)) return;
+};
+// All that is listed, by the threads of one CTA
+struct Flat {
+    const float *x;
+    int n;
+    template <typename F> __device__ __forceinline__ void over(float above, F each) const {
+        for (int i = (int)threadIdx.x; i < n; i += 4 * SAMPLE_THREADS) {
+            float y[4];
+#pragma unroll
+            for (int u = 0; u < 4; u++) y[u] = i + u * SAMPLE_THREADS < n ? x[i + u * SAMPLE_THREADS] : neg_inf();
+#pragma unroll
+            for (int u = 0; u < 4; u++)
+                if (y[u] > above) each(y[u]);
         }
-        for (int v0 = sl.v0; v0 < sl.v1; v0 += 32) {
-            const int v = v0 + lane;
-            const bool in = v < sl.v1;
-            if (in) unpack<T>(sl.vec(v), x);
-            if (f(x, sl.lead + v * VEC<T>, in ? VEC<T> : 0)) return;
-        }
-        if (sl.tail_n) {
-            const bool in = lane < sl.tail_n;
-            x[0] = in ? sl.at(sl.tail_at + lane) : neg_inf();
-            f(x, sl.tail_at + lane, in ? 1 : 0);
+    }
+};
+// A warp's listed logits
+struct Listed {
+    const float *x;
+    int n, lane;
+    template <typename F> __device__ __forceinline__ void over(float above, F each) const {
+        for (int i = lane; i < n; i += 128) {
+            float y[4];
+#pragma unroll
+            for (int u = 0; u < 4; u++) y[u] = i + 32 * u < n ? x[i + 32 * u] : neg_inf();
+#pragma unroll
+            for (int u = 0; u < 4; u++)
+                if (y[u] > above) each(y[u]);
         }
     }
 };
@@ -206,32 +318,58 @@ struct Border {
     unsigned long long ties;
 };
 
-// The border of the run, largest first, of the logits above `from.above` and from.ties equal to it, whose measure (1 each, or their weights)
-// reaches `share` of the whole or, where `count` is given, that number; `from` itself where the run takes all of it.
-template <bool WEIGHTS, typename T> __device__ __forceinline__ Border find_border(SampleShared &s, const Share<T> &sh, const Weight &weight, const Border from, float top, double share,
-                                                                                  unsigned long long count, int parts, int rank) {
+// The border of the run, largest first, whose measure (1 each, or their weights) reaches `target`, or `share` of the whole where that is 0.  The run begins with
+// logits that measure `base` together and are not looked at, goes on with those of the source from `top` down to above from.above, and ends with from.ties
+// that equal it: `from` itself where the run takes all of it.
+template <bool WEIGHTS, int PARTS, typename T, typename S> __device__ __noinline__ Border find_border(SampleShared &s, const S &source, const Weight &weight, const Border from, float top, unsigned long long base,
+                                                                                                     double share, unsigned long long target) {
     const int tid = (int)threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    unsigned lo = key_of<T>(from.above) + 1, hi = key_of<T>(top);
-    unsigned long long base = 0, target = count;
+    unsigned lo = key_of<T>(from.above), hi = key_of<T>(top);
     const unsigned long long end = from.ties * (WEIGHTS ? weight(from.above) : 1ull);  // what equals the lower border
     for (bool first = true;; first = false) {
-        int shift = 0;
-        while ((hi - lo) >> shift >= (unsigned)BINS) shift++;
-        for (int i = tid; i < BINS; i += SAMPLE_THREADS) s.bin[i] = 0;
+        const int shift = max(0, 32 - __clz(hi - lo) - 10);  // BINS of them
+        static_assert(BINS == 1 << 10, "bins of the search");
+        for (int i = tid; i < BINS; i += SAMPLE_THREADS) s.bin[0][i] = s.bin[1][i] = 0;
         __syncthreads();
-        const float above = logit_of<T>(lo - 1), below = logit_of<T>(hi);
-        sh.over(first ? from.above : above, [&](float x) {
+        const float above = first ? from.above : fmaxf(from.above, logit_of<T>(lo - 1)), below = logit_of<T>(hi);
+        source.over(above, [&](float x) {
             if (!first && x > below) return;
-            atomicAdd(&s.bin[(hi - key_of<T>(x)) >> shift], WEIGHTS ? weight(x) : 1ull);
+            const unsigned b = (hi - key_of<T>(x)) >> shift;
+            if constexpr (WEIGHTS) {
+                const unsigned long long w = weight(x);
+                const unsigned low = (unsigned)w, old = atomicAdd(&s.bin[0][b], low);
+                const unsigned high = (unsigned)(w >> 32) + (old + low < old);
+                if (high) atomicAdd(&s.bin[1][b], high);
+            } else {
+                atomicAdd(&s.bin[0][b], 1u);
+            }
         });
-        meet(parts);
-        // a thread adds up neighbouring bins of all CTAs
+        meet<PARTS>();
+        // a thread adds up neighbouring bins; those of the other CTAs are fetched by warps in one piece
         constexpr int EACH = BINS / SAMPLE_THREADS;
         unsigned long long n[EACH], sum = 0;
+        if constexpr (PARTS > 1) {
+            unsigned low[EACH][PARTS], high[EACH][PARTS];
+#pragma unroll
+            for (int i = 0; i < EACH; i++)
+#pragma unroll
+                for (int r = 0; r < PARTS; r++) {
+                    low[i][r] = peer_u32<PARTS>(&s.bin[0][tid + i * SAMPLE_THREADS], r);
+                    high[i][r] = WEIGHTS ? peer_u32<PARTS>(&s.bin[1][tid + i * SAMPLE_THREADS], r) : 0;
+                }
+#pragma unroll
+            for (int i = 0; i < EACH; i++) {
+                unsigned long long all = 0;
+#pragma unroll
+                for (int r = 0; r < PARTS; r++) all += (unsigned long long)high[i][r] << 32 | low[i][r];
+                s.merged[tid + i * SAMPLE_THREADS] = all;
+            }
+            __syncthreads();
+        }
 #pragma unroll
         for (int i = 0; i < EACH; i++) {
-            n[i] = 0;
-            for (int r = 0; r < parts; r++) n[i] += parts == 1 ? s.bin[tid * EACH + i] : peer_load_u64(peer_smem(&s.bin[tid * EACH + i], r));
+            const int b = tid * EACH + i;
+            n[i] = PARTS > 1 ? s.merged[b] : (unsigned long long)s.bin[1][b] << 32 | s.bin[0][b];
             sum += n[i];
         }
         const unsigned long long up_to = warp_scan_u64(sum, lane);
@@ -239,14 +377,18 @@ template <bool WEIGHTS, typename T> __device__ __forceinline__ Border find_borde
         if (tid == 0) s.crossing = -1;
         __syncthreads();
         unsigned long long before = base + up_to - sum, total = base;
+#pragma unroll
         for (int w = 0; w < SAMPLE_WARPS; w++) {
-            if (w < warp) before += s.scan[w];
-            total += s.scan[w];
+            const unsigned long long t = s.scan[w];
+            if (w < warp) before += t;
+            total += t;
         }
-        if (first && WEIGHTS) target = (unsigned long long)ceil(share * (double)(total + end));
-        if (target < 1) target = 1;
+        if (first && target == 0) {
+            target = (unsigned long long)ceil(share * (double)(total + end));
+            if (target < 1) target = 1;
+        }
         if (first && target > total) {  // the run goes to the lower border
-            meet(parts);
+            meet<PARTS>();
             if (target >= total + end) return from;
             const unsigned long long each = WEIGHTS ? weight(from.above) : 1ull;
             return Border{from.above, (target - total + each - 1) / each};
@@ -259,7 +401,7 @@ template <bool WEIGHTS, typename T> __device__ __forceinline__ Border find_borde
             }
             before += n[i];
         }
-        meet(parts);  // nobody reads the other CTAs' bins any more
+        meet<PARTS>();  // nobody reads the other CTAs' bins any more
         const unsigned at = (unsigned)s.crossing;
         base = s.base;
         __syncthreads();
@@ -268,165 +410,499 @@ template <bool WEIGHTS, typename T> __device__ __forceinline__ Border find_borde
         if (hi - lo > width) lo = hi - width;
         if (shift == 0) {
             const float value = logit_of<T>(hi);
-            const unsigned long long each = WEIGHTS ? weight(value) : 1ull;
+            if (!WEIGHTS) return Border{value, target - base};
+            const unsigned long long each = weight(value);
             return Border{value, (target - base + each - 1) / each};
         }
     }
 }
 
-template <typename T> __global__ void __launch_bounds__(SAMPLE_THREADS, 2) sample_kernel(const SampleParams p) {
-    __shared__ SampleShared s;
-    const int tid = (int)threadIdx.x, lane = tid & 31, warp = tid >> 5, parts = p.parts, rank = parts == 1 ? 0 : cluster_rank();
+// Where the border of a run is likely to be, from a sample of the row: above `lo`, at or below `hi` (+inf: the list may begin with the largest).
+struct Bracket {
+    float lo, hi;
+};
+// One step of 32 vectors in `stride` is counted into bins of equal width below the row's maximum.  What the sample says of the row's count above (weight below) a bin
+// is off by its standard deviation, s times the root of the sum of squares of what was counted; the bracket is four of them wide to both sides,
+// and one element that the sample missed.  Where the border is not in it after all, the search over the whole row takes over.
+// By the threads of one CTA, which leave it in s.lo and s.hi.
+template <bool WEIGHTS, typename T> __device__ __noinline__ void find_bracket(SampleShared &s, const Share<T> &sh, float window, float top, float per_bin, float octaves, float want, float room) {
+    const int tid = (int)threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    constexpr int warps = SAMPLE_WARPS, AHEAD = 4;
+    unsigned *const bin = s.bin[0];
+    for (int i = tid; i < BINS; i += SAMPLE_THREADS) bin[i] = 0;
+    if (tid == 0) s.from = s.to = BINS;
+    __syncthreads();
+    const int nvec = (sh.sl.tail_at - sh.sl.lead) / VEC<T>, steps = (nvec / warps + 32) / 32;  // of a warp, the most
+    int stride = nvec * VEC<T> / 16384;
+    stride = stride < 1 ? 1 : stride;
+    const float scale = (float)(warps * steps) / (float)((warps * steps + stride - 1) / stride);
+    for (int i = (stride - warp * steps % stride) % stride; i < steps; i += stride * AHEAD) {
+        uint4 q[AHEAD];
+#pragma unroll
+        for (int u = 0; u < AHEAD; u++) q[u] = sh.vector_or_none(sh.sl.v0 + 32 * (i + u * stride) + lane);
+#pragma unroll
+        for (int u = 0; u < AHEAD; u++) {
+            float x[VEC<T>];
+            unpack<T>(q[u], x);
+#pragma unroll
+            for (int j = 0; j < VEC<T>; j++)
+                if (x[j] > window) atomicAdd(&bin[min(BINS - 1, (int)((top - x[j]) * per_bin))], 1u);
+        }
+    }
+    __syncthreads();
+    // bins in the order of the search: from the largest logits by count, from the smallest by weight
+    constexpr int EACH = BINS / SAMPLE_THREADS;
+    float3 n[EACH], sum = make_float3(0.f, 0.f, 0.f);  // measure, its square, count
+    float one[EACH];
+#pragma unroll
+    for (int i = 0; i < EACH; i++) {
+        const unsigned all = bin[WEIGHTS ? BINS - 1 - (tid * EACH + i) : tid * EACH + i];
+        one[i] = WEIGHTS ? exp2_fast(-((float)(BINS - 1 - (tid * EACH + i)) + 0.5f) * octaves) : 1.f;
+        sum.x += (float)all * one[i];
+        sum.y += (float)all * one[i] * one[i];
+        sum.z += (float)all;
+        n[i] = sum;
+    }
+    float3 upto = sum;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const float x = __shfl_up_sync(FULL, upto.x, o), y = __shfl_up_sync(FULL, upto.y, o), z = __shfl_up_sync(FULL, upto.z, o);
+        if (lane >= o) upto.x += x, upto.y += y, upto.z += z;
+    }
+    if (lane == 31) s.scan3[warp] = upto;
+    __syncthreads();
+    float3 before = make_float3(upto.x - sum.x, upto.y - sum.y, upto.z - sum.z);
+    float all = 0.f;
+#pragma unroll
+    for (int w = 0; w < SAMPLE_WARPS; w++) {
+        const float3 t = s.scan3[w];
+        if (w < warp) before.x += t.x, before.y += t.y, before.z += t.z;
+        all += t.z;
+    }
+    want /= scale;
+    unsigned surely = BINS, may = BINS;
+#pragma unroll
+    for (int i = EACH - 1; i >= 0; i--) {
+        const float m = before.x + n[i].x, off = 4.f * sqrtf(before.y + n[i].y + one[i] * one[i]) + (WEIGHTS ? 0.5f * octaves * want : 0.f);  // half a bin's width is what the weights of its logits may be off by
+        if (m - off >= want) surely = tid * EACH + i;     // the border is in this bin or before it
+        if (m + off > want) may = tid * EACH + i;         // or may be
+    }
+    surely = __reduce_min_sync(FULL, surely);
+    may = __reduce_min_sync(FULL, may);
+    if (lane == 0) {
+        atomicMin(&s.to, surely);
+        atomicMin(&s.from, may);
+    }
+    __syncthreads();
+    const unsigned from = s.from, to = s.to;
+    // how many logits there are above the bracket's lower end, in the sample
+    const unsigned last = WEIGHTS ? from : to;
+    if (last == BINS) {
+        if (tid == 0) s.upto = all;
+    } else {
+#pragma unroll
+        for (int i = 0; i < EACH; i++)
+            if (last == (unsigned)(tid * EACH + i)) s.upto = WEIGHTS ? all - before.z - (i ? n[i ? i - 1 : 0].z : 0.f) : before.z + n[i].z;
+    }
+    __syncthreads();
+    if (tid == 0) {
+        auto edge = [&](unsigned b) { return top - (float)b / per_bin; };  // the upper one of bin b
+        float lo, hi;
+        if constexpr (WEIGHTS) {
+            lo = from == 0 ? window : from == BINS ? edge(1) : edge(BINS - from);
+            hi = to == BINS ? __int_as_float(0x7f800000) : edge(BINS - 1 - to);
+        } else {
+            lo = to == BINS ? window : edge(to + 1);
+            hi = from == 0 ? __int_as_float(0x7f800000) : edge(from);
+        }
+        s.hi = s.upto * scale < room ? __int_as_float(0x7f800000) : hi;  // few enough to be listed as a whole
+        s.lo = lo > window ? lo : window;
+    }
+}
+
+// Logits between the bracket's ends into the warp's list.  SUMS: the weights of all logits and of those above the bracket, and how many the latter are.
+template <bool SUMS, typename T> __device__ __noinline__ void gather(SampleShared &s, const Share<T> &sh, const Weight &weight, const Bracket br) {
+    const int lane = (int)threadIdx.x & 31, warp = (int)threadIdx.x >> 5;
+    unsigned long long all = 0, above = 0;
+    unsigned count = 0, calls = 0, n = 0;
+    sh.template walk<4>([&](const float *x, int col) {
+        unsigned chosen = 0;
+#pragma unroll
+        for (int i = 0; i < VEC<T>; i++) {
+            const bool over = x[i] > br.hi;
+            if (x[i] > br.lo && !over) chosen |= 1u << i;
+            if constexpr (SUMS) {
+                const unsigned long long w = weight.beside_one(x[i]);
+                all += w;
+                if (over) above += w, count++;
+            }
+        }
+        calls++;
+        if (!__any_sync(FULL, chosen != 0)) return;
+        const unsigned mine = __popc(chosen), upto = warp_scan_u32(mine, lane);
+        unsigned at = n + upto - mine;
+        n += __shfl_sync(FULL, upto, 31);
+        for (; chosen && at < LISTED; chosen &= chosen - 1, at++) {
+            const int c = col + __ffs(chosen) - 1;
+            s.list_x[warp][at] = sh.sl.at(c);
+            s.list_col[warp][at] = c;
+        }
+    });
+    if constexpr (SUMS) {
+        all = warp_sum_u64(all - (unsigned long long)calls * VEC<T> * Weight::ONE);
+        above = warp_sum_u64(above - (unsigned long long)count * Weight::ONE);
+        count = __reduce_add_sync(FULL, count);
+    }
+    if (lane == 0) {
+        s.weight[warp] = all;
+        s.above[warp] = above;
+        s.count[warp] = count;
+        s.listed[warp] = n;
+    }
+}
+
+template <typename T, int PARTS> __global__ void __launch_bounds__(SAMPLE_THREADS, 4) sample_kernel(const SampleParams p) {
+    extern __shared__ __align__(16) char smem[];
+    SampleShared &s = *reinterpret_cast<SampleShared *>(smem);
+    const int tid = (int)threadIdx.x, lane = tid & 31, warp = tid >> 5, rank = PARTS == 1 ? 0 : cluster_rank();
+    const int me = rank * SAMPLE_WARPS + warp;
+    constexpr int WARPS = PARTS * SAMPLE_WARPS;
+    constexpr float INF = __builtin_huge_valf();
     if (tid < 32) s.table[tid] = ldexp(exp2((double)tid / 32), p.scale_bits);
-    for (unsigned row = blockIdx.x / parts; row < p.x.rows; row += gridDim.x / parts) {
-        const Share<T> sh(static_cast<const T *>(p.x.x) + p.x.offset(row), p.x.vocab, rank * SAMPLE_WARPS + warp, parts * SAMPLE_WARPS);
-        const double tau = p.temperatures ? (double)p.temperatures[row] : p.temperature, top_p = p.top_ps ? (double)p.top_ps[row] : p.top_p, min_p = p.min_ps ? (double)p.min_ps[row] : p.min_p;
+    for (unsigned row = blockIdx.x / PARTS; row < p.x.rows; row += gridDim.x / PARTS) {
+        const T *const logits = static_cast<const T *>(p.x.x) + p.x.offset(row);
+        const Share<T> sh(logits, p.x.vocab, me, WARPS);
+        const double tau = p.temperatures ? (double)p.temperatures[row] : p.temperature, min_p = p.min_ps ? (double)p.min_ps[row] : p.min_p;
+        double top_p = p.top_ps ? (double)p.top_ps[row] : p.top_p;
         const int64_t top_k = p.top_ks ? p.top_ks[row] : p.top_k;
         const float u = p.uniform[row];
+        const bool meant = tau >= 0 && tau <= 1e30 && u == u && top_p == top_p && min_p == min_p;
+        if (top_p < 0) top_p = 0;
+        const bool by_count = top_k > 0 && top_k < p.x.vocab, by_weight = top_p < 1;
 
-        const float warp_top = sh.top();
-        if (lane == 0) s.warp_top[warp] = warp_top;
-        if (tid == 0) s.first = 0xffffffffu;
-        __syncthreads();
-        float top = s.warp_top[0];
-        for (int w = 1; w < SAMPLE_WARPS; w++) top = max_or_nan(top, s.warp_top[w]);
-        if (parts > 1) {
-            if (tid == 0) s.top = top;
-            meet(parts);
-            for (int r = 0; r < parts; r++) top = max_or_nan(top, __uint_as_float(peer_u32(&s.top, r)));
+        // the maximum, and about the softmax's sum where a share of it is asked for
+        const double inverse = 1 / tau;
+        const float a = (float)(1.4426950408889634 * inverse);
+        float warp_top;
+        if (by_weight && !by_count && tau >= 1e-30) {
+            RunningStats<T, false> stats;
+            warp_top = sh.top(&stats, a);
+            const Stats st = warp_merge(stats.st, a);
+            if (lane == 0) s.stats[warp] = st;
+        } else {
+            warp_top = sh.top((RunningStats<T, false> *)nullptr, a);
         }
+        if (lane == 0) s.warp_top[warp] = warp_top;
+        if (tid == 0) s.hit = -1;
+        meet<PARTS>();
+        float top = neg_inf();
+        of_warps<PARTS>([&](int r, int w, bool there) { top = max_or_nan(top, there ? peer_f32<PARTS>(&s.warp_top[w], r) : neg_inf()); });
+#pragma unroll
+        for (int o = 16; o; o >>= 1) top = max_or_nan(top, __shfl_xor_sync(FULL, top, o));
         // NaN or +inf among the logits, nothing but -inf, or settings that mean nothing
-        if (!(fabsf(top) < __int_as_float(0x7f800000)) || !(tau >= 0) || tau > 1e30 || u != u || top_p != top_p || min_p != min_p) {
+        if (!(fabsf(top) < INF) || !meant) {
             if (rank == 0 && tid == 0) {
                 p.tokens[row] = -1;
                 p.log_prob[row] = __int_as_float(0x7fffffff);
             }
-            meet(parts);
+            meet<PARTS>();
             continue;
         }
         if (tau < 1e-30) {  // the first of the largest
-            if (warp_top == top)
-                sh.in_order([&](const float *x, int col, int n) {
-                    int at = -1;
-                    for (int i = n - 1; i >= 0; i--)
-                        if (x[i] == top) at = col + i;
-                    const unsigned found = __reduce_min_sync(FULL, (unsigned)at);  // -1 is the largest
-                    if (found == 0xffffffffu) return false;
-                    if (lane == 0) atomicMin(&s.first, found);
-                    return true;
+            unsigned found = 0xffffffffu;
+            if (warp_top == top) {
+                sh.template walk<4>([&](const float *x, int col) {
+#pragma unroll
+                    for (int i = VEC<T> - 1; i >= 0; i--)
+                        if (x[i] == top) found = min(found, (unsigned)(col + i));
                 });
-            meet(parts);
-            if (rank == 0 && tid == 0) {
-                unsigned first = s.first;
-                for (int r = 1; r < parts; r++) first = min(first, peer_u32(&s.first, r));
-                p.tokens[row] = (int64_t)first;
-                p.log_prob[row] = 0.f;
+                found = __reduce_min_sync(FULL, found);
             }
-            meet(parts);
+            if (lane == 0) s.first[warp] = found;
+            meet<PARTS>();
+            if (rank == 0 && warp == 0) {
+                found = 0xffffffffu;
+                of_warps<PARTS>([&](int r, int w, bool there) { found = min(found, there ? peer_u32<PARTS>(&s.first[w], r) : 0xffffffffu); });
+                found = __reduce_min_sync(FULL, found);
+                if (lane == 0) {
+                    p.tokens[row] = (int64_t)found;
+                    p.log_prob[row] = 0.f;
+                }
+            }
+            meet<PARTS>();
             continue;
         }
 
-        const double per_logit = 32 * 1.4426950408889634 / tau;
-        const Weight weight{(double)top, per_logit, -32.0 * (p.scale_bits + 1), s.table};
+        const double per_logit = 32 * 1.4426950408889634 * inverse;
+        const Weight weight(top, per_logit, p.scale_bits, s.table);
         // all that has a weight
-        Border kept{-__int_as_float(0x7f800000), 0};
+        Border kept{-INF, 0};
         {
-            const float lowest = __double2float_rd((double)top + weight.lowest / per_logit);
+            const float lowest = __double2float_rd((double)top - (p.scale_bits + 1) * 0.6931471805599454 * tau);
             if (lowest > kept.above) kept.above = lowest;
             const unsigned key = key_of<T>(kept.above);  // a logit of the type, or what lies between two of them
             kept.above = logit_of<T>(key > key_of<T>(neg_inf()) ? key - 1 : key);
         }
-        const double floor_p = min_p > 0 ? (double)top + tau * log(min_p < 1 ? min_p : 1) : -1e300;
-        auto apply_min_p = [&] {  // nothing at or below the largest float under the border
-            const float at_least = floor_p < -3e38 ? neg_inf() : __double2float_ru(floor_p);
-            const float below = at_least == neg_inf() ? neg_inf() : nextafterf(at_least, neg_inf());
+        const float window = kept.above;
+
+        // the border of the run that is kept
+        bool both = false;    // the first CTA has looked for both borders
+        bool listed = false;  // what is kept: the list's part of it, and all above the bracket
+        Bracket br{window, INF};
+        if (by_count || by_weight) {
+            const float octaves = (float)(p.scale_bits + 1) / BINS, per_bin = a / octaves;  // of a bin; bins of a logit
+            if (rank == 0) {
+                const Share<T> whole(logits, p.x.vocab, warp, SAMPLE_WARPS);
+                const float room = 0.3f * (float)min(FLAT, WARPS * LISTED);
+                if (by_count) {
+                    find_bracket<false>(s, whole, window, top, per_bin, octaves, (float)top_k, room);
+                } else {
+                    float z = 0.f;  // in units of the largest weight
+                    of_warps<PARTS>([&](int r, int w, bool there) {
+                        const float m = peer_f32<PARTS>(&s.stats[w].m, r), sum = there ? peer_f32<PARTS>(&s.stats[w].s, r) : 0.f;
+                        if (sum > 0.f) z += sum * exp2_fast((m - top) * a);
+                    });
+                    z = warp_sum(z);
+                    find_bracket<true>(s, whole, window, top, per_bin, octaves, (float)(1 - top_p) * z, room);
+                }
+            }
+            meet<PARTS>();
+            br.lo = peer_f32<PARTS>(&s.lo, 0);
+            br.hi = peer_f32<PARTS>(&s.hi, 0);
+        }
+        if ((by_count || by_weight) && br.lo < top) {
+            const bool sums = !by_count || br.hi < INF;
+            if (sums) gather<true>(s, sh, weight, br);
+            else gather<false>(s, sh, weight, br);
+            meet<PARTS>();
+            unsigned long long all = 0, above = 0;
+            unsigned count = 0, entries = 0, most = 0, mine = 0;
+            int round = 0;
+            of_warps<PARTS>([&](int r, int w, bool there) {
+                unsigned n = peer_u32<PARTS>(&s.listed[w], r);
+                if (!there) n = 0;
+                const unsigned upto = entries + warp_scan_u32(n, lane);
+                if (me / 32 == round) mine = __shfl_sync(FULL, upto - n, me % 32);
+                entries = __shfl_sync(FULL, upto, 31);
+                most = max(most, n);
+                if (sums) {
+                    const unsigned long long z = peer_u64<PARTS>(&s.weight[w], r), over = peer_u64<PARTS>(&s.above[w], r);
+                    const unsigned c = peer_u32<PARTS>(&s.count[w], r);
+                    if (there) all += z, above += over, count += c;
+                }
+                round++;
+            });
+            most = __reduce_max_sync(FULL, most);
+            if (sums) {
+                all = warp_sum_u64(all);
+                above = warp_sum_u64(above);
+                count = __reduce_add_sync(FULL, count);
+            }
+            unsigned long long target = by_count ? (unsigned long long)top_k : (unsigned long long)ceil(top_p * (double)all);
+            if (target < 1) target = 1;
+            const bool all_kept = by_count && br.lo == window && target > (unsigned long long)count + entries;  // fewer than k have a weight
+            const bool in_list = most <= LISTED && (by_count ? count < target && (target <= count + entries || all_kept) : above < target);
+            if (in_list && entries > FLAT) {  // every CTA in its lists
+                const Listed list{s.list_x[warp], (int)s.listed[warp], lane};
+                const Border found = by_count ? find_border<false, PARTS, T>(s, list, weight, Border{br.lo, 0}, fminf(br.hi, top), count, 0.0, target)
+                                              : find_border<true, PARTS, T>(s, list, weight, Border{br.lo, 0}, fminf(br.hi, top), above, 0.0, target);
+                if (found.ties > 0) kept = found, listed = true;
+            } else if (in_list) {
+                // the first CTA looks for the border in all lists
+                both = by_count && by_weight && br.hi == INF;
+                for (int i = lane; i < (int)s.listed[warp]; i += 32) {
+                    if constexpr (PARTS == 1) s.flat[mine + i] = s.list_x[warp][i];
+                    else asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(peer_smem(&s.flat[mine + i], 0)), "f"(s.list_x[warp][i]) : "memory");
+                }
+                meet<PARTS>();
+                if (rank == 0) {
+                    const Flat flat{s.flat, (int)entries};
+                    const Border from{br.lo, 0};
+                    const float high = fminf(br.hi, top);
+                    Border found = kept;
+                    bool there = true;
+                    if (by_count) {
+                        if (!all_kept) found = find_border<false, 1, T>(s, flat, weight, from, high, count, 0.0, target);
+                        if (both) found = find_border<true, 1, T>(s, flat, weight, found, top, 0, top_p, 0);
+                    } else {
+                        found = find_border<true, 1, T>(s, flat, weight, from, high, above, 0.0, target);
+                        there = found.ties > 0 || br.lo == window;  // the latter: rounded up, all of it
+                    }
+                    if (tid == 0) {
+                        s.border = there ? found.above : INF;
+                        s.border_ties = found.ties;
+                    }
+                }
+                meet<PARTS>();
+                const Border found{peer_f32<PARTS>(&s.border, 0), peer_u64<PARTS>(&s.border_ties, 0)};
+                if (found.above < INF) kept = found, listed = true;
+            }
+        }
+        if (!listed && by_count) kept = find_border<false, PARTS, T>(s, sh, weight, kept, top, 0, 0.0, (unsigned long long)top_k);  // over the whole row
+        if (by_weight && (!listed || (by_count && !both))) {
+            kept = find_border<true, PARTS, T>(s, sh, weight, kept, top, 0, top_p, 0);
+            listed = false;
+        }
+        if (min_p > 0) {  // nothing at or below the largest float under the border
+            const double floor_p = (double)top + tau * log(min_p < 1 ? min_p : 1);
+            const float at_least = floor_p < -3e38 ? -INF : __double2float_ru(floor_p);
+            const float below = at_least == -INF ? -INF : nextafterf(at_least, -INF);
             if (below >= kept.above) kept = Border{below, 0};
-        };
-        if (top_k > 0 && top_k < p.x.vocab) kept = find_border<false>(s, sh, weight, kept, top, 0.0, (unsigned long long)top_k, parts, rank);
-        if (top_p < 1) kept = find_border<true>(s, sh, weight, kept, top, top_p < 0 ? 0 : top_p, 0, parts, rank);
-        apply_min_p();
+        }
+        if (br.hi < INF && kept.above >= br.hi) listed = false;
 
         // sums of the warps' shares, in the order of the columns
         unsigned long long sum = 0;
         unsigned ties = 0;
-        if (kept.ties) {
-            const float under = nextafterf(kept.above, neg_inf());
-            sh.over(under, [&](float x) {
-                if (x == kept.above) ties++;
-                else sum += weight(x);
+        auto count_in = [&](float x) {
+            if (x == kept.above) ties++;
+            else sum += weight(x);
+        };
+        const float under = kept.ties ? nextafterf(kept.above, -INF) : kept.above;
+        if (listed) {
+            if (br.hi < INF && lane == 0) sum = s.above[warp];
+            Listed{s.list_x[warp], (int)s.listed[warp], lane}.over(under, count_in);
+        } else if (kept.above == window && !kept.ties) {
+            unsigned calls = 0;
+            sh.template walk<4>([&](const float *x, int) {
+#pragma unroll
+                for (int i = 0; i < VEC<T>; i++) sum += weight.beside_one(x[i]);
+                calls++;
             });
+            sum -= (unsigned long long)calls * VEC<T> * Weight::ONE;
         } else {
-            sh.over(kept.above, [&](float x) { sum += weight(x); });
+            sh.over(under, count_in);
         }
         sum = warp_sum_u64(sum);
         ties = __reduce_add_sync(FULL, ties);
         if (lane == 0) {
-            s.warp_weight[warp] = sum;
-            s.warp_ties[warp] = ties;
+            s.kept_weight[warp] = sum;
+            s.kept_ties[warp] = ties;
         }
-        meet(parts);
+        meet<PARTS>();
         const unsigned long long each = kept.ties ? weight(kept.above) : 0;
         unsigned long long all = 0, before = 0, ties_seen = 0, mine = 0, ties_before = 0;
-        const int me = rank * SAMPLE_WARPS + warp;
-        for (int r = 0; r < parts; r++)
-            for (int w0 = 0; w0 < SAMPLE_WARPS; w0 += 32) {
-                static_assert(SAMPLE_WARPS <= 32, "a lane for each warp");
-                const bool in = lane < SAMPLE_WARPS;
-                const unsigned long long ws = in ? (parts == 1 ? s.warp_weight[lane] : peer_load_u64(peer_smem(&s.warp_weight[lane], r))) : 0;
-                const unsigned long long wt = in ? (parts == 1 ? s.warp_ties[lane] : peer_u32(&s.warp_ties[lane], r)) : 0;
-                const unsigned long long t_upto = ties_seen + warp_scan_u64(wt, lane), t_before = t_upto - wt;
-                const unsigned long long k_before = min(t_before, kept.ties), k_upto = min(t_upto, kept.ties);
-                const unsigned long long kept_w = ws + (k_upto - k_before) * each, upto = all + warp_scan_u64(kept_w, lane);
-                const int at = me - r * SAMPLE_WARPS;
-                if (at >= 0 && at < SAMPLE_WARPS) {
-                    before = __shfl_sync(FULL, upto - kept_w, at);
-                    mine = __shfl_sync(FULL, kept_w, at);
-                    ties_before = __shfl_sync(FULL, t_before, at);
-                }
-                all = __shfl_sync(FULL, upto, 31);
+        int round = 0;
+        of_warps<PARTS>([&](int r, int w, bool there) {
+            unsigned long long ws = peer_u64<PARTS>(&s.kept_weight[w], r);
+            unsigned wt = peer_u32<PARTS>(&s.kept_ties[w], r);
+            if (!there) ws = wt = 0;
+            unsigned long long t_before = 0, kept_w = ws;
+            if (kept.ties) {
+                const unsigned long long t_upto = ties_seen + warp_scan_u32(wt, lane);
+                t_before = t_upto - wt;
+                kept_w += (min(t_upto, kept.ties) - min(t_before, kept.ties)) * each;
                 ties_seen = __shfl_sync(FULL, t_upto, 31);
             }
-        // floor(u * all), exactly: u = m 2^-b
+            const unsigned long long upto = all + warp_scan_u64(kept_w, lane);
+            if (me / 32 == round) {
+                before = __shfl_sync(FULL, upto - kept_w, me % 32);
+                mine = __shfl_sync(FULL, kept_w, me % 32);
+                ties_before = __shfl_sync(FULL, t_before, me % 32);
+            }
+            all = __shfl_sync(FULL, upto, 31);
+            round++;
+        });
+        // floor(u * all), exactly: u = m 2^exponent
         unsigned long long target = 0;
         if (u >= 1.f) target = all - 1;
         else if (u > 0.f) {
             int exponent;
-            const float m = frexpf(u, &exponent);  // u = m 2^exponent, m in [1/2, 1)
-            const unsigned long long mantissa = (unsigned long long)(unsigned)(m * 16777216.f) << 40;  // m 2^64
-            const unsigned long long high = __umul64hi(mantissa, all);
+            const float m = frexpf(u, &exponent);  // in [1/2, 1)
+            const unsigned long long high = __umul64hi((unsigned long long)(unsigned)(m * 16777216.f) << 40, all);
             target = exponent <= -64 ? 0 : high >> -exponent;
         }
-        if (target >= before && target - before < mine) {
-            unsigned long long at = before, seen = ties_before;
-            sh.in_order([&](const float *x, int col, int n) {
-                unsigned long long part = 0;
-                unsigned mine_ties = 0;
-                for (int i = 0; i < n; i++) mine_ties += x[i] == kept.above;
-                unsigned long long ties_here = warp_scan_u64((unsigned long long)mine_ties, lane), t = seen + ties_here - mine_ties;
-                for (int i = 0; i < n; i++) {
-                    if (x[i] > kept.above) part += weight(x[i]);
-                    else if (x[i] == kept.above && t++ < kept.ties) part += each;
+        const bool hit = target >= before && target - before < mine;
+        auto found = [&](float x, int col, double log_all) {
+            p.tokens[row] = col;
+            p.log_prob[row] = (float)(((double)x - (double)top) * inverse - log_all);
+        };
+        if (listed && br.hi == INF) {
+            if (hit) {
+                unsigned long long at = before, seen = ties_before;
+                const int n = (int)s.listed[warp];
+                const double log_all = log(ldexp((double)all, -p.scale_bits));
+                for (int i0 = 0; i0 < n && at <= target; i0 += 32) {
+                    const int i = i0 + lane;
+                    const float x = i < n ? s.list_x[warp][i] : -INF;
+                    const bool tie = i < n && x == kept.above;
+                    const unsigned same = __ballot_sync(FULL, tie);
+                    const bool in = i < n && (x > kept.above || (tie && seen + __popc(same & ((1u << lane) - 1)) < kept.ties));
+                    const unsigned long long w = in ? weight(x) : 0, upto = at + warp_scan_u64(w, lane);
+                    if (target >= upto - w && target < upto) found(x, s.list_col[warp][i], log_all);
+                    at = __shfl_sync(FULL, upto, 31);
+                    seen += __popc(same);
                 }
-                const unsigned long long upto = at + warp_scan_u64(part, lane);
-                if (target >= upto - part && target < upto) {
-                    unsigned long long c = upto - part;
-                    t = seen + ties_here - mine_ties;
-                    for (int i = 0; i < n; i++) {
-                        if (x[i] > kept.above) c += weight(x[i]);
-                        else if (x[i] == kept.above && t++ < kept.ties) c += each;
-                        if (target < c) {
-                            p.tokens[row] = col + i;
-                            p.log_prob[row] = (float)(((double)x[i] - (double)top) / tau - log(ldexp((double)all, -p.scale_bits)));
-                            break;
+            }
+        } else {
+            // the warps of the CTA cut the share that the number falls into once more
+            if (hit && lane == 0) {
+                s.hit = warp;
+                s.before = before;
+                s.seen = ties_before;
+            }
+            __syncthreads();
+            if (s.hit >= 0) {
+                const Share<T> all_of_it(logits, p.x.vocab, rank * SAMPLE_WARPS + s.hit, WARPS), part(all_of_it, min(warp, SAMPLE_WARPS - 2), SAMPLE_WARPS - 1);
+                sum = 0;
+                ties = 0;
+                if (warp < SAMPLE_WARPS - 1) {
+                    part.template walk<2>([&](const float *x, int) {
+#pragma unroll
+                        for (int i = 0; i < VEC<T>; i++) {
+                            const unsigned long long w = weight(x[i]);
+                            if (x[i] > kept.above) sum += w;
+                            else if (x[i] == kept.above && kept.ties) ties++;
                         }
-                    }
+                    });
+                } else {
+                    const double log_all = log(ldexp((double)all, -p.scale_bits));
+                    if (lane == 0) s.log_all = log_all;
                 }
-                at = __shfl_sync(FULL, upto, 31);
-                seen += __shfl_sync(FULL, ties_here, 31);
-                return at > target;
-            });
+                sum = warp_sum_u64(sum);
+                ties = __reduce_add_sync(FULL, ties);
+                if (lane == 0) {
+                    s.part_weight[warp] = sum;
+                    s.part_ties[warp] = ties;
+                }
+                __syncthreads();
+                const unsigned long long ws = lane < SAMPLE_WARPS ? s.part_weight[lane] : 0, wt = lane < SAMPLE_WARPS ? s.part_ties[lane] : 0;
+                const unsigned long long t_upto = s.seen + warp_scan_u64(wt, lane), t_before = t_upto - wt, k_before = min(t_before, kept.ties), k_upto = min(t_upto, kept.ties);
+                const unsigned long long kept_w = ws + (k_upto - k_before) * each, upto = s.before + warp_scan_u64(kept_w, lane);
+                unsigned long long at = __shfl_sync(FULL, upto - kept_w, warp), seen = __shfl_sync(FULL, t_before, warp);
+                const unsigned long long end = __shfl_sync(FULL, upto, warp);
+                if (target >= at && target < end)
+                    part.template walk<2>([&](const float *x, int col) {
+                        if (at > target) return;
+                        unsigned long long w[VEC<T>], here = 0, t = 0;
+                        if (kept.ties) {
+                            unsigned n = 0;
+#pragma unroll
+                            for (int i = 0; i < VEC<T>; i++) n += x[i] == kept.above;
+                            const unsigned upto = warp_scan_u32(n, lane);
+                            t = seen + upto - n;
+                            seen += __shfl_sync(FULL, upto, 31);
+                        }
+#pragma unroll
+                        for (int i = 0; i < VEC<T>; i++) {
+                            w[i] = weight(x[i]);
+                            if (!(x[i] > kept.above)) w[i] = x[i] == kept.above && t++ < kept.ties ? each : 0;
+                            here += w[i];
+                        }
+                        const unsigned long long upto = at + warp_scan_u64(here, lane);
+                        if (target >= upto - here && target < upto) {
+                            unsigned long long c = upto - here;
+#pragma unroll
+                            for (int i = 0; i < VEC<T>; i++) {
+                                if (target >= c && target < c + w[i]) found(x[i], col + i, s.log_all);
+                                c += w[i];
+                            }
+                        }
+                        at = __shfl_sync(FULL, upto, 31);
+                    });
+            }
         }
-        meet(parts);  // the next row writes what was read here
+        meet<PARTS>();  // the next row writes what was read here
     }
 }
 
@@ -435,12 +911,57 @@ static int sample_parts(int64_t rows, int vocab, int sms) {
     int best = 1;
     double best_time = 1e300;
     for (int parts = 1; parts <= 8; parts *= 2) {
-        if (parts > 1 && vocab < parts * 4096) break;
-        const int64_t slots = (int64_t)sms * 2 / parts, rounds = (rows + slots - 1) / slots;
-        const double time = (double)rounds * ((double)vocab / parts + (parts > 1 ? 6000 + 1000 * parts : 4000));
+        if (parts > 1 && vocab < parts * 2048) break;
+        const int64_t slots = (int64_t)sms * 4 / parts - (parts > 2 ? sms / (6 * parts) : 0), rounds = (rows + slots - 1) / slots;
+        const double time = (double)rounds * ((double)vocab / parts + (parts > 1 ? 3000 + 500 * parts : 2000));
         if (time < best_time) best_time = time, best = parts;
     }
     return best;
+}
+
+// Clusters of the kernel that the device holds at once, asked for once: SMs that are left over when clusters are placed hold none (148 clusters of four would
+// be 142 and, behind them, six).
+template <typename T, int PARTS> static int resident_clusters(int *out) {
+    static std::atomic<int> known[kMaxDevices];
+    int dev = 0;
+    NMG_CUDA(cudaGetDevice(&dev));
+    *out = dev < kMaxDevices ? known[dev].load(std::memory_order_relaxed) : 0;
+    if (*out > 0) return NMG_OK;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(PARTS * 1024);
+    cfg.blockDim = dim3(SAMPLE_THREADS);
+    cfg.dynamicSmemBytes = sizeof(SampleShared);
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = PARTS;
+    attr.val.clusterDim.y = 1;
+    attr.val.clusterDim.z = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    NMG_CUDA(cudaOccupancyMaxActiveClusters(out, sample_kernel<T, PARTS>, &cfg));
+    if (*out < 1) NMG_FAIL(NMG_ERR_CUDA, "no cluster of the sampling kernel fits the device");
+    if (dev < kMaxDevices) known[dev].store(*out, std::memory_order_relaxed);
+    return NMG_OK;
+}
+template <typename T, int PARTS> static int launch_sample(const SampleParams &p, cudaStream_t st) {
+    NMG_ALLOW_SMEM(sizeof(SampleShared), sample_kernel<T, PARTS>);
+    int clusters;
+    if (const int rc = resident_clusters<T, PARTS>(&clusters)) return rc;
+    if (p.x.rows > INT32_MAX) NMG_FAIL(NMG_ERR_UNSUPPORTED, "%lld rows are more than one launch takes", (long long)p.x.rows);
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)((p.x.rows < clusters ? p.x.rows : clusters) * PARTS));
+    cfg.blockDim = dim3(SAMPLE_THREADS);
+    cfg.dynamicSmemBytes = sizeof(SampleShared);
+    cfg.stream = st;
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = PARTS;
+    attr.val.clusterDim.y = 1;
+    attr.val.clusterDim.z = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    NMG_CUDA(cudaLaunchKernelEx(&cfg, sample_kernel<T, PARTS>, p));
+    return NMG_OK;
 }
 
 }  // namespace nmg
@@ -451,7 +972,7 @@ extern "C" int nmg_sample_tokens(const void *logits, int64_t rows, int64_t inner
                                  const float *temperatures, double temperature, const int64_t *top_ks, int64_t top_k, const float *top_ps, double top_p,
                                  const float *min_ps, double min_p, int64_t *tokens, float *log_prob, void *stream) {
     if (vocab < 1 || vocab > INT32_MAX - 64) NMG_FAIL(NMG_ERR_INVALID, "vocab must be 1 .. 2^31 - 65, got %lld", (long long)vocab);
-    SampleParams p{{logits, rows, inner_rows, ld, ld_outer, (int)vocab}, 1, uniform, temperatures, top_ps, min_ps, top_ks, temperature, top_p, min_p, top_k, 46, tokens, log_prob};
+    SampleParams p{{logits, rows, inner_rows, ld, ld_outer, (int)vocab}, uniform, temperatures, top_ps, min_ps, top_ks, temperature, top_p, min_p, top_k, 46, tokens, log_prob};
     int rc, sms;
     if ((rc = check_logits(p.x, dtype, 1.f))) return rc;
     if (!uniform || !tokens || !log_prob) NMG_FAIL(NMG_ERR_INVALID, "uniform, tokens and log_prob must be non-NULL");
@@ -463,7 +984,13 @@ extern "C" int nmg_sample_tokens(const void *logits, int64_t rows, int64_t inner
     int bits = 0;
     while ((int64_t)1 << bits < vocab) bits++;
     if (p.scale_bits > 62 - bits) p.scale_bits = 62 - bits;
-    p.parts = sample_parts(rows, p.x.vocab, sms);
-    NMG_DISPATCH_DTYPE(dtype, T, return launch_rows(sample_kernel<T>, rows, Deal{SAMPLE_THREADS, p.parts}, sms, 0, sizeof(SampleShared) + 1024, (cudaStream_t)stream, p));
+    const int parts = sample_parts(rows, p.x.vocab, sms);
+    cudaStream_t st = (cudaStream_t)stream;
+    NMG_DISPATCH_DTYPE(dtype, T, {
+        if (parts == 1) return launch_sample<T, 1>(p, st);
+        if (parts == 2) return launch_sample<T, 2>(p, st);
+        if (parts == 4) return launch_sample<T, 4>(p, st);
+        return launch_sample<T, 8>(p, st);
+    });
     return NMG_OK;
 }
