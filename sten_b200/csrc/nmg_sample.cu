@@ -26,8 +26,8 @@ struct SampleParams {
     float *log_prob;
 };
 
-constexpr int SAMPLE_THREADS = 256, SAMPLE_WARPS = SAMPLE_THREADS / 32, BINS = 1024, LISTED = 448, FLAT = 4096;
-struct SampleShared {
+constexpr int SAMPLE_THREADS = 256, SAMPLE_WARPS = SAMPLE_THREADS / 32, BINS = 1024, LISTED = 384, FLAT = 4096, CHECKS = 64, SAMPLE_PER_SM = 4;
+template <typename T> struct SampleShared {
     unsigned bin[2][BINS];  // low and high words: additions of 64 bits to shared memory are loops of compare-and-swap, which all lanes that add to one bin go through
     double table[32];       // 2^(s + j / 32)
     unsigned long long scan[SAMPLE_WARPS];
@@ -38,6 +38,8 @@ struct SampleShared {
     unsigned first[SAMPLE_WARPS];
     unsigned long long weight[SAMPLE_WARPS], above[SAMPLE_WARPS], kept_weight[SAMPLE_WARPS];
     unsigned count[SAMPLE_WARPS], listed[SAMPLE_WARPS], kept_ties[SAMPLE_WARPS];
+    // sums of a warp's share up to the end of each of its pieces
+    unsigned long long check[SAMPLE_WARPS][CHECKS];
     // and the warps of a CTA
     unsigned long long part_weight[SAMPLE_WARPS];
     unsigned part_ties[SAMPLE_WARPS];
@@ -51,13 +53,14 @@ struct SampleShared {
     float border;
     unsigned long long border_ties;
     union {
-        float flat[FLAT];                 // of the first CTA: all warps' lists
+        T flat[FLAT];                     // of the first CTA: all warps' lists
         unsigned long long merged[BINS];  // bins of all CTAs
     };
     // a warp's logits between two borders, in the order of their columns
-    float list_x[SAMPLE_WARPS][LISTED];
+    T list_x[SAMPLE_WARPS][LISTED];
     int list_col[SAMPLE_WARPS][LISTED];
 };
+static_assert(4 * (sizeof(SampleShared<float>) + 1024) <= 228 << 10, "four CTAs an SM");
 
 // Logits in their order as integers, equal ones equal (-0 is 0).  The low bits that no logit of the type has are left out.
 template <typename T> constexpr int KEY_SHIFT = sizeof(T) == 4 ? 0 : DT<T>::id == NMG_BF16 ? 16 : 13;
@@ -207,6 +210,19 @@ template <typename T> struct Share {
         if (part) sl.lead_n = 0;
         if (part + 1 < parts) sl.tail_n = 0;
     }
+    // Pieces of so many vectors, at most CHECKS; the first has the elements before the vectors, the last those behind them.
+    __device__ __forceinline__ int piece_vectors() const { return ((sl.v1 - sl.v0 + 128 * CHECKS - 1) / (128 * CHECKS)) * 128; }
+    __device__ __forceinline__ int pieces() const { return max(1, (sl.v1 - sl.v0 + max(128, piece_vectors()) - 1) / max(128, piece_vectors())); }
+    __device__ __forceinline__ int piece_of(int col) const { return col < sl.lead ? 0 : col >= sl.tail_at ? pieces() - 1 : ((col - sl.lead) / VEC<T> - sl.v0) / max(128, piece_vectors()); }
+    __device__ __forceinline__ Share piece(int i) const {
+        Share r = *this;
+        const int n = max(128, piece_vectors());
+        r.sl.v0 = min(sl.v1, sl.v0 + i * n);
+        r.sl.v1 = min(sl.v1, r.sl.v0 + n);
+        if (i) r.sl.lead_n = 0;
+        if (i + 1 < pieces()) r.sl.tail_n = 0;
+        return r;
+    }
     __device__ __forceinline__ uint4 vector_or_none(int v) const {
         const uint32_t none = neg_inf_word<T>();
         return v < sl.v1 ? sl.vec(v) : make_uint4(none, none, none, none);
@@ -229,6 +245,12 @@ template <typename T> struct Share {
     // f(x, column of x[0]) for neighbouring elements a lane (a vector, or one element and -inf behind it) in the order of their columns: those of a lane,
     // of the next lane, of the next call.  All lanes are there.
     template <int N, typename F> __device__ __forceinline__ void walk(F f) const {
+        walk<N>(f, [](int) {});
+    }
+    // the same; end(i) behind the piece i (N = 4)
+    template <int N, typename F, typename E> __device__ __forceinline__ void walk(F f, E end) const {
+        const int per = max(128, piece_vectors());
+        int piece = 0, next = sl.v0 + per;
         float x[VEC<T>];
         auto single = [&](int col, bool in) {
             x[0] = in ? sl.at(col) : neg_inf();
@@ -243,8 +265,13 @@ template <typename T> struct Share {
                 unpack<T>(q[u], x);
                 f(x, sl.lead + (v + 32 * u) * VEC<T>);
             }
+            if (N == 4 && v - lane + 128 >= next && next < sl.v1) {
+                end(piece++);
+                next += per;
+            }
         });
         if (sl.tail_n) single(sl.tail_at + lane, lane < sl.tail_n);
+        end(piece);
     }
     // each(logit) over elements above `above`, in no order
     template <typename F> __device__ __forceinline__ void over(float above, F each) const {
@@ -282,14 +309,14 @@ template <typename T> struct Share {
     }
 };
 // All that is listed, by the threads of one CTA
-struct Flat {
-    const float *x;
+template <typename T> struct Flat {
+    const T *x;
     int n;
     template <typename F> __device__ __forceinline__ void over(float above, F each) const {
         for (int i = (int)threadIdx.x; i < n; i += 4 * SAMPLE_THREADS) {
             float y[4];
 #pragma unroll
-            for (int u = 0; u < 4; u++) y[u] = i + u * SAMPLE_THREADS < n ? x[i + u * SAMPLE_THREADS] : neg_inf();
+            for (int u = 0; u < 4; u++) y[u] = i + u * SAMPLE_THREADS < n ? DT<T>::to_f32(x[i + u * SAMPLE_THREADS]) : neg_inf();
 #pragma unroll
             for (int u = 0; u < 4; u++)
                 if (y[u] > above) each(y[u]);
@@ -297,14 +324,14 @@ struct Flat {
     }
 };
 // A warp's listed logits
-struct Listed {
-    const float *x;
+template <typename T> struct Listed {
+    const T *x;
     int n, lane;
     template <typename F> __device__ __forceinline__ void over(float above, F each) const {
         for (int i = lane; i < n; i += 128) {
             float y[4];
 #pragma unroll
-            for (int u = 0; u < 4; u++) y[u] = i + 32 * u < n ? x[i + 32 * u] : neg_inf();
+            for (int u = 0; u < 4; u++) y[u] = i + 32 * u < n ? DT<T>::to_f32(x[i + 32 * u]) : neg_inf();
 #pragma unroll
             for (int u = 0; u < 4; u++)
                 if (y[u] > above) each(y[u]);
@@ -321,7 +348,7 @@ struct Border {
 // The border of the run, largest first, whose measure (1 each, or their weights) reaches `target`, or `share` of the whole where that is 0.  The run begins with
 // logits that measure `base` together and are not looked at, goes on with those of the source from `top` down to above from.above, and ends with from.ties
 // that equal it: `from` itself where the run takes all of it.
-template <bool WEIGHTS, int PARTS, typename T, typename S> __device__ __noinline__ Border find_border(SampleShared &s, const S &source, const Weight &weight, const Border from, float top, unsigned long long base,
+template <bool WEIGHTS, int PARTS, typename T, typename S> __device__ __noinline__ Border find_border(SampleShared<T> &s, const S &source, const Weight &weight, const Border from, float top, unsigned long long base,
                                                                                                      double share, unsigned long long target) {
     const int tid = (int)threadIdx.x, lane = tid & 31, warp = tid >> 5;
     unsigned lo = key_of<T>(from.above), hi = key_of<T>(top);
@@ -424,19 +451,19 @@ struct Bracket {
 // One step of 32 vectors in `stride` is counted into bins of equal width below the row's maximum.  What the sample says of the row's count above (weight below) a bin
 // is off by its standard deviation, s times the root of the sum of squares of what was counted; the bracket is four of them wide to both sides,
 // and one element that the sample missed.  Where the border is not in it after all, the search over the whole row takes over.
-// By the threads of one CTA, which leave it in s.lo and s.hi.
-template <bool WEIGHTS, typename T> __device__ __noinline__ void find_bracket(SampleShared &s, const Share<T> &sh, float window, float top, float per_bin, float octaves, float want, float room) {
-    const int tid = (int)threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    constexpr int warps = SAMPLE_WARPS, AHEAD = 4;
+// The counting is done by all, and says how many logits one of the sample stands for.
+template <int PARTS, typename T> __device__ __noinline__ float take_sample(SampleShared<T> &s, const Share<T> &sh, float window, float top, float per_bin, int elements, int warp_of_row) {
+    const int tid = (int)threadIdx.x, lane = tid & 31;
+    constexpr int warps = PARTS * SAMPLE_WARPS, AHEAD = 4;
     unsigned *const bin = s.bin[0];
     for (int i = tid; i < BINS; i += SAMPLE_THREADS) bin[i] = 0;
     if (tid == 0) s.from = s.to = BINS;
     __syncthreads();
     const int nvec = (sh.sl.tail_at - sh.sl.lead) / VEC<T>, steps = (nvec / warps + 32) / 32;  // of a warp, the most
-    int stride = nvec * VEC<T> / 16384;
+    int stride = nvec * VEC<T> / elements;
     stride = stride < 1 ? 1 : stride;
     const float scale = (float)(warps * steps) / (float)((warps * steps + stride - 1) / stride);
-    for (int i = (stride - warp * steps % stride) % stride; i < steps; i += stride * AHEAD) {
+    for (int i = (stride - warp_of_row * steps % stride) % stride; i < steps; i += stride * AHEAD) {
         uint4 q[AHEAD];
 #pragma unroll
         for (int u = 0; u < AHEAD; u++) q[u] = sh.vector_or_none(sh.sl.v0 + 32 * (i + u * stride) + lane);
@@ -449,9 +476,30 @@ template <bool WEIGHTS, typename T> __device__ __noinline__ void find_bracket(Sa
                 if (x[j] > window) atomicAdd(&bin[min(BINS - 1, (int)((top - x[j]) * per_bin))], 1u);
         }
     }
-    __syncthreads();
-    // bins in the order of the search: from the largest logits by count, from the smallest by weight
+    meet<PARTS>();
+    return scale;
+}
+// The rest is done by the first CTA, which leaves the bracket in s.lo and s.hi.
+template <bool WEIGHTS, int PARTS, typename T> __device__ __noinline__ void find_bracket(SampleShared<T> &s, float scale, float window, float top, float per_bin, float octaves, float want, float room) {
+    const int tid = (int)threadIdx.x, lane = tid & 31, warp = tid >> 5;
     constexpr int EACH = BINS / SAMPLE_THREADS;
+    unsigned *const bin = s.bin[0];
+    if constexpr (PARTS > 1) {
+        unsigned c[EACH][PARTS];
+#pragma unroll
+        for (int i = 0; i < EACH; i++)
+#pragma unroll
+            for (int r = 0; r < PARTS; r++) c[i][r] = r ? peer_u32<PARTS>(&bin[tid + i * SAMPLE_THREADS], r) : bin[tid + i * SAMPLE_THREADS];
+#pragma unroll
+        for (int i = 0; i < EACH; i++) {
+            unsigned all = 0;
+#pragma unroll
+            for (int r = 0; r < PARTS; r++) all += c[i][r];
+            bin[tid + i * SAMPLE_THREADS] = all;
+        }
+        __syncthreads();
+    }
+    // bins in the order of the search: from the largest logits by count, from the smallest by weight
     float3 n[EACH], sum = make_float3(0.f, 0.f, 0.f);  // measure, its square, count
     float one[EACH];
 #pragma unroll
@@ -521,7 +569,7 @@ template <bool WEIGHTS, typename T> __device__ __noinline__ void find_bracket(Sa
 }
 
 // Logits between the bracket's ends into the warp's list.  SUMS: the weights of all logits and of those above the bracket, and how many the latter are.
-template <bool SUMS, typename T> __device__ __noinline__ void gather(SampleShared &s, const Share<T> &sh, const Weight &weight, const Bracket br) {
+template <bool SUMS, typename T> __device__ __noinline__ void gather(SampleShared<T> &s, const Share<T> &sh, const Weight &weight, const Bracket br) {
     const int lane = (int)threadIdx.x & 31, warp = (int)threadIdx.x >> 5;
     unsigned long long all = 0, above = 0;
     unsigned count = 0, calls = 0, n = 0;
@@ -544,8 +592,13 @@ template <bool SUMS, typename T> __device__ __noinline__ void gather(SampleShare
         n += __shfl_sync(FULL, upto, 31);
         for (; chosen && at < LISTED; chosen &= chosen - 1, at++) {
             const int c = col + __ffs(chosen) - 1;
-            s.list_x[warp][at] = sh.sl.at(c);
+            s.list_x[warp][at] = sh.sl.row[c];
             s.list_col[warp][at] = c;
+        }
+    }, [&](int piece) {
+        if constexpr (SUMS) {
+            const unsigned long long upto = warp_sum_u64(above - (unsigned long long)count * Weight::ONE);
+            if (lane == 0) s.check[warp][piece] = upto;
         }
     });
     if constexpr (SUMS) {
@@ -561,9 +614,9 @@ template <bool SUMS, typename T> __device__ __noinline__ void gather(SampleShare
     }
 }
 
-template <typename T, int PARTS> __global__ void __launch_bounds__(SAMPLE_THREADS, 4) sample_kernel(const SampleParams p) {
+template <typename T, int PARTS> __global__ void __launch_bounds__(SAMPLE_THREADS, SAMPLE_PER_SM) sample_kernel(const SampleParams p) {
     extern __shared__ __align__(16) char smem[];
-    SampleShared &s = *reinterpret_cast<SampleShared *>(smem);
+    SampleShared<T> &s = *reinterpret_cast<SampleShared<T> *>(smem);
     const int tid = (int)threadIdx.x, lane = tid & 31, warp = tid >> 5, rank = PARTS == 1 ? 0 : cluster_rank();
     const int me = rank * SAMPLE_WARPS + warp;
     constexpr int WARPS = PARTS * SAMPLE_WARPS;
@@ -651,11 +704,11 @@ template <typename T, int PARTS> __global__ void __launch_bounds__(SAMPLE_THREAD
         Bracket br{window, INF};
         if (by_count || by_weight) {
             const float octaves = (float)(p.scale_bits + 1) / BINS, per_bin = a / octaves;  // of a bin; bins of a logit
+            const float scale = take_sample<PARTS>(s, sh, window, top, per_bin, by_count ? 4096 : 16384, me);
             if (rank == 0) {
-                const Share<T> whole(logits, p.x.vocab, warp, SAMPLE_WARPS);
                 const float room = 0.3f * (float)min(FLAT, WARPS * LISTED);
                 if (by_count) {
-                    find_bracket<false>(s, whole, window, top, per_bin, octaves, (float)top_k, room);
+                    find_bracket<false, PARTS>(s, scale, window, top, per_bin, octaves, (float)top_k, room);
                 } else {
                     float z = 0.f;  // in units of the largest weight
                     of_warps<PARTS>([&](int r, int w, bool there) {
@@ -663,7 +716,7 @@ template <typename T, int PARTS> __global__ void __launch_bounds__(SAMPLE_THREAD
                         if (sum > 0.f) z += sum * exp2_fast((m - top) * a);
                     });
                     z = warp_sum(z);
-                    find_bracket<true>(s, whole, window, top, per_bin, octaves, (float)(1 - top_p) * z, room);
+                    find_bracket<true, PARTS>(s, scale, window, top, per_bin, octaves, (float)(1 - top_p) * z, room);
                 }
             }
             meet<PARTS>();
@@ -703,7 +756,7 @@ template <typename T, int PARTS> __global__ void __launch_bounds__(SAMPLE_THREAD
             const bool all_kept = by_count && br.lo == window && target > (unsigned long long)count + entries;  // fewer than k have a weight
             const bool in_list = most <= LISTED && (by_count ? count < target && (target <= count + entries || all_kept) : above < target);
             if (in_list && entries > FLAT) {  // every CTA in its lists
-                const Listed list{s.list_x[warp], (int)s.listed[warp], lane};
+                const Listed<T> list{s.list_x[warp], (int)s.listed[warp], lane};
                 const Border found = by_count ? find_border<false, PARTS, T>(s, list, weight, Border{br.lo, 0}, fminf(br.hi, top), count, 0.0, target)
                                               : find_border<true, PARTS, T>(s, list, weight, Border{br.lo, 0}, fminf(br.hi, top), above, 0.0, target);
                 if (found.ties > 0) kept = found, listed = true;
@@ -712,11 +765,12 @@ template <typename T, int PARTS> __global__ void __launch_bounds__(SAMPLE_THREAD
                 both = by_count && by_weight && br.hi == INF;
                 for (int i = lane; i < (int)s.listed[warp]; i += 32) {
                     if constexpr (PARTS == 1) s.flat[mine + i] = s.list_x[warp][i];
-                    else asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(peer_smem(&s.flat[mine + i], 0)), "f"(s.list_x[warp][i]) : "memory");
+                    else if constexpr (sizeof(T) == 4) asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(peer_smem(&s.flat[mine + i], 0)), "f"(s.list_x[warp][i]) : "memory");
+                    else asm volatile("st.shared::cluster.u16 [%0], %1;" ::"r"(peer_smem(&s.flat[mine + i], 0)), "h"(*reinterpret_cast<const uint16_t *>(&s.list_x[warp][i])) : "memory");
                 }
                 meet<PARTS>();
                 if (rank == 0) {
-                    const Flat flat{s.flat, (int)entries};
+                    const Flat<T> flat{s.flat, (int)entries};
                     const Border from{br.lo, 0};
                     const float high = fminf(br.hi, top);
                     Border found = kept;
@@ -759,16 +813,21 @@ template <typename T, int PARTS> __global__ void __launch_bounds__(SAMPLE_THREAD
             else sum += weight(x);
         };
         const float under = kept.ties ? nextafterf(kept.above, -INF) : kept.above;
+        bool checked = listed && br.hi < INF;  // there are sums of the share's pieces, but for what is listed
         if (listed) {
             if (br.hi < INF && lane == 0) sum = s.above[warp];
-            Listed{s.list_x[warp], (int)s.listed[warp], lane}.over(under, count_in);
+            Listed<T>{s.list_x[warp], (int)s.listed[warp], lane}.over(under, count_in);
         } else if (kept.above == window && !kept.ties) {
             unsigned calls = 0;
             sh.template walk<4>([&](const float *x, int) {
 #pragma unroll
                 for (int i = 0; i < VEC<T>; i++) sum += weight.beside_one(x[i]);
                 calls++;
+            }, [&](int piece) {
+                const unsigned long long upto = warp_sum_u64(sum - (unsigned long long)calls * VEC<T> * Weight::ONE);
+                if (lane == 0) s.check[warp][piece] = upto;
             });
+            checked = true;
             sum -= (unsigned long long)calls * VEC<T> * Weight::ONE;
         } else {
             sh.over(under, count_in);
@@ -824,7 +883,7 @@ template <typename T, int PARTS> __global__ void __launch_bounds__(SAMPLE_THREAD
                 const double log_all = log(ldexp((double)all, -p.scale_bits));
                 for (int i0 = 0; i0 < n && at <= target; i0 += 32) {
                     const int i = i0 + lane;
-                    const float x = i < n ? s.list_x[warp][i] : -INF;
+                    const float x = i < n ? DT<T>::to_f32(s.list_x[warp][i]) : -INF;
                     const bool tie = i < n && x == kept.above;
                     const unsigned same = __ballot_sync(FULL, tie);
                     const bool in = i < n && (x > kept.above || (tie && seen + __popc(same & ((1u << lane) - 1)) < kept.ties));
@@ -835,71 +894,117 @@ template <typename T, int PARTS> __global__ void __launch_bounds__(SAMPLE_THREAD
                 }
             }
         } else {
-            // the warps of the CTA cut the share that the number falls into once more
-            if (hit && lane == 0) {
-                s.hit = warp;
-                s.before = before;
-                s.seen = ties_before;
-            }
-            __syncthreads();
-            if (s.hit >= 0) {
-                const Share<T> all_of_it(logits, p.x.vocab, rank * SAMPLE_WARPS + s.hit, WARPS), part(all_of_it, min(warp, SAMPLE_WARPS - 2), SAMPLE_WARPS - 1);
-                sum = 0;
-                ties = 0;
-                if (warp < SAMPLE_WARPS - 1) {
-                    part.template walk<2>([&](const float *x, int) {
+            // the token among those of a part, of which `at` are before, and `seen` equal to the border
+            auto find_in = [&](const Share<T> &part, unsigned long long at, unsigned long long seen, double log_all) {
+                part.template walk<1>([&](const float *x, int col) {
+                    if (at > target) return;
+                    unsigned long long w[VEC<T>], here = 0, t = 0;
+                    if (kept.ties) {
+                        unsigned n = 0;
+#pragma unroll
+                        for (int i = 0; i < VEC<T>; i++) n += x[i] == kept.above;
+                        const unsigned upto = warp_scan_u32(n, lane);
+                        t = seen + upto - n;
+                        seen += __shfl_sync(FULL, upto, 31);
+                    }
+#pragma unroll
+                    for (int i = 0; i < VEC<T>; i++) {
+                        w[i] = weight(x[i]);
+                        if (!(x[i] > kept.above)) w[i] = x[i] == kept.above && t++ < kept.ties ? each : 0;
+                        here += w[i];
+                    }
+                    const unsigned long long upto = at + warp_scan_u64(here, lane);
+                    if (target >= upto - here && target < upto) {
+                        unsigned long long c = upto - here;
 #pragma unroll
                         for (int i = 0; i < VEC<T>; i++) {
-                            const unsigned long long w = weight(x[i]);
-                            if (x[i] > kept.above) sum += w;
-                            else if (x[i] == kept.above && kept.ties) ties++;
+                            if (target >= c && target < c + w[i]) found(x[i], col + i, log_all);
+                            c += w[i];
                         }
-                    });
-                } else {
+                    }
+                    at = __shfl_sync(FULL, upto, 31);
+                });
+            };
+            if (checked) {
+                if (hit) {
                     const double log_all = log(ldexp((double)all, -p.scale_bits));
-                    if (lane == 0) s.log_all = log_all;
-                }
-                sum = warp_sum_u64(sum);
-                ties = __reduce_add_sync(FULL, ties);
-                if (lane == 0) {
-                    s.part_weight[warp] = sum;
-                    s.part_ties[warp] = ties;
-                }
-                __syncthreads();
-                const unsigned long long ws = lane < SAMPLE_WARPS ? s.part_weight[lane] : 0, wt = lane < SAMPLE_WARPS ? s.part_ties[lane] : 0;
-                const unsigned long long t_upto = s.seen + warp_scan_u64(wt, lane), t_before = t_upto - wt, k_before = min(t_before, kept.ties), k_upto = min(t_upto, kept.ties);
-                const unsigned long long kept_w = ws + (k_upto - k_before) * each, upto = s.before + warp_scan_u64(kept_w, lane);
-                unsigned long long at = __shfl_sync(FULL, upto - kept_w, warp), seen = __shfl_sync(FULL, t_before, warp);
-                const unsigned long long end = __shfl_sync(FULL, upto, warp);
-                if (target >= at && target < end)
-                    part.template walk<2>([&](const float *x, int col) {
-                        if (at > target) return;
-                        unsigned long long w[VEC<T>], here = 0, t = 0;
-                        if (kept.ties) {
-                            unsigned n = 0;
-#pragma unroll
-                            for (int i = 0; i < VEC<T>; i++) n += x[i] == kept.above;
-                            const unsigned upto = warp_scan_u32(n, lane);
-                            t = seen + upto - n;
-                            seen += __shfl_sync(FULL, upto, 31);
-                        }
-#pragma unroll
-                        for (int i = 0; i < VEC<T>; i++) {
-                            w[i] = weight(x[i]);
-                            if (!(x[i] > kept.above)) w[i] = x[i] == kept.above && t++ < kept.ties ? each : 0;
-                            here += w[i];
-                        }
-                        const unsigned long long upto = at + warp_scan_u64(here, lane);
-                        if (target >= upto - here && target < upto) {
-                            unsigned long long c = upto - here;
-#pragma unroll
-                            for (int i = 0; i < VEC<T>; i++) {
-                                if (target >= c && target < c + w[i]) found(x[i], col + i, s.log_all);
-                                c += w[i];
+                    // what the list adds to each piece: bins that nobody uses any more
+                static_assert(CHECKS == 64, "two pieces a lane");
+                    unsigned *const low = s.bin[0], *const high = s.bin[1], *const tied = s.bin[0] + CHECKS;
+                    unsigned long long in[2] = {0, 0};
+                    unsigned ties_in[2] = {0, 0};
+                    if (listed) {
+                        for (int i = lane; i < CHECKS; i += 32) low[i] = high[i] = tied[i] = 0;
+                        __syncwarp();
+                        unsigned long long seen = ties_before;
+                        for (int i0 = 0; i0 < (int)s.listed[warp]; i0 += 32) {
+                            const int i = i0 + lane;
+                            const float x = i < (int)s.listed[warp] ? DT<T>::to_f32(s.list_x[warp][i]) : -INF;
+                            const bool tie = kept.ties && x == kept.above;
+                            const unsigned same = __ballot_sync(FULL, tie);
+                            const bool kept_tie = tie && seen + __popc(same & ((1u << lane) - 1)) < kept.ties;
+                            seen += __popc(same);
+                            if (x > kept.above || tie) {
+                                const int c = sh.piece_of(s.list_col[warp][i]);
+                                const unsigned long long w = tie ? (kept_tie ? each : 0) : weight(x);
+                                const unsigned word = (unsigned)w, old = atomicAdd(&low[c], word), carry = (unsigned)(w >> 32) + (old + word < old);
+                                if (carry) atomicAdd(&high[c], carry);
+                                if (tie) atomicAdd(&tied[c], 1u);
                             }
                         }
-                        at = __shfl_sync(FULL, upto, 31);
-                    });
+                        __syncwarp();
+#pragma unroll
+                        for (int i = 0; i < 2; i++) {
+                            in[i] = (unsigned long long)high[2 * lane + i] << 32 | low[2 * lane + i];
+                            ties_in[i] = tied[2 * lane + i];
+                        }
+                    }
+                    const unsigned long long listed_upto = warp_scan_u64(in[0] + in[1], lane);
+                    const unsigned ties_upto = warp_scan_u32(ties_in[0] + ties_in[1], lane);
+                    const int pieces = sh.pieces();
+                    unsigned long long upto[2];
+#pragma unroll
+                    for (int i = 0; i < 2; i++) upto[i] = before + s.check[warp][min(pieces - 1, 2 * lane + i)] + listed_upto - (i ? 0 : in[1]);
+                    const unsigned first = __ballot_sync(FULL, target < upto[0]), second = __ballot_sync(FULL, target < upto[1]);  // from some piece on
+                    const int at_lane = __ffs(second) - 1;
+                    const bool of_two = first >> at_lane & 1;  // the first of the lane's two
+                    const unsigned long long last = __shfl_up_sync(FULL, upto[1], 1);
+                    const unsigned long long from0 = lane ? last : before;
+                    const unsigned long long at = __shfl_sync(FULL, of_two ? from0 : upto[0], at_lane);
+                    const unsigned seen = __shfl_sync(FULL, ties_upto - ties_in[1] - (of_two ? ties_in[0] : 0), at_lane);
+                    find_in(sh.piece(2 * at_lane + (of_two ? 0 : 1)), at, ties_before + seen, log_all);
+                }
+            } else {
+                // the warps of the CTA cut the share that the number falls into once more
+                if (hit && lane == 0) {
+                    s.hit = warp;
+                    s.before = before;
+                    s.seen = ties_before;
+                }
+                __syncthreads();
+                if (s.hit >= 0) {
+                    const Share<T> all_of_it(logits, p.x.vocab, rank * SAMPLE_WARPS + s.hit, WARPS), part(all_of_it, min(warp, SAMPLE_WARPS - 2), SAMPLE_WARPS - 1);
+                    sum = 0;
+                    ties = 0;
+                    if (warp < SAMPLE_WARPS - 1) {
+                        part.over(under, count_in);
+                    } else {
+                        const double log_all = log(ldexp((double)all, -p.scale_bits));
+                        if (lane == 0) s.log_all = log_all;
+                    }
+                    sum = warp_sum_u64(sum);
+                    ties = __reduce_add_sync(FULL, ties);
+                    if (lane == 0) {
+                        s.part_weight[warp] = sum;
+                        s.part_ties[warp] = ties;
+                    }
+                    __syncthreads();
+                    const unsigned long long ws = lane < SAMPLE_WARPS ? s.part_weight[lane] : 0, wt = lane < SAMPLE_WARPS ? s.part_ties[lane] : 0;
+                    const unsigned long long t_upto = s.seen + warp_scan_u64(wt, lane), t_before = t_upto - wt, k_before = min(t_before, kept.ties), k_upto = min(t_upto, kept.ties);
+                    const unsigned long long kept_w = ws + (k_upto - k_before) * each, upto = s.before + warp_scan_u64(kept_w, lane);
+                    const unsigned long long at = __shfl_sync(FULL, upto - kept_w, warp), seen = __shfl_sync(FULL, t_before, warp), end = __shfl_sync(FULL, upto, warp);
+                    if (target >= at && target < end) find_in(part, at, seen, s.log_all);
+                }
             }
         }
         meet<PARTS>();  // the next row writes what was read here
@@ -912,7 +1017,7 @@ static int sample_parts(int64_t rows, int vocab, int sms) {
     double best_time = 1e300;
     for (int parts = 1; parts <= 8; parts *= 2) {
         if (parts > 1 && vocab < parts * 2048) break;
-        const int64_t slots = (int64_t)sms * 4 / parts - (parts > 2 ? sms / (6 * parts) : 0), rounds = (rows + slots - 1) / slots;
+        const int64_t slots = (int64_t)sms * SAMPLE_PER_SM / parts - (parts > 2 ? sms / (6 * parts) : 0), rounds = (rows + slots - 1) / slots;
         const double time = (double)rounds * ((double)vocab / parts + (parts > 1 ? 3000 + 500 * parts : 2000));
         if (time < best_time) best_time = time, best = parts;
     }
@@ -930,7 +1035,7 @@ template <typename T, int PARTS> static int resident_clusters(int *out) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(PARTS * 1024);
     cfg.blockDim = dim3(SAMPLE_THREADS);
-    cfg.dynamicSmemBytes = sizeof(SampleShared);
+    cfg.dynamicSmemBytes = sizeof(SampleShared<T>);
     cudaLaunchAttribute attr;
     attr.id = cudaLaunchAttributeClusterDimension;
     attr.val.clusterDim.x = PARTS;
@@ -944,14 +1049,14 @@ template <typename T, int PARTS> static int resident_clusters(int *out) {
     return NMG_OK;
 }
 template <typename T, int PARTS> static int launch_sample(const SampleParams &p, cudaStream_t st) {
-    NMG_ALLOW_SMEM(sizeof(SampleShared), sample_kernel<T, PARTS>);
+    NMG_ALLOW_SMEM(sizeof(SampleShared<T>), sample_kernel<T, PARTS>);
     int clusters;
     if (const int rc = resident_clusters<T, PARTS>(&clusters)) return rc;
     if (p.x.rows > INT32_MAX) NMG_FAIL(NMG_ERR_UNSUPPORTED, "%lld rows are more than one launch takes", (long long)p.x.rows);
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)((p.x.rows < clusters ? p.x.rows : clusters) * PARTS));
     cfg.blockDim = dim3(SAMPLE_THREADS);
-    cfg.dynamicSmemBytes = sizeof(SampleShared);
+    cfg.dynamicSmemBytes = sizeof(SampleShared<T>);
     cfg.stream = st;
     cudaLaunchAttribute attr;
     attr.id = cudaLaunchAttributeClusterDimension;
