@@ -29,10 +29,15 @@ struct SampleParams {
 constexpr int SAMPLE_THREADS = 256, SAMPLE_WARPS = SAMPLE_THREADS / 32, BINS = 1024, LISTED = 384, FLAT = 4096, CHECKS = 64, SAMPLE_PER_SM = 4;
 template <typename T> struct SampleShared {
     unsigned bin[2][BINS];  // low and high words: additions of 64 bits to shared memory are loops of compare-and-swap, which all lanes that add to one bin go through
-    double table[32];       // 2^(s + j / 32)
+    double table[32];       // 2^(s + j / 32), less j 2^15 in the first word
     unsigned long long scan[SAMPLE_WARPS];
     float3 scan3[SAMPLE_WARPS];
     // what the CTAs of a cluster tell each other, a warp each
+    struct Settings {  // of the first CTA: what all of them go by, whoever writes to the caller's arrays meanwhile
+        double tau, top_p, min_p;
+        long long top_k;
+        float u;
+    } settings;
     float warp_top[SAMPLE_WARPS];
     Stats stats[SAMPLE_WARPS];
     unsigned first[SAMPLE_WARPS];
@@ -48,7 +53,9 @@ template <typename T> struct SampleShared {
     int crossing, hit;
     unsigned from, to;
     float upto, lo, hi;
-    double log_all;
+    // of the first CTA: what is written for the row
+    float token_logit;
+    int token;
     // found by the first CTA for all
     float border;
     unsigned long long border_ties;
@@ -122,12 +129,12 @@ struct Weight {
         table = table_;
     }
     // A float times 2^-896 in 64 bits, by words (the conversion instruction is slow, and the exponent's bias stays as it is; -inf becomes -2^-768)
-    static __device__ __forceinline__ double widen(float x) {
+    template <typename T = float> static __device__ __forceinline__ double widen(float x) {
         const int b = __float_as_int(x);
-        return __hiloint2double((b >> 3) & 0x8fffffff, b << 29);
+        return __hiloint2double((b >> 3) & 0x8fffffff, sizeof(T) == 2 && DT<T>::id == NMG_BF16 ? 0 : b << 29);  // bf16 has no bits for the second word
     }
-    __device__ __forceinline__ unsigned long long beside_one(float x) const {  // ONE + the weight
-        const double d = (widen(x) - top) * per_logit;
+    template <typename T = float> __device__ __forceinline__ unsigned long long beside_one(float x) const {  // ONE + the weight (T: the logit's type)
+        const double d = (widen<T>(x) - top) * per_logit;
         const double t = __hiloint2double((int)min((unsigned)__double2hiint(d), least), __double2loint(d));  // negative: the larger word is the lower number
         const double y = t + MAGIC, r = t - (y - MAGIC);
         const int k = __double2loint(y);
@@ -135,7 +142,7 @@ struct Weight {
         q = fma(r, q, 0.0002345961982011260327);
         q = fma(r, q, 0.02166084939218784396);
         const double a = table[k & 31];
-        const double w = __hiloint2double(__double2hiint(a) + ((k & ~31) << 15), __double2loint(a));
+        const double w = __hiloint2double(__double2hiint(a) + (k << 15), __double2loint(a));  // k / 32 to the exponent; the table has the rest of k off
         return (unsigned long long)__double_as_longlong(fma(w, r * q, w) + 4503599627370496.0);
     }
     __device__ __forceinline__ unsigned long long operator()(float x) const { return beside_one(x) - ONE; }
@@ -429,10 +436,11 @@ template <bool WEIGHTS, int PARTS, typename T, typename S> __device__ __noinline
             before += n[i];
         }
         meet<PARTS>();  // nobody reads the other CTAs' bins any more
-        const unsigned at = (unsigned)s.crossing;
+        const int at = s.crossing;
         base = s.base;
         __syncthreads();
-        hi -= at << shift;
+        if (at < 0) return from;  // only where somebody writes to the logits meanwhile
+        hi -= (unsigned)at << shift;
         const unsigned width = (1u << shift) - 1;
         if (hi - lo > width) lo = hi - width;
         if (shift == 0) {
@@ -580,20 +588,35 @@ template <bool SUMS, typename T> __device__ __noinline__ void gather(SampleShare
             const bool over = x[i] > br.hi;
             if (x[i] > br.lo && !over) chosen |= 1u << i;
             if constexpr (SUMS) {
-                const unsigned long long w = weight.beside_one(x[i]);
+                const unsigned long long w = weight.template beside_one<T>(x[i]);
                 all += w;
                 if (over) above += w, count++;
             }
         }
         calls++;
-        if (!__any_sync(FULL, chosen != 0)) return;
-        const unsigned mine = __popc(chosen), upto = warp_scan_u32(mine, lane);
-        unsigned at = n + upto - mine;
-        n += __shfl_sync(FULL, upto, 31);
+        const unsigned some = __ballot_sync(FULL, chosen != 0);
+        if (!some) return;
+        unsigned upto, total;
+        if (__any_sync(FULL, (chosen & (chosen - 1)) != 0)) {
+            const unsigned mine = __popc(chosen);
+            upto = warp_scan_u32(mine, lane) - mine;
+            total = __shfl_sync(FULL, upto + mine, 31);
+        } else {  // one a lane at most
+            upto = __popc(some & ((1u << lane) - 1));
+            total = __popc(some);
+        }
+        unsigned at = n + upto;
+        n += total;
         for (; chosen && at < LISTED; chosen &= chosen - 1, at++) {
-            const int c = col + __ffs(chosen) - 1;
-            s.list_x[warp][at] = sh.sl.row[c];
-            s.list_col[warp][at] = c;
+            const int i = __ffs(chosen) - 1;
+            float y = i & 1 ? x[1] : x[0];
+#pragma unroll
+            for (int j = 2; j < VEC<T>; j += 2) {
+                const float z = i & 1 ? x[j + 1] : x[j];
+                if ((i & ~1) == j) y = z;
+            }
+            s.list_x[warp][at] = DT<T>::from_f32(y);
+            s.list_col[warp][at] = col + i;
         }
     }, [&](int piece) {
         if constexpr (SUMS) {
@@ -621,23 +644,21 @@ template <typename T, int PARTS> __global__ void __launch_bounds__(SAMPLE_THREAD
     const int me = rank * SAMPLE_WARPS + warp;
     constexpr int WARPS = PARTS * SAMPLE_WARPS;
     constexpr float INF = __builtin_huge_valf();
-    if (tid < 32) s.table[tid] = ldexp(exp2((double)tid / 32), p.scale_bits);
+    if (tid < 32) {
+        const double a = ldexp(exp2((double)tid / 32), p.scale_bits);
+        s.table[tid] = __hiloint2double(__double2hiint(a) - (tid << 15), __double2loint(a));
+    }
     for (unsigned row = blockIdx.x / PARTS; row < p.x.rows; row += gridDim.x / PARTS) {
         const T *const logits = static_cast<const T *>(p.x.x) + p.x.offset(row);
         const Share<T> sh(logits, p.x.vocab, me, WARPS);
-        const double tau = p.temperatures ? (double)p.temperatures[row] : p.temperature, min_p = p.min_ps ? (double)p.min_ps[row] : p.min_p;
-        double top_p = p.top_ps ? (double)p.top_ps[row] : p.top_p;
-        const int64_t top_k = p.top_ks ? p.top_ks[row] : p.top_k;
-        const float u = p.uniform[row];
-        const bool meant = tau >= 0 && tau <= 1e30 && u == u && top_p == top_p && min_p == min_p;
-        if (top_p < 0) top_p = 0;
-        const bool by_count = top_k > 0 && top_k < p.x.vocab, by_weight = top_p < 1;
+        typename SampleShared<T>::Settings set{p.temperatures ? (double)p.temperatures[row] : p.temperature, p.top_ps ? (double)p.top_ps[row] : p.top_p, p.min_ps ? (double)p.min_ps[row] : p.min_p,
+                                               p.top_ks ? (long long)p.top_ks[row] : (long long)p.top_k, p.uniform[row]};
+        if (rank == 0 && tid == 0) s.settings = set;
 
         // the maximum, and about the softmax's sum where a share of it is asked for
-        const double inverse = 1 / tau;
-        const float a = (float)(1.4426950408889634 * inverse);
+        float a = (float)(1.4426950408889634 / set.tau);
         float warp_top;
-        if (by_weight && !by_count && tau >= 1e-30) {
+        if (set.top_p < 1 && !(set.top_k > 0 && set.top_k < p.x.vocab) && set.tau >= 1e-30) {
             RunningStats<T, false> stats;
             warp_top = sh.top(&stats, a);
             const Stats st = warp_merge(stats.st, a);
@@ -648,6 +669,17 @@ template <typename T, int PARTS> __global__ void __launch_bounds__(SAMPLE_THREAD
         if (lane == 0) s.warp_top[warp] = warp_top;
         if (tid == 0) s.hit = -1;
         meet<PARTS>();
+        set.tau = __longlong_as_double((long long)peer_u64<PARTS>(&s.settings.tau, 0));
+        set.top_p = __longlong_as_double((long long)peer_u64<PARTS>(&s.settings.top_p, 0));
+        set.min_p = __longlong_as_double((long long)peer_u64<PARTS>(&s.settings.min_p, 0));
+        set.top_k = (long long)peer_u64<PARTS>(&s.settings.top_k, 0);
+        set.u = peer_f32<PARTS>(&s.settings.u, 0);
+        const double tau = set.tau, min_p = set.min_p, inverse = 1 / tau, top_p = set.top_p < 0 ? 0 : set.top_p;
+        const int64_t top_k = set.top_k;
+        const float u = set.u;
+        const bool meant = tau >= 0 && tau <= 1e30 && u == u && set.top_p == set.top_p && min_p == min_p;
+        const bool by_count = top_k > 0 && top_k < p.x.vocab, by_weight = top_p < 1;
+        a = (float)(1.4426950408889634 * inverse);
         float top = neg_inf();
         of_warps<PARTS>([&](int r, int w, bool there) { top = max_or_nan(top, there ? peer_f32<PARTS>(&s.warp_top[w], r) : neg_inf()); });
 #pragma unroll
@@ -821,14 +853,14 @@ template <typename T, int PARTS> __global__ void __launch_bounds__(SAMPLE_THREAD
             unsigned calls = 0;
             sh.template walk<4>([&](const float *x, int) {
 #pragma unroll
-                for (int i = 0; i < VEC<T>; i++) sum += weight.beside_one(x[i]);
+                for (int i = 0; i < VEC<T>; i++) sum += weight.template beside_one<T>(x[i]);
                 calls++;
             }, [&](int piece) {
                 const unsigned long long upto = warp_sum_u64(sum - (unsigned long long)calls * VEC<T> * Weight::ONE);
                 if (lane == 0) s.check[warp][piece] = upto;
             });
-            checked = true;
             sum -= (unsigned long long)calls * VEC<T> * Weight::ONE;
+            checked = true;
         } else {
             sh.over(under, count_in);
         }
@@ -872,15 +904,19 @@ template <typename T, int PARTS> __global__ void __launch_bounds__(SAMPLE_THREAD
             target = exponent <= -64 ? 0 : high >> -exponent;
         }
         const bool hit = target >= before && target - before < mine;
-        auto found = [&](float x, int col, double log_all) {
-            p.tokens[row] = col;
-            p.log_prob[row] = (float)(((double)x - (double)top) * inverse - log_all);
+        auto found = [&](float x, int col) {  // for the first CTA, which has the logarithm by then
+            if constexpr (PARTS == 1) {
+                s.token_logit = x;
+                s.token = col;
+            } else {
+                asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(peer_smem(&s.token_logit, 0)), "f"(x) : "memory");
+                asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(peer_smem(&s.token, 0)), "r"(col) : "memory");
+            }
         };
         if (listed && br.hi == INF) {
             if (hit) {
                 unsigned long long at = before, seen = ties_before;
                 const int n = (int)s.listed[warp];
-                const double log_all = log(ldexp((double)all, -p.scale_bits));
                 for (int i0 = 0; i0 < n && at <= target; i0 += 32) {
                     const int i = i0 + lane;
                     const float x = i < n ? DT<T>::to_f32(s.list_x[warp][i]) : -INF;
@@ -888,14 +924,14 @@ template <typename T, int PARTS> __global__ void __launch_bounds__(SAMPLE_THREAD
                     const unsigned same = __ballot_sync(FULL, tie);
                     const bool in = i < n && (x > kept.above || (tie && seen + __popc(same & ((1u << lane) - 1)) < kept.ties));
                     const unsigned long long w = in ? weight(x) : 0, upto = at + warp_scan_u64(w, lane);
-                    if (target >= upto - w && target < upto) found(x, s.list_col[warp][i], log_all);
+                    if (target >= upto - w && target < upto) found(x, s.list_col[warp][i]);
                     at = __shfl_sync(FULL, upto, 31);
                     seen += __popc(same);
                 }
             }
         } else {
             // the token among those of a part, of which `at` are before, and `seen` equal to the border
-            auto find_in = [&](const Share<T> &part, unsigned long long at, unsigned long long seen, double log_all) {
+            auto find_in = [&](const Share<T> &part, unsigned long long at, unsigned long long seen) {
                 part.template walk<1>([&](const float *x, int col) {
                     if (at > target) return;
                     unsigned long long w[VEC<T>], here = 0, t = 0;
@@ -918,7 +954,7 @@ template <typename T, int PARTS> __global__ void __launch_bounds__(SAMPLE_THREAD
                         unsigned long long c = upto - here;
 #pragma unroll
                         for (int i = 0; i < VEC<T>; i++) {
-                            if (target >= c && target < c + w[i]) found(x[i], col + i, log_all);
+                            if (target >= c && target < c + w[i]) found(x[i], col + i);
                             c += w[i];
                         }
                     }
@@ -927,9 +963,8 @@ template <typename T, int PARTS> __global__ void __launch_bounds__(SAMPLE_THREAD
             };
             if (checked) {
                 if (hit) {
-                    const double log_all = log(ldexp((double)all, -p.scale_bits));
                     // what the list adds to each piece: bins that nobody uses any more
-                static_assert(CHECKS == 64, "two pieces a lane");
+                    static_assert(CHECKS == 64, "two pieces a lane");
                     unsigned *const low = s.bin[0], *const high = s.bin[1], *const tied = s.bin[0] + CHECKS;
                     unsigned long long in[2] = {0, 0};
                     unsigned ties_in[2] = {0, 0};
@@ -937,6 +972,7 @@ template <typename T, int PARTS> __global__ void __launch_bounds__(SAMPLE_THREAD
                         for (int i = lane; i < CHECKS; i += 32) low[i] = high[i] = tied[i] = 0;
                         __syncwarp();
                         unsigned long long seen = ties_before;
+#pragma unroll 4
                         for (int i0 = 0; i0 < (int)s.listed[warp]; i0 += 32) {
                             const int i = i0 + lane;
                             const float x = i < (int)s.listed[warp] ? DT<T>::to_f32(s.list_x[warp][i]) : -INF;
@@ -966,13 +1002,13 @@ template <typename T, int PARTS> __global__ void __launch_bounds__(SAMPLE_THREAD
 #pragma unroll
                     for (int i = 0; i < 2; i++) upto[i] = before + s.check[warp][min(pieces - 1, 2 * lane + i)] + listed_upto - (i ? 0 : in[1]);
                     const unsigned first = __ballot_sync(FULL, target < upto[0]), second = __ballot_sync(FULL, target < upto[1]);  // from some piece on
-                    const int at_lane = __ffs(second) - 1;
+                    const int at_lane = second ? __ffs(second) - 1 : 31;  // there is one, unless somebody writes to the logits meanwhile
                     const bool of_two = first >> at_lane & 1;  // the first of the lane's two
                     const unsigned long long last = __shfl_up_sync(FULL, upto[1], 1);
                     const unsigned long long from0 = lane ? last : before;
                     const unsigned long long at = __shfl_sync(FULL, of_two ? from0 : upto[0], at_lane);
                     const unsigned seen = __shfl_sync(FULL, ties_upto - ties_in[1] - (of_two ? ties_in[0] : 0), at_lane);
-                    find_in(sh.piece(2 * at_lane + (of_two ? 0 : 1)), at, ties_before + seen, log_all);
+                    find_in(sh.piece(2 * at_lane + (of_two ? 0 : 1)), at, ties_before + seen);
                 }
             } else {
                 // the warps of the CTA cut the share that the number falls into once more
@@ -983,15 +1019,10 @@ template <typename T, int PARTS> __global__ void __launch_bounds__(SAMPLE_THREAD
                 }
                 __syncthreads();
                 if (s.hit >= 0) {
-                    const Share<T> all_of_it(logits, p.x.vocab, rank * SAMPLE_WARPS + s.hit, WARPS), part(all_of_it, min(warp, SAMPLE_WARPS - 2), SAMPLE_WARPS - 1);
+                    const Share<T> all_of_it(logits, p.x.vocab, rank * SAMPLE_WARPS + s.hit, WARPS), part(all_of_it, warp, SAMPLE_WARPS);
                     sum = 0;
                     ties = 0;
-                    if (warp < SAMPLE_WARPS - 1) {
-                        part.over(under, count_in);
-                    } else {
-                        const double log_all = log(ldexp((double)all, -p.scale_bits));
-                        if (lane == 0) s.log_all = log_all;
-                    }
+                    part.over(under, count_in);
                     sum = warp_sum_u64(sum);
                     ties = __reduce_add_sync(FULL, ties);
                     if (lane == 0) {
@@ -1003,11 +1034,16 @@ template <typename T, int PARTS> __global__ void __launch_bounds__(SAMPLE_THREAD
                     const unsigned long long t_upto = s.seen + warp_scan_u64(wt, lane), t_before = t_upto - wt, k_before = min(t_before, kept.ties), k_upto = min(t_upto, kept.ties);
                     const unsigned long long kept_w = ws + (k_upto - k_before) * each, upto = s.before + warp_scan_u64(kept_w, lane);
                     const unsigned long long at = __shfl_sync(FULL, upto - kept_w, warp), seen = __shfl_sync(FULL, t_before, warp), end = __shfl_sync(FULL, upto, warp);
-                    if (target >= at && target < end) find_in(part, at, seen, s.log_all);
+                    if (target >= at && target < end) find_in(part, at, seen);
                 }
             }
         }
+        const double log_all = rank == 0 && warp == SAMPLE_WARPS - 1 ? log(ldexp((double)all, -p.scale_bits)) : 0.0;
         meet<PARTS>();  // the next row writes what was read here
+        if (rank == 0 && tid == SAMPLE_THREADS - 32) {
+            p.tokens[row] = s.token;
+            p.log_prob[row] = (float)(((double)s.token_logit - (double)top) * inverse - log_all);
+        }
     }
 }
 
