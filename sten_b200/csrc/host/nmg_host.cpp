@@ -993,7 +993,8 @@ at::Tensor f32_rows(const at::Tensor &t) { return t.defined() ? packed_rows(t) :
 void set_item(PyObject *tuple, Py_ssize_t i, const at::Tensor &t) { PyTuple_SET_ITEM(tuple, i, t.defined() ? THPVariable_Wrap(t) : Py_NewRef(Py_None)); }
 
 // A library call that failed where no interpreter is at hand: in the backward pass, on one of autograd's threads.
-void check_backward(int status) { TORCH_CHECK(status == NMG_OK, "nmg_b200 status ", status, ": ", nmg_last_error()); }
+// The text is put together without streams: a number through one ended the process (the locale of this library's own copy of the C++ runtime).
+void check_backward(int status) { TORCH_CHECK(status == NMG_OK, "nmg_b200 status " + std::to_string(status) + ": " + nmg_last_error()); }
 
 // Forward-mode derivatives: a tangent that is there must not be left out, which would read as a derivative of zero.
 bool has_tangent(const at::Tensor &t) { return t.defined() && t._fw_grad(/*level=*/0).defined(); }
