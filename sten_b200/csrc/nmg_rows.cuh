@@ -18,6 +18,18 @@ template <typename T, int V> struct Raw {
             else w[i] = reinterpret_cast<const uint4 *>(p)[i];
         }
     }
+    __device__ __forceinline__ void fill(float v) {
+#pragma unroll
+        for (int i = 0; i < N; i++) {
+            if constexpr (V == 1) w[i] = DT<T>::from_f32(v);
+            else {
+                float f[VEC<T>];
+#pragma unroll
+                for (int j = 0; j < VEC<T>; j++) f[j] = v;
+                w[i] = pack<T>(f);
+            }
+        }
+    }
     __device__ __forceinline__ void unpacked(float *f) const {
 #pragma unroll
         for (int i = 0; i < N; i++) {
