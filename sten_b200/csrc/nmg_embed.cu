@@ -4,9 +4,9 @@
 //
 // Both are bound by HBM.  Gradient: the tokens are sorted by their id, so that the rows of g that belong to one row of the matrix stand
 // together and are added in the order of their positions, whatever runs when, in 32 bits and rounded once.  Three launches:
-//   sort_kernel    one cluster sorts (id, position) in two or three radix passes; the other CTAs fill d_weight with zeros meanwhile
+//   sort_kernel    one cluster sorts (id, position) in two or three radix passes; the other CTAs fill d_weight's first rows with zeros meanwhile
 //   sum_kernel     the sorted list is cut into pieces of equal length, a warp for 32 vectors of columns of each; ids that lie within a piece
-//                  are finished, the sums of those that cross its ends are left in the workspace
+//                  are finished, the sums of those that cross its ends are left in the workspace.  Other CTAs fill the other rows that have no id
 //   join_kernel    puts the latter together
 #include "nmg_rows.cuh"
 
@@ -49,6 +49,7 @@ template <typename T, int V> __global__ void __launch_bounds__(LOOKUP_THREADS) e
 }
 
 // ---- the tokens in the order of their ids
+constexpr int FILL_BYTES = 32 << 10;  // of zeros that the copy engine writes at once
 constexpr int SORT_THREADS = 1024, SORT_WARPS = SORT_THREADS / 32, DIGIT_BITS = 9, DIGITS = 1 << DIGIT_BITS;
 struct SortParams {
     EmbedIds e;
@@ -72,14 +73,28 @@ __device__ __forceinline__ void cluster_barrier() {
     cluster_barrier_arrive();
     cluster_barrier_wait();
 }
+// `bytes` consecutive bytes to global memory, a multiple of 16 with both addresses 16-byte aligned
+__device__ __forceinline__ void bulk_store(void *gdst, const void *smem_src, int bytes) {
+    asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(gdst), "r"(smem_u32(smem_src)), "r"(bytes) : "memory");
+}
 __global__ void __launch_bounds__(SORT_THREADS) sort_kernel(const SortParams p) {
     extern __shared__ __align__(16) char smem[];
     const int rank = cluster_rank(), tid = (int)threadIdx.x, lane = tid & 31, warp = tid >> 5;
     if ((int)blockIdx.x >= p.parts) {  // not of the cluster that sorts
-        const int64_t vectors = p.fill_bytes / 16, step = (int64_t)(gridDim.x - p.parts) * SORT_THREADS;
-        uint4 *to = static_cast<uint4 *>(p.fill);
-        for (int64_t i = (int64_t)(blockIdx.x - p.parts) * SORT_THREADS + tid; i < vectors; i += step) to[i] = make_uint4(0u, 0u, 0u, 0u);
-        if ((int)blockIdx.x == p.parts && tid < (int)(p.fill_bytes & 15)) static_cast<char *>(p.fill)[vectors * 16 + tid] = 0;
+        for (int i = tid; i < FILL_BYTES / 16; i += SORT_THREADS) reinterpret_cast<uint4 *>(smem)[i] = make_uint4(0u, 0u, 0u, 0u);
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncthreads();
+        const int64_t chunks = (p.fill_bytes + FILL_BYTES - 1) / FILL_BYTES, whole = p.fill_bytes & ~(int64_t)15;
+        char *const to = static_cast<char *>(p.fill);
+        if (tid == 0) {
+            for (int64_t i = blockIdx.x - p.parts; i < chunks; i += gridDim.x - p.parts) {
+                const int64_t at = i * FILL_BYTES, left = whole - at;
+                if (left > 0) bulk_store(to + at, smem, (int)(left < FILL_BYTES ? left : FILL_BYTES));
+            }
+            asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+            asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+        }
+        if ((int)blockIdx.x == p.parts && tid < (int)(p.fill_bytes & 15)) to[whole + tid] = 0;
         return;
     }
     SortShared &s = *reinterpret_cast<SortShared *>(smem);
@@ -101,22 +116,28 @@ __global__ void __launch_bounds__(SORT_THREADS) sort_kernel(const SortParams p) 
         for (unsigned i = begin + lane; i < end; i += 32) atomicAdd(&s.count[warp][key_at(i) >> shift & mask], 1u);
         __syncthreads();
         if (tid < DIGITS) {
-            unsigned sum = 0;
+            unsigned sum = 0, n[SORT_WARPS];
+#pragma unroll
+            for (int w = 0; w < SORT_WARPS; w++) n[w] = s.count[w][tid];
+#pragma unroll
             for (int w = 0; w < SORT_WARPS; w++) {
-                const unsigned n = s.count[w][tid];
                 s.count[w][tid] = sum;
-                sum += n;
+                sum += n[w];
             }
             s.total[tid] = sum;
         }
         cluster_barrier();
-        unsigned before = 0, all = 0;
-        if (tid < DIGITS)
-            for (int r = 0; r < p.parts; r++) {
-                const unsigned n = peer_load_u32(peer_smem(&s.total[tid], r));
-                if (r < rank) before += n;
-                all += n;
+        unsigned before = 0, all = 0, n[8] = {};
+        if (tid < DIGITS) {
+#pragma unroll
+            for (int r = 0; r < 8; r++)  // all on their way before the first is looked at
+                if (r < p.parts) n[r] = peer_load_u32(peer_smem(&s.total[tid], r));
+#pragma unroll
+            for (int r = 0; r < 8; r++) {
+                if (r < rank) before += n[r];
+                all += n[r];
             }
+        }
         unsigned scan = all;  // over the digits
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -159,6 +180,8 @@ struct SumParams {
     int64_t ld;
     float scale;
     void *d_weight;
+    int64_t filled;  // rows from here on are not zero yet: those without an id are filled beside the sums
+    unsigned sum_ctas;
     float *part;  // [pieces][2][width]: of the id that began before the piece, and of the one that goes on behind it
 };
 constexpr int SUM_WARPS = 4;
@@ -182,10 +205,31 @@ template <typename T, int V, int K> struct Columns {
     }
     __device__ __forceinline__ float *part(const SumParams &p, unsigned piece, int which) const { return p.part + ((int64_t)piece * 2 + which) * p.width; }
 };
+// A warp's 32 rows: a lane looks for one of them in the sorted list, and those that are not there become zero.
+template <typename T, int V> __device__ __forceinline__ void fill_rows(const SumParams &p, int64_t item, int lane) {
+    const int64_t first = p.filled + item * 32, row = first + lane;
+    if (first >= p.vocab) return;
+    unsigned lo = 0, hi = p.tokens;  // the first key that is not below the row
+    while (lo < hi) {
+        const unsigned mid = (lo + hi) / 2;
+        if (p.key[mid] < row) lo = mid + 1;
+        else hi = mid;
+    }
+    unsigned empty = __ballot_sync(FULL, row < p.vocab && !(lo < p.tokens && p.key[lo] == row));
+    float zero[V] = {};
+    for (; empty; empty &= empty - 1) {
+        T *to = static_cast<T *>(p.d_weight) + (first + __ffs(empty) - 1) * p.width;
+        for (int c = lane * V; c < p.width; c += 32 * V) store_access<T, V>(to + c, zero);
+    }
+}
 template <typename T, int V, int K, int AHEAD> __global__ void __launch_bounds__(SUM_WARPS * 32) sum_kernel(const SumParams p) {
     dependents_wait();
     dependents_launch();
     const int lane = (int)threadIdx.x & 31;
+    if (blockIdx.x >= p.sum_ctas) {
+        fill_rows<T, V>(p, (int64_t)(blockIdx.x - p.sum_ctas) * SUM_WARPS + (threadIdx.x >> 5), lane);
+        return;
+    }
     const int64_t item = (int64_t)blockIdx.x * SUM_WARPS + (threadIdx.x >> 5);
     if (item >= (int64_t)p.pieces * p.slabs) return;
     const unsigned piece = (unsigned)(item / p.slabs), begin = piece * p.length, end = min(p.tokens, begin + p.length);
@@ -200,9 +244,7 @@ template <typename T, int V, int K, int AHEAD> __global__ void __launch_bounds__
         float *to = col.part(p, piece, which);
 #pragma unroll
         for (int k = 0; k < K; k++)
-            if (col.c[k] < p.width)
-#pragma unroll
-                for (int i = 0; i < V; i++) to[col.c[k] + i] = acc[k * V + i];
+            if (col.c[k] < p.width) store_access<float, V>(to + col.c[k], acc + k * V);
     };
     for (unsigned i0 = begin; i0 < end; i0 += 32) {
         const unsigned i = i0 + lane;
@@ -261,17 +303,25 @@ template <typename T, int V, int K, int AHEAD> __global__ void __launch_bounds__
     if (id == p.vocab || p.key[end] != id || (begin > 0 && p.key[begin] == id && p.key[begin - 1] == id)) return;
     const Columns<T, V, K> col((int)(item % p.slabs));
     unsigned last = piece + 1;  // the last piece that the id is in
-    while (last + 1 < p.pieces && p.key[(last + 1) * p.length] == id) last++;
+    for (;;) {
+        const unsigned next = last + 1 + (threadIdx.x & 31);
+        const unsigned there = __ballot_sync(FULL, next < p.pieces && p.key[next * p.length] == id);
+        last += there == FULL ? 32 : __ffs(~there) - 1;
+        if (there != FULL) break;
+    }
     float acc[K * V];
     auto add = [&](const float *from, bool first) {
 #pragma unroll
         for (int k = 0; k < K; k++)
-            if (col.c[k] < p.width)
+            if (col.c[k] < p.width) {
+                float f[V];
+                load_access<float, V>(from + col.c[k], f);
 #pragma unroll
-                for (int i = 0; i < V; i++) acc[k * V + i] = from[col.c[k] + i] + (first ? 0.f : acc[k * V + i]);
+                for (int i = 0; i < V; i++) acc[k * V + i] = f[i] + (first ? 0.f : acc[k * V + i]);
+            }
     };
     add(col.part(p, piece, 1), true);
-#pragma unroll 4
+#pragma unroll 8
     for (unsigned q = piece + 1; q <= last; q++) add(col.part(p, q, 0), false);
     col.store_row(p, id, acc);
 }
@@ -305,7 +355,9 @@ template <typename T, int V, int K, int AHEAD> static int launch_sums(SumParams 
     p.length = cut.length;
     p.pieces = cut.count;
     auto ctas = [&](int64_t pieces) { return dim3((unsigned)((pieces * p.slabs + SUM_WARPS - 1) / SUM_WARPS)); };
-    if (const int rc = launch_early(sum_kernel<T, V, K, AHEAD>, ctas(p.pieces), dim3(SUM_WARPS * 32), 0, st, p)) return rc;
+    p.sum_ctas = ctas(p.pieces).x;
+    const int64_t fill_ctas = (p.vocab - p.filled + 32 * SUM_WARPS - 1) / (32 * SUM_WARPS);
+    if (const int rc = launch_early(sum_kernel<T, V, K, AHEAD>, dim3((unsigned)(p.sum_ctas + fill_ctas)), dim3(SUM_WARPS * 32), 0, st, p)) return rc;
     if (p.pieces > 1) return launch_early(join_kernel<T, V, K, AHEAD>, ctas(p.pieces - 1), dim3(SUM_WARPS * 32), 0, st, p);
     return NMG_OK;
 }
@@ -348,13 +400,16 @@ extern "C" int nmg_embedding_backward(const void *g, int64_t ld_g, int64_t token
     if ((rc = device_sms(&sms))) return rc;
     cudaStream_t st = (cudaStream_t)stream;
     unsigned *list = static_cast<unsigned *>(workspace);
-    SortParams s{{ids, id_bytes, vocab}, padding, (unsigned)tokens, 0, 0, 1, {list, list + 2 * tokens}, {list + tokens, list + 3 * tokens}, d_weight, vocab * width * (int64_t)dtype_size(dtype)};
+    const int64_t row_bytes = width * (int64_t)dtype_size(dtype);
+    int64_t filled = (((int64_t)88 << 20) + tokens * 1024) / row_bytes;  // what the other SMs write while one cluster sorts (20 us for 12288 tokens)
+    if (filled > vocab) filled = vocab;
+    SortParams s{{ids, id_bytes, vocab}, padding, (unsigned)tokens, 0, 0, 1, {list, list + 2 * tokens}, {list + tokens, list + 3 * tokens}, d_weight, filled * row_bytes};
     int bits = 1;
     while (vocab >> bits) bits++;  // ids and vocab itself
     s.passes = (bits + DIGIT_BITS - 1) / DIGIT_BITS;
     s.digit_bits = (bits + s.passes - 1) / s.passes;
     while (s.parts < 8 && tokens > (int64_t)s.parts * 1024) s.parts *= 2;
-    const int64_t wanted = (s.fill_bytes + SORT_THREADS * 64 - 1) / (SORT_THREADS * 64), most = (int64_t)sms * 2 - s.parts;  // CTAs that fill
+    const int64_t wanted = (s.fill_bytes + FILL_BYTES - 1) / FILL_BYTES, most = (int64_t)sms * 2 - s.parts;  // CTAs that fill
     const int64_t fill = ((wanted < most ? wanted : most) + s.parts - 1) / s.parts * s.parts;
     NMG_ALLOW_SMEM(sizeof(SortShared), sort_kernel);
     cudaLaunchConfig_t cfg = {};
@@ -370,7 +425,7 @@ extern "C" int nmg_embedding_backward(const void *g, int64_t ld_g, int64_t token
     cfg.attrs = &attr;
     cfg.numAttrs = 1;
     NMG_CUDA(cudaLaunchKernelEx(&cfg, sort_kernel, s));
-    const SumParams p{s.key[0], s.pos[0], (unsigned)tokens, (unsigned)vocab, 0, 0, (int)width, 0, g, ld_g, scale, d_weight, reinterpret_cast<float *>(static_cast<char *>(workspace) + list_bytes(tokens))};
+    const SumParams p{s.key[0], s.pos[0], (unsigned)tokens, (unsigned)vocab, 0, 0, (int)width, 0, g, ld_g, scale, d_weight, filled, 0, reinterpret_cast<float *>(static_cast<char *>(workspace) + list_bytes(tokens))};
     const bool vectors = whole_vectors(g, ld_g, dtype) && whole_vectors(d_weight, width, dtype);
     NMG_DISPATCH_DTYPE(dtype, T, {
         if (vectors) return launch_sums<T, VEC<T>, 8 / VEC<T>, 8>(p, st);
