@@ -113,6 +113,7 @@ __global__ void __launch_bounds__(SORT_THREADS) sort_kernel(const SortParams p) 
         };
         for (int d = lane; d < DIGITS; d += 32) s.count[warp][d] = 0;
         __syncwarp();
+#pragma unroll 8
         for (unsigned i = begin + lane; i < end; i += 32) atomicAdd(&s.count[warp][key_at(i) >> shift & mask], 1u);
         __syncthreads();
         if (tid < DIGITS) {
@@ -151,19 +152,29 @@ __global__ void __launch_bounds__(SORT_THREADS) sort_kernel(const SortParams p) 
             s.base[tid] = scan - all + before;
         }
         __syncthreads();
-        for (unsigned i0 = begin; i0 < end; i0 += 32) {
-            const unsigned i = i0 + lane;
-            const bool there = i < end;
-            const unsigned key = there ? key_at(i) : 0, pos = there ? (pass ? __ldcg(pos_in + i) : i) : 0, d = there ? key >> shift & mask : DIGITS;
-            const unsigned same = __match_any_sync(FULL, d);
-            unsigned at = 0;
-            if (there) at = s.base[d] + s.count[warp][d] + __popc(same & ((1u << lane) - 1));
-            __syncwarp();
-            if (there && (same >> lane) == 1u) s.count[warp][d] += __popc(same);
-            __syncwarp();
-            if (there) {
-                key_out[at] = key;
-                pos_out[at] = pos;
+        // four steps of 32 are fetched at once
+        for (unsigned i0 = begin; i0 < end; i0 += 128) {
+            unsigned key[4], pos[4];
+#pragma unroll
+            for (int u = 0; u < 4; u++) {
+                const unsigned i = i0 + 32 * u + lane;
+                key[u] = i < end ? key_at(i) : 0;
+                pos[u] = i < end ? (pass ? __ldcg(pos_in + i) : i) : 0;
+            }
+#pragma unroll
+            for (int u = 0; u < 4; u++) {
+                if (i0 + 32 * u >= end) break;
+                const bool there = i0 + 32 * u + lane < end;
+                const unsigned d = there ? key[u] >> shift & mask : DIGITS, same = __match_any_sync(FULL, d);
+                unsigned at = 0;
+                if (there) at = s.base[d] + s.count[warp][d] + __popc(same & ((1u << lane) - 1));
+                __syncwarp();
+                if (there && (same >> lane) == 1u) s.count[warp][d] += __popc(same);
+                __syncwarp();
+                if (there) {
+                    key_out[at] = key[u];
+                    pos_out[at] = pos[u];
+                }
             }
         }
         __threadfence();
