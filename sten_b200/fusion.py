@@ -6,7 +6,8 @@ The reference runs ``F.linear`` and leaves bias, activation and residual to sepa
 rewires the two module shapes every BERT-style encoder is made of:
 
 * ``dense`` + ``intermediate_act_fn`` (exact GELU)            -> one call with ``activation="gelu"``
-* ``dense`` + ``dropout`` + ``LayerNorm(hidden + input)``     -> one call with ``residual=input`` followed by the LayerNorm
+* ``dense`` + ``dropout`` + ``LayerNorm(hidden + input)``     -> one call with ``residual=input`` followed by the LayerNorm, which
+  ``layer_norms=True`` makes a call of ``layer_norm``
 
 Only modules whose ``dense.weight`` is a grouped n:m parameter are touched, and only while gradients are disabled and
 dropout is inactive; otherwise the module's own forward runs.
@@ -18,6 +19,7 @@ import torch
 from . import ops
 from .dispatch import SparseTensorWrapper
 from .grouped_nm_tensor import GroupedNMTensor
+from .hidden import layer_norm
 
 
 def _nmg_weight(linear):
@@ -62,14 +64,27 @@ def _fused_output_forward(self, hidden_states, input_tensor):
     dropout_off = (not self.training) or getattr(self.dropout, "p", 0.0) == 0.0
     if gnm is None or torch.is_grad_enabled() or not dropout_off or not hidden_states.is_cuda:
         return self._sten_unfused_forward(hidden_states, input_tensor)
-    return self.LayerNorm(sparse_linear_fused(hidden_states, gnm, self.dense.bias, residual=input_tensor))
+    h, norm = sparse_linear_fused(hidden_states, gnm, self.dense.bias, residual=input_tensor), self.LayerNorm
+    if self._sten_layer_norm and _is_plain_layer_norm(norm, h):
+        return layer_norm(h, norm.weight, norm.bias, eps=norm.eps)
+    return norm(h)
 
 
-def fuse_linear_epilogues(model):
+def _is_plain_layer_norm(norm, x):
+    return (type(norm) is torch.nn.LayerNorm and norm.normalized_shape == x.shape[-1:] and not norm._forward_hooks and not norm._forward_pre_hooks
+            and all(p is None or (p.is_cuda and p.dtype in (x.dtype, torch.float32)) for p in (norm.weight, norm.bias))
+            and (norm.weight is None or norm.bias is None or norm.weight.dtype == norm.bias.dtype))
+
+
+def fuse_linear_epilogues(model, layer_norms=False):
     """Rewire ``dense`` + GELU and ``dense`` + residual + LayerNorm modules of ``model`` whose dense weight is grouped n:m.
-    Returns the number of modules rewired.  Idempotent."""
+    ``layer_norms``: the norm behind the residual runs as ``layer_norm`` too where it is a plain ``torch.nn.LayerNorm`` of the last
+    dimension; its results differ from torch's by roundings.  Returns the number of modules rewired.  Idempotent; modules that are
+    rewired already take the new choice of ``layer_norms``."""
     count = 0
     for mod in model.modules():
+        if hasattr(mod, "_sten_layer_norm"):
+            mod._sten_layer_norm = bool(layer_norms)
         dense = getattr(mod, "dense", None)
         if not isinstance(dense, torch.nn.Linear) or _nmg_weight(dense) is None or hasattr(mod, "_sten_unfused_forward"):
             continue
@@ -79,6 +94,7 @@ def fuse_linear_epilogues(model):
             count += 1
         elif hasattr(mod, "LayerNorm") and hasattr(mod, "dropout"):
             mod._sten_unfused_forward = mod.forward
+            mod._sten_layer_norm = bool(layer_norms)
             mod.forward = types.MethodType(_fused_output_forward, mod)
             count += 1
     return count
