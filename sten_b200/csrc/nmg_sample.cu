@@ -364,6 +364,7 @@ template <bool WEIGHTS, int PARTS, typename T, typename S> __device__ __noinline
         const int shift = max(0, 32 - __clz(hi - lo) - 10);  // BINS of them
         static_assert(BINS == 1 << 10, "bins of the search");
         for (int i = tid; i < BINS; i += SAMPLE_THREADS) s.bin[0][i] = s.bin[1][i] = 0;
+        if (tid == 0) s.from = 0xffffffffu, s.to = 0;
         __syncthreads();
         const float above = first ? from.above : fmaxf(from.above, logit_of<T>(lo - 1)), below = logit_of<T>(hi);
         source.over(above, [&](float x) {
@@ -440,10 +441,33 @@ template <bool WEIGHTS, int PARTS, typename T, typename S> __device__ __noinline
         base = s.base;
         __syncthreads();
         if (at < 0) return from;  // only where somebody writes to the logits meanwhile
-        hi -= (unsigned)at << shift;
-        const unsigned width = (1u << shift) - 1;
-        if (hi - lo > width) lo = hi - width;
-        if (shift == 0) {
+        if constexpr (PARTS == 1) {
+            if (shift) {  // the smallest and the largest of the bin, which are often one
+                unsigned least = 0xffffffffu, most = 0;
+                source.over(above, [&](float x) {
+                    const unsigned key = key_of<T>(x);
+                    if (key <= hi && (hi - key) >> shift == (unsigned)at) least = min(least, key), most = max(most, key);
+                });
+                least = __reduce_min_sync(FULL, least);
+                most = __reduce_max_sync(FULL, most);
+                if (lane == 0 && most >= least) {
+                    atomicMin(&s.from, least);
+                    atomicMax(&s.to, most);
+                }
+                __syncthreads();
+                lo = s.from;
+                hi = s.to;
+                __syncthreads();
+                if (lo > hi) return from;  // as above
+            } else {
+                lo = hi -= (unsigned)at;
+            }
+        } else {
+            hi -= (unsigned)at << shift;
+            const unsigned width = (1u << shift) - 1;
+            if (hi - lo > width) lo = hi - width;
+        }
+        if (shift == 0 || (PARTS == 1 && lo == hi)) {
             const float value = logit_of<T>(hi);
             if (!WEIGHTS) return Border{value, target - base};
             const unsigned long long each = weight(value);
@@ -734,11 +758,12 @@ template <typename T, int PARTS> __global__ void __launch_bounds__(SAMPLE_THREAD
         bool both = false;    // the first CTA has looked for both borders
         bool listed = false;  // what is kept: the list's part of it, and all above the bracket
         Bracket br{window, INF};
-        if (by_count || by_weight) {
+        const bool direct = p.x.vocab <= min(FLAT, WARPS * (LISTED - 16));  // the row is short: all that has a weight is listed
+        if ((by_count || by_weight) && !direct) {
             const float octaves = (float)(p.scale_bits + 1) / BINS, per_bin = a / octaves;  // of a bin; bins of a logit
             const float scale = take_sample<PARTS>(s, sh, window, top, per_bin, by_count ? 4096 : 16384, me);
             if (rank == 0) {
-                const float room = 0.3f * (float)min(FLAT, WARPS * LISTED);
+                const float room = fminf(0.85f * FLAT, 0.6f * WARPS * LISTED);
                 if (by_count) {
                     find_bracket<false, PARTS>(s, scale, window, top, per_bin, octaves, (float)top_k, room);
                 } else {
@@ -756,7 +781,7 @@ template <typename T, int PARTS> __global__ void __launch_bounds__(SAMPLE_THREAD
             br.hi = peer_f32<PARTS>(&s.hi, 0);
         }
         if ((by_count || by_weight) && br.lo < top) {
-            const bool sums = !by_count || br.hi < INF;
+            const bool sums = !direct && (!by_count || br.hi < INF);
             if (sums) gather<true>(s, sh, weight, br);
             else gather<false>(s, sh, weight, br);
             meet<PARTS>();
@@ -785,8 +810,9 @@ template <typename T, int PARTS> __global__ void __launch_bounds__(SAMPLE_THREAD
             }
             unsigned long long target = by_count ? (unsigned long long)top_k : (unsigned long long)ceil(top_p * (double)all);
             if (target < 1) target = 1;
+            if (direct && !by_count) target = 0;  // that share of what is listed
             const bool all_kept = by_count && br.lo == window && target > (unsigned long long)count + entries;  // fewer than k have a weight
-            const bool in_list = most <= LISTED && (by_count ? count < target && (target <= count + entries || all_kept) : above < target);
+            const bool in_list = most <= LISTED && (by_count ? count < target && (target <= count + entries || all_kept) : direct || above < target);
             if (in_list && entries > FLAT) {  // every CTA in its lists
                 const Listed<T> list{s.list_x[warp], (int)s.listed[warp], lane};
                 const Border found = by_count ? find_border<false, PARTS, T>(s, list, weight, Border{br.lo, 0}, fminf(br.hi, top), count, 0.0, target)
@@ -811,7 +837,7 @@ template <typename T, int PARTS> __global__ void __launch_bounds__(SAMPLE_THREAD
                         if (!all_kept) found = find_border<false, 1, T>(s, flat, weight, from, high, count, 0.0, target);
                         if (both) found = find_border<true, 1, T>(s, flat, weight, found, top, 0, top_p, 0);
                     } else {
-                        found = find_border<true, 1, T>(s, flat, weight, from, high, above, 0.0, target);
+                        found = find_border<true, 1, T>(s, flat, weight, from, high, above, top_p, target);
                         there = found.ties > 0 || br.lo == window;  // the latter: rounded up, all of it
                     }
                     if (tid == 0) {
