@@ -305,10 +305,13 @@ template <typename T> struct Share {
             m = sl.at(c);
             if (stats) stats->st.template add_one<false>(m, a), stats->refer(a);
         }
-        steps<4>([&](const uint4 *q, int) {
+        steps<8>([&](const uint4 *q, int) {
 #pragma unroll
-            for (int u = 0; u < 4; u++) m = max_or_nan(m, vector_max_or_nan<T>(q[u]));
-            if (stats) stats->add(q, a);
+            for (int u = 0; u < 8; u++) m = max_or_nan(m, vector_max_or_nan<T>(q[u]));
+            if (stats) {
+                stats->add(q, a);
+                stats->add(q + 4, a);
+            }
         });
 #pragma unroll
         for (int o = 16; o; o >>= 1) m = max_or_nan(m, __shfl_xor_sync(FULL, m, o));
@@ -369,7 +372,7 @@ template <bool WEIGHTS, int PARTS, typename T, typename S> __device__ __noinline
         const float above = first ? from.above : fmaxf(from.above, logit_of<T>(lo - 1)), below = logit_of<T>(hi);
         source.over(above, [&](float x) {
             if (!first && x > below) return;
-            const unsigned b = (hi - key_of<T>(x)) >> shift;
+            const unsigned b = min((hi - key_of<T>(x)) >> shift, (unsigned)BINS - 1);  // none is above hi, unless somebody writes to the logits meanwhile
             if constexpr (WEIGHTS) {
                 const unsigned long long w = weight(x);
                 const unsigned low = (unsigned)w, old = atomicAdd(&s.bin[0][b], low);
@@ -505,7 +508,7 @@ template <int PARTS, typename T> __device__ __noinline__ float take_sample(Sampl
             unpack<T>(q[u], x);
 #pragma unroll
             for (int j = 0; j < VEC<T>; j++)
-                if (x[j] > window) atomicAdd(&bin[min(BINS - 1, (int)((top - x[j]) * per_bin))], 1u);
+                if (x[j] > window) atomicAdd(&bin[max(0, min(BINS - 1, (int)((top - x[j]) * per_bin)))], 1u);
         }
     }
     meet<PARTS>();
