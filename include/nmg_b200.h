@@ -311,7 +311,7 @@ int nmg_sample_tokens(const void *logits, int64_t rows, int64_t inner_rows, int6
  *   h = x, or with a residual sum = x + residual rounded to dtype, which is written
  *   y = (h - mean) rstd weight + bias,  rstd = 1 / sqrt(mean of (h - mean)^2 + eps);  stats [rows][2] (8-byte aligned, may be NULL): mean, rstd
  * nmg_layer_norm_backward takes h (x or sum) and stats, the gradient of y and (or NULL) that of sum, and writes d_x, which is the residual's
- * gradient too, d_weight and d_bias, each unless NULL.  The sums over rows are added in 32 bits in a fixed order.  The workspace (16-byte
+ * gradient too, d_weight and d_bias, each unless NULL.  The sums over rows are added in a fixed order, a CTA's in 32 bits.  The workspace (16-byte
  * aligned) is needed for d_weight and d_bias only; its size depends on the current device.  No output may overlap an input. */
 int nmg_layer_norm(const void *x, int64_t ld_x, const void *residual, int64_t ld_residual, int64_t rows, int64_t width, int dtype,
                    const void *weight, const void *bias, int param_dtype, float eps, void *y, void *sum, float *stats, void *stream);

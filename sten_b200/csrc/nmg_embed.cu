@@ -8,6 +8,8 @@
 //   sum_kernel     the sorted list is cut into pieces of equal length, a warp for 32 vectors of columns of each; ids that lie within a piece
 //                  are finished, the sums of those that cross its ends are left in the workspace.  Other CTAs fill the other rows that have no id
 //   join_kernel    puts the latter together
+// 16384 tokens of 131072 x 4096 bf16: 20 + 185 + 8 us, 1.2 GB at 5.6 TB/s in the second (writing alone reaches 5.4); 12288 of 30522 x 1024 fp32: 20 + 25 + 8.  The sort is
+// latency: its cluster meets twice a pass.  Filling all of the matrix during the sort, before the sums: 198 + 40 + 8.
 #include "nmg_rows.cuh"
 
 namespace nmg {
@@ -20,7 +22,7 @@ struct EmbedIds {
     __device__ __forceinline__ bool valid(int64_t id) const { return id >= 0 && id < vocab; }
 };
 
-// A thread takes LOOKUPS accesses of V columns, a CTA's threads neighbouring ones.
+// A thread takes LOOKUPS accesses of V columns, a CTA's threads neighbouring ones.  16384 rows of 8 KB 33 us (8 TB/s: ids that come again are found in L2).
 constexpr int LOOKUP_THREADS = 256, LOOKUPS = 4;
 template <typename T, int V> __global__ void __launch_bounds__(LOOKUP_THREADS) embed_kernel(const EmbedIds e, const T *weight, int64_t ld, int64_t tokens, int width, float scale, T *out) {
     const unsigned each = (unsigned)(width / V);

@@ -11,6 +11,10 @@
 // Which token a number falls to turns on sums of up to a hundred thousand weights that differ by millionths, so 32 bits would draw another
 // token for one row in forty.  Weights are therefore integers, w 2^s rounded (s = 62 - log2 of the vocabulary, at most 46; w from a polynomial
 // in 64-bit floating point, relative error 2^-42): sums are exact, and the same for every way a row is cut.  Weights below 2^-(s+1) count as zero.
+//
+// A row is read once from memory for its maximum and again from L2.  1024 x 131072 bf16 without filters 190 us: 28 instructions a logit, of which 21 are the weight's, at
+// half the issue slots (floor: 41 us of memory, 106 of issue).  256 x 131072 with top_p = 0.95 and a fifth of the tokens kept 136, 64 x 131072 with settings of every row 52,
+// 97 x 50021 fp32 with all filters 39, one row of 30522 fp16 with top-k and top-p 19: these are chains of ten or so phases with a meeting each.
 #include "nmg_rows.cuh"
 
 namespace nmg {
