@@ -488,7 +488,7 @@ struct Bracket {
     float lo, hi;
 };
 // One step of 32 vectors in `stride` is counted into bins of equal width below the row's maximum.  What the sample says of the row's count above (weight below) a bin
-// is off by its standard deviation, s times the root of the sum of squares of what was counted; the bracket is four of them wide to both sides,
+// is off by its standard deviation, the root of the sum of squares of what was counted and, of that, the part the sample left out; the bracket is four of them wide to both sides,
 // and one element that the sample missed.  Where the border is not in it after all, the search over the whole row takes over.
 // The counting is done by all, and says how many logits one of the sample stands for.
 template <int PARTS, typename T> __device__ __noinline__ float take_sample(SampleShared<T> &s, const Share<T> &sh, float window, float top, float per_bin, int elements, int warp_of_row) {
@@ -567,10 +567,11 @@ template <bool WEIGHTS, int PARTS, typename T> __device__ __noinline__ void find
         all += t.z;
     }
     want /= scale;
+    const float missed = 1.f - 1.f / scale;  // a sample of the whole row is off by nothing
     unsigned surely = BINS, may = BINS;
 #pragma unroll
     for (int i = EACH - 1; i >= 0; i--) {
-        const float m = before.x + n[i].x, off = 4.f * sqrtf(before.y + n[i].y + one[i] * one[i]) + (WEIGHTS ? 0.5f * octaves * want : 0.f);  // half a bin's width is what the weights of its logits may be off by
+        const float m = before.x + n[i].x, off = 4.f * sqrtf(missed * (before.y + n[i].y) + one[i] * one[i]) + (WEIGHTS ? 0.5f * octaves * want : 0.f);  // half a bin's width is what the weights of its logits may be off by
         if (m - off >= want) surely = tid * EACH + i;     // the border is in this bin or before it
         if (m + off > want) may = tid * EACH + i;         // or may be
     }
@@ -768,7 +769,10 @@ template <typename T, int PARTS> __global__ void __launch_bounds__(SAMPLE_THREAD
         const bool direct = p.x.vocab <= min(FLAT, WARPS * (LISTED - 16));  // the row is short: all that has a weight is listed
         if ((by_count || by_weight) && !direct) {
             const float octaves = (float)(p.scale_bits + 1) / BINS, per_bin = a / octaves;  // of a bin; bins of a logit
-            const float scale = take_sample<PARTS>(s, sh, window, top, per_bin, by_count ? 4096 : 16384, me);
+            // By weight half of a long row, by count more the further down the border is: 1024 x 131072 bf16 with top_p = 0.95 takes 435 us, with a sample of
+            // 16384 (whose bracket the lists do not hold, so that the search goes over the row) 1536; with top_k = 50 a sample of 65536 would take 163, not 145.
+            const int elements = by_weight && !by_count ? max(65536, p.x.vocab / 2) : top_k > 8192 ? 65536 : 16384;
+            const float scale = take_sample<PARTS>(s, sh, window, top, per_bin, elements, me);
             if (rank == 0) {
                 const float room = fminf(0.85f * FLAT, 0.6f * WARPS * LISTED);
                 if (by_count) {
@@ -1081,10 +1085,12 @@ template <typename T, int PARTS> __global__ void __launch_bounds__(SAMPLE_THREAD
 }
 
 // A row is shared by as many CTAs as keep the SMs filled, two of them to an SM; each has some thousand logits at least.
-static int sample_parts(int64_t rows, int vocab, int sms) {
+// `deep`: the border may lie far down.  Then a long row takes two at least, whose lists hold twice as many logits of its bracket: 1024 x 131072 bf16
+// with top_p = 0.9 takes 443 us, by one CTA a row 421, but of logits spread by 1 instead of 2.5 479 and 1484; the first of 65536 by count 440 and 794.
+static int sample_parts(int64_t rows, int vocab, bool deep, int sms) {
     int best = 1;
     double best_time = 1e300;
-    for (int parts = 1; parts <= 8; parts *= 2) {
+    for (int parts = deep && vocab > 65536 ? 2 : 1; parts <= 8; parts *= 2) {
         if (parts > 1 && vocab < parts * 2048) break;
         const int64_t slots = (int64_t)sms * SAMPLE_PER_SM / parts - (parts > 2 ? sms / (6 * parts) : 0), rounds = (rows + slots - 1) / slots;
         const double time = (double)rounds * ((double)vocab / parts + (parts > 1 ? 3000 + 500 * parts : 2000));
@@ -1158,7 +1164,8 @@ extern "C" int nmg_sample_tokens(const void *logits, int64_t rows, int64_t inner
     int bits = 0;
     while ((int64_t)1 << bits < vocab) bits++;
     if (p.scale_bits > 62 - bits) p.scale_bits = 62 - bits;
-    const int parts = sample_parts(rows, p.x.vocab, sms);
+    const bool deep = top_ks || top_k > 2048 || (top_k == 0 && (top_ps || top_p < 1));
+    const int parts = sample_parts(rows, p.x.vocab, deep, sms);
     cudaStream_t st = (cudaStream_t)stream;
     NMG_DISPATCH_DTYPE(dtype, T, {
         if (parts == 1) return launch_sample<T, 1>(p, st);

@@ -100,6 +100,16 @@ def test_rows_and_clusters(rows, setting):
         assert torch.equal(part.tokens, o.tokens[a:b]) and torch.equal(part.log_prob, o.log_prob[a:b])
 
 
+@pytest.mark.parametrize("scale", [0.3, 1.0, 2.5])  # the narrower, the more logits there are beside the border
+@pytest.mark.parametrize("setting", [dict(top_p=0.9), dict(top_k=2048), dict(top_k=50000), dict(top_k=9000, top_p=0.7)])
+def test_long_rows_with_borders_far_down(setting, scale):
+    x, u = logits(600, 90001, BF16, seed=3, scale=scale, ahead=False)
+    o = sten.sample_tokens(x, u, **setting)  # by the CTAs that many rows get
+    some = torch.arange(0, 600, 40, device="cuda")
+    few = check(x[some], u[some], **setting)
+    assert torch.equal(few.tokens, o.tokens[some]) and torch.equal(few.log_prob, o.log_prob[some])
+
+
 @pytest.mark.parametrize("dtype", [F32, BF16])
 def test_settings_of_every_row(dtype):
     x, u = logits(60, 5003, dtype)
