@@ -194,10 +194,10 @@ struct SumParams {
     float scale;
     void *d_weight;
     int64_t filled;  // rows from here on are not zero yet: those without an id are filled beside the sums
-    unsigned sum_ctas;
+    unsigned sum_ctas, fill_rows;  // fill_rows: of a warp, at most 32
     float *part;  // [pieces][2][width]: of the id that began before the piece, and of the one that goes on behind it
 };
-constexpr int SUM_WARPS = 4;
+constexpr int SUM_WARPS = 4, FILL_WARPS = 4096;
 
 template <typename T, int V, int K> struct Columns {
     int c[K];
@@ -218,9 +218,9 @@ template <typename T, int V, int K> struct Columns {
     }
     __device__ __forceinline__ float *part(const SumParams &p, unsigned piece, int which) const { return p.part + ((int64_t)piece * 2 + which) * p.width; }
 };
-// A warp's 32 rows: a lane looks for one of them in the sorted list, and those that are not there become zero.
-template <typename T, int V> __device__ __forceinline__ void fill_rows(const SumParams &p, int64_t item, int lane) {
-    const int64_t first = p.filled + item * 32, row = first + lane;
+// Some rows of a warp: a lane looks for one of them in the sorted list, and those that are not there become zero.
+template <typename T> __device__ __forceinline__ void fill_rows(const SumParams &p, int64_t item, int lane) {
+    const int64_t first = p.filled + item * p.fill_rows, row = first + lane;
     if (first >= p.vocab) return;
     unsigned lo = 0, hi = p.tokens;  // the first key that is not below the row
     while (lo < hi) {
@@ -228,11 +228,15 @@ template <typename T, int V> __device__ __forceinline__ void fill_rows(const Sum
         if (p.key[mid] < row) lo = mid + 1;
         else hi = mid;
     }
-    unsigned empty = __ballot_sync(FULL, row < p.vocab && !(lo < p.tokens && p.key[lo] == row));
-    float zero[V] = {};
+    unsigned empty = __ballot_sync(FULL, lane < (int)p.fill_rows && row < p.vocab && !(lo < p.tokens && p.key[lo] == row));
     for (; empty; empty &= empty - 1) {
-        T *to = static_cast<T *>(p.d_weight) + (first + __ffs(empty) - 1) * p.width;
-        for (int c = lane * V; c < p.width; c += 32 * V) store_access<T, V>(to + c, zero);
+        T *const to = static_cast<T *>(p.d_weight) + (first + __ffs(empty) - 1) * p.width;
+        // elements before the first whole vector (of a row that begins between two), vectors, elements
+        const int head = min(p.width, (int)(-(intptr_t)to & 15) / (int)sizeof(T)), vectors = (p.width - head) / VEC<T>;
+        uint4 *const v = reinterpret_cast<uint4 *>(to + head);
+        for (int c = lane; c < vectors; c += 32) v[c] = make_uint4(0u, 0u, 0u, 0u);
+        if (lane < head) to[lane] = DT<T>::from_f32(0.f);
+        if (head + vectors * VEC<T> + lane < p.width) to[head + vectors * VEC<T> + lane] = DT<T>::from_f32(0.f);
     }
 }
 template <typename T, int V, int K, int AHEAD> __global__ void __launch_bounds__(SUM_WARPS * 32) sum_kernel(const SumParams p) {
@@ -240,7 +244,7 @@ template <typename T, int V, int K, int AHEAD> __global__ void __launch_bounds__
     dependents_launch();
     const int lane = (int)threadIdx.x & 31;
     if (blockIdx.x >= p.sum_ctas) {
-        fill_rows<T, V>(p, (int64_t)(blockIdx.x - p.sum_ctas) * SUM_WARPS + (threadIdx.x >> 5), lane);
+        fill_rows<T>(p, (int64_t)(blockIdx.x - p.sum_ctas) * SUM_WARPS + (threadIdx.x >> 5), lane);
         return;
     }
     const int64_t item = (int64_t)blockIdx.x * SUM_WARPS + (threadIdx.x >> 5);
@@ -369,7 +373,11 @@ template <typename T, int V, int K, int AHEAD> static int launch_sums(SumParams 
     p.pieces = cut.count;
     auto ctas = [&](int64_t pieces) { return dim3((unsigned)((pieces * p.slabs + SUM_WARPS - 1) / SUM_WARPS)); };
     p.sum_ctas = ctas(p.pieces).x;
-    const int64_t fill_ctas = (p.vocab - p.filled + 32 * SUM_WARPS - 1) / (32 * SUM_WARPS);
+    // Few rows of a large matrix are shared by more warps: 2 tokens of a matrix of 9333 x 7641 fp32 take 56 us (zeros alone: 44), by 32 rows a warp 90.
+    const int64_t empty = p.vocab - p.filled;
+    p.fill_rows = 32;
+    while (p.fill_rows > 1 && empty / p.fill_rows < FILL_WARPS) p.fill_rows /= 2;
+    const int64_t fill_ctas = (empty + p.fill_rows * SUM_WARPS - 1) / (p.fill_rows * SUM_WARPS);
     if (const int rc = launch_early(sum_kernel<T, V, K, AHEAD>, dim3((unsigned)(p.sum_ctas + fill_ctas)), dim3(SUM_WARPS * 32), 0, st, p)) return rc;
     if (p.pieces > 1) return launch_early(join_kernel<T, V, K, AHEAD>, ctas(p.pieces - 1), dim3(SUM_WARPS * 32), 0, st, p);
     return NMG_OK;
@@ -438,7 +446,7 @@ extern "C" int nmg_embedding_backward(const void *g, int64_t ld_g, int64_t token
     cfg.attrs = &attr;
     cfg.numAttrs = 1;
     NMG_CUDA(cudaLaunchKernelEx(&cfg, sort_kernel, s));
-    const SumParams p{s.key[0], s.pos[0], (unsigned)tokens, (unsigned)vocab, 0, 0, (int)width, 0, g, ld_g, scale, d_weight, filled, 0, reinterpret_cast<float *>(static_cast<char *>(workspace) + list_bytes(tokens))};
+    const SumParams p{s.key[0], s.pos[0], (unsigned)tokens, (unsigned)vocab, 0, 0, (int)width, 0, g, ld_g, scale, d_weight, filled, 0, 32, reinterpret_cast<float *>(static_cast<char *>(workspace) + list_bytes(tokens))};
     const bool vectors = whole_vectors(g, ld_g, dtype) && whole_vectors(d_weight, width, dtype);
     NMG_DISPATCH_DTYPE(dtype, T, {
         if (vectors) return launch_sums<T, VEC<T>, 8 / VEC<T>, 8>(p, st);

@@ -80,6 +80,13 @@ def test_widths(dtype, width):
     case("words", 777, 333, width, dtype, scale=width ** 0.5, padding=0, seed=width)
 
 
+@pytest.mark.parametrize("dtype,vocab,width", [(F32, 9333, 7641), (F16, 5000, 20003), (BF16, 70001, 1001), (F32, 40, 900000), (F16, 90, 700008)])
+def test_large_matrices_with_few_tokens(dtype, vocab, width):
+    stale = [torch.full((vocab, width), float("nan"), dtype=dtype, device="cuda") for _ in range(3)]  # what the gradient's memory may hold before
+    del stale
+    case("even", 7, vocab, width, dtype)
+
+
 def test_pieces_longer_than_the_shortest():
     case("words", 120000, 3000, 1024, BF16)   # pieces of 96 positions and more
     case("one", 70000, 3, 2048, F32)
