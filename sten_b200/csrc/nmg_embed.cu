@@ -8,7 +8,7 @@
 //   sum_kernel     the sorted list is cut into pieces of equal length, a warp for 32 vectors of columns of each; ids that lie within a piece
 //                  are finished, the sums of those that cross its ends are left in the workspace.  Other CTAs fill the other rows that have no id
 //   join_kernel    puts the latter together
-// 16384 tokens of 131072 x 4096 bf16: 20 + 185 + 8 us, 1.2 GB at 5.6 TB/s in the second (writing alone reaches 5.4); 12288 of 30522 x 1024 fp32: 20 + 25 + 8.  The sort is
+// 16384 tokens of 131072 x 4096 bf16: 27 + 174 + 11 us, 1.2 GB in all; 12288 of 30522 x 1024 fp32: 20 + 25 + 8.  The sort is
 // latency: its cluster meets twice a pass.  Filling all of the matrix during the sort, before the sums: 198 + 40 + 8.
 #include "nmg_rows.cuh"
 
