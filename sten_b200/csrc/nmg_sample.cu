@@ -83,6 +83,8 @@ template <typename T> __device__ __forceinline__ float logit_of(unsigned key) {
     const unsigned b = key << KEY_SHIFT<T>;
     return __uint_as_float(b & 0x80000000u ? b ^ 0x80000000u : KEY_SHIFT<T> ? ~(b | ((1u << KEY_SHIFT<T>) - 1)) : ~b);
 }
+// A float that the logits of a key are above, and those of smaller keys are not.  Under the key of 0 is that of -0, which no logit has and 0 is not above.
+template <typename T> __device__ __forceinline__ float under_key(unsigned key) { return logit_of<T>(key - (key == 0x80000000u >> KEY_SHIFT<T> ? 2 : 1)); }
 
 __device__ __forceinline__ float max_or_nan(float a, float b) {
     float r;
@@ -373,10 +375,11 @@ template <bool WEIGHTS, int PARTS, typename T, typename S> __device__ __noinline
         for (int i = tid; i < BINS; i += SAMPLE_THREADS) s.bin[0][i] = s.bin[1][i] = 0;
         if (tid == 0) s.from = 0xffffffffu, s.to = 0;
         __syncthreads();
-        const float above = first ? from.above : fmaxf(from.above, logit_of<T>(lo - 1)), below = logit_of<T>(hi);
+        const float above = first ? from.above : fmaxf(from.above, under_key<T>(lo));
         source.over(above, [&](float x) {
-            if (!first && x > below) return;
-            const unsigned b = min((hi - key_of<T>(x)) >> shift, (unsigned)BINS - 1);  // none is above hi, unless somebody writes to the logits meanwhile
+            const unsigned key = key_of<T>(x);
+            if (key > hi) return;  // of the first bins; hi need not be a logit's key
+            const unsigned b = min((hi - key) >> shift, (unsigned)BINS - 1);  // fewer than BINS, unless somebody writes to the logits meanwhile
             if constexpr (WEIGHTS) {
                 const unsigned long long w = weight(x);
                 const unsigned low = (unsigned)w, old = atomicAdd(&s.bin[0][b], low);
@@ -757,8 +760,8 @@ template <typename T, int PARTS> __global__ void __launch_bounds__(SAMPLE_THREAD
         {
             const float lowest = __double2float_rd((double)top - (p.scale_bits + 1) * 0.6931471805599454 * tau);
             if (lowest > kept.above) kept.above = lowest;
-            const unsigned key = key_of<T>(kept.above);  // a logit of the type, or what lies between two of them
-            kept.above = logit_of<T>(key > key_of<T>(neg_inf()) ? key - 1 : key);
+            const unsigned key = key_of<T>(kept.above);  // of a logit of the type, or of what lies between two of them
+            if (key > key_of<T>(neg_inf())) kept.above = under_key<T>(key);
         }
         const float window = kept.above;
 
