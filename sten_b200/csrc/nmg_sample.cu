@@ -359,11 +359,13 @@ template <typename T> struct Listed {
 struct Border {
     float above;
     unsigned long long ties;
+    __device__ __forceinline__ bool lost() const { return above != above; }
 };
 
 // The border of the run, largest first, whose measure (1 each, or their weights) reaches `target`, or `share` of the whole where that is 0.  The run begins with
 // logits that measure `base` together and are not looked at, goes on with those of the source from `top` down to above from.above, and ends with from.ties
-// that equal it: `from` itself where the run takes all of it.
+// that equal it: `from` itself where the run takes all of it.  A border that is not where the pass before saw it, as where somebody writes to the logits
+// meanwhile, is lost (NaN).
 template <bool WEIGHTS, int PARTS, typename T, typename S> __device__ __noinline__ Border find_border(SampleShared<T> &s, const S &source, const Weight &weight, const Border from, float top, unsigned long long base,
                                                                                                      double share, unsigned long long target) {
     const int tid = (int)threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -450,7 +452,8 @@ template <bool WEIGHTS, int PARTS, typename T, typename S> __device__ __noinline
         const int at = s.crossing;
         base = s.base;
         __syncthreads();
-        if (at < 0) return from;  // only where somebody writes to the logits meanwhile
+        const Border lost{__int_as_float(0x7fffffff), 0};
+        if (at < 0) return lost;
         if constexpr (PARTS == 1) {
             if (shift) {  // the smallest and the largest of the bin, which are often one
                 unsigned least = 0xffffffffu, most = 0;
@@ -468,7 +471,7 @@ template <bool WEIGHTS, int PARTS, typename T, typename S> __device__ __noinline
                 lo = s.from;
                 hi = s.to;
                 __syncthreads();
-                if (lo > hi) return from;  // as above
+                if (lo > hi) return lost;
             } else {
                 lo = hi -= (unsigned)at;
             }
@@ -689,6 +692,10 @@ template <typename T, int PARTS> __global__ void __launch_bounds__(SAMPLE_THREAD
         typename SampleShared<T>::Settings set{p.temperatures ? (double)p.temperatures[row] : p.temperature, p.top_ps ? (double)p.top_ps[row] : p.top_p, p.min_ps ? (double)p.min_ps[row] : p.min_p,
                                                p.top_ks ? (long long)p.top_ks[row] : (long long)p.top_k, p.uniform[row]};
         if (rank == 0 && tid == 0) s.settings = set;
+        if (rank == 0 && tid == SAMPLE_THREADS - 32) {  // who wrote the last row's: what is said where no share has the token, as above
+            s.token = -1;
+            s.token_logit = __int_as_float(0x7fffffff);
+        }
 
         // the maximum, and about the softmax's sum where a share of it is asked for
         float a = (float)(1.4426950408889634 / set.tau);
@@ -865,9 +872,17 @@ template <typename T, int PARTS> __global__ void __launch_bounds__(SAMPLE_THREAD
             }
         }
         if (!listed && by_count) kept = find_border<false, PARTS, T>(s, sh, weight, kept, top, 0, 0.0, (unsigned long long)top_k);  // over the whole row
-        if (by_weight && (!listed || (by_count && !both))) {
+        if (by_weight && (!listed || (by_count && !both)) && !kept.lost()) {
             kept = find_border<true, PARTS, T>(s, sh, weight, kept, top, 0, top_p, 0);
             listed = false;
+        }
+        if (kept.lost()) {  // in all CTAs: they have the same bins.  Nothing is drawn rather than from all
+            if (rank == 0 && tid == 0) {
+                p.tokens[row] = -1;
+                p.log_prob[row] = __int_as_float(0x7fffffff);
+            }
+            meet<PARTS>();
+            continue;
         }
         if (min_p > 0) {  // nothing at or below the largest float under the border
             const double floor_p = (double)top + tau * log(min_p < 1 ? min_p : 1);
