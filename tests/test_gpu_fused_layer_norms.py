@@ -1,0 +1,75 @@
+"""fuse_linear_epilogues(layer_norms=True) replaces a norm only where the call does what the module would have done."""
+import copy
+import io
+
+import pytest
+import torch
+
+import sten_b200 as sten
+from gpu_util import cuda
+
+pytestmark = pytest.mark.gpu
+
+
+class Output(torch.nn.Module):
+    def __init__(self, hidden=64):
+        super().__init__()
+        self.dense, self.dropout, self.LayerNorm = torch.nn.Linear(2 * hidden, hidden), torch.nn.Dropout(0.0), torch.nn.LayerNorm(hidden)
+
+    def forward(self, hidden_states, input_tensor):
+        return self.LayerNorm(self.dropout(self.dense(hidden_states)) + input_tensor)
+
+
+def rewired(layer_norms=True, change=lambda norm: None):
+    torch.manual_seed(0)
+    model = torch.nn.Sequential(Output()).half().to(cuda()).eval()
+    change(model[0].LayerNorm)
+    sb = sten.SparsityBuilder()
+    sb.set_weight("0.dense.weight", initial_sparsifier=sten.GroupedNMSparsifier(n=2, m=4, g=16), out_format=sten.GroupedNMTensor)
+    model = sb.sparsify_model_inplace(model)
+    assert sten.fuse_linear_epilogues(model, layer_norms=layer_norms) == 1
+    return model[0]
+
+
+@pytest.fixture
+def replaced(monkeypatch):
+    """How often the package's norm ran."""
+    calls, real = [], sten.fusion.layer_norm
+    monkeypatch.setattr(sten.fusion, "layer_norm", lambda *a, **k: calls.append(1) or real(*a, **k))
+    return calls
+
+
+def operands(hidden=64):
+    gen = torch.Generator(device="cuda").manual_seed(1)
+    return torch.randn(3, 128, 2 * hidden, device="cuda", generator=gen).half(), torch.randn(3, 128, hidden, device="cuda", generator=gen).half()
+
+
+def run(mod):
+    with torch.no_grad():
+        return mod(*operands())
+
+
+def test_a_plain_norm_is_replaced(replaced):
+    ours = run(rewired())
+    torchs = run(rewired(layer_norms=False))
+    assert len(replaced) == 1 and ours.dtype == torch.float16
+    # both compute in 32 bits and round once: a step of fp16 apart at most, where the two values before are on either side of a border
+    assert bool(((ours.float() - torchs.float()).abs() <= 2.0 ** -10 * torchs.float().abs() + 2.0 ** -20).all())
+
+
+def test_modules_that_were_rewired_before_there_was_a_choice(replaced):
+    """As they come out of a pickle: without the attribute that holds the choice."""
+    mod = rewired(layer_norms=False)
+    want = run(mod)
+    del mod.__dict__["_sten_layer_norm"]
+    assert torch.equal(run(mod), want) and not replaced
+    holder = torch.nn.Sequential(mod)
+    assert sten.fuse_linear_epilogues(holder, layer_norms=True) == 0
+    run(mod)
+    assert len(replaced) == 1
+    assert sten.fuse_linear_epilogues(holder) == 0 and torch.equal(run(mod), want)
+    file = io.BytesIO()
+    torch.save(mod, file)
+    file.seek(0)
+    back = torch.load(file, weights_only=False)
+    assert torch.equal(run(back), want) and torch.equal(run(copy.deepcopy(mod)), want)
