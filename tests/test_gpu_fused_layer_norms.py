@@ -57,6 +57,27 @@ def test_a_plain_norm_is_replaced(replaced):
     assert bool(((ours.float() - torchs.float()).abs() <= 2.0 ** -10 * torchs.float().abs() + 2.0 ** -20).all())
 
 
+class Masked:
+    """The smallest payload: whatever has a dense form."""
+
+    def __init__(self, dense):
+        self.dense, self.shape, self.dtype, self.device = dense, dense.shape, dense.dtype, dense.device
+
+    def to_dense(self):
+        return self.dense
+
+
+def test_a_norm_of_sparse_parameters_runs_itself(replaced):
+    """Through the dispatcher, as before."""
+    outs = []
+    for layer_norms in (False, True):
+        mod = rewired(layer_norms)
+        dense = mod.LayerNorm.weight.detach() * 3
+        mod.LayerNorm.weight = sten.SparseParameterWrapper(sten.SparseTensorWrapper.wrapped_from_dense(Masked(dense), dense))
+        outs.append(run(mod))
+    assert torch.equal(*outs) and not replaced
+
+
 def test_modules_that_were_rewired_before_there_was_a_choice(replaced):
     """As they come out of a pickle: without the attribute that holds the choice."""
     mod = rewired(layer_norms=False)
