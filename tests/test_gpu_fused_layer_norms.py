@@ -57,6 +57,15 @@ def test_a_plain_norm_is_replaced(replaced):
     assert bool(((ours.float() - torchs.float()).abs() <= 2.0 ** -10 * torchs.float().abs() + 2.0 ** -20).all())
 
 
+def test_under_autocast_the_modules_own_norm_runs(replaced):
+    with torch.autocast("cuda", dtype=torch.float16):
+        ours, torchs = run(rewired()), run(rewired(layer_norms=False))
+    assert not replaced and ours.dtype == torchs.dtype == torch.float32 and torch.equal(ours, torchs)
+    with torch.autocast("cuda", enabled=False):
+        run(rewired())
+    assert len(replaced) == 1
+
+
 class Masked:
     """The smallest payload: whatever has a dense form."""
 
