@@ -15,6 +15,7 @@ dropout is inactive; otherwise the module's own forward runs.
 import types
 
 import torch
+from torch.nn.modules import module as _module
 
 from . import ops
 from .dispatch import SparseTensorWrapper
@@ -72,7 +73,8 @@ def _fused_output_forward(self, hidden_states, input_tensor):
 
 def _is_plain_layer_norm(norm, x):
     """Whether ``norm(x)`` is layer_norm of its parameters and nothing else.  Under autocast torch's norm returns fp32."""
-    return (type(norm) is torch.nn.LayerNorm and not torch.is_autocast_enabled("cuda") and norm.normalized_shape == x.shape[-1:] and not norm._forward_hooks and not norm._forward_pre_hooks
+    return (type(norm) is torch.nn.LayerNorm and not torch.is_autocast_enabled("cuda") and norm.normalized_shape == x.shape[-1:] and "forward" not in norm.__dict__
+            and not norm._forward_hooks and not norm._forward_pre_hooks and not _module._global_forward_hooks and not _module._global_forward_pre_hooks
             and all(p is None or (type(p) in (torch.Tensor, torch.nn.Parameter) and p.is_cuda and p.dtype in (x.dtype, torch.float32)) for p in (norm.weight, norm.bias))
             and (norm.weight is None or norm.bias is None or norm.weight.dtype == norm.bias.dtype))
 

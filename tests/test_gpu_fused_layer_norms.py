@@ -66,6 +66,42 @@ def test_under_autocast_the_modules_own_norm_runs(replaced):
     assert len(replaced) == 1
 
 
+def test_a_forward_of_the_instances_own_runs(replaced):
+    def change(norm):
+        norm.forward = lambda x, real=norm.forward: real(x) + 100
+    ours, torchs = run(rewired(change=change)), run(rewired(layer_norms=False, change=change))
+    assert not replaced and torch.equal(ours, torchs) and float(ours.float().min()) > 50
+
+
+@pytest.mark.parametrize("kind", ["forward", "forward_pre", "module", "module_pre"])
+def test_hooks_run(replaced, kind):
+    mod, seen = rewired(), []
+
+    def hook(m, *rest):
+        if m is mod.LayerNorm:
+            seen.append(1)
+    register = {"forward": mod.LayerNorm.register_forward_hook, "forward_pre": mod.LayerNorm.register_forward_pre_hook,
+                "module": torch.nn.modules.module.register_module_forward_hook, "module_pre": torch.nn.modules.module.register_module_forward_pre_hook}[kind]
+    handle = register(hook)
+    try:
+        out = run(mod)
+    finally:
+        handle.remove()
+    assert seen == [1] and not replaced and torch.equal(out, run(rewired(layer_norms=False)))
+
+
+def test_norms_of_other_kinds_run_themselves(replaced):
+    class Scaled(torch.nn.LayerNorm):
+        def forward(self, x):
+            return super().forward(x) * 2
+    torchs = run(rewired(layer_norms=False))
+    mod = rewired()
+    norm = Scaled(64).half().to(cuda())
+    norm.load_state_dict(mod.LayerNorm.state_dict())
+    mod.LayerNorm = norm
+    assert torch.equal(run(mod), torchs * 2) and not replaced
+
+
 class Masked:
     """The smallest payload: whatever has a dense form."""
 
