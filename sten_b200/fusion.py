@@ -66,7 +66,7 @@ def _fused_output_forward(self, hidden_states, input_tensor):
     if gnm is None or torch.is_grad_enabled() or not dropout_off or not hidden_states.is_cuda:
         return self._sten_unfused_forward(hidden_states, input_tensor)
     h, norm = sparse_linear_fused(hidden_states, gnm, self.dense.bias, residual=input_tensor), self.LayerNorm
-    if getattr(self, "_sten_layer_norm", False) and _is_plain_layer_norm(norm, h):
+    if self._sten_layer_norm and _is_plain_layer_norm(norm, h):
         return layer_norm(h, norm.weight, norm.bias, eps=norm.eps)
     return norm(h)
 
@@ -86,7 +86,7 @@ def fuse_linear_epilogues(model, layer_norms=False):
     rewired already take the new choice of ``layer_norms``."""
     count = 0
     for mod in model.modules():
-        if getattr(getattr(mod, "forward", None), "__func__", None) is _fused_output_forward:  # one from an earlier version's pickle has no choice yet
+        if hasattr(mod, "_sten_layer_norm"):
             mod._sten_layer_norm = bool(layer_norms)
         dense = getattr(mod, "dense", None)
         if not isinstance(dense, torch.nn.Linear) or _nmg_weight(dense) is None or hasattr(mod, "_sten_unfused_forward"):

@@ -1,7 +1,4 @@
 """fuse_linear_epilogues(layer_norms=True) replaces a norm only where the call does what the module would have done."""
-import copy
-import io
-
 import pytest
 import torch
 
@@ -121,21 +118,3 @@ def test_a_norm_of_sparse_parameters_runs_itself(replaced):
         mod.LayerNorm.weight = sten.SparseParameterWrapper(sten.SparseTensorWrapper.wrapped_from_dense(Masked(dense), dense))
         outs.append(run(mod))
     assert torch.equal(*outs) and not replaced
-
-
-def test_modules_that_were_rewired_before_there_was_a_choice(replaced):
-    """As they come out of a pickle: without the attribute that holds the choice."""
-    mod = rewired(layer_norms=False)
-    want = run(mod)
-    del mod.__dict__["_sten_layer_norm"]
-    assert torch.equal(run(mod), want) and not replaced
-    holder = torch.nn.Sequential(mod)
-    assert sten.fuse_linear_epilogues(holder, layer_norms=True) == 0
-    run(mod)
-    assert len(replaced) == 1
-    assert sten.fuse_linear_epilogues(holder) == 0 and torch.equal(run(mod), want)
-    file = io.BytesIO()
-    torch.save(mod, file)
-    file.seek(0)
-    back = torch.load(file, weights_only=False)
-    assert torch.equal(run(back), want) and torch.equal(run(copy.deepcopy(mod)), want)
