@@ -106,17 +106,20 @@ __global__ void __launch_bounds__(SORT_THREADS) sort_kernel(const SortParams p) 
     const unsigned mask = (1u << p.digit_bits) - 1;
     for (int pass = 0; pass < p.passes; pass++) {
         const int from = (p.passes - pass) & 1, shift = pass * p.digit_bits;
-        const unsigned *key_in = p.key[from], *pos_in = p.pos[from];
-        unsigned *key_out = p.key[from ^ 1], *pos_out = p.pos[from ^ 1];
-        auto key_at = [&](unsigned i) -> unsigned {
+        unsigned *key_in = p.key[from], *key_out = p.key[from ^ 1], *pos_out = p.pos[from ^ 1];
+        const unsigned *pos_in = p.pos[from];
+        // An id is read once: what is counted and what is placed are the same, whoever writes to the ids meanwhile.
+        auto taken = [&](unsigned i) -> unsigned {
             if (pass) return __ldcg(key_in + i);
             const int64_t id = p.e.at(i);
-            return p.e.valid(id) && id != p.padding ? (unsigned)id : (unsigned)p.e.vocab;  // those without a gradient are last
+            const unsigned key = p.e.valid(id) && id != p.padding ? (unsigned)id : (unsigned)p.e.vocab;  // those without a gradient are last
+            key_in[i] = key;  // for the same lane below
+            return key;
         };
         for (int d = lane; d < DIGITS; d += 32) s.count[warp][d] = 0;
         __syncwarp();
 #pragma unroll 8
-        for (unsigned i = begin + lane; i < end; i += 32) atomicAdd(&s.count[warp][key_at(i) >> shift & mask], 1u);
+        for (unsigned i = begin + lane; i < end; i += 32) atomicAdd(&s.count[warp][taken(i) >> shift & mask], 1u);
         __syncthreads();
         if (tid < DIGITS) {
             unsigned sum = 0, n[SORT_WARPS];
@@ -160,7 +163,7 @@ __global__ void __launch_bounds__(SORT_THREADS) sort_kernel(const SortParams p) 
 #pragma unroll
             for (int u = 0; u < 4; u++) {
                 const unsigned i = i0 + 32 * u + lane;
-                key[u] = i < end ? key_at(i) : 0;
+                key[u] = i < end ? __ldcg(key_in + i) : 0;
                 pos[u] = i < end ? (pass ? __ldcg(pos_in + i) : i) : 0;
             }
 #pragma unroll
