@@ -751,9 +751,9 @@ template <typename T, int PARTS> __global__ void __launch_bounds__(SAMPLE_THREAD
                 found = 0xffffffffu;
                 of_warps<PARTS>([&](int r, int w, bool there) { found = min(found, there ? peer_u32<PARTS>(&s.first[w], r) : 0xffffffffu); });
                 found = __reduce_min_sync(FULL, found);
-                if (lane == 0) {
-                    p.tokens[row] = (int64_t)found;
-                    p.log_prob[row] = 0.f;
+                if (lane == 0) {  // none: somebody wrote to the logits meanwhile
+                    p.tokens[row] = found == 0xffffffffu ? -1 : (int64_t)found;
+                    p.log_prob[row] = found == 0xffffffffu ? __int_as_float(0x7fffffff) : 0.f;
                 }
             }
             meet<PARTS>();

@@ -46,3 +46,33 @@ def test_lost_borders_are_told(dtype, rows):
     for s in settings:  # and after the writes everything is as before
         a, b = sten.sample_tokens(x, u, temperature=50.0, **s), sten.sample_tokens(versions[0], u, temperature=50.0, **s)
         assert torch.equal(a.tokens, b.tokens) and torch.equal(a.log_prob, b.log_prob) and bool(among[a.tokens].all())
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("rows", [1, 8, 600])
+def test_a_largest_logit_that_is_gone(dtype, rows):
+    """Temperature 0: one of the columns that are the largest in some version, or -1 with NaN."""
+    vocab, columns = 131072, (77, 130000)
+    x = torch.zeros(rows, vocab, dtype=dtype, device="cuda")
+    versions = [x.clone(), x.clone()]
+    for v, c, top in zip(versions, columns, (50.0, 60.0)):
+        v[:, c] = top
+    u = torch.full((rows,), 0.5, device="cuda")
+    x.copy_(versions[0])
+    sten.sample_tokens(x, u, temperature=0.0)
+    writes = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(writes):
+        for i in range(40):
+            x.copy_(versions[(i + 1) % 2])
+    torch.cuda.synchronize()
+    side, drawn = torch.cuda.Stream(), []
+    for i in range(100):
+        with torch.cuda.stream(side):
+            writes.replay()
+        drawn.append(sten.sample_tokens(x, u, temperature=0.0))
+    torch.cuda.synchronize()
+    tokens, log_prob = torch.stack([d.tokens for d in drawn]), torch.stack([d.log_prob for d in drawn])
+    none = tokens == -1
+    # where a version is half written, neither of the two may be there: the first of the zeros
+    assert bool((none | (tokens == columns[0]) | (tokens == columns[1]) | (tokens == 0)).all())
+    assert bool(torch.isnan(log_prob[none]).all()) and bool((log_prob[~none] == 0).all())
