@@ -300,8 +300,9 @@ int nmg_distill_backward(const void *logits, int64_t rows, int64_t inner_rows, i
  * Each setting is one number for all rows or, where its array is not NULL, one for each row (the number is then not looked at; values
  * beyond a setting's range mean the nearest one in it).  A temperature of 0 takes the first of the largest logits, with log-probability 0;
  * u >= 1 takes the last token that is left.  A row that holds NaN or +inf or nothing but -inf, or one with a temperature below 0 or above 1e30
- * or a NaN among its settings has token -1 and log-probability NaN.  Tokens of less than 2^-(s+1) times the largest one's probability are never drawn (s =
- * min(46, 62 - log2 vocab)). */
+ * or a NaN among its settings has token -1 and log-probability NaN; so may one that is written to during the call.  Probabilities are rounded to multiples of 2^-s
+ * of the largest one's (s = min(46, 62 - log2 vocab rounded up)): tokens of less than 2^-(s+1) times that are never drawn, and n tokens together are off by
+ * n 2^-(s+1) of it at most (2^-29 for 131072 tokens, 2^-23 for 2^20). */
 int nmg_sample_tokens(const void *logits, int64_t rows, int64_t inner_rows, int64_t ld, int64_t ld_outer, int64_t vocab, int dtype,
                       const float *uniform, const float *temperatures, double temperature, const int64_t *top_ks, int64_t top_k,
                       const float *top_ps, double top_p, const float *min_ps, double min_p, int64_t *tokens, float *log_prob, void *stream);

@@ -4,7 +4,7 @@
 //
 // Both are bound by HBM.  Gradient: the tokens are sorted by their id, so that the rows of g that belong to one row of the matrix stand
 // together and are added in the order of their positions, whatever runs when, in 32 bits and rounded once.  Three launches:
-//   sort_kernel    one cluster sorts (id, position) in two or three radix passes; the other CTAs fill d_weight's first rows with zeros meanwhile
+//   sort_kernel    one cluster sorts (id, position) in a radix pass for every nine bits of the vocabulary (one to four); the other CTAs fill d_weight's first rows with zeros meanwhile
 //   sum_kernel     the sorted list is cut into pieces of equal length, a warp for 32 vectors of columns of each; ids that lie within a piece
 //                  are finished, the sums of those that cross its ends are left in the workspace.  Other CTAs fill the other rows that have no id
 //   join_kernel    puts the latter together

@@ -356,6 +356,7 @@ template <typename T, typename P> __global__ void __launch_bounds__(WIDE_THREADS
 
 // Gradients.  CTAs stay, as above, and sum g_y k and g_y of their columns in registers.  A CTA's groups are put together at the end, the CTAs by
 // column_totals_kernel, all in a fixed order.  Of 32 elements a thread only the sums stay in registers: the row is read from shared memory twice.
+// (By single elements even they do not: with the parameters' gradients the compiler spills 1000 bytes of stores and 1300 of loads a thread.)
 // 16384 x 8192 bf16 143 us (5.5 TB/s), 12288 x 1024 fp16 with the sum's gradient 25, and 6 for the totals.  One CTA an SM: twice as many would write
 // and read twice as many partial sums (10 MB here).
 template <typename T, typename P, int V, int E, bool SUM, bool PARAMS> __global__ void __launch_bounds__(512) norm_grad_kernel(const NormGradParams p, int threads, RingShape shape, int *status) {

@@ -12,7 +12,8 @@
 // token for one row in forty.  Weights are therefore integers, w 2^s rounded (s = 62 - log2 of the vocabulary, at most 46; w from a polynomial
 // in 64-bit floating point, relative error 2^-42): sums are exact, and the same for every way a row is cut.  Weights below 2^-(s+1) count as zero.
 //
-// A row is read once from memory for its maximum and again from L2.  1024 x 131072 bf16 without filters 190 us: 28 instructions a logit, of which 21 are the weight's, at
+// A row is read for its maximum and again for its weights, the second time from L2 where the rows in flight fit into it (592 of 131072 bf16, 155 MB, do not: 312 MB come from
+// HBM).  1024 x 131072 bf16 without filters 188 us: 28 instructions a logit, of which 21 are the weight's, at
 // half the issue slots (floor: 41 us of memory, 106 of issue).  256 x 131072 with top_p = 0.95 and a fifth of the tokens kept 136, 64 x 131072 with settings of every row 52,
 // 97 x 50021 fp32 with all filters 39, one row of 30522 fp16 with top-k and top-p 19: these are chains of ten or so phases with a meeting each.
 #include "nmg_rows.cuh"
@@ -30,6 +31,9 @@ struct SampleParams {
     float *log_prob;
 };
 
+// Four CTAs an SM leave a thread 64 registers, of which values that live across the phases spill (16-bit logits: 230 to 300 bytes of stores and 530 to 730 of loads in the
+// code, fp32 120 to 140 and 310 to 530; gather<true> another 60 to 150).  Three, with 80 registers, spill 120 to 145 and 350 to 500 and are slower by top-p (163 us beside 138
+// at 256 x 131072 bf16) and equal without filters (204 beside 206 at 1024 x 131072, both of an earlier form).
 constexpr int SAMPLE_THREADS = 256, SAMPLE_WARPS = SAMPLE_THREADS / 32, BINS = 1024, LISTED = 384, FLAT = 4096, CHECKS = 64, SAMPLE_PER_SM = 4;
 template <typename T> struct SampleShared {
     unsigned bin[2][BINS];  // low and high words: additions of 64 bits to shared memory are loops of compare-and-swap, which all lanes that add to one bin go through
@@ -784,6 +788,7 @@ template <typename T, int PARTS> __global__ void __launch_bounds__(SAMPLE_THREAD
             const int elements = by_weight && !by_count ? max(65536, p.x.vocab / 2) : top_k > 8192 ? 65536 : 16384;
             const float scale = take_sample<PARTS>(s, sh, window, top, per_bin, elements, me);
             if (rank == 0) {
+                // what the lists hold, less what the sample may be off by and, in the warps' lists, what one share may have more of than the others
                 const float room = fminf(0.85f * FLAT, 0.6f * WARPS * LISTED);
                 if (by_count) {
                     find_bracket<false, PARTS>(s, scale, window, top, per_bin, octaves, (float)top_k, room);
@@ -1102,7 +1107,10 @@ template <typename T, int PARTS> __global__ void __launch_bounds__(SAMPLE_THREAD
     }
 }
 
-// A row is shared by as many CTAs as keep the SMs filled, two of them to an SM; each has some thousand logits at least.
+// A row is shared by as many CTAs as make the least of rounds x (logits of a CTA + what its phases and meetings cost beside them, in logits), clusters of more than two at the
+// number that is resident; each has two thousand logits at least.  us by 1, 2, 4, 8 CTAs, bf16 without filters: one row of 131072 43, 27, 19, 15; 148 rows 46, 37, 46, 55; 1024 rows
+// 190, 193, 227, 304; 64 rows of 20011 15, 15, 15, 21; 592 rows 32, 49, 69, 125.  One cost for all settings is coarse: of 66 calls with 20011 and 131072 logits, without
+// filters, by top-p and by top-k, half have another best, faster by 1.24 on average and 1.75 at most (64 rows of 20011 by top-k 50: 8 CTAs 29, one 16; 700 rows of 131072: 4 CTAs 155, one 107).
 // `deep`: the border may lie far down.  Then a long row takes two at least, whose lists hold twice as many logits of its bracket: 1024 x 131072 bf16
 // with top_p = 0.9 takes 443 us, by one CTA a row 421, but of logits spread by 1 instead of 2.5 479 and 1484; the first of 65536 by count 440 and 794.
 static int sample_parts(int64_t rows, int vocab, bool deep, int sms) {

@@ -82,7 +82,8 @@ def _is_plain_layer_norm(norm, x):
 def fuse_linear_epilogues(model, layer_norms=False):
     """Rewire ``dense`` + GELU and ``dense`` + residual + LayerNorm modules of ``model`` whose dense weight is grouped n:m.
     ``layer_norms``: the norm behind the residual runs as ``layer_norm`` too where it is a plain ``torch.nn.LayerNorm`` of the last
-    dimension; its results differ from torch's by roundings.  Returns the number of modules rewired.  Idempotent; modules that are
+    dimension; its results differ from torch's by roundings.  The module itself still runs under autocast (its result is fp32 there), and where it
+    has a ``forward`` of its own, hooks (its own or those of all modules) or sparse parameters.  Returns the number of modules rewired.  Idempotent; modules that are
     rewired already take the new choice of ``layer_norms``."""
     count = 0
     for mod in model.modules():

@@ -64,7 +64,7 @@ def sample_tokens(logits, uniform, *, temperature=1.0, top_k=0, top_p=1.0, min_p
     exceed ``uniform`` times their sum; ``log_prob`` is its log-probability among what is left.  Each setting is a number or a tensor with
     one for each row (float32; ``top_k`` int64).  ``temperature`` 0 takes the first of the largest logits.
 
-    A row that holds NaN or +inf, or is -inf throughout, gives token -1 and log-probability NaN.  The same logits, number and settings give
+    A row that holds NaN or +inf, or is -inf throughout, gives token -1 and log-probability NaN (so may one that is written to meanwhile).  The same logits, number and settings give
     the same token in every call, whatever else is in the batch.  Not differentiable: ``token_log_probs`` is."""
     return SampledTokens(*nat.host().sample_tokens(_dense(logits), uniform, temperature, top_k, top_p, min_p))
 
